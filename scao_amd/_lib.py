@@ -1,4 +1,4 @@
-"""ctypes binding of the gfx950 C ABI (include/scao_amd.h).
+"""ctypes binding of the gfx950 C ABI (include/scao_amd.h, include/scao_train.h).
 
 The shared object is built in-tree by ``scao_amd.build`` into
 ``scao_amd/_lib/libscao_amd.so``.  It links the HIP runtime by soname; torch
@@ -21,7 +21,7 @@ import torch  # noqa: F401  -- loads torch's HIP runtime before ours
 HERE = os.path.dirname(os.path.abspath(__file__))
 LIB_PATH = os.environ.get("SCAO_AMD_LIB", os.path.join(HERE, "_lib", "libscao_amd.so"))
 
-ABI_VERSION = 14
+ABI_VERSION = 15
 SLOT_WIDTH = 3
 FLAT_CHUNK = 4096
 PROJ_COLS = 256
@@ -94,6 +94,10 @@ FILTER_MASK, FILTER_FIRST = 1, 2
 LOOKAHEAD_DESC = np.dtype([
     ("p", "u8"), ("slow", "u8"), ("numel", "i8"), ("dtype", "i4"), ("pad0", "i4"),
 ], align=True)
+
+TENSOR_DESC = np.dtype([
+    ("data", "u8"), ("numel", "i8"), ("dtype", "i4"), ("pad0", "i4"),
+], align=True)
 FILTER_WORK_WORDS = 2 * 2048 + 16
 FILTER_COMPACT_WORD = 2 * 2048 + 11   # 1 when the refinement passes read the candidates
 FILTER_REGION = 2048                  # candidate slots per chunk (SCAO_FLAT_CHUNK / 2)
@@ -105,7 +109,8 @@ STRUCTS = {0: (PARAM_DESC, [n for n in PARAM_DESC.names if n != "pad0"]),
            4: (GRAM_DESC, list(GRAM_DESC.names)),
            5: (PREP_DESC, list(PREP_DESC.names)),
            6: (FILTER_DESC, list(FILTER_DESC.names)),
-           7: (LOOKAHEAD_DESC, [n for n in LOOKAHEAD_DESC.names if n != "pad0"])}
+           7: (LOOKAHEAD_DESC, [n for n in LOOKAHEAD_DESC.names if n != "pad0"]),
+           8: (TENSOR_DESC, [n for n in TENSOR_DESC.names if n != "pad0"])}
 
 _VP, _I, _I64, _D = ctypes.c_void_p, ctypes.c_int, ctypes.c_int64, ctypes.c_double
 
@@ -154,6 +159,13 @@ SIGNATURES = {
     "scao_lookahead": (_I, [_VP, _I, _VP, ctypes.c_float, _VP]),
 }
 
+# include/scao_train.h
+TRAIN_SIGNATURES = {
+    "scao_grad_norm_workspace": (_I64, [_VP, _I]),
+    "scao_grad_norm": (_I, [_VP, _I, _I, _D, _VP, _VP, _VP]),
+    "scao_grad_clip": (_I, [_VP, _I, _I, _D, _D, _VP, _VP, _VP]),
+}
+
 
 class ScaoLibError(RuntimeError):
     pass
@@ -169,7 +181,7 @@ def _load():
             f"scao_amd: HIP library not found at {LIB_PATH}. Build it with "
             "`python -m scao_amd.build` (hipcc, gfx950). There is no CPU or torch fallback.")
     lib = ctypes.CDLL(LIB_PATH)
-    for name, (res, args) in SIGNATURES.items():
+    for name, (res, args) in {**SIGNATURES, **TRAIN_SIGNATURES}.items():
         fn = getattr(lib, name)
         fn.restype = res
         fn.argtypes = args

@@ -4,6 +4,7 @@
 #include <stddef.h>
 #include <stdio.h>
 
+#include "../../include/scao_train.h"
 #include "scao_common.hpp"
 
 static thread_local char g_err[512] = "";
@@ -104,6 +105,12 @@ extern "C" int scao_struct_layout(int which, int64_t* out, int cap) {
       typedef scao_lookahead_desc S;
       PUT(sizeof(S));
       PUT(offsetof(S, p)); PUT(offsetof(S, slow)); PUT(offsetof(S, numel)); PUT(offsetof(S, dtype));
+      break;
+    }
+    case 8: {
+      typedef scao_tensor_desc S;
+      PUT(sizeof(S));
+      PUT(offsetof(S, data)); PUT(offsetof(S, numel)); PUT(offsetof(S, dtype));
       break;
     }
     default:
