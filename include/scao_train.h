@@ -39,6 +39,42 @@ int scao_grad_norm(const scao_tensor_desc* tensors, int n, int norm_type, double
 int scao_grad_clip(const scao_tensor_desc* tensors, int n, int norm_type, double scale,
                    double max_norm, float* norm, void* workspace, void* stream);
 
+/* ---- gated feed-forward block ---------------------------------------------
+ * a = x Wg^T, b = x Wu^T, h = f(a) * b, y = h Wd^T, all row-major: x tokens x d,
+ * Wg and Wu f x d, Wd d x f, y tokens x d, with unit column stride and any row
+ * stride of at least a row; fp32, bf16 or fp16, one type for all.  Sums are
+ * fp32.  With `saved` (scao_ffn_saved_bytes() bytes) the forward pass keeps h, a
+ * and b for scao_ffn_backward: dh = dy Wd, da = dh * b * f'(a), db = dh * f(a),
+ * dx = da Wg + db Wu, dWg = da^T x, dWu = db^T x, dWd = dy^T h, each written
+ * densely (row strides d, d, d, f) unless its pointer is null.  No atomics: the
+ * same call gives the same bits.  workspace: the *_workspace() bytes for the
+ * same descriptor, aligned to 256, as is `saved`. */
+enum scao_activation {
+  SCAO_ACT_SILU = 0,        /* a / (1 + exp(-a))                                 */
+  SCAO_ACT_GELU = 1,        /* a (1 + erf(a / sqrt 2)) / 2                       */
+  SCAO_ACT_GELU_TANH = 2,   /* a (1 + tanh(sqrt(2/pi) (a + 0.044715 a^3))) / 2   */
+  SCAO_ACT_RELU = 3,        /* a where a > 0, else 0                             */
+  SCAO_ACT_SIGMOID = 4      /* 1 / (1 + exp(-a))                                 */
+};
+typedef struct scao_ffn_desc {   /* HOST */
+  const void* x;
+  const void* w_gate;
+  const void* w_up;
+  const void* w_down;
+  int64_t ldx, ld_gate, ld_up, ld_down;   /* row strides in elements             */
+  int64_t tokens, d, f;                   /* all at least 1                      */
+  int32_t dtype;            /* enum scao_dtype                                   */
+  int32_t act;              /* enum scao_activation                              */
+} scao_ffn_desc;
+int64_t scao_ffn_saved_bytes(const scao_ffn_desc* desc);
+int64_t scao_ffn_forward_workspace(const scao_ffn_desc* desc, int save);
+int scao_ffn_forward(const scao_ffn_desc* desc, void* y, void* saved, void* workspace,
+                     void* stream);
+int64_t scao_ffn_backward_workspace(const scao_ffn_desc* desc, const void* dy, int64_t ld_dy);
+int scao_ffn_backward(const scao_ffn_desc* desc, const void* dy, int64_t ld_dy, const void* saved,
+                      void* dx, void* dw_gate, void* dw_up, void* dw_down, void* workspace,
+                      void* stream);
+
 #ifdef __cplusplus
 }
 #endif

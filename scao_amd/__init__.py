@@ -9,6 +9,7 @@ phase behaviour; its step runs as batched hand-written HIP kernels
 from .optimizer import SCAO, scao_sub1b, scao_1b, scao_3b, scao_7b, scao_40b, scao_125b
 from .preconditioner import SparsePreconditioner
 from .utils import matrix_power_neg_quarter, adaptive_rank
+from .ffn import GatedFFN, gated_ffn
 from .grad_clip import clip_grad_norm_, global_grad_norm
 from . import logging as scao_logging
 
@@ -20,6 +21,8 @@ __all__ = [
     "SparsePreconditioner",
     "matrix_power_neg_quarter",
     "adaptive_rank",
+    "GatedFFN",
+    "gated_ffn",
     "clip_grad_norm_",
     "global_grad_norm",
     "scao_logging",

@@ -98,6 +98,11 @@ LOOKAHEAD_DESC = np.dtype([
 TENSOR_DESC = np.dtype([
     ("data", "u8"), ("numel", "i8"), ("dtype", "i4"), ("pad0", "i4"),
 ], align=True)
+FFN_DESC = np.dtype([
+    ("x", "u8"), ("w_gate", "u8"), ("w_up", "u8"), ("w_down", "u8"), ("ldx", "i8"),
+    ("ld_gate", "i8"), ("ld_up", "i8"), ("ld_down", "i8"), ("tokens", "i8"), ("d", "i8"),
+    ("f", "i8"), ("dtype", "i4"), ("act", "i4"),
+], align=True)
 FILTER_WORK_WORDS = 2 * 2048 + 16
 FILTER_COMPACT_WORD = 2 * 2048 + 11   # 1 when the refinement passes read the candidates
 FILTER_REGION = 2048                  # candidate slots per chunk (SCAO_FLAT_CHUNK / 2)
@@ -110,7 +115,8 @@ STRUCTS = {0: (PARAM_DESC, [n for n in PARAM_DESC.names if n != "pad0"]),
            5: (PREP_DESC, list(PREP_DESC.names)),
            6: (FILTER_DESC, list(FILTER_DESC.names)),
            7: (LOOKAHEAD_DESC, [n for n in LOOKAHEAD_DESC.names if n != "pad0"]),
-           8: (TENSOR_DESC, [n for n in TENSOR_DESC.names if n != "pad0"])}
+           8: (TENSOR_DESC, [n for n in TENSOR_DESC.names if n != "pad0"]),
+           9: (FFN_DESC, list(FFN_DESC.names))}
 
 _VP, _I, _I64, _D = ctypes.c_void_p, ctypes.c_int, ctypes.c_int64, ctypes.c_double
 
@@ -164,6 +170,11 @@ TRAIN_SIGNATURES = {
     "scao_grad_norm_workspace": (_I64, [_VP, _I]),
     "scao_grad_norm": (_I, [_VP, _I, _I, _D, _VP, _VP, _VP]),
     "scao_grad_clip": (_I, [_VP, _I, _I, _D, _D, _VP, _VP, _VP]),
+    "scao_ffn_saved_bytes": (_I64, [_VP]),
+    "scao_ffn_forward_workspace": (_I64, [_VP, _I]),
+    "scao_ffn_forward": (_I, [_VP, _VP, _VP, _VP, _VP]),
+    "scao_ffn_backward_workspace": (_I64, [_VP, _VP, _I64]),
+    "scao_ffn_backward": (_I, [_VP, _VP, _I64, _VP, _VP, _VP, _VP, _VP, _VP, _VP]),
 }
 
 

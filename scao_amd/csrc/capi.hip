@@ -113,6 +113,15 @@ extern "C" int scao_struct_layout(int which, int64_t* out, int cap) {
       PUT(offsetof(S, data)); PUT(offsetof(S, numel)); PUT(offsetof(S, dtype));
       break;
     }
+    case 9: {
+      typedef scao_ffn_desc S;
+      PUT(sizeof(S));
+      PUT(offsetof(S, x)); PUT(offsetof(S, w_gate)); PUT(offsetof(S, w_up));
+      PUT(offsetof(S, w_down)); PUT(offsetof(S, ldx)); PUT(offsetof(S, ld_gate));
+      PUT(offsetof(S, ld_up)); PUT(offsetof(S, ld_down)); PUT(offsetof(S, tokens));
+      PUT(offsetof(S, d)); PUT(offsetof(S, f)); PUT(offsetof(S, dtype)); PUT(offsetof(S, act));
+      break;
+    }
     default:
       return 0;
   }

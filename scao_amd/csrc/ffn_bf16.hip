@@ -1,0 +1,6 @@
+// The gated feed-forward block's kernels for bf16.
+#include "ffn_kernels.hpp"
+
+namespace scao {
+FfnLaunchers ffn_bf16() { return {launch_product<SCAO_BF16>, launch_pack<SCAO_BF16>}; }
+}

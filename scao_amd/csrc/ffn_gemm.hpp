@@ -1,0 +1,273 @@
+// Tiled matrix products of the gated feed-forward block on gfx950's bf16 and
+// fp16 matrix cores, with the block's epilogues.
+//
+//   C[m][n] = sum over segments s and k of A_s[m][k] B_s[n][k]
+//
+// An operand is stored either with k contiguous ("rows": element (r, k) at
+// r*ld + k) or with r contiguous ("cols": k*ld + r); the six products of the
+// block's forward and backward pass need rows x rows, rows x cols and cols x
+// cols.  Segments add products of different operands of one shape: da Wg + db
+// Wu, and the six partial products of an fp32 product on bf16 cores.
+//
+// A workgroup owns a BM x BN tile of C and walks k in steps of 64.  Each step's
+// two tiles go from global memory to LDS without passing registers (16 bytes a
+// lane), one step ahead of the products, into the other of two stages.  The
+// buffer descriptor's bound and an out-of-range lane offset give zeros outside
+// the operands, so no edge needs a branch.
+//
+// LDS layout.  The direct load writes lane l's 16 bytes at l*16, so tiles are
+// permuted by choosing which 16 bytes a lane fetches:
+//   rows: a row's 64 k are 8 chunks of 16 bytes; chunk c of row r lies at c ^
+//         (r & 7), so that the 16 rows a fragment read touches spread over all
+//         banks;
+//   cols: a k's R elements are R/16 chunks of 32 bytes; chunk c of k lies at
+//         c ^ f(k), f(k) = (k & 3) | (k >> 3 & 1) << 2: a transposing read takes
+//         32 bytes of 16 different k.
+#pragma once
+
+#include "../../include/scao_train.h"
+#include "scao_common.hpp"
+
+namespace scao {
+
+typedef _Float16 v8h __attribute__((ext_vector_type(8)));
+typedef short v4s __attribute__((ext_vector_type(4)));
+typedef short v8s __attribute__((ext_vector_type(8)));
+typedef int v4i __attribute__((ext_vector_type(4)));
+typedef __attribute__((address_space(3))) char lchar;
+typedef __attribute__((address_space(3))) v4s lv4s;
+typedef __attribute__((address_space(3))) v8s lv8s;
+
+constexpr int FFN_BK = 64;
+constexpr int FFN_MAX_SEG = 12;
+
+enum { ROWS = 0, COLS = 1 };
+
+// one 16x16x32 product: lane l supplies P[l%16][8*(l/16)+e] and Q[l%16][8*(l/16)+e];
+// element r of the result is the product of P's row 4*(l/16)+r and Q's row l%16
+template <bool F16>
+__device__ __forceinline__ v4f mma(v8s p, v8s q, v4f c) {
+  if (F16)
+    return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(v8h, p),
+                                                  __builtin_bit_cast(v8h, q), c, 0, 0, 0);
+  return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(v8bf, p),
+                                                 __builtin_bit_cast(v8bf, q), c, 0, 0, 0);
+}
+
+// 16 bytes a lane from global memory to LDS at lds + 16*lane.  The compiler
+// neither counts this load nor waits for it: ffn_wait_all does.
+__device__ __forceinline__ void load_lds(v4i rsrc, uint32_t lds, uint32_t voff) {
+  asm volatile("s_mov_b32 m0, %0\n\tbuffer_load_dwordx4 %1, %2, 0 offen lds" ::"s"(lds), "v"(voff),
+               "s"(rsrc)
+               : "memory");
+}
+// every load of this wave has arrived in LDS and every LDS read of it has been
+// answered, and every other wave says the same
+__device__ __forceinline__ void wait_all() {
+  asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory");
+}
+
+constexpr uint32_t OUT_OF_RANGE = 0x80000000u;
+
+__device__ __forceinline__ v4i buffer_of(const void* p, int64_t bytes) {
+  const uint64_t a = (uint64_t)(uintptr_t)p;
+  const int64_t n = bytes < 0 ? 0 : bytes > 0x7fffffff ? 0x7fffffff : bytes;
+  v4i r;
+  r[0] = __builtin_amdgcn_readfirstlane((int)(uint32_t)a);
+  r[1] = __builtin_amdgcn_readfirstlane((int)(uint32_t)(a >> 32) & 0xffff);
+  r[2] = __builtin_amdgcn_readfirstlane((int)n);
+  r[3] = 0x00020000;
+  return r;
+}
+
+// One operand's share of a step: R rows (of C's dimension) by 64 k, 16-bit.
+template <int L, int R, int NW>
+struct Tile {
+  static constexpr int BYTES = R * FFN_BK * 2;
+  static constexpr int LOADS = BYTES / 1024 / NW;   // per wave and step
+  static constexpr int KROW = R * 2;                // cols: bytes of one k
+  static_assert(BYTES % (1024 * NW) == 0, "whole loads a wave");
+
+  // byte offset, relative to the step's origin, of what lane `lane` of load i
+  // of wave w fetches
+  static __device__ uint32_t offset(int i, int w, int lane, int64_t ld) {
+    const int at = (i * NW + w) * 1024 + lane * 16;
+    if (L == ROWS) {
+      const int r = at / 128, c = (at % 128) / 16 ^ (r & 7);
+      return (uint32_t)(r * ld * 2 + c * 16);
+    }
+    const int k = at / KROW, p = (at % KROW) / 16;
+    return (uint32_t)(k * ld * 2 + (((p >> 1) ^ fold(k)) * 2 + (p & 1)) * 16);
+  }
+  // its position in the dimension that has to be checked by hand: k for rows
+  // (a row's tail is followed by the next row), r for cols
+  static __device__ int inner(int i, int w, int lane) {
+    const int at = (i * NW + w) * 1024 + lane * 16;
+    if (L == ROWS) return ((at % 128) / 16 ^ ((at / 128) & 7)) * 8;
+    const int k = at / KROW, p = (at % KROW) / 16;
+    return (((p >> 1) ^ fold(k)) * 2 + (p & 1)) * 8;
+  }
+  static __device__ int fold(int k) { return (k & 3) | ((k >> 3 & 1) << 2); }
+
+  // fragment of 16 rows from row r0 (a multiple of 16), k = 32 ks + 0..31
+  static __device__ v8s frag(const lchar* t, int r0, int ks, int lane) {
+    const int q = lane & 15, g = lane >> 4;
+    if (L == ROWS) {
+      const int r = r0 + q;
+      return *(const lv8s*)(t + r * 128 + ((ks * 4 + g) ^ (r & 7)) * 16);
+    }
+    const int k = ks * 32 + 8 * g + (q >> 2);
+    const lchar* p = t + k * KROW + ((r0 >> 4) ^ fold(k)) * 32 + (q & 3) * 8;
+    const v4s lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lv4s*)p);
+    const v4s hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lv4s*)(p + 4 * KROW));
+    return __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7);
+  }
+};
+
+// Where the products' operands lie.  The second half of b[] holds the up
+// projection's segments where the first holds the gate's (GATED).
+struct FfnOperands {
+  const void* a[FFN_MAX_SEG];
+  const void* b[FFN_MAX_SEG];
+  int64_t lda, ldb;
+  int M, N, K;          // C's sizes (N: one projection's with GATED), k of one segment
+  int nseg;
+  int splits;           // parts of the k steps of all segments
+  int tiles_m, tiles_n;
+};
+
+// The tile of workgroup `b`.  Consecutive workgroups go to different XCDs, each
+// with an L2 of its own: the tiles are dealt out so that one XCD gets a
+// contiguous piece of an order that walks C in bands of 8 tile rows.
+__device__ __forceinline__ void tile_of(int b, int tm, int tn, int& m, int& n) {
+  const int total = tm * tn, per = total / 8, rest = total % 8;
+  const int x = b % 8, y = b / 8;
+  const int t = x * per + (x < rest ? x : rest) + y;
+  constexpr int BAND = 8;
+  const int band = t / (BAND * tn), rows = min(BAND, tm - band * BAND);
+  const int in = t - band * BAND * tn;
+  m = band * BAND + in % rows;
+  n = in / rows;
+}
+
+// GATED: B's tile rows 0 .. BN/2-1 are gate rows, the others the same columns'
+// up rows; each wave's fragments are half of either.
+template <int BM, int BN, int WM, int WN, int LA, int LB, bool F16, bool GATED>
+struct Gemm {
+  static constexpr int NW = WM * WN, THREADS = NW * 64;
+  static constexpr int MI = BM / WM / 16, NJ = BN / WN / 16;
+  using TA = Tile<LA, BM, NW>;
+  using TB = Tile<LB, BN, NW>;
+  static constexpr int STAGE = TA::BYTES + TB::BYTES;
+  static constexpr int COLS_N = GATED ? BN / 2 : BN;   // of C
+  static_assert(!GATED || LB == ROWS, "gated products have weights in rows");
+
+  const FfnOperands& o;
+  lchar* lds;
+  int wave, lane, wm, wn, m0, n0;
+  uint32_t offa[TA::LOADS], offb[TB::LOADS];
+  int ina[TA::LOADS], inb[TB::LOADS];
+
+  __device__ Gemm(const FfnOperands& ops, lchar* l, int tm, int tn) : o(ops), lds(l) {
+    wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    lane = threadIdx.x & 63;
+    wm = wave / WN;
+    wn = wave % WN;
+    m0 = tm * BM;
+    n0 = tn * COLS_N;
+#pragma unroll
+    for (int i = 0; i < TA::LOADS; ++i) {
+      offa[i] = TA::offset(i, wave, lane, o.lda);
+      ina[i] = TA::inner(i, wave, lane);
+      if (LA == COLS && m0 + ina[i] >= o.M) offa[i] = OUT_OF_RANGE;
+    }
+#pragma unroll
+    for (int i = 0; i < TB::LOADS; ++i) {
+      offb[i] = TB::offset(i, wave, lane, o.ldb);
+      if (GATED && up_half(i)) offb[i] -= (uint32_t)(BN / 2 * o.ldb * 2);
+      inb[i] = TB::inner(i, wave, lane);
+      if (LB == COLS && n0 + inb[i] >= o.N) offb[i] = OUT_OF_RANGE;
+    }
+  }
+  __device__ bool up_half(int i) const { return (i * NW + wave) * 8 >= BN / 2; }
+
+  // C row of the first of fragment i's rows, C column of fragment j's
+  __device__ int frag_m(int i) const { return wm * (BM / WM) + i * 16; }
+  __device__ int frag_n(int j) const {   // LDS row
+    if (GATED) return (j < NJ / 2 ? 0 : BN / 2) + wn * (BN / 2 / WN) + (j % (NJ / 2)) * 16;
+    return wn * (BN / WN) + j * 16;
+  }
+
+  template <int L>
+  static __device__ v4i buffer(const void* p, int64_t ld, int r0, int rows, int k0, int K) {
+    // rows: up to row rows-1's k K-1; cols: up to k K-1's row rows-1.  A 16-byte
+    // load that the bound cuts gives zeros whole, so the contiguous size counts
+    // with the padding to 8 elements that every row of an operand has.
+    const char* base = (const char*)p;
+    if (L == ROWS)
+      return buffer_of(base + ((int64_t)r0 * ld + k0) * 2,
+                       ((int64_t)(rows - 1 - r0) * ld + ((K + 7) & ~7) - k0) * 2);
+    return buffer_of(base + ((int64_t)k0 * ld + r0) * 2,
+                     ((int64_t)(K - 1 - k0) * ld + ((rows + 7) & ~7) - r0) * 2);
+  }
+
+  __device__ void fetch(int stage, int seg, int k0) const {
+    const uint32_t at = (uint32_t)(uintptr_t)(lds + stage * STAGE);
+    const v4i ra = buffer<LA>(o.a[seg], o.lda, m0, o.M, k0, o.K);
+#pragma unroll
+    for (int i = 0; i < TA::LOADS; ++i)
+      load_lds(ra, at + (i * NW + wave) * 1024,
+               LA == ROWS && k0 + ina[i] >= o.K ? OUT_OF_RANGE : offa[i]);
+    const v4i rb = buffer<LB>(o.b[seg], o.ldb, n0, o.N, k0, o.K);
+    const v4i ru = GATED ? buffer<LB>(o.b[seg + FFN_MAX_SEG / 2], o.ldb, n0, o.N, k0, o.K) : rb;
+#pragma unroll
+    for (int i = 0; i < TB::LOADS; ++i)
+      load_lds(GATED && up_half(i) ? ru : rb, at + TA::BYTES + (i * NW + wave) * 1024,
+               LB == ROWS && k0 + inb[i] >= o.K ? OUT_OF_RANGE : offb[i]);
+  }
+
+  __device__ void products(int stage, v4f (&acc)[MI][NJ]) const {
+    const lchar* ta = lds + stage * STAGE;
+    const lchar* tb = ta + TA::BYTES;
+#pragma unroll
+    for (int ks = 0; ks < 2; ++ks) {
+      v8s a[MI], b[NJ];
+#pragma unroll
+      for (int j = 0; j < NJ; ++j) b[j] = TB::frag(tb, frag_n(j), ks, lane);
+#pragma unroll
+      for (int i = 0; i < MI; ++i) a[i] = TA::frag(ta, frag_m(i), ks, lane);
+#pragma unroll
+      for (int i = 0; i < MI; ++i)
+#pragma unroll
+        for (int j = 0; j < NJ; ++j) acc[i][j] = mma<F16>(b[j], a[i], acc[i][j]);
+    }
+  }
+
+  // the k steps [begin, end) of all segments' steps in order
+  __device__ void run(int begin, int end, v4f (&acc)[MI][NJ]) const {
+#pragma unroll
+    for (int i = 0; i < MI; ++i)
+#pragma unroll
+      for (int j = 0; j < NJ; ++j) acc[i][j] = v4f{0.f, 0.f, 0.f, 0.f};
+    if (begin >= end) return;
+    const int steps = (o.K + FFN_BK - 1) / FFN_BK;
+    int seg = begin / steps, k0 = (begin % steps) * FFN_BK;
+    fetch(0, seg, k0);
+    int stage = 0;
+    for (int s = begin; s < end; ++s) {
+      wait_all();
+      if (s + 1 < end) {
+        k0 += FFN_BK;
+        if (k0 >= o.K) {
+          k0 = 0;
+          ++seg;
+        }
+        fetch(stage ^ 1, seg, k0);
+      }
+      products(stage, acc);
+      stage ^= 1;
+    }
+  }
+};
+
+}  // namespace scao

@@ -1,0 +1,380 @@
+// The kernels of the gated feed-forward block: the tiled products with their
+// epilogues, the join of a product that was split over k, and the packing of
+// operands.  One translation unit instantiates them for each type.
+//
+//   a = x Wg^T, b = x Wu^T, h = f(a) * b, y = h Wd^T
+//   dh = dy Wd, da = dh * b * f'(a), db = dh * f(a)
+//   dx = da Wg + db Wu, dWg = da^T x, dWu = db^T x, dWd = dy^T h
+//
+// Roundings of the 16-bit types: h, da and db, which enter further products on
+// the matrix cores, to the type itself, once each; nothing else before the
+// outputs.  a and b, which only enter f' and elementwise products, are kept for
+// the backward pass with 16 significant bits (24 of a float's 32): rounded to 8
+// (bf16) they would add as much error to da and db as those' own rounding.  In
+// fp32 nothing is rounded below it: h, da and db are kept as three bf16 parts
+// that add up to them, and a product of two such sums is six products of parts
+// (see mfma_x6) run as six segments of one bf16 product.
+#pragma once
+
+#include "ffn_gemm.hpp"
+
+namespace scao {
+
+enum { EPI_STORE = 0, EPI_GATED = 1, EPI_DACT = 2 };
+
+struct FfnEpilogue {
+  void* out;            // STORE: rows of C; GATED: h; DACT: da, and db next to it
+  void* out2;           // STORE: rows from `second` on, or null
+  int64_t ldo;
+  int64_t plane;        // GATED, DACT in fp32: elements from one part to the next
+  int rows, second;     // STORE: rows of either output, C's row where the second begins
+  int cols;             // columns written
+  int fi, fj;           // fragments of 16 rows and of 16 columns of a and b kept
+  void* ab;             // a and b by fragments, or null (GATED: nothing is kept)
+  int act;
+  float* partial;       // split products: the parts, by fragments
+};
+
+// ------------------------------------------------------- activations -------
+// 1 / (1 + exp(-z)) from the hardware's exp2 and reciprocal (an ulp each).  The
+// product z log2(e) is kept as a sum of two floats where the result is fp32:
+// its rounding alone would be |z| 6e-8 of the result.
+template <bool F32>
+__device__ __forceinline__ float logistic(float z) {
+  constexpr float L2E = 1.44269504f, L2E_LO = 1.92596303e-8f;
+  float e;
+  const float t = -z * L2E;
+  if (F32) {
+    const float lo = fmaf(-z, L2E, -t) - z * L2E_LO;
+    // the correction only where it is a number (t finite) and matters
+    const float p = __builtin_amdgcn_exp2f(t);
+    e = fabsf(t) < 126.f ? fmaf(p, lo * 0.69314718f, p) : p;
+  } else {
+    e = __builtin_amdgcn_exp2f(t);
+  }
+  return __builtin_amdgcn_rcpf(1.f + e);
+}
+
+// f(a) and f'(a)
+template <int ACT, bool F32>
+__device__ __forceinline__ void activation(float a, float& f, float& g) {
+  if (ACT == SCAO_ACT_SILU) {
+    const float s = logistic<F32>(a);
+    f = a * s;
+    g = s * fmaf(a, 1.f - s, 1.f);
+  } else if (ACT == SCAO_ACT_SIGMOID) {
+    const float s = logistic<F32>(a);
+    f = s;
+    g = s * (1.f - s);
+  } else if (ACT == SCAO_ACT_RELU) {
+    // a NaN stays one, as in a product with (a > 0)
+    f = a > 0.f ? a : a * 0.f;
+    g = a > 0.f ? 1.f : 0.f;
+  } else if (ACT == SCAO_ACT_GELU) {
+    const float c = 0.5f * erfcf(a * -0.70710678f);
+    f = a * c;
+    g = fmaf(a * 0.39894228f, expf(-0.5f * a * a), c);
+  } else {   // a/2 (1 + tanh u) = a logistic(2u), u = sqrt(2/pi) (a + 0.044715 a^3)
+    const float a2 = a * a;
+    const float s = logistic<F32>(1.59576912f * fmaf(0.044715f * a2, a, a));
+    f = a * s;
+    g = fmaf(a * s * (1.f - s), 1.59576912f * fmaf(0.134145f, a2, 1.f), s);
+  }
+}
+
+// --------------------------------------------------------- stores ----------
+// TYPE: enum scao_dtype of the block.  Four values of one row as an operand of a
+// further product: one 16-bit value each, or three bf16 parts in three planes.
+template <int TYPE>
+__device__ __forceinline__ void put_operand(void* base, int64_t at, int64_t plane, v4f x) {
+  uint16_t* p = (uint16_t*)base + at;
+  if (TYPE == SCAO_F32) {
+    v2u h, m, l;
+    uint32_t w[3];
+#pragma unroll
+    for (int t = 0; t < 2; ++t) {
+      split3_pk(x[2 * t], x[2 * t + 1], w[0], w[1], w[2]);
+      h[t] = w[0];
+      m[t] = w[1];
+      l[t] = w[2];
+    }
+    *(gv2u*)p = h;
+    *(gv2u*)(p + plane) = m;
+    *(gv2u*)(p + 2 * plane) = l;
+  } else if (TYPE == SCAO_BF16) {
+    *(gv2u*)p = v2u{pk_bf16(x[0], x[1]), pk_bf16(x[2], x[3])};
+  } else {
+    *(gv2u*)p = v4f_to_halves(SCAO_F16, x);
+  }
+}
+
+// a and b of one fragment, four of either a lane.  16-bit types: 16 bytes of
+// upper halves a lane, then, behind all fragments', 8 bytes of the next 8 bits.
+template <int TYPE>
+__host__ __device__ constexpr int64_t ab_bytes(int64_t fi, int64_t fj) {
+  return fi * fj * 64 * (TYPE == SCAO_F32 ? 32 : 24);
+}
+typedef __attribute__((address_space(1))) v4u_t gv4u_a16;
+typedef __attribute__((address_space(1))) v2u gv2u_a8;
+
+template <int TYPE>
+__device__ __forceinline__ void put_ab(void* ab, int64_t frags, int64_t frag, int lane, v4f a,
+                                       v4f b) {
+  const int64_t at = frag * 64 + lane;
+  v4u_t ua = __builtin_bit_cast(v4u_t, a), ub = __builtin_bit_cast(v4u_t, b);
+  if (TYPE == SCAO_F32) {
+    ((gv4u_a16*)ab)[2 * at] = ua;
+    ((gv4u_a16*)ab)[2 * at + 1] = ub;
+    return;
+  }
+  v4u_t hi;
+  v2u lo;
+  // byte selectors of v_perm_b32: 0-3 of the second word, 4-7 of the first
+  hi[0] = __builtin_amdgcn_perm(ua[1], ua[0], 0x07060302u);
+  hi[1] = __builtin_amdgcn_perm(ua[3], ua[2], 0x07060302u);
+  hi[2] = __builtin_amdgcn_perm(ub[1], ub[0], 0x07060302u);
+  hi[3] = __builtin_amdgcn_perm(ub[3], ub[2], 0x07060302u);
+  lo[0] = __builtin_amdgcn_perm(ua[1], ua[0], 0x0c0c0501u) |
+          __builtin_amdgcn_perm(ua[3], ua[2], 0x05010c0cu);
+  lo[1] = __builtin_amdgcn_perm(ub[1], ub[0], 0x0c0c0501u) |
+          __builtin_amdgcn_perm(ub[3], ub[2], 0x05010c0cu);
+  ((gv4u_a16*)ab)[at] = hi;
+  ((gv2u_a8*)((char*)ab + frags * 1024))[at] = lo;
+}
+template <int TYPE>
+__device__ __forceinline__ void get_ab(const void* ab, int64_t frags, int64_t frag, int lane,
+                                       v4f& a, v4f& b) {
+  const int64_t at = frag * 64 + lane;
+  if (TYPE == SCAO_F32) {
+    a = __builtin_bit_cast(v4f, (v4u_t)((const gv4u_a16*)ab)[2 * at]);
+    b = __builtin_bit_cast(v4f, (v4u_t)((const gv4u_a16*)ab)[2 * at + 1]);
+    return;
+  }
+  const v4u_t hi = ((const gv4u_a16*)ab)[at];
+  const v2u lo = ((const gv2u_a8*)((const char*)ab + frags * 1024))[at];
+#pragma unroll
+  for (int t = 0; t < 4; ++t) {
+    // bytes 1 (from lo), 2 and 3 (from hi) of the float; byte 0 is zero
+    const uint32_t half = t & 1 ? 0x0706000cu : 0x0504000cu;
+    a[t] = __uint_as_float(__builtin_amdgcn_perm(hi[t / 2], lo[0], half | (uint32_t)t << 8));
+    b[t] = __uint_as_float(__builtin_amdgcn_perm(hi[2 + t / 2], lo[1], half | (uint32_t)t << 8));
+  }
+}
+
+// ------------------------------------------------------ epilogues ----------
+// Four consecutive columns n .. n+3 of row m of C.
+template <int TYPE>
+__device__ __forceinline__ void epi_store(const FfnEpilogue& e, int m, int n, v4f c) {
+  void* out = e.out;
+  if (m >= e.second) {
+    m -= e.second;
+    out = e.out2;
+  }
+  if (m >= e.rows || n >= e.cols || !out) return;
+  const int64_t at = (int64_t)m * e.ldo + n;
+  const int left = e.cols - n;
+  st4(out, TYPE, at, c, left >= 4, left >= 4 ? 15 : (1 << left) - 1);
+}
+
+template <int TYPE, int ACT>
+__device__ __forceinline__ void epi_gated(const FfnEpilogue& e, int m, int n, int lane, v4f a,
+                                          v4f b) {
+  v4f h;
+#pragma unroll
+  for (int t = 0; t < 4; ++t) {
+    float f, g;
+    activation<ACT, TYPE == SCAO_F32>(a[t], f, g);
+    h[t] = f * b[t];
+  }
+  if (m < e.rows && n < e.cols)
+    put_operand<TYPE>(e.out, (int64_t)m * e.ldo + n, e.plane, h);
+  const int fi = m >> 4, fj = n >> 4;
+  if (e.ab && fi < e.fi && fj < e.fj)
+    put_ab<TYPE>(e.ab, (int64_t)e.fi * e.fj, (int64_t)fi * e.fj + fj, lane, a, b);
+}
+
+template <int TYPE, int ACT>
+__device__ __forceinline__ void epi_dact(const FfnEpilogue& e, int m, int n, int lane, v4f dh) {
+  const int fi = m >> 4, fj = n >> 4;
+  if (fi >= e.fi || fj >= e.fj) return;
+  v4f a, b, da, db;
+  get_ab<TYPE>(e.ab, (int64_t)e.fi * e.fj, (int64_t)fi * e.fj + fj, lane, a, b);
+#pragma unroll
+  for (int t = 0; t < 4; ++t) {
+    float f, g;
+    activation<ACT, TYPE == SCAO_F32>(a[t], f, g);
+    da[t] = dh[t] * b[t] * g;
+    db[t] = dh[t] * f;
+  }
+  if (m < e.rows && n < e.cols) {
+    const int64_t at = (int64_t)m * e.ldo + n;
+    put_operand<TYPE>(e.out, at, e.plane, da);
+    put_operand<TYPE>(e.out, at + e.ldo / 2, e.plane, db);
+  }
+}
+
+// f(act) for every activation, outside of the unrolled loops
+#define FFN_FOR_ACT(act, CALL)            \
+  switch (act) {                          \
+    case SCAO_ACT_SILU: CALL(SCAO_ACT_SILU); break;           \
+    case SCAO_ACT_GELU: CALL(SCAO_ACT_GELU); break;           \
+    case SCAO_ACT_GELU_TANH: CALL(SCAO_ACT_GELU_TANH); break; \
+    case SCAO_ACT_RELU: CALL(SCAO_ACT_RELU); break;           \
+    default: CALL(SCAO_ACT_SIGMOID); break;                   \
+  }
+
+// ------------------------------------------------------- products ----------
+typedef __attribute__((address_space(1))) v4f gv4f_a16;
+
+template <class G, int TYPE, int EPI>
+__global__ __launch_bounds__(G::THREADS, 2) void k_ffn_gemm(const FfnOperands o,
+                                                            const FfnEpilogue e) {
+  __shared__ __attribute__((aligned(1024))) char smem[2 * G::STAGE];
+  const int tiles = o.tiles_m * o.tiles_n;
+  const int part = blockIdx.x / tiles;
+  int tm, tn;
+  tile_of(blockIdx.x - part * tiles, o.tiles_m, o.tiles_n, tm, tn);
+  G g(o, (lchar*)smem, tm, tn);
+  const int steps = o.nseg * ((o.K + FFN_BK - 1) / FFN_BK);
+  const int per = (steps + o.splits - 1) / o.splits;
+  v4f acc[G::MI][G::NJ];
+  g.run(part * per, min(steps, part * per + per), acc);
+
+  const int lane = g.lane, dm = lane & 15, dn = 4 * (lane >> 4);
+  if (o.splits > 1) {
+    // C's fragments in order, a projection's behind the other's (GATED)
+    constexpr int H = EPI == EPI_GATED ? 2 : 1;
+    const int64_t fj = o.tiles_n * (G::COLS_N / 16), fi = o.tiles_m * (int64_t)(G::TA::BYTES / 2048);
+    gv4f_a16* to = (gv4f_a16*)e.partial + part * fi * fj * H * 64;
+#pragma unroll
+    for (int i = 0; i < G::MI; ++i)
+#pragma unroll
+      for (int j = 0; j < G::NJ; ++j) {
+        const int half = EPI == EPI_GATED && j >= G::NJ / 2;
+        const int n = g.n0 + g.frag_n(j) - half * G::COLS_N;
+        to[(((g.m0 + g.frag_m(i)) / 16 + half * fi) * fj + n / 16) * 64 + lane] = acc[i][j];
+      }
+    return;
+  }
+  if constexpr (EPI == EPI_STORE) {
+#pragma unroll
+    for (int i = 0; i < G::MI; ++i)
+#pragma unroll
+      for (int j = 0; j < G::NJ; ++j)
+        epi_store<TYPE>(e, g.m0 + g.frag_m(i) + dm, g.n0 + g.frag_n(j) + dn, acc[i][j]);
+  } else {
+#define FFN_EPILOGUE(ACT)                                                                     \
+  _Pragma("unroll") for (int i = 0; i < G::MI; ++i) {                                         \
+    const int m = g.m0 + g.frag_m(i) + dm;                                                    \
+    if constexpr (EPI == EPI_GATED) {                                                         \
+      _Pragma("unroll") for (int j = 0; j < G::NJ / 2; ++j)                                   \
+          epi_gated<TYPE, ACT>(e, m, g.n0 + g.frag_n(j) + dn, lane, acc[i][j],                \
+                               acc[i][j + G::NJ / 2]);                                        \
+    } else {                                                                                  \
+      _Pragma("unroll") for (int j = 0; j < G::NJ; ++j)                                       \
+          epi_dact<TYPE, ACT>(e, m, g.n0 + g.frag_n(j) + dn, lane, acc[i][j]);                \
+    }                                                                                         \
+  }
+    FFN_FOR_ACT(e.act, FFN_EPILOGUE)
+#undef FFN_EPILOGUE
+  }
+}
+
+// The parts of a split product, added in order, and its epilogue: a wave takes
+// a fragment.
+template <int TYPE, int EPI>
+__global__ __launch_bounds__(256) void k_ffn_join(const FfnEpilogue e, int splits, int fi, int fj) {
+  constexpr int H = EPI == EPI_GATED ? 2 : 1;
+  const int64_t frag = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6);
+  if (frag >= (int64_t)fi * fj) return;
+  const int lane = threadIdx.x & 63;
+  const int m = (int)(frag / fj) * 16 + (lane & 15), n = (int)(frag % fj) * 16 + 4 * (lane >> 4);
+  const gv4f_a16* p = (const gv4f_a16*)e.partial + frag * 64 + lane;
+  const int64_t all = (int64_t)fi * fj * 64;
+  v4f a = {0.f, 0.f, 0.f, 0.f}, b = a;
+  for (int s = 0; s < splits; ++s) {
+    a += p[s * all * H];
+    if (EPI == EPI_GATED) b += p[s * all * H + all];
+  }
+  if constexpr (EPI == EPI_STORE) {
+    epi_store<TYPE>(e, m, n, a);
+  } else {
+#define FFN_EPILOGUE(ACT)                                                   \
+  if constexpr (EPI == EPI_GATED) epi_gated<TYPE, ACT>(e, m, n, lane, a, b); \
+  else epi_dact<TYPE, ACT>(e, m, n, lane, a);
+    FFN_FOR_ACT(e.act, FFN_EPILOGUE)
+#undef FFN_EPILOGUE
+  }
+}
+
+// --------------------------------------------------------- packing ---------
+// rows x cols elements with any row stride and start, as a product's operand:
+// rows of `ldo` elements (cols rounded up to 8, the rest zero), 16-byte aligned;
+// an fp32 one as three bf16 planes that add up to it.  Eight columns a thread.
+template <int TYPE>
+__global__ __launch_bounds__(256) void k_ffn_pack(const void* src, int64_t lds_, int64_t rows,
+                                                  int cols, void* dst, int ldo, int64_t plane) {
+  const int per = ldo / 8;
+  const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x;
+  if (i >= rows * per) return;
+  const int64_t r = i / per;
+  const int c = (int)(i % per) * 8;
+#pragma unroll
+  for (int t = 0; t < 8; t += 4) {
+    const int left = cols - c - t;
+    const v4f x = ld4(src, TYPE, r * lds_ + c + t, left >= 4,
+                      left >= 4 ? 15 : left <= 0 ? 0 : (1 << left) - 1);
+    put_operand<TYPE>(dst, r * ldo + c + t, plane, x);
+  }
+}
+
+// --------------------------------------------------------- launches --------
+// The products by the layouts of their operands and their epilogue.
+enum { FFN_GATE_UP, FFN_DOWN, FFN_DH, FFN_DX, FFN_DW };
+
+template <int TYPE, int TILE, int WM, int WN, int LA, int LB, int EPI>
+void launch_gemm(const FfnOperands& o, const FfnEpilogue& e, hipStream_t st) {
+  using G = Gemm<TILE, TILE, WM, WN, LA, LB, TYPE == SCAO_F16, EPI == EPI_GATED>;
+  const int tiles = o.tiles_m * o.tiles_n;
+  k_ffn_gemm<G, TYPE, EPI><<<tiles * o.splits, G::THREADS, 0, st>>>(o, e);
+  if (o.splits == 1) return;
+  const int fi = o.tiles_m * (TILE / 16), fj = o.tiles_n * (G::COLS_N / 16);
+  const int64_t frags = (int64_t)fi * fj;
+  k_ffn_join<TYPE, EPI><<<(int)((frags + 3) / 4), 256, 0, st>>>(e, o.splits, fi, fj);
+}
+
+template <int TYPE, int LA, int LB, int EPI>
+void launch_tile(int tile, const FfnOperands& o, const FfnEpilogue& e, hipStream_t st) {
+  if (tile == 256) launch_gemm<TYPE, 256, 2, 4, LA, LB, EPI>(o, e, st);
+  else launch_gemm<TYPE, 128, 2, 2, LA, LB, EPI>(o, e, st);
+}
+
+template <int TYPE>
+void launch_product(int kind, int tile, const FfnOperands& o, const FfnEpilogue& e,
+                    hipStream_t st) {
+  switch (kind) {
+    case FFN_GATE_UP: launch_tile<TYPE, ROWS, ROWS, EPI_GATED>(tile, o, e, st); break;
+    case FFN_DOWN: launch_tile<TYPE, ROWS, ROWS, EPI_STORE>(tile, o, e, st); break;
+    case FFN_DH: launch_tile<TYPE, ROWS, COLS, EPI_DACT>(tile, o, e, st); break;
+    case FFN_DX: launch_tile<TYPE, ROWS, COLS, EPI_STORE>(tile, o, e, st); break;
+    default: launch_tile<TYPE, COLS, COLS, EPI_STORE>(tile, o, e, st); break;
+  }
+}
+
+template <int TYPE>
+void launch_pack(const void* src, int64_t ld, int64_t rows, int cols, void* dst, int ldo,
+                 int64_t plane, hipStream_t st) {
+  const int64_t n = rows * (ldo / 8);
+  k_ffn_pack<TYPE><<<(int)((n + 255) / 256), 256, 0, st>>>(src, ld, rows, cols, dst, ldo, plane);
+}
+
+// instantiated in ffn_f32.hip, ffn_bf16.hip and ffn_f16.hip
+struct FfnLaunchers {
+  void (*product)(int, int, const FfnOperands&, const FfnEpilogue&, hipStream_t);
+  void (*pack)(const void*, int64_t, int64_t, int, void*, int, int64_t, hipStream_t);
+};
+FfnLaunchers ffn_f32();
+FfnLaunchers ffn_bf16();
+FfnLaunchers ffn_f16();
+
+}  // namespace scao

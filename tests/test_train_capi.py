@@ -89,3 +89,65 @@ def test_workspace_holds_every_launch():
     assert lib.scao_grad_norm_workspace(t.ctypes.data, 0) == 0
     assert lib.scao_grad_norm_workspace(t.ctypes.data, 1) == 2048 * 8
     assert lib.scao_grad_norm_workspace(t.ctypes.data, 400) == 3 * 2048 * 8
+
+
+def _ffn(**kw):
+    from scao_amd import _lib as L
+    base = dict(x=4096, w_gate=4096, w_up=4096, w_down=4096, ldx=16, ld_gate=16, ld_up=16,
+                ld_down=24, tokens=3, d=16, f=24, dtype=1, act=0)
+    base.update(kw)
+    t = np.zeros(1, dtype=L.FFN_DESC)
+    for k, v in base.items():
+        t[k] = v
+    return t
+
+
+BAD_FFN = [dict(x=0), dict(w_gate=0), dict(w_up=4097), dict(w_down=0), dict(ldx=15),
+           dict(ld_gate=15), dict(ld_up=8), dict(ld_down=23), dict(ldx=1 << 21), dict(tokens=0),
+           dict(tokens=-1), dict(tokens=1 << 31), dict(d=0), dict(d=1 << 21), dict(f=0),
+           dict(f=1 << 20), dict(dtype=3), dict(dtype=-1), dict(act=5), dict(act=-1),
+           dict(x=4098, dtype=0)]
+
+
+@pytest.mark.parametrize("kw", BAD_FFN)
+def test_ffn_refuses_bad_descriptors(kw):
+    from scao_amd import _lib as L
+    lib = L.lib()
+    t = _ffn(**kw)
+    at = t.ctypes.data
+    assert lib.scao_ffn_forward(at, P, None, P, None) == 1
+    assert lib.scao_last_error().startswith(b"scao_ffn_forward:")
+    assert lib.scao_ffn_backward(at, P, 16, P, P, P, P, P, P, None) == 1
+    assert lib.scao_last_error().startswith(b"scao_ffn_backward:")
+    assert lib.scao_ffn_forward_workspace(at, 0) == 0
+    assert lib.scao_ffn_backward_workspace(at, P, 16) == 0
+
+
+def test_ffn_refuses_bad_buffers():
+    from scao_amd import _lib as L
+    lib = L.lib()
+    t = _ffn()
+    at = t.ctypes.data
+    assert lib.scao_ffn_forward(None, P, None, P, None) == 1
+    assert lib.scao_ffn_backward(None, P, 16, P, P, P, P, P, P, None) == 1
+    for y, saved, work in ((None, None, P), (17, None, P), (P, 8, P), (P, None, 8), (P, None, None)):
+        assert lib.scao_ffn_forward(at, y, saved, work, None) == 1
+    for args in ((None, 16, P, P, P, P, P, P), (P, 15, P, P, P, P, P, P),
+                 (P, 16, None, P, P, P, P, P), (P, 16, P, P, P, P, P, None),
+                 (P, 16, P, 17, P, P, P, P), (P, 16, P, P, P, P, 17, P)):
+        assert lib.scao_ffn_backward(at, *args, None) == 1
+
+
+def test_ffn_sizes_of_buffers():
+    """h, a and b: what the header's formulas need and no packing for operands
+    that can be loaded as they are."""
+    from scao_amd import _lib as L
+    lib = L.lib()
+    t = _ffn(tokens=32, d=64, f=48, ldx=64, ld_gate=64, ld_up=64, ld_down=48)
+    frags = 2 * 3
+    assert lib.scao_ffn_saved_bytes(t.ctypes.data) == 32 * 48 * 2 + frags * 64 * 24
+    assert lib.scao_ffn_forward_workspace(t.ctypes.data, 1) == 0
+    assert lib.scao_ffn_forward_workspace(t.ctypes.data, 0) == 32 * 48 * 2
+    t = _ffn(tokens=32, d=64, f=48, ldx=64, ld_gate=64, ld_up=64, ld_down=48, dtype=0)
+    assert lib.scao_ffn_saved_bytes(t.ctypes.data) == 3 * 32 * 48 * 2 + frags * 64 * 32
+    assert lib.scao_ffn_forward_workspace(t.ctypes.data, 1) >= 3 * 2 * (32 * 64 + 3 * 64 * 48)
