@@ -55,16 +55,16 @@ __device__ __forceinline__ v4f mma(v8s p, v8s q, v4f c) {
 }
 
 // 16 bytes a lane from global memory to LDS at lds + 16*lane.  The compiler
-// neither counts this load nor waits for it: ffn_wait_all does.
+// neither counts this load nor waits for it: wait_loads does, which it cannot pass.
 __device__ __forceinline__ void load_lds(v4i rsrc, uint32_t lds, uint32_t voff) {
   asm volatile("s_mov_b32 m0, %0\n\tbuffer_load_dwordx4 %1, %2, 0 offen lds" ::"s"(lds), "v"(voff),
-               "s"(rsrc)
-               : "memory");
+               "s"(rsrc));
 }
-// every load of this wave has arrived in LDS and every LDS read of it has been
-// answered, and every other wave says the same
-__device__ __forceinline__ void wait_all() {
-  asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory");
+// all but the last N loads of this wave have arrived in LDS and every LDS read
+// of it has been answered, and every other wave says the same
+template <int N>
+__device__ __forceinline__ void wait_loads() {
+  asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)\n\ts_barrier" ::"n"(N) : "memory");
 }
 
 constexpr uint32_t OUT_OF_RANGE = 0x80000000u;
@@ -158,7 +158,7 @@ struct Gemm {
   static constexpr int MI = BM / WM / 16, NJ = BN / WN / 16;
   using TA = Tile<LA, BM, NW>;
   using TB = Tile<LB, BN, NW>;
-  static constexpr int STAGE = TA::BYTES + TB::BYTES;
+  static constexpr int LDS = 3 * TA::BYTES + 2 * TB::BYTES;
   static constexpr int COLS_N = GATED ? BN / 2 : BN;   // of C
   static_assert(!GATED || LB == ROWS, "gated products have weights in rows");
 
@@ -198,48 +198,101 @@ struct Gemm {
     return wn * (BN / WN) + j * 16;
   }
 
+  // Where an operand's next step begins and how many bytes are left of it from
+  // there.  rows: up to row rows-1's k K-1; cols: up to k K-1's row rows-1.  A
+  // 16-byte load that the bound cuts gives zeros whole, so the contiguous size
+  // counts with the padding to 8 elements that every row of an operand has.
+  struct Cursor {
+    const char* at;
+    int64_t left;
+    __device__ v4i buffer() const { return buffer_of(at, left); }
+  };
   template <int L>
-  static __device__ v4i buffer(const void* p, int64_t ld, int r0, int rows, int k0, int K) {
-    // rows: up to row rows-1's k K-1; cols: up to k K-1's row rows-1.  A 16-byte
-    // load that the bound cuts gives zeros whole, so the contiguous size counts
-    // with the padding to 8 elements that every row of an operand has.
+  static __device__ Cursor cursor(const void* p, int64_t ld, int r0, int rows, int k0, int K) {
     const char* base = (const char*)p;
     if (L == ROWS)
-      return buffer_of(base + ((int64_t)r0 * ld + k0) * 2,
-                       ((int64_t)(rows - 1 - r0) * ld + ((K + 7) & ~7) - k0) * 2);
-    return buffer_of(base + ((int64_t)k0 * ld + r0) * 2,
-                     ((int64_t)(K - 1 - k0) * ld + ((rows + 7) & ~7) - r0) * 2);
+      return Cursor{base + ((int64_t)r0 * ld + k0) * 2,
+                    ((int64_t)(rows - 1 - r0) * ld + ((K + 7) & ~7) - k0) * 2};
+    return Cursor{base + ((int64_t)k0 * ld + r0) * 2,
+                  ((int64_t)(K - 1 - k0) * ld + ((rows + 7) & ~7) - r0) * 2};
+  }
+  template <int L>
+  static __device__ void advance(Cursor& c, int64_t ld) {
+    const int64_t step = L == ROWS ? FFN_BK * 2 : ld * FFN_BK * 2;
+    c.at += step;
+    c.left -= step;
   }
 
-  __device__ void fetch(int stage, int seg, int k0) const {
-    const uint32_t at = (uint32_t)(uintptr_t)(lds + stage * STAGE);
-    const v4i ra = buffer<LA>(o.a[seg], o.lda, m0, o.M, k0, o.K);
-#pragma unroll
-    for (int i = 0; i < TA::LOADS; ++i)
-      load_lds(ra, at + (i * NW + wave) * 1024,
-               LA == ROWS && k0 + ina[i] >= o.K ? OUT_OF_RANGE : offa[i]);
-    const v4i rb = buffer<LB>(o.b[seg], o.ldb, n0, o.N, k0, o.K);
-    const v4i ru = GATED ? buffer<LB>(o.b[seg + FFN_MAX_SEG / 2], o.ldb, n0, o.N, k0, o.K) : rb;
-#pragma unroll
-    for (int i = 0; i < TB::LOADS; ++i)
-      load_lds(GATED && up_half(i) ? ru : rb, at + TA::BYTES + (i * NW + wave) * 1024,
-               LB == ROWS && k0 + inb[i] >= o.K ? OUT_OF_RANGE : offb[i]);
+  // The steps that are still to be fetched, in order.
+  struct Walk {
+    int seg, k0;
+    Cursor a, b, u;
+  };
+  __device__ void seek(Walk& w) const {
+    w.a = cursor<LA>(o.a[w.seg], o.lda, m0, o.M, w.k0, o.K);
+    w.b = cursor<LB>(o.b[w.seg], o.ldb, n0, o.N, w.k0, o.K);
+    if (GATED) w.u = cursor<LB>(o.b[w.seg + FFN_MAX_SEG / 2], o.ldb, n0, o.N, w.k0, o.K);
+  }
+  __device__ void next(Walk& w) const {
+    w.k0 += FFN_BK;
+    if (w.k0 < o.K) {
+      advance<LA>(w.a, o.lda);
+      advance<LB>(w.b, o.ldb);
+      if (GATED) advance<LB>(w.u, o.ldb);
+    } else {
+      w.k0 = 0;
+      w.seg = min(w.seg + 1, o.nseg - 1);
+      seek(w);
+    }
   }
 
-  __device__ void products(int stage, v4f (&acc)[MI][NJ]) const {
-    const lchar* ta = lds + stage * STAGE;
-    const lchar* tb = ta + TA::BYTES;
+  // What the loads of one operand's next step need; the up rows of B's tile
+  // come from a buffer of their own.
+  struct Fetch {
+    v4i buf, up;
+    uint32_t lds;
+    int k0;
+  };
+  __device__ Fetch fetch_a(const Walk& w, int at) const {
+    const v4i b = w.a.buffer();
+    return Fetch{b, b, (uint32_t)(uintptr_t)(lds + at) + wave * 1024, w.k0};
+  }
+  __device__ Fetch fetch_b(const Walk& w, int at) const {
+    const v4i b = w.b.buffer();
+    return Fetch{b, GATED ? w.u.buffer() : b, (uint32_t)(uintptr_t)(lds + at) + wave * 1024, w.k0};
+  }
+  __device__ void load_a(const Fetch& f, int i) const {
+    load_lds(f.buf, f.lds + i * NW * 1024,
+             LA == ROWS && f.k0 + ina[i] >= o.K ? OUT_OF_RANGE : offa[i]);
+  }
+  __device__ void load_b(const Fetch& f, int i) const {
+    load_lds(GATED && up_half(i) ? f.up : f.buf, f.lds + i * NW * 1024,
+             LB == ROWS && f.k0 + inb[i] >= o.K ? OUT_OF_RANGE : offb[i]);
+  }
+
+  // Half a step: the products of the fragments a, b, row of fragments after row,
+  // with the LDS reads of the next half's (na, nb: k = 32 ks .. of the tiles at
+  // ta, tb) and one operand's loads of a later step dealt out between the rows.
+  // A wave issues in order, so a queue of loads or reads ahead of the products
+  // would idle the matrix cores until it drains.
+  template <bool LOAD_A>
+  __device__ void half(const v8s (&a)[MI], const v8s (&b)[NJ], v4f (&acc)[MI][NJ], int ta, int tb,
+                       int ks, v8s (&na)[MI], v8s (&nb)[NJ], const Fetch& f) const {
+    constexpr int LOADS = LOAD_A ? TA::LOADS : TB::LOADS;
 #pragma unroll
-    for (int ks = 0; ks < 2; ++ks) {
-      v8s a[MI], b[NJ];
+    for (int i = 0; i < MI; ++i) {
 #pragma unroll
-      for (int j = 0; j < NJ; ++j) b[j] = TB::frag(tb, frag_n(j), ks, lane);
+      for (int j = i * NJ / MI; j < (i + 1) * NJ / MI; ++j)
+        nb[j] = TB::frag(lds + tb, frag_n(j), ks, lane);
+      na[i] = TA::frag(lds + ta, frag_m(i), ks, lane);
 #pragma unroll
-      for (int i = 0; i < MI; ++i) a[i] = TA::frag(ta, frag_m(i), ks, lane);
+      for (int j = 0; j < NJ; ++j) acc[i][j] = mma<F16>(b[j], a[i], acc[i][j]);
 #pragma unroll
-      for (int i = 0; i < MI; ++i)
-#pragma unroll
-        for (int j = 0; j < NJ; ++j) acc[i][j] = mma<F16>(b[j], a[i], acc[i][j]);
+      for (int l = i * LOADS / MI; l < (i + 1) * LOADS / MI; ++l) {
+        if (LOAD_A) load_a(f, l);
+        else load_b(f, l);
+      }
+      __builtin_amdgcn_sched_barrier(0);
     }
   }
 
@@ -251,21 +304,48 @@ struct Gemm {
       for (int j = 0; j < NJ; ++j) acc[i][j] = v4f{0.f, 0.f, 0.f, 0.f};
     if (begin >= end) return;
     const int steps = (o.K + FFN_BK - 1) / FFN_BK;
-    int seg = begin / steps, k0 = (begin % steps) * FFN_BK;
-    fetch(0, seg, k0);
-    int stage = 0;
+    Walk w;
+    w.seg = begin / steps;
+    w.k0 = (begin % steps) * FFN_BK;
+    seek(w);
+    // A's tiles of this step, the next and the one after, B's of this and the next
+    int a0_ = 0, a1_ = TA::BYTES, a2_ = 2 * TA::BYTES;
+    int b0_ = 3 * TA::BYTES, b1_ = b0_ + TB::BYTES;
+    auto fetch = [&](int at_a, int at_b) {
+      const Fetch fa = fetch_a(w, at_a), fb = fetch_b(w, at_b);
+#pragma unroll
+      for (int l = 0; l < TA::LOADS; ++l) load_a(fa, l);
+#pragma unroll
+      for (int l = 0; l < TB::LOADS; ++l) load_b(fb, l);
+      next(w);
+    };
+    fetch(a0_, b0_);
+    wait_loads<0>();
+    if (begin + 1 < end) fetch(a1_, b1_);
+    v8s fa0[MI], fb0[NJ], fa1[MI], fb1[NJ];
+#pragma unroll
+    for (int j = 0; j < NJ; ++j) fb0[j] = TB::frag(lds + b0_, frag_n(j), 0, lane);
+#pragma unroll
+    for (int i = 0; i < MI; ++i) fa0[i] = TA::frag(lds + a0_, frag_m(i), 0, lane);
     for (int s = begin; s < end; ++s) {
-      wait_all();
-      if (s + 1 < end) {
-        k0 += FFN_BK;
-        if (k0 >= o.K) {
-          k0 = 0;
-          ++seg;
-        }
-        fetch(stage ^ 1, seg, k0);
-      }
-      products(stage, acc);
-      stage ^= 1;
+      // behind the last step there is nothing to load: empty buffers
+      if (s + 2 >= end) w.a.left = w.b.left = w.u.left = 0;
+      const Fetch fa = fetch_a(w, a2_), fb = fetch_b(w, b0_);
+      __builtin_amdgcn_sched_barrier(0);
+      half<true>(fa0, fb0, acc, a0_, b0_, 1, fa1, fb1, fa);
+      // all but A's tile of the step after the next one has arrived, and nobody
+      // reads this step's tiles any more
+      wait_loads<TA::LOADS>();
+      __builtin_amdgcn_sched_barrier(0);
+      // (after the last step the reads are of no use, within LDS)
+      half<false>(fa1, fb1, acc, a1_, b1_, 0, fa0, fb0, fb);
+      next(w);
+      const int a = a0_, b = b0_;
+      a0_ = a1_;
+      a1_ = a2_;
+      a2_ = a;
+      b0_ = b1_;
+      b1_ = b;
     }
   }
 };

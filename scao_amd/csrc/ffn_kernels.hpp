@@ -229,7 +229,7 @@ typedef __attribute__((address_space(1))) v4f gv4f_a16;
 template <class G, int TYPE, int EPI>
 __global__ __launch_bounds__(G::THREADS, 2) void k_ffn_gemm(const FfnOperands o,
                                                             const FfnEpilogue e) {
-  __shared__ __attribute__((aligned(1024))) char smem[2 * G::STAGE];
+  __shared__ __attribute__((aligned(1024))) char smem[G::LDS];
   const int tiles = o.tiles_m * o.tiles_n;
   const int part = blockIdx.x / tiles;
   int tm, tn;
