@@ -2,7 +2,7 @@
 // the launches.  The kernels are in ffn_kernels.hpp and ffn_gemm.hpp.
 #include <algorithm>
 
-#include "ffn_kernels.hpp"
+#include "ffn_few.hpp"
 
 using namespace scao;
 
@@ -47,12 +47,14 @@ struct Block {
       : s(d), st((hipStream_t)stream), ws(workspace), dry(count),
         parts(d.dtype == SCAO_F32 ? 3 : 1), fp(round_up(d.f, 8)) {}
 
-  // The user's matrix itself where its rows can be loaded 16 bytes at a time,
-  // else a packed copy.
+  // whether a matrix's rows can be loaded 16 bytes at a time
+  bool direct(const void* p, int64_t ld, int64_t rows, int64_t cols) const {
+    return s.dtype != SCAO_F32 && (uintptr_t)p % 16 == 0 && (ld % 8 == 0 || rows == 1) &&
+           cols % 8 == 0;
+  }
+  // The user's matrix itself where it can be, else a packed copy.
   Operand operand(const void* p, int64_t ld, int64_t rows, int64_t cols) {
-    if (s.dtype != SCAO_F32 && (uintptr_t)p % 16 == 0 && (ld % 8 == 0 || rows == 1) &&
-        cols % 8 == 0)
-      return Operand{p, rows == 1 ? round_up(cols, 8) : ld, 0};
+    if (direct(p, ld, rows, cols)) return Operand{p, rows == 1 ? cols : ld, 0};
     Operand o;
     o.ld = round_up(cols, 8);
     o.plane = rows * o.ld;
@@ -64,23 +66,39 @@ struct Block {
   }
 
   // Tile and parts of k for an M x N product of `steps` k steps: the least
-  // estimated time.  A 256 x 256 tile's step takes 1.68 us with one workgroup a
-  // CU (1276 TFLOP/s), a 128 x 128 tile's 0.99 us with two (1090 TFLOP/s) and
-  // 0.62 us alone; a split costs a launch and 8 bytes of traffic a part and
-  // element.
-  static void choose(int64_t M, int64_t N, int64_t steps, bool gated, int& tile, int& splits) {
+  // estimated time.  us of a step with one workgroup a CU and with all a CU
+  // holds, and of a tile's beginning and end, fitted to the times of every tile
+  // and part count of 225 products (8 to 4096 tokens, 256 x 704 to 4096 x 14336):
+  // the choice is 1.7% slower than the best on the geometric average, 17% at
+  // most.  For example dx of 24 tokens, 2048 x 8192: 32 x 128 tiles in one part
+  // 116 us, in 16 parts 21.8; of 4096 tokens: 256 x 256 in one part 285, in two
+  // 183, 128 x 128 in one 251.
+  static void choose(int64_t M, int64_t N, int64_t steps, bool gated, bool tokens, int& tile,
+                     int& splits) {
+    struct Cost {
+      int slots;
+      double lone, full, ends;
+    };
+    static const Cost costs[FFN_TILES] = {
+        {256, 1.15, 1.50, 4.9}, {512, 0.62, 1.14, 5.2}, {512, 0.56, 0.70, 3.0}, {768, 0.44, 0.96, 1.7}};
     double best = 1e30;
-    for (int t : {256, 128}) {
-      const int64_t cols = gated ? t / 2 : t;
-      const int64_t tiles = ((M + t - 1) / t) * ((N + cols - 1) / cols);
+    for (int t = 0; t < (tokens ? FFN_TILES : FFN_64x128); ++t) {
+      const Cost& c = costs[t];
+      const int64_t cols = gated ? FFN_BN[t] / 2 : FFN_BN[t];
+      const int64_t tiles = ((M + FFN_BM[t] - 1) / FFN_BM[t]) * ((N + cols - 1) / cols);
       for (int64_t n : {1, 2, 3, 4, 6, 8, 12, 16, 24, 32}) {
-        if (n > 1 && (n * 4 > steps || tiles * n > 1024)) break;
+        if (n > 1 && (n * 2 > steps || tiles * n > 2048)) break;
         const int64_t per = (steps + n - 1) / n, groups = tiles * n;
-        double us;
-        if (t == 256) us = ((groups + 255) / 256) * (per * 1.68 + 3);
-        else if (groups <= 256) us = per * 0.62 + 2;
-        else us = ((groups + 511) / 512) * (per * 0.99 + 3);
-        if (n > 1) us += 4 + 8e-6 * n * (double)M * N * (gated ? 2 : 1) / 4;
+        const int64_t rounds = groups / c.slots, rest = groups % c.slots;
+        double us = rounds * (per * c.full + c.ends);
+        if (rest) {
+          const double crowd = c.slots == 256 ? rest / 256.0
+                               : rest <= 256  ? 0.0
+                                              : (rest - 256.0) / (c.slots - 256.0);
+          us += per * (c.lone + (c.full - c.lone) * crowd) + c.ends;
+        }
+        // the join: a launch, and 8 bytes a part and element
+        if (n > 1) us += 2 + 8 / 7.4e6 * n * (double)M * N * (gated ? 2 : 1);
         if (us < best) {
           best = us;
           tile = t;
@@ -107,13 +125,15 @@ struct Block {
     const bool gated = kind == FFN_GATE_UP;
     const int64_t steps = (int64_t)o.nseg * ((o.K + FFN_BK - 1) / FFN_BK);
     int tile = 0;
-    choose(o.M, o.N, steps, gated, tile, o.splits);
-    o.tiles_m = (o.M + tile - 1) / tile;
-    o.tiles_n = (o.N + (gated ? tile / 2 : tile) - 1) / (gated ? tile / 2 : tile);
+    choose(o.M, o.N, steps, gated, kind != FFN_DW, tile, o.splits);
+    const int cols = gated ? FFN_BN[tile] / 2 : FFN_BN[tile];
+    o.tiles_m = (o.M + FFN_BM[tile] - 1) / FFN_BM[tile];
+    o.tiles_n = (o.N + cols - 1) / cols;
     e.partial = nullptr;
     if (o.splits > 1) {
       const int64_t at = ws.used;   // given back: the next product may write it
-      e.partial = (float*)ws.take((int64_t)o.splits * o.tiles_m * o.tiles_n * tile * tile * 4);
+      e.partial = (float*)ws.take((int64_t)o.splits * o.tiles_m * o.tiles_n * FFN_BM[tile] *
+                                  FFN_BN[tile] * 4);
       peak = std::max(peak, ws.used);
       ws.used = at;
     }
@@ -155,7 +175,32 @@ struct Block {
     return e;
   }
 
+  // Whether the forward pass alone goes without tiles.  bf16, 2048 x 8192: 8
+  // tokens 30 us against 32, 16 tokens 35 against 33; 4096 x 14336: 4 tokens 73
+  // against 78, 16 tokens 93 against 79.  The tiles' operands have to be packed
+  // in fp32 and where rows begin off 16 bytes, which takes longer than the
+  // product: fp32, 4096 x 14336, 64 tokens 394 us against 789.
+  bool few() const {
+    if (s.tokens <= 8) return true;
+    return s.tokens <= FFN_FEW_TOKENS &&
+           !(direct(s.w_gate, s.ld_gate, s.f, s.d) && direct(s.w_up, s.ld_up, s.f, s.d) &&
+             direct(s.w_down, s.ld_down, s.d, s.f));
+  }
+  // h in the block's type, nothing packed
+  int forward_few(void* y) {
+    void* h = ws.take(s.tokens * s.f * size_of(s.dtype));
+    if (dry) return SCAO_OK;
+    FfnFew o{s.x, s.w_gate, s.w_up, s.ldx, s.ld_gate, s.ld_up, (int)s.tokens, (int)s.f, (int)s.d};
+    FfnEpilogue e = store(h, s.tokens, s.f);
+    e.act = s.act;
+    launchers(s.dtype).few(o, e, true, st);
+    o = FfnFew{h, s.w_down, nullptr, s.f, s.ld_down, 0, (int)s.tokens, (int)s.d, (int)s.f};
+    launchers(s.dtype).few(o, store(y, s.tokens, s.d), false, st);
+    return SCAO_OK;
+  }
+
   int forward(void* y, void* saved, bool save) {
+    if (!save && few()) return forward_few(y);
     const Operand x = operand(s.x, s.ldx, s.tokens, s.d);
     Operand g = operand(s.w_gate, s.ld_gate, s.f, s.d), u = operand(s.w_up, s.ld_up, s.f, s.d);
     if (g.ld != u.ld) pair(g, u);

@@ -57,8 +57,9 @@ __device__ __forceinline__ v4f mma(v8s p, v8s q, v4f c) {
 // 16 bytes a lane from global memory to LDS at lds + 16*lane.  The compiler
 // neither counts this load nor waits for it: wait_loads does, which it cannot pass.
 __device__ __forceinline__ void load_lds(v4i rsrc, uint32_t lds, uint32_t voff) {
-  asm volatile("s_mov_b32 m0, %0\n\tbuffer_load_dwordx4 %1, %2, 0 offen lds" ::"s"(lds), "v"(voff),
-               "s"(rsrc));
+  asm volatile("s_mov_b32 m0, %0\n\tbuffer_load_dwordx4 %1, %2, 0 offen lds" ::"s"(
+                   __builtin_amdgcn_readfirstlane(lds)),
+               "v"(voff), "s"(rsrc));
 }
 // all but the last N loads of this wave have arrived in LDS and every LDS read
 // of it has been answered, and every other wave says the same
@@ -90,7 +91,7 @@ struct Tile {
 
   // byte offset, relative to the step's origin, of what lane `lane` of load i
   // of wave w fetches
-  static __device__ uint32_t offset(int i, int w, int lane, int64_t ld) {
+  static __device__ __forceinline__ uint32_t offset(int i, int w, int lane, int64_t ld) {
     const int at = (i * NW + w) * 1024 + lane * 16;
     if (L == ROWS) {
       const int r = at / 128, c = (at % 128) / 16 ^ (r & 7);
@@ -101,16 +102,16 @@ struct Tile {
   }
   // its position in the dimension that has to be checked by hand: k for rows
   // (a row's tail is followed by the next row), r for cols
-  static __device__ int inner(int i, int w, int lane) {
+  static __device__ __forceinline__ int inner(int i, int w, int lane) {
     const int at = (i * NW + w) * 1024 + lane * 16;
     if (L == ROWS) return ((at % 128) / 16 ^ ((at / 128) & 7)) * 8;
     const int k = at / KROW, p = (at % KROW) / 16;
     return (((p >> 1) ^ fold(k)) * 2 + (p & 1)) * 8;
   }
-  static __device__ int fold(int k) { return (k & 3) | ((k >> 3 & 1) << 2); }
+  static __device__ __forceinline__ int fold(int k) { return (k & 3) | ((k >> 3 & 1) << 2); }
 
   // fragment of 16 rows from row r0 (a multiple of 16), k = 32 ks + 0..31
-  static __device__ v8s frag(const lchar* t, int r0, int ks, int lane) {
+  static __device__ __forceinline__ v8s frag(const lchar* t, int r0, int ks, int lane) {
     const int q = lane & 15, g = lane >> 4;
     if (L == ROWS) {
       const int r = r0 + q;
@@ -154,7 +155,7 @@ __device__ __forceinline__ void tile_of(int b, int tm, int tn, int& m, int& n) {
 // up rows; each wave's fragments are half of either.
 template <int BM, int BN, int WM, int WN, int LA, int LB, bool F16, bool GATED>
 struct Gemm {
-  static constexpr int NW = WM * WN, THREADS = NW * 64;
+  static constexpr int NW = WM * WN, THREADS = NW * 64, BM_ = BM;
   static constexpr int MI = BM / WM / 16, NJ = BN / WN / 16;
   using TA = Tile<LA, BM, NW>;
   using TB = Tile<LB, BN, NW>;
@@ -168,7 +169,7 @@ struct Gemm {
   uint32_t offa[TA::LOADS], offb[TB::LOADS];
   int ina[TA::LOADS], inb[TB::LOADS];
 
-  __device__ Gemm(const FfnOperands& ops, lchar* l, int tm, int tn) : o(ops), lds(l) {
+  __device__ __forceinline__ Gemm(const FfnOperands& ops, lchar* l, int tm, int tn) : o(ops), lds(l) {
     wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     lane = threadIdx.x & 63;
     wm = wave / WN;
@@ -189,11 +190,11 @@ struct Gemm {
       if (LB == COLS && n0 + inb[i] >= o.N) offb[i] = OUT_OF_RANGE;
     }
   }
-  __device__ bool up_half(int i) const { return (i * NW + wave) * 8 >= BN / 2; }
+  __device__ __forceinline__ bool up_half(int i) const { return (i * NW + wave) * 8 >= BN / 2; }
 
   // C row of the first of fragment i's rows, C column of fragment j's
-  __device__ int frag_m(int i) const { return wm * (BM / WM) + i * 16; }
-  __device__ int frag_n(int j) const {   // LDS row
+  __device__ __forceinline__ int frag_m(int i) const { return wm * (BM / WM) + i * 16; }
+  __device__ __forceinline__ int frag_n(int j) const {   // LDS row
     if (GATED) return (j < NJ / 2 ? 0 : BN / 2) + wn * (BN / 2 / WN) + (j % (NJ / 2)) * 16;
     return wn * (BN / WN) + j * 16;
   }
@@ -208,7 +209,7 @@ struct Gemm {
     __device__ v4i buffer() const { return buffer_of(at, left); }
   };
   template <int L>
-  static __device__ Cursor cursor(const void* p, int64_t ld, int r0, int rows, int k0, int K) {
+  static __device__ __forceinline__ Cursor cursor(const void* p, int64_t ld, int r0, int rows, int k0, int K) {
     const char* base = (const char*)p;
     if (L == ROWS)
       return Cursor{base + ((int64_t)r0 * ld + k0) * 2,
@@ -217,7 +218,7 @@ struct Gemm {
                   ((int64_t)(K - 1 - k0) * ld + ((rows + 7) & ~7) - r0) * 2};
   }
   template <int L>
-  static __device__ void advance(Cursor& c, int64_t ld) {
+  static __device__ __forceinline__ void advance(Cursor& c, int64_t ld) {
     const int64_t step = L == ROWS ? FFN_BK * 2 : ld * FFN_BK * 2;
     c.at += step;
     c.left -= step;
@@ -228,12 +229,12 @@ struct Gemm {
     int seg, k0;
     Cursor a, b, u;
   };
-  __device__ void seek(Walk& w) const {
+  __device__ __forceinline__ void seek(Walk& w) const {
     w.a = cursor<LA>(o.a[w.seg], o.lda, m0, o.M, w.k0, o.K);
     w.b = cursor<LB>(o.b[w.seg], o.ldb, n0, o.N, w.k0, o.K);
     if (GATED) w.u = cursor<LB>(o.b[w.seg + FFN_MAX_SEG / 2], o.ldb, n0, o.N, w.k0, o.K);
   }
-  __device__ void next(Walk& w) const {
+  __device__ __forceinline__ void next(Walk& w) const {
     w.k0 += FFN_BK;
     if (w.k0 < o.K) {
       advance<LA>(w.a, o.lda);
@@ -253,19 +254,19 @@ struct Gemm {
     uint32_t lds;
     int k0;
   };
-  __device__ Fetch fetch_a(const Walk& w, int at) const {
+  __device__ __forceinline__ Fetch fetch_a(const Walk& w, int at) const {
     const v4i b = w.a.buffer();
     return Fetch{b, b, (uint32_t)(uintptr_t)(lds + at) + wave * 1024, w.k0};
   }
-  __device__ Fetch fetch_b(const Walk& w, int at) const {
+  __device__ __forceinline__ Fetch fetch_b(const Walk& w, int at) const {
     const v4i b = w.b.buffer();
     return Fetch{b, GATED ? w.u.buffer() : b, (uint32_t)(uintptr_t)(lds + at) + wave * 1024, w.k0};
   }
-  __device__ void load_a(const Fetch& f, int i) const {
+  __device__ __forceinline__ void load_a(const Fetch& f, int i) const {
     load_lds(f.buf, f.lds + i * NW * 1024,
              LA == ROWS && f.k0 + ina[i] >= o.K ? OUT_OF_RANGE : offa[i]);
   }
-  __device__ void load_b(const Fetch& f, int i) const {
+  __device__ __forceinline__ void load_b(const Fetch& f, int i) const {
     load_lds(GATED && up_half(i) ? f.up : f.buf, f.lds + i * NW * 1024,
              LB == ROWS && f.k0 + inb[i] >= o.K ? OUT_OF_RANGE : offb[i]);
   }
@@ -276,7 +277,7 @@ struct Gemm {
   // A wave issues in order, so a queue of loads or reads ahead of the products
   // would idle the matrix cores until it drains.
   template <bool LOAD_A>
-  __device__ void half(const v8s (&a)[MI], const v8s (&b)[NJ], v4f (&acc)[MI][NJ], int ta, int tb,
+  __device__ __forceinline__ void half(const v8s (&a)[MI], const v8s (&b)[NJ], v4f (&acc)[MI][NJ], int ta, int tb,
                        int ks, v8s (&na)[MI], v8s (&nb)[NJ], const Fetch& f) const {
     constexpr int LOADS = LOAD_A ? TA::LOADS : TB::LOADS;
 #pragma unroll
@@ -297,7 +298,7 @@ struct Gemm {
   }
 
   // the k steps [begin, end) of all segments' steps in order
-  __device__ void run(int begin, int end, v4f (&acc)[MI][NJ]) const {
+  __device__ __forceinline__ void run(int begin, int end, v4f (&acc)[MI][NJ]) const {
 #pragma unroll
     for (int i = 0; i < MI; ++i)
 #pragma unroll

@@ -71,9 +71,19 @@ __device__ __forceinline__ void activation(float a, float& f, float& g) {
     f = a > 0.f ? a : a * 0.f;
     g = a > 0.f ? 1.f : 0.f;
   } else if (ACT == SCAO_ACT_GELU) {
-    const float c = 0.5f * erfcf(a * -0.70710678f);
+    // erfc(z) = t (a1 + t (a2 + ... )) exp(-z^2), t = 1 / (1 + 0.3275911 z), z >= 0,
+    // to 1.5e-7 (Abramowitz and Stegun, Handbook of Mathematical Functions,
+    // 7.1.26); exp(-z^2) = exp(-a^2/2) is the derivative's too
+    const float t = __builtin_amdgcn_rcpf(fmaf(0.3275911f * 0.70710678f, fabsf(a), 1.f));
+    const float ex = __builtin_amdgcn_exp2f(-0.72134752f * (a * a));
+    float p = fmaf(t, 1.061405429f, -1.453152027f);
+    p = fmaf(t, p, 1.421413741f);
+    p = fmaf(t, p, -0.284496736f);
+    p = fmaf(t, p, 0.254829592f);
+    const float tail = 0.5f * p * t * ex;
+    const float c = a < 0.f ? tail : 1.f - tail;
     f = a * c;
-    g = fmaf(a * 0.39894228f, expf(-0.5f * a * a), c);
+    g = fmaf(a * 0.39894228f, ex, c);
   } else {   // a/2 (1 + tanh u) = a logistic(2u), u = sqrt(2/pi) (a + 0.044715 a^3)
     const float a2 = a * a;
     const float s = logistic<F32>(1.59576912f * fmaf(0.044715f * a2, a, a));
@@ -83,28 +93,61 @@ __device__ __forceinline__ void activation(float a, float& f, float& g) {
 }
 
 // --------------------------------------------------------- stores ----------
-// TYPE: enum scao_dtype of the block.  Four values of one row as an operand of a
-// further product: one 16-bit value each, or three bf16 parts in three planes.
+// TYPE: enum scao_dtype of the block.  Four values of one row as 16-bit words of
+// each plane of an operand: the value, or (fp32) its three bf16 parts.
 template <int TYPE>
-__device__ __forceinline__ void put_operand(void* base, int64_t at, int64_t plane, v4f x) {
-  uint16_t* p = (uint16_t*)base + at;
-  if (TYPE == SCAO_F32) {
-    v2u h, m, l;
-    uint32_t w[3];
+constexpr int PLANES = TYPE == SCAO_F32 ? 3 : 1;
+template <int TYPE>
+__device__ __forceinline__ void operand_words(v4f x, v2u (&w)[PLANES<TYPE>]) {
+  if constexpr (TYPE == SCAO_F32) {
 #pragma unroll
     for (int t = 0; t < 2; ++t) {
-      split3_pk(x[2 * t], x[2 * t + 1], w[0], w[1], w[2]);
-      h[t] = w[0];
-      m[t] = w[1];
-      l[t] = w[2];
+      uint32_t h, m, l;
+      split3_pk(x[2 * t], x[2 * t + 1], h, m, l);
+      w[0][t] = h;
+      w[1][t] = m;
+      w[2][t] = l;
     }
-    *(gv2u*)p = h;
-    *(gv2u*)(p + plane) = m;
-    *(gv2u*)(p + 2 * plane) = l;
   } else if (TYPE == SCAO_BF16) {
-    *(gv2u*)p = v2u{pk_bf16(x[0], x[1]), pk_bf16(x[2], x[3])};
+    w[0] = v2u{pk_bf16(x[0], x[1]), pk_bf16(x[2], x[3])};
   } else {
-    *(gv2u*)p = v4f_to_halves(SCAO_F16, x);
+    w[0] = v4f_to_halves(SCAO_F16, x);
+  }
+}
+template <int TYPE>
+__device__ __forceinline__ void put_operand(void* base, int64_t at, int64_t plane, v4f x) {
+  v2u w[PLANES<TYPE>];
+  operand_words<TYPE>(x, w);
+#pragma unroll
+  for (int i = 0; i < PLANES<TYPE>; ++i) *(gv2u*)((uint16_t*)base + at + i * plane) = w[i];
+}
+
+// Two fragments next to each other: lane group g (16 lanes) holds columns 4g ..
+// 4g+3 of either.  The odd groups of the first change places with the even ones
+// of the second, after which a lane holds eight columns in order, those from
+// pair_column(lane) on: one 16-byte store, 64 bytes of a row side by side.
+__device__ __forceinline__ int pair_column(int lane) {
+  return (lane >> 4 & 1) * 16 + (lane >> 5) * 8;
+}
+__device__ __forceinline__ v4u_t join_pair(v2u p, v2u q) {
+  const auto a = __builtin_amdgcn_permlane16_swap(p[0], q[0], false, false);
+  const auto b = __builtin_amdgcn_permlane16_swap(p[1], q[1], false, false);
+  return v4u_t{a[0], b[0], a[1], b[1]};
+}
+typedef __attribute__((address_space(1))) v4u_t gv4u_a16;
+typedef v4u_t v4u_a2 __attribute__((aligned(2)));
+typedef __attribute__((address_space(1))) v4u_a2 gv4u_a2;
+// at: the element of this lane's first column
+template <int TYPE>
+__device__ __forceinline__ void put_operand_pair(void* base, int64_t at, int64_t plane, bool in,
+                                                 v4f x, v4f y) {
+  v2u p[PLANES<TYPE>], q[PLANES<TYPE>];
+  operand_words<TYPE>(x, p);
+  operand_words<TYPE>(y, q);
+#pragma unroll
+  for (int i = 0; i < PLANES<TYPE>; ++i) {
+    const v4u_t w = join_pair(p[i], q[i]);
+    if (in) *(gv4u_a16*)((uint16_t*)base + at + i * plane) = w;
   }
 }
 
@@ -114,7 +157,6 @@ template <int TYPE>
 __host__ __device__ constexpr int64_t ab_bytes(int64_t fi, int64_t fj) {
   return fi * fj * 64 * (TYPE == SCAO_F32 ? 32 : 24);
 }
-typedef __attribute__((address_space(1))) v4u_t gv4u_a16;
 typedef __attribute__((address_space(1))) v2u gv2u_a8;
 
 template <int TYPE>
@@ -142,24 +184,36 @@ __device__ __forceinline__ void put_ab(void* ab, int64_t frags, int64_t frag, in
   ((gv2u_a8*)((char*)ab + frags * 1024))[at] = lo;
 }
 template <int TYPE>
-__device__ __forceinline__ void get_ab(const void* ab, int64_t frags, int64_t frag, int lane,
-                                       v4f& a, v4f& b) {
-  const int64_t at = frag * 64 + lane;
-  if (TYPE == SCAO_F32) {
-    a = __builtin_bit_cast(v4f, (v4u_t)((const gv4u_a16*)ab)[2 * at]);
-    b = __builtin_bit_cast(v4f, (v4u_t)((const gv4u_a16*)ab)[2 * at + 1]);
-    return;
+struct Kept {
+  v4u_t hi;   // fp32: a
+  v4u_t lo;   // fp32: b; else two words
+  __device__ __forceinline__ void load(const void* ab, int64_t frags, int64_t frag, int lane) {
+    const int64_t at = frag * 64 + lane;
+    if (TYPE == SCAO_F32) {
+      hi = ((const gv4u_a16*)ab)[2 * at];
+      lo = ((const gv4u_a16*)ab)[2 * at + 1];
+    } else {
+      hi = ((const gv4u_a16*)ab)[at];
+      const v2u w = ((const gv2u_a8*)((const char*)ab + frags * 1024))[at];
+      lo[0] = w[0];
+      lo[1] = w[1];
+    }
   }
-  const v4u_t hi = ((const gv4u_a16*)ab)[at];
-  const v2u lo = ((const gv2u_a8*)((const char*)ab + frags * 1024))[at];
+  __device__ __forceinline__ void get(v4f& a, v4f& b) const {
+    if (TYPE == SCAO_F32) {
+      a = __builtin_bit_cast(v4f, hi);
+      b = __builtin_bit_cast(v4f, lo);
+      return;
+    }
 #pragma unroll
-  for (int t = 0; t < 4; ++t) {
-    // bytes 1 (from lo), 2 and 3 (from hi) of the float; byte 0 is zero
-    const uint32_t half = t & 1 ? 0x0706000cu : 0x0504000cu;
-    a[t] = __uint_as_float(__builtin_amdgcn_perm(hi[t / 2], lo[0], half | (uint32_t)t << 8));
-    b[t] = __uint_as_float(__builtin_amdgcn_perm(hi[2 + t / 2], lo[1], half | (uint32_t)t << 8));
+    for (int t = 0; t < 4; ++t) {
+      // bytes 1 (from lo), 2 and 3 (from hi) of the float; byte 0 is zero
+      const uint32_t half = t & 1 ? 0x0706000cu : 0x0504000cu;
+      a[t] = __uint_as_float(__builtin_amdgcn_perm(hi[t / 2], lo[0], half | (uint32_t)t << 8));
+      b[t] = __uint_as_float(__builtin_amdgcn_perm(hi[2 + t / 2], lo[1], half | (uint32_t)t << 8));
+    }
   }
-}
+};
 
 // ------------------------------------------------------ epilogues ----------
 // Four consecutive columns n .. n+3 of row m of C.
@@ -176,9 +230,41 @@ __device__ __forceinline__ void epi_store(const FfnEpilogue& e, int m, int n, v4
   st4(out, TYPE, at, c, left >= 4, left >= 4 ? 15 : (1 << left) - 1);
 }
 
+// the same of two fragments next to each other, the first at column n
+template <int TYPE>
+__device__ __forceinline__ void epi_store_pair(const FfnEpilogue& e, int m, int n, int lane, v4f c,
+                                               v4f d) {
+  if (TYPE == SCAO_F32) {
+    n += 4 * (lane >> 4);
+    epi_store<TYPE>(e, m, n, c);
+    epi_store<TYPE>(e, m, n + 16, d);
+    return;
+  }
+  v2u p[1], q[1];
+  operand_words<TYPE == SCAO_F32 ? SCAO_BF16 : TYPE>(c, p);
+  operand_words<TYPE == SCAO_F32 ? SCAO_BF16 : TYPE>(d, q);
+  const v4u_t w = join_pair(p[0], q[0]);
+  n += pair_column(lane);
+  void* out = e.out;
+  if (m >= e.second) {
+    m -= e.second;
+    out = e.out2;
+  }
+  if (m >= e.rows || n >= e.cols || !out) return;
+  uint16_t* to = (uint16_t*)out + (int64_t)m * e.ldo + n;
+  if (n + 8 <= e.cols) {
+    *(gv4u_a2*)to = w;
+  } else {
+#pragma unroll
+    for (int t = 0; t < 8; ++t)
+      if (n + t < e.cols) ((gu16*)to)[t] = (uint16_t)(w[t / 2] >> (16 * (t & 1)));
+  }
+}
+
+// h of a fragment, a and b kept
 template <int TYPE, int ACT>
-__device__ __forceinline__ void epi_gated(const FfnEpilogue& e, int m, int n, int lane, v4f a,
-                                          v4f b) {
+__device__ __forceinline__ v4f epi_gated(const FfnEpilogue& e, int m, int n, int lane, v4f a,
+                                         v4f b) {
   v4f h;
 #pragma unroll
   for (int t = 0; t < 4; ++t) {
@@ -186,19 +272,21 @@ __device__ __forceinline__ void epi_gated(const FfnEpilogue& e, int m, int n, in
     activation<ACT, TYPE == SCAO_F32>(a[t], f, g);
     h[t] = f * b[t];
   }
-  if (m < e.rows && n < e.cols)
-    put_operand<TYPE>(e.out, (int64_t)m * e.ldo + n, e.plane, h);
   const int fi = m >> 4, fj = n >> 4;
   if (e.ab && fi < e.fi && fj < e.fj)
     put_ab<TYPE>(e.ab, (int64_t)e.fi * e.fj, (int64_t)fi * e.fj + fj, lane, a, b);
+  return h;
 }
 
+// where a fragment's a and b are kept; one outside of what is kept repeats the
+// last one and writes nothing
+__device__ __forceinline__ int64_t kept_at(const FfnEpilogue& e, int m, int n) {
+  return (int64_t)min(m >> 4, e.fi - 1) * e.fj + min(n >> 4, e.fj - 1);
+}
 template <int TYPE, int ACT>
-__device__ __forceinline__ void epi_dact(const FfnEpilogue& e, int m, int n, int lane, v4f dh) {
-  const int fi = m >> 4, fj = n >> 4;
-  if (fi >= e.fi || fj >= e.fj) return;
-  v4f a, b, da, db;
-  get_ab<TYPE>(e.ab, (int64_t)e.fi * e.fj, (int64_t)fi * e.fj + fj, lane, a, b);
+__device__ __forceinline__ void epi_dact(const Kept<TYPE>& k, v4f dh, v4f& da, v4f& db) {
+  v4f a, b;
+  k.get(a, b);
 #pragma unroll
   for (int t = 0; t < 4; ++t) {
     float f, g;
@@ -206,22 +294,23 @@ __device__ __forceinline__ void epi_dact(const FfnEpilogue& e, int m, int n, int
     da[t] = dh[t] * b[t] * g;
     db[t] = dh[t] * f;
   }
-  if (m < e.rows && n < e.cols) {
-    const int64_t at = (int64_t)m * e.ldo + n;
-    put_operand<TYPE>(e.out, at, e.plane, da);
-    put_operand<TYPE>(e.out, at + e.ldo / 2, e.plane, db);
-  }
 }
 
-// f(act) for every activation, outside of the unrolled loops
-#define FFN_FOR_ACT(act, CALL)            \
-  switch (act) {                          \
-    case SCAO_ACT_SILU: CALL(SCAO_ACT_SILU); break;           \
-    case SCAO_ACT_GELU: CALL(SCAO_ACT_GELU); break;           \
-    case SCAO_ACT_GELU_TANH: CALL(SCAO_ACT_GELU_TANH); break; \
-    case SCAO_ACT_RELU: CALL(SCAO_ACT_RELU); break;           \
-    default: CALL(SCAO_ACT_SIGMOID); break;                   \
+// f with the activation as a type, chosen outside of the unrolled loops
+template <int ACT>
+struct Activation {
+  static constexpr int value = ACT;
+};
+template <class F>
+__device__ __forceinline__ void for_activation(int act, F&& f) {
+  switch (act) {
+    case SCAO_ACT_SILU: f(Activation<SCAO_ACT_SILU>{}); break;
+    case SCAO_ACT_GELU: f(Activation<SCAO_ACT_GELU>{}); break;
+    case SCAO_ACT_GELU_TANH: f(Activation<SCAO_ACT_GELU_TANH>{}); break;
+    case SCAO_ACT_RELU: f(Activation<SCAO_ACT_RELU>{}); break;
+    default: f(Activation<SCAO_ACT_SIGMOID>{}); break;
   }
+}
 
 // ------------------------------------------------------- products ----------
 typedef __attribute__((address_space(1))) v4f gv4f_a16;
@@ -244,7 +333,7 @@ __global__ __launch_bounds__(G::THREADS, 2) void k_ffn_gemm(const FfnOperands o,
   if (o.splits > 1) {
     // C's fragments in order, a projection's behind the other's (GATED)
     constexpr int H = EPI == EPI_GATED ? 2 : 1;
-    const int64_t fj = o.tiles_n * (G::COLS_N / 16), fi = o.tiles_m * (int64_t)(G::TA::BYTES / 2048);
+    const int64_t fj = o.tiles_n * (G::COLS_N / 16), fi = o.tiles_m * (int64_t)(G::BM_ / 16);
     gv4f_a16* to = (gv4f_a16*)e.partial + part * fi * fj * H * 64;
 #pragma unroll
     for (int i = 0; i < G::MI; ++i)
@@ -256,27 +345,78 @@ __global__ __launch_bounds__(G::THREADS, 2) void k_ffn_gemm(const FfnOperands o,
       }
     return;
   }
+  // pairs of fragments next to each other where a wave has them
+  constexpr int NH = EPI == EPI_GATED ? G::NJ / 2 : G::NJ, STEP = NH % 2 ? 1 : 2;
+  const int dp = STEP == 2 ? pair_column(lane) : dn;
   if constexpr (EPI == EPI_STORE) {
 #pragma unroll
     for (int i = 0; i < G::MI; ++i)
 #pragma unroll
-      for (int j = 0; j < G::NJ; ++j)
-        epi_store<TYPE>(e, g.m0 + g.frag_m(i) + dm, g.n0 + g.frag_n(j) + dn, acc[i][j]);
+      for (int j = 0; j < NH; j += STEP) {
+        const int m = g.m0 + g.frag_m(i) + dm, n = g.n0 + g.frag_n(j);
+        if constexpr (STEP == 2) epi_store_pair<TYPE>(e, m, n, lane, acc[i][j], acc[i][j + 1]);
+        else epi_store<TYPE>(e, m, n + dn, acc[i][j]);
+      }
+  } else if constexpr (EPI == EPI_GATED) {
+    auto epilogue = [&](auto act) __attribute__((always_inline)) {
+      constexpr int ACT = decltype(act)::value;
+#pragma unroll
+      for (int i = 0; i < G::MI; ++i)
+#pragma unroll
+        for (int j = 0; j < NH; j += STEP) {
+          const int m = g.m0 + g.frag_m(i) + dm, n = g.n0 + g.frag_n(j);
+          const v4f h = epi_gated<TYPE, ACT>(e, m, n + dn, lane, acc[i][j], acc[i][j + NH]);
+          const bool in = m < e.rows && n + dp < e.cols;
+          const int64_t at = (int64_t)m * e.ldo + n + dp;
+          if constexpr (STEP == 2)
+            put_operand_pair<TYPE>(e.out, at, e.plane, in, h,
+                                   epi_gated<TYPE, ACT>(e, m, n + 16 + dn, lane, acc[i][j + 1],
+                                                        acc[i][j + 1 + NH]));
+          else if (in) put_operand<TYPE>(e.out, at, e.plane, h);
+        }
+    };
+    for_activation(e.act, epilogue);
   } else {
-#define FFN_EPILOGUE(ACT)                                                                     \
-  _Pragma("unroll") for (int i = 0; i < G::MI; ++i) {                                         \
-    const int m = g.m0 + g.frag_m(i) + dm;                                                    \
-    if constexpr (EPI == EPI_GATED) {                                                         \
-      _Pragma("unroll") for (int j = 0; j < G::NJ / 2; ++j)                                   \
-          epi_gated<TYPE, ACT>(e, m, g.n0 + g.frag_n(j) + dn, lane, acc[i][j],                \
-                               acc[i][j + G::NJ / 2]);                                        \
-    } else {                                                                                  \
-      _Pragma("unroll") for (int j = 0; j < G::NJ; ++j)                                       \
-          epi_dact<TYPE, ACT>(e, m, g.n0 + g.frag_n(j) + dn, lane, acc[i][j]);                \
-    }                                                                                         \
-  }
-    FFN_FOR_ACT(e.act, FFN_EPILOGUE)
-#undef FFN_EPILOGUE
+    // A wait for loads also waits for the stores before them, so the kept values
+    // of many fragments are loaded at a time (dh of 4096 tokens x 8192 with k =
+    // 64, so nearly the epilogue alone: 123 us one fragment at a time, 83 with
+    // 16); more than 8 do not fit beside the 256 x 256 tile's sums.
+    auto epilogue = [&](auto act) __attribute__((always_inline)) {
+      constexpr int ACT = decltype(act)::value;
+      constexpr int BATCH = G::MI * G::NJ > 16 ? 1 : G::MI < 4 ? G::MI : 4;
+#pragma unroll
+      for (int i0 = 0; i0 < G::MI; i0 += BATCH) {
+        Kept<TYPE> k[BATCH][NH];
+#pragma unroll
+        for (int i = 0; i < BATCH; ++i)
+#pragma unroll
+          for (int j = 0; j < NH; ++j)
+            k[i][j].load(e.ab, (int64_t)e.fi * e.fj,
+                         kept_at(e, g.m0 + g.frag_m(i0 + i), g.n0 + g.frag_n(j)), lane);
+        __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+        for (int i = 0; i < BATCH; ++i)
+#pragma unroll
+          for (int j = 0; j < NH; j += STEP) {
+            __builtin_amdgcn_sched_barrier(0);
+            const int m = g.m0 + g.frag_m(i0 + i) + dm, n = g.n0 + g.frag_n(j) + dp;
+            const bool in = m < e.rows && n < e.cols;
+            const int64_t at = (int64_t)m * e.ldo + n;
+            v4f da, db, da2, db2;
+            epi_dact<TYPE, ACT>(k[i][j], acc[i0 + i][j], da, db);
+            if constexpr (STEP == 2) {
+              epi_dact<TYPE, ACT>(k[i][j + 1], acc[i0 + i][j + 1], da2, db2);
+              put_operand_pair<TYPE>(e.out, at, e.plane, in, da, da2);
+              put_operand_pair<TYPE>(e.out, at + e.ldo / 2, e.plane, in, db, db2);
+            } else if (in) {
+              put_operand<TYPE>(e.out, at, e.plane, da);
+              put_operand<TYPE>(e.out, at + e.ldo / 2, e.plane, db);
+            }
+          }
+        __builtin_amdgcn_sched_barrier(0);
+      }
+    };
+    for_activation(e.act, epilogue);
   }
 }
 
@@ -299,11 +439,24 @@ __global__ __launch_bounds__(256) void k_ffn_join(const FfnEpilogue e, int split
   if constexpr (EPI == EPI_STORE) {
     epi_store<TYPE>(e, m, n, a);
   } else {
-#define FFN_EPILOGUE(ACT)                                                   \
-  if constexpr (EPI == EPI_GATED) epi_gated<TYPE, ACT>(e, m, n, lane, a, b); \
-  else epi_dact<TYPE, ACT>(e, m, n, lane, a);
-    FFN_FOR_ACT(e.act, FFN_EPILOGUE)
-#undef FFN_EPILOGUE
+    Kept<TYPE> k;
+    if (EPI == EPI_DACT) k.load(e.ab, (int64_t)e.fi * e.fj, kept_at(e, m, n), lane);
+    const bool in = m < e.rows && n < e.cols;
+    const int64_t at = (int64_t)m * e.ldo + n;
+    for_activation(e.act, [&](auto act) {
+      constexpr int ACT = decltype(act)::value;
+      if constexpr (EPI == EPI_GATED) {
+        const v4f h = epi_gated<TYPE, ACT>(e, m, n, lane, a, b);
+        if (in) put_operand<TYPE>(e.out, at, e.plane, h);
+      } else {
+        v4f da, db;
+        epi_dact<TYPE, ACT>(k, a, da, db);
+        if (in) {
+          put_operand<TYPE>(e.out, at, e.plane, da);
+          put_operand<TYPE>(e.out, at + e.ldo / 2, e.plane, db);
+        }
+      }
+    });
   }
 }
 
@@ -332,21 +485,29 @@ __global__ __launch_bounds__(256) void k_ffn_pack(const void* src, int64_t lds_,
 // The products by the layouts of their operands and their epilogue.
 enum { FFN_GATE_UP, FFN_DOWN, FFN_DH, FFN_DX, FFN_DW };
 
+// The tiles, and how many columns of C one covers: half of BN for GATE_UP.
+enum { FFN_256x256, FFN_128x128, FFN_64x128, FFN_32x128, FFN_TILES };
+constexpr int FFN_BM[FFN_TILES] = {256, 128, 64, 32}, FFN_BN[FFN_TILES] = {256, 128, 128, 128};
+
 template <int TYPE, int TILE, int WM, int WN, int LA, int LB, int EPI>
 void launch_gemm(const FfnOperands& o, const FfnEpilogue& e, hipStream_t st) {
-  using G = Gemm<TILE, TILE, WM, WN, LA, LB, TYPE == SCAO_F16, EPI == EPI_GATED>;
+  using G = Gemm<FFN_BM[TILE], FFN_BN[TILE], WM, WN, LA, LB, TYPE == SCAO_F16, EPI == EPI_GATED>;
   const int tiles = o.tiles_m * o.tiles_n;
   k_ffn_gemm<G, TYPE, EPI><<<tiles * o.splits, G::THREADS, 0, st>>>(o, e);
   if (o.splits == 1) return;
-  const int fi = o.tiles_m * (TILE / 16), fj = o.tiles_n * (G::COLS_N / 16);
+  const int fi = o.tiles_m * (FFN_BM[TILE] / 16), fj = o.tiles_n * (G::COLS_N / 16);
   const int64_t frags = (int64_t)fi * fj;
   k_ffn_join<TYPE, EPI><<<(int)((frags + 3) / 4), 256, 0, st>>>(e, o.splits, fi, fj);
 }
 
 template <int TYPE, int LA, int LB, int EPI>
 void launch_tile(int tile, const FfnOperands& o, const FfnEpilogue& e, hipStream_t st) {
-  if (tile == 256) launch_gemm<TYPE, 256, 2, 4, LA, LB, EPI>(o, e, st);
-  else launch_gemm<TYPE, 128, 2, 2, LA, LB, EPI>(o, e, st);
+  if (tile == FFN_256x256) launch_gemm<TYPE, FFN_256x256, 2, 4, LA, LB, EPI>(o, e, st);
+  else if (tile == FFN_128x128) launch_gemm<TYPE, FFN_128x128, 2, 2, LA, LB, EPI>(o, e, st);
+  else if constexpr (LA == ROWS) {   // A's rows are tokens: there may be few
+    if (tile == FFN_64x128) launch_gemm<TYPE, FFN_64x128, 1, 4, LA, LB, EPI>(o, e, st);
+    else launch_gemm<TYPE, FFN_32x128, 1, 4, LA, LB, EPI>(o, e, st);
+  }
 }
 
 template <int TYPE>
@@ -368,10 +529,12 @@ void launch_pack(const void* src, int64_t ld, int64_t rows, int cols, void* dst,
   k_ffn_pack<TYPE><<<(int)((n + 255) / 256), 256, 0, st>>>(src, ld, rows, cols, dst, ldo, plane);
 }
 
+struct FfnFew;
 // instantiated in ffn_f32.hip, ffn_bf16.hip and ffn_f16.hip
 struct FfnLaunchers {
   void (*product)(int, int, const FfnOperands&, const FfnEpilogue&, hipStream_t);
   void (*pack)(const void*, int64_t, int64_t, int, void*, int, int64_t, hipStream_t);
+  void (*few)(const FfnFew&, const FfnEpilogue&, bool, hipStream_t);
 };
 FfnLaunchers ffn_f32();
 FfnLaunchers ffn_bf16();

@@ -91,6 +91,17 @@ def test_few_tokens(hip_device, dtype, tokens, d, f):
 
 
 @pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("tokens", [1, 15, 16, 17, 32, 33, 48, 63, 64, 65])
+@pytest.mark.parametrize("d,f,skip", [(32, 33, 0), (31, 100, 1), (520, 264, 0), (2050, 70, 3)])
+def test_serving_sizes(hip_device, dtype, tokens, d, f, skip):
+    """The forward pass alone around the sizes where its kernels change, with
+    rows that start and end anywhere."""
+    ins = _inputs(hip_device, tokens, d, f, dtype, seed=tokens, skip=skip)
+    y = scao_amd.gated_ffn(*ins[:4], activation=ACTS[tokens % 5])
+    _compare(dict(y=y), reference(*ins, ACTS[tokens % 5]), dtype)
+
+
+@pytest.mark.parametrize("dtype", TYPES)
 def test_many_tiles(hip_device, dtype):
     _check(hip_device, 2050, 1032, 2056, dtype)
 
@@ -164,7 +175,8 @@ def test_shapes_of_x_and_views(hip_device):
     assert torch.equal(scao_amd.gated_ffn(x, gate.t().contiguous().t(), up, down), flat)
     x3 = x.reshape(3, 20, 32).transpose(0, 1).detach().requires_grad_()
     y = scao_amd.gated_ffn(x3, gate, up, down)
-    assert torch.equal(y, flat.reshape(3, 20, 32).transpose(0, 1))
+    kept = scao_amd.gated_ffn(x.detach().requires_grad_(), gate, up, down)   # as for training
+    assert torch.equal(y, kept.reshape(3, 20, 32).transpose(0, 1))
     y.sum().backward()   # an expanded gradient of the output
     assert x3.grad.shape == x3.shape and bool(x3.grad.isfinite().all())
     one = torch.ones(60, 32, dtype=torch.bfloat16, device=hip_device)
