@@ -70,7 +70,13 @@ int64_t scao_ffn_saved_bytes(const scao_ffn_desc* desc);
 int64_t scao_ffn_forward_workspace(const scao_ffn_desc* desc, int save);
 int scao_ffn_forward(const scao_ffn_desc* desc, void* y, void* saved, void* workspace,
                      void* stream);
-int64_t scao_ffn_backward_workspace(const scao_ffn_desc* desc, const void* dy, int64_t ld_dy);
+/* grads: which of them are wanted */
+#define SCAO_FFN_DX 1
+#define SCAO_FFN_DGATE 2
+#define SCAO_FFN_DUP 4
+#define SCAO_FFN_DDOWN 8
+int64_t scao_ffn_backward_workspace(const scao_ffn_desc* desc, const void* dy, int64_t ld_dy,
+                                    int grads);
 int scao_ffn_backward(const scao_ffn_desc* desc, const void* dy, int64_t ld_dy, const void* saved,
                       void* dx, void* dw_gate, void* dw_up, void* dw_down, void* workspace,
                       void* stream);

@@ -173,7 +173,7 @@ TRAIN_SIGNATURES = {
     "scao_ffn_saved_bytes": (_I64, [_VP]),
     "scao_ffn_forward_workspace": (_I64, [_VP, _I]),
     "scao_ffn_forward": (_I, [_VP, _VP, _VP, _VP, _VP]),
-    "scao_ffn_backward_workspace": (_I64, [_VP, _VP, _I64]),
+    "scao_ffn_backward_workspace": (_I64, [_VP, _VP, _I64, _I]),
     "scao_ffn_backward": (_I, [_VP, _VP, _I64, _VP, _VP, _VP, _VP, _VP, _VP, _VP]),
 }
 

@@ -52,53 +52,81 @@ struct Block {
     return s.dtype != SCAO_F32 && (uintptr_t)p % 16 == 0 && (ld % 8 == 0 || rows == 1) &&
            cols % 8 == 0;
   }
-  // The user's matrix itself where it can be, else a packed copy.
-  Operand operand(const void* p, int64_t ld, int64_t rows, int64_t cols) {
-    if (direct(p, ld, rows, cols)) return Operand{p, rows == 1 ? cols : ld, 0};
+  // The user's matrix itself where it can be, else a copy that pack() makes.
+  FfnPack packs{};
+  Operand operand(const void* p, int64_t ld, int64_t rows, int64_t cols, bool as_is = true) {
+    if (as_is && direct(p, ld, rows, cols)) return Operand{p, rows == 1 ? cols : ld, 0};
     Operand o;
     o.ld = round_up(cols, 8);
     o.plane = rows * o.ld;
     o.p = ws.take(parts * o.plane * 2);
-    if (!dry)
-      launchers(s.dtype).pack(p, ld, rows, (int)cols, const_cast<void*>(o.p), (int)o.ld, o.plane,
-                              st);
+    packs.m[packs.n++] = {p, const_cast<void*>(o.p), ld, o.plane, rows, (int)cols, (int)o.ld,
+                          packs.groups};
+    packs.groups += (rows * (o.ld / 8) + 255) / 256;
     return o;
   }
+  // gate and up weights, with one row stride
+  void gate_up(Operand& g, Operand& u) {
+    const bool same = s.ld_gate == s.ld_up;
+    g = operand(s.w_gate, s.ld_gate, s.f, s.d, same);
+    // (either alone may start off 16 bytes: then their strides agree only packed)
+    u = operand(s.w_up, s.ld_up, s.f, s.d, same && g.p == s.w_gate);
+    if (g.ld != u.ld) g = operand(s.w_gate, s.ld_gate, s.f, s.d, false);
+  }
+  void pack() {
+    if (packs.n && !dry) launchers(s.dtype).pack(packs, st);
+  }
 
-  // Tile and parts of k for an M x N product of `steps` k steps: the least
-  // estimated time.  us of a step with one workgroup a CU and with all a CU
-  // holds, and of a tile's beginning and end, fitted to the times of every tile
-  // and part count of 225 products (8 to 4096 tokens, 256 x 704 to 4096 x 14336):
-  // the choice is 1.7% slower than the best on the geometric average, 17% at
-  // most.  For example dx of 24 tokens, 2048 x 8192: 32 x 128 tiles in one part
-  // 116 us, in 16 parts 21.8; of 4096 tokens: 256 x 256 in one part 285, in two
-  // 183, 128 x 128 in one 251.
-  static void choose(int64_t M, int64_t N, int64_t steps, bool gated, bool tokens, int& tile,
-                     int& splits) {
-    struct Cost {
-      int slots;
-      double lone, full, ends;
-    };
+  // Estimated us of products on tiles: us of a k step with one workgroup a CU
+  // and with all a CU holds, and of a tile's beginning and end, fitted to the
+  // times of every tile and part count of 225 products (8 to 4096 tokens, 256 x
+  // 704 to 4096 x 14336): the choice is 1.7% slower than the best on the
+  // geometric average, 17% at most.  For example dx of 24 tokens, 2048 x 8192: 32
+  // x 128 tiles in one part 116 us, in 16 parts 21.8; of 4096 tokens: 256 x 256
+  // in one part 285, in two 183, 128 x 128 in one 251.
+  struct Cost {
+    int slots;
+    double lone, full, ends;
+    double step(int64_t groups) const {
+      const double crowd = groups >= slots  ? 1.0
+                           : slots == 256   ? groups / 256.0
+                           : groups <= 256  ? 0.0
+                                            : (groups - 256.0) / (slots - 256.0);
+      return lone + (full - lone) * crowd;
+    }
+  };
+  struct Shape {
+    int64_t M, N, steps;
+    bool gated;
+    int64_t tiles(int t) const {
+      const int64_t cols = gated ? FFN_BN[t] / 2 : FFN_BN[t];
+      return ((M + FFN_BM[t] - 1) / FFN_BM[t]) * ((N + cols - 1) / cols);
+    }
+    // the join: a launch, 8 bytes a part and element, and the epilogue's own
+    // `moved`, which a tile's end would overlap better
+    double moved;
+    double join(int64_t n) const {
+      return n == 1 ? 0.0 : 2 + (8 / 7.4e6 * n * (gated ? 2 : 1) + moved / 5e6) * M * N;
+    }
+    bool may_split(int t, int64_t n) const {
+      return n == 1 || (n * 2 <= steps && tiles(t) * n <= 2048);
+    }
+  };
+  static const Cost& cost(int tile) {
     static const Cost costs[FFN_TILES] = {
         {256, 1.15, 1.50, 4.9}, {512, 0.62, 1.14, 5.2}, {512, 0.56, 0.70, 3.0}, {768, 0.44, 0.96, 1.7}};
+    return costs[tile];
+  }
+  static double choose(const Shape& s, bool tokens, int& tile, int& splits) {
     double best = 1e30;
     for (int t = 0; t < (tokens ? FFN_TILES : FFN_64x128); ++t) {
-      const Cost& c = costs[t];
-      const int64_t cols = gated ? FFN_BN[t] / 2 : FFN_BN[t];
-      const int64_t tiles = ((M + FFN_BM[t] - 1) / FFN_BM[t]) * ((N + cols - 1) / cols);
+      const Cost& c = cost(t);
       for (int64_t n : {1, 2, 3, 4, 6, 8, 12, 16, 24, 32}) {
-        if (n > 1 && (n * 2 > steps || tiles * n > 2048)) break;
-        const int64_t per = (steps + n - 1) / n, groups = tiles * n;
-        const int64_t rounds = groups / c.slots, rest = groups % c.slots;
-        double us = rounds * (per * c.full + c.ends);
-        if (rest) {
-          const double crowd = c.slots == 256 ? rest / 256.0
-                               : rest <= 256  ? 0.0
-                                              : (rest - 256.0) / (c.slots - 256.0);
-          us += per * (c.lone + (c.full - c.lone) * crowd) + c.ends;
-        }
-        // the join: a launch, and 8 bytes a part and element
-        if (n > 1) us += 2 + 8 / 7.4e6 * n * (double)M * N * (gated ? 2 : 1);
+        if (!s.may_split(t, n)) break;
+        const int64_t per = (s.steps + n - 1) / n, groups = s.tiles(t) * n;
+        const int64_t rest = groups % c.slots;
+        double us = (groups / c.slots) * (per * c.full + c.ends) + s.join(n);
+        if (rest) us += per * c.step(rest) + c.ends;
         if (us < best) {
           best = us;
           tile = t;
@@ -106,6 +134,44 @@ struct Block {
         }
       }
     }
+    return best;
+  }
+  // two products in one launch: `a` workgroups of one length, then as many of
+  // the other's as fit where these leave room
+  static double choose_pair(const Shape& x, const Shape& y, int& tile, int& nx, int& ny) {
+    double best = 1e30;
+    for (int t : {FFN_256x256, FFN_128x128}) {
+      const Cost& c = cost(t);
+      for (int64_t n : {1, 2, 4, 8, 16}) {
+        if (!x.may_split(t, n)) break;
+        for (int64_t m : {1, 2, 4, 8, 16}) {
+          if (!y.may_split(t, m)) break;
+          int64_t ga = x.tiles(t) * n, gb = y.tiles(t) * m;
+          const double step = c.step(ga + gb);
+          double a = ((x.steps + n - 1) / n) * step + c.ends, b = ((y.steps + m - 1) / m) * step + c.ends;
+          if (a < b) {
+            std::swap(a, b);
+            std::swap(ga, gb);
+          }
+          // the first's rounds, its last one on `rest` workgroups' places
+          const int64_t rounds = ga / c.slots, rest = ga % c.slots;
+          const double lo = rounds * a, hi = rest ? lo + a : lo;
+          double us = std::max(hi, (ga * a + gb * b) / c.slots);
+          // places for the second's beside and behind them
+          while ((int64_t)((us - lo) / b + 1e-9) * (c.slots - rest) +
+                     (int64_t)((us - hi) / b + 1e-9) * rest < gb)
+            us += 0.25 * b;
+          us += x.join(n) + y.join(m);
+          if (us < best) {
+            best = us;
+            tile = t;
+            nx = (int)n;
+            ny = (int)m;
+          }
+        }
+      }
+    }
+    return best;
   }
 
   // a segment for every product of parts that counts: the small ones first
@@ -121,25 +187,54 @@ struct Block {
     return n;
   }
 
-  int product(int kind, FfnOperands& o, FfnEpilogue& e) {
-    const bool gated = kind == FFN_GATE_UP;
-    const int64_t steps = (int64_t)o.nseg * ((o.K + FFN_BK - 1) / FFN_BK);
-    int tile = 0;
-    choose(o.M, o.N, steps, gated, kind != FFN_DW, tile, o.splits);
-    const int cols = gated ? FFN_BN[tile] / 2 : FFN_BN[tile];
+  Shape shape(int kind, const FfnOperands& o) const {
+    const double bytes = kind == FFN_GATE_UP ? 8 : kind == FFN_DH ? 10 : 0;
+    return Shape{o.M, o.N, (int64_t)o.nseg * ((o.K + FFN_BK - 1) / FFN_BK), kind == FFN_GATE_UP,
+                 s.dtype == SCAO_F32 ? 2 * bytes : bytes};
+  }
+  // the tiles' counts, and room for the parts of a split product
+  void cut(int kind, int tile, FfnOperands& o, FfnEpilogue& e) {
+    const int cols = kind == FFN_GATE_UP ? FFN_BN[tile] / 2 : FFN_BN[tile];
     o.tiles_m = (o.M + FFN_BM[tile] - 1) / FFN_BM[tile];
     o.tiles_n = (o.N + cols - 1) / cols;
     e.partial = nullptr;
-    if (o.splits > 1) {
-      const int64_t at = ws.used;   // given back: the next product may write it
+    if (o.splits > 1)
       e.partial = (float*)ws.take((int64_t)o.splits * o.tiles_m * o.tiles_n * FFN_BM[tile] *
                                   FFN_BN[tile] * 4);
-      peak = std::max(peak, ws.used);
-      ws.used = at;
+    peak = std::max(peak, ws.used);
+  }
+  struct Product {
+    int kind;
+    FfnOperands o;
+    FfnEpilogue e;
+  };
+  void run(Product& p) {
+    const int64_t at = ws.used;   // the parts' room is given back
+    int tile = 0;
+    choose(shape(p.kind, p.o), p.kind != FFN_DW, tile, p.o.splits);
+    cut(p.kind, tile, p.o, p.e);
+    ws.used = at;
+    if (!dry) launchers(s.dtype).product(p.kind, tile, p.o, p.e, st);
+  }
+  // dh or dx, and a dW that does not need it
+  void run(Product& p, Product& w) {
+    const Shape x = shape(p.kind, p.o), y = shape(w.kind, w.o);
+    int tile = 0, nx = 0, ny = 0, t, n;
+    const double apart = choose(x, true, t, n) + choose(y, false, t, n) + 3;
+    // large products lose a few per cent side by side, two working sets in an L2:
+    // 8192 tokens, 4096 x 14336, the whole pass 6560 us apart and 6700 in pairs
+    if (1.06 * choose_pair(x, y, tile, nx, ny) > apart) {
+      run(p);
+      run(w);
+      return;
     }
-    if (dry) return SCAO_OK;
-    launchers(s.dtype).product(kind, tile, o, e, st);
-    return SCAO_OK;
+    const int64_t at = ws.used;
+    p.o.splits = nx;
+    w.o.splits = ny;
+    cut(p.kind, tile, p.o, p.e);
+    cut(w.kind, tile, w.o, w.e);
+    ws.used = at;
+    if (!dry) launchers(s.dtype).pair(p.kind, tile, p.o, p.e, w.o, w.e, st);
   }
   int64_t peak = 0;
   int64_t need() { return std::max(peak, ws.used); }
@@ -202,118 +297,101 @@ struct Block {
   int forward(void* y, void* saved, bool save) {
     if (!save && few()) return forward_few(y);
     const Operand x = operand(s.x, s.ldx, s.tokens, s.d);
-    Operand g = operand(s.w_gate, s.ld_gate, s.f, s.d), u = operand(s.w_up, s.ld_up, s.f, s.d);
-    if (g.ld != u.ld) pair(g, u);
+    Operand g, u;
+    gate_up(g, u);
     const Operand down = operand(s.w_down, s.ld_down, s.d, s.f);
     Operand h;
     h.ld = fp;
     h.plane = s.tokens * fp;
     h.p = save ? saved : ws.take(h_bytes());
-    FfnOperands o{};
-    o.M = (int)s.tokens;
-    o.N = (int)s.f;
-    o.K = (int)s.d;
-    o.lda = x.ld;
-    o.ldb = g.ld;
+    pack();
+    Product p{FFN_GATE_UP};
+    p.o.M = (int)s.tokens;
+    p.o.N = (int)s.f;
+    p.o.K = (int)s.d;
+    p.o.lda = x.ld;
+    p.o.ldb = g.ld;
     const void* pu[FFN_MAX_SEG];
-    o.nseg = segments(parts, x, 0, g, o.a, o.b);
-    segments(parts, x, 0, u, pu, o.b + FFN_MAX_SEG / 2);
-    FfnEpilogue e = kept(const_cast<void*>(h.p), save && saved ? (char*)saved + h_bytes() : nullptr,
-                         fp);
-    if (int rc = product(FFN_GATE_UP, o, e)) return rc;
-    o = FfnOperands{};
-    o.M = (int)s.tokens;
-    o.N = (int)s.d;
-    o.K = (int)s.f;
-    o.lda = h.ld;
-    o.ldb = down.ld;
-    o.nseg = segments(parts, h, 0, down, o.a, o.b);
-    e = store(y, s.tokens, s.d);
-    return product(FFN_DOWN, o, e);
+    p.o.nseg = segments(parts, x, 0, g, p.o.a, p.o.b);
+    segments(parts, x, 0, u, pu, p.o.b + FFN_MAX_SEG / 2);
+    p.e = kept(const_cast<void*>(h.p), save && saved ? (char*)saved + h_bytes() : nullptr, fp);
+    run(p);
+    Product q{FFN_DOWN};
+    q.o.M = (int)s.tokens;
+    q.o.N = (int)s.d;
+    q.o.K = (int)s.f;
+    q.o.lda = h.ld;
+    q.o.ldb = down.ld;
+    q.o.nseg = segments(parts, h, 0, down, q.o.a, q.o.b);
+    q.e = store(y, s.tokens, s.d);
+    run(q);
+    return SCAO_OK;
   }
 
-  // gate and up weights with one row stride
-  void pair(Operand& g, Operand& u) {
-    const int64_t ld = round_up(s.d, 8);
-    auto packed = [&](const void* p, int64_t from, Operand& o) {
-      if (o.ld == ld && o.p != p) return;
-      o.ld = ld;
-      o.plane = s.f * ld;
-      o.p = ws.take(parts * o.plane * 2);
-      if (!dry) launchers(s.dtype).pack(p, from, s.f, (int)s.d, const_cast<void*>(o.p), (int)ld,
-                                        o.plane, st);
-    };
-    packed(s.w_gate, s.ld_gate, g);
-    packed(s.w_up, s.ld_up, u);
-  }
-
+  // grads: SCAO_FFN_DX | ... wanted
   int backward(const void* dy_, int64_t ld_dy, const void* saved, void* dx, void* dgate, void* dup,
-               void* ddown, bool all) {
-    const bool need_w = all || dgate || dup, need_x = all || dx;
+               void* ddown, int grads) {
+    const bool gate = grads & SCAO_FFN_DGATE, up = grads & SCAO_FFN_DUP;
+    const bool want_down = grads & SCAO_FFN_DDOWN, want_x = grads & SCAO_FFN_DX;
+    const bool want_dh = gate || up || want_x;
     const Operand dy = operand(dy_, ld_dy, s.tokens, s.d);
-    Operand h;
+    Operand h, down, x, g, u, dab;
     h.p = saved;
     h.ld = fp;
     h.plane = s.tokens * fp;
-    if (all || ddown) {
-      FfnOperands o{};
-      o.M = (int)s.d;
-      o.N = (int)s.f;
-      o.K = (int)s.tokens;
-      o.lda = dy.ld;
-      o.ldb = h.ld;
-      o.nseg = segments(parts, dy, 0, h, o.a, o.b);
-      FfnEpilogue e = store(ddown, s.d, s.f);
-      if (int rc = product(FFN_DW, o, e)) return rc;
+    if (want_dh) down = operand(s.w_down, s.ld_down, s.d, s.f);
+    if (gate || up) x = operand(s.x, s.ldx, s.tokens, s.d);
+    if (want_x) gate_up(g, u);
+    if (want_dh) {   // da in the first fp columns, db in the others
+      dab.ld = 2 * fp;
+      dab.plane = s.tokens * dab.ld;
+      dab.p = ws.take(parts * dab.plane * 2);
     }
-    if (!need_w && !need_x) return SCAO_OK;
-    const Operand down = operand(s.w_down, s.ld_down, s.d, s.f);
-    Operand dab;   // da in the first fp columns, db in the others
-    dab.ld = 2 * fp;
-    dab.plane = s.tokens * dab.ld;
-    dab.p = ws.take(parts * dab.plane * 2);
-    {
-      FfnOperands o{};
-      o.M = (int)s.tokens;
-      o.N = (int)s.f;
-      o.K = (int)s.d;
-      o.lda = dy.ld;
-      o.ldb = down.ld;
-      o.nseg = segments(parts, dy, 0, down, o.a, o.b);
-      FfnEpilogue e = kept(const_cast<void*>(dab.p),
-                           saved ? (char*)const_cast<void*>(saved) + h_bytes() : nullptr, 2 * fp);
-      if (int rc = product(FFN_DH, o, e)) return rc;
-    }
-    if (need_w) {
-      const Operand x = operand(s.x, s.ldx, s.tokens, s.d);
-      FfnOperands o{};
-      const bool gate = all || dgate, up = all || dup;
-      const int64_t from = gate ? 0 : fp;
-      o.M = (int)((gate && up ? fp : 0) + s.f);
-      o.N = (int)s.d;
-      o.K = (int)s.tokens;
-      o.lda = dab.ld;
-      o.ldb = x.ld;
-      o.nseg = segments(parts, dab, from, x, o.a, o.b);
-      FfnEpilogue e = store(gate ? dgate : dup, s.f, s.d);
-      e.out2 = dup;
-      e.second = gate && up ? (int)fp : 0x7fffffff;
-      if (int rc = product(FFN_DW, o, e)) return rc;
-    }
-    if (need_x) {
-      Operand g = operand(s.w_gate, s.ld_gate, s.f, s.d), u = operand(s.w_up, s.ld_up, s.f, s.d);
-      if (g.ld != u.ld) pair(g, u);
-      FfnOperands o{};
-      o.M = (int)s.tokens;
-      o.N = (int)s.d;
-      o.K = (int)s.f;
-      o.lda = dab.ld;
-      o.ldb = g.ld;
-      o.nseg = segments(parts, dab, 0, g, o.a, o.b);
-      o.nseg += segments(parts, dab, fp, u, o.a + o.nseg, o.b + o.nseg);
-      FfnEpilogue e = store(dx, s.tokens, s.d);
-      if (int rc = product(FFN_DX, o, e)) return rc;
-    }
+    pack();
+
+    Product wd{FFN_DW}, dh{FFN_DH}, wgu{FFN_DW}, px{FFN_DX};
+    wd.o.M = (int)s.d;
+    wd.o.N = (int)s.f;
+    wd.o.K = (int)s.tokens;
+    wd.o.lda = dy.ld;
+    wd.o.ldb = h.ld;
+    wd.o.nseg = segments(parts, dy, 0, h, wd.o.a, wd.o.b);
+    wd.e = store(ddown, s.d, s.f);
+
+    dh.o.M = (int)s.tokens;
+    dh.o.N = (int)s.f;
+    dh.o.K = (int)s.d;
+    dh.o.lda = dy.ld;
+    dh.o.ldb = down.ld;
+    dh.o.nseg = segments(parts, dy, 0, down, dh.o.a, dh.o.b);
+    dh.e = kept(const_cast<void*>(dab.p),
+                saved ? (char*)const_cast<void*>(saved) + h_bytes() : nullptr, 2 * fp);
+
+    wgu.o.M = (int)((gate && up ? fp : 0) + s.f);
+    wgu.o.N = (int)s.d;
+    wgu.o.K = (int)s.tokens;
+    wgu.o.lda = dab.ld;
+    wgu.o.ldb = x.ld;
+    wgu.o.nseg = segments(parts, dab, gate ? 0 : fp, x, wgu.o.a, wgu.o.b);
+    wgu.e = store(gate ? dgate : dup, s.f, s.d);
+    wgu.e.out2 = dup;
+    wgu.e.second = gate && up ? (int)fp : 0x7fffffff;
+
+    px.o.M = (int)s.tokens;
+    px.o.N = (int)s.d;
+    px.o.K = (int)s.f;
+    px.o.lda = dab.ld;
+    px.o.ldb = g.ld;
+    px.o.nseg = segments(parts, dab, 0, g, px.o.a, px.o.b);
+    px.o.nseg += segments(parts, dab, fp, u, px.o.a + px.o.nseg, px.o.b + px.o.nseg);
+    px.e = store(dx, s.tokens, s.d);
+
+    if (want_down && want_dh) run(dh, wd);
+    else if (want_dh) run(dh);
+    else if (want_down) run(wd);
+    if ((gate || up) && want_x) run(px, wgu);
+    else if (want_x) run(px);
+    else if (gate || up) run(wgu);
     return SCAO_OK;
   }
 };
@@ -378,10 +456,10 @@ extern "C" int scao_ffn_forward(const scao_ffn_desc* d, void* y, void* saved, vo
 }
 
 extern "C" int64_t scao_ffn_backward_workspace(const scao_ffn_desc* d, const void* dy,
-                                               int64_t ld_dy) {
+                                               int64_t ld_dy, int grads) {
   if (check_inputs("scao_ffn_backward_workspace", d)) return 0;
   Block b(*d, nullptr, nullptr, true);
-  b.backward(dy, ld_dy, nullptr, nullptr, nullptr, nullptr, nullptr, true);
+  b.backward(dy, ld_dy, nullptr, nullptr, nullptr, nullptr, nullptr, grads);
   return b.need();
 }
 
@@ -391,12 +469,16 @@ extern "C" int scao_ffn_backward(const scao_ffn_desc* d, const void* dy, int64_t
   const char* who = "scao_ffn_backward";
   if (int rc = check_inputs(who, d)) return rc;
   if (int rc = check_matrix(who, "dy", dy, ld_dy, d->tokens, d->d, d->dtype)) return rc;
-  SCAO_CHECK_ARG(saved && workspace && (uintptr_t)saved % 16 == 0 && (uintptr_t)workspace % 16 == 0,
-                 "%s: saved or workspace is null or not aligned", who);
+  const int grads = (dx ? SCAO_FFN_DX : 0) | (dw_gate ? SCAO_FFN_DGATE : 0) |
+                    (dw_up ? SCAO_FFN_DUP : 0) | (dw_down ? SCAO_FFN_DDOWN : 0);
+  SCAO_CHECK_ARG(saved && (uintptr_t)saved % 16 == 0 && (uintptr_t)workspace % 16 == 0,
+                 "%s: saved is null, or it or workspace not aligned", who);
+  SCAO_CHECK_ARG(workspace || scao_ffn_backward_workspace(d, dy, ld_dy, grads) == 0,
+                 "%s: null workspace", who);
   for (void* p : {dx, dw_gate, dw_up, dw_down})
     SCAO_CHECK_ARG((uintptr_t)p % size_of(d->dtype) == 0, "%s: a gradient is not aligned", who);
   Block b(*d, workspace, stream, false);
-  if (int rc = b.backward(dy, ld_dy, saved, dx, dw_gate, dw_up, dw_down, false)) return rc;
+  if (int rc = b.backward(dy, ld_dy, saved, dx, dw_gate, dw_up, dw_down, grads)) return rc;
   SCAO_LAUNCH_CHECK(who);
   return SCAO_OK;
 }

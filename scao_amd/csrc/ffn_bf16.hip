@@ -3,6 +3,6 @@
 
 namespace scao {
 FfnLaunchers ffn_bf16() {
-  return {launch_product<SCAO_BF16>, launch_pack<SCAO_BF16>, launch_few<SCAO_BF16>};
+  return {launch_product<SCAO_BF16>, launch_pair<SCAO_BF16>, launch_pack<SCAO_BF16>, launch_few<SCAO_BF16>};
 }
 }  // namespace scao

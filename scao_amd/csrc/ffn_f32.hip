@@ -3,6 +3,6 @@
 
 namespace scao {
 FfnLaunchers ffn_f32() {
-  return {launch_product<SCAO_F32>, launch_pack<SCAO_F32>, launch_few<SCAO_F32>};
+  return {launch_product<SCAO_F32>, launch_pair<SCAO_F32>, launch_pack<SCAO_F32>, launch_few<SCAO_F32>};
 }
 }  // namespace scao

@@ -315,14 +315,14 @@ __device__ __forceinline__ void for_activation(int act, F&& f) {
 // ------------------------------------------------------- products ----------
 typedef __attribute__((address_space(1))) v4f gv4f_a16;
 
+// Workgroup `block` of one product: a tile, or one part of its k steps.
 template <class G, int TYPE, int EPI>
-__global__ __launch_bounds__(G::THREADS, 2) void k_ffn_gemm(const FfnOperands o,
-                                                            const FfnEpilogue e) {
-  __shared__ __attribute__((aligned(1024))) char smem[G::LDS];
+__device__ __forceinline__ void ffn_tile(char* smem, const FfnOperands& o, const FfnEpilogue& e,
+                                         int block) {
   const int tiles = o.tiles_m * o.tiles_n;
-  const int part = blockIdx.x / tiles;
+  const int part = block / tiles;
   int tm, tn;
-  tile_of(blockIdx.x - part * tiles, o.tiles_m, o.tiles_n, tm, tn);
+  tile_of(block - part * tiles, o.tiles_m, o.tiles_n, tm, tn);
   G g(o, (lchar*)smem, tm, tn);
   const int steps = o.nseg * ((o.K + FFN_BK - 1) / FFN_BK);
   const int per = (steps + o.splits - 1) / o.splits;
@@ -420,6 +420,41 @@ __global__ __launch_bounds__(G::THREADS, 2) void k_ffn_gemm(const FfnOperands o,
   }
 }
 
+template <class G, int TYPE, int EPI>
+__global__ __launch_bounds__(G::THREADS, 2) void k_ffn_gemm(const FfnOperands o,
+                                                            const FfnEpilogue e) {
+  __shared__ __attribute__((aligned(1024))) char smem[G::LDS];
+  ffn_tile<G, TYPE, EPI>(smem, o, e, blockIdx.x);
+}
+
+// Two products that do not need each other in one launch: the second one's tiles
+// fill the CUs that the first one's last round would leave idle.  na: workgroups
+// of the first.  `mixed` eights of either take turns (eight, so that a tile keeps
+// its XCD), so that dh's epilogue moves its bytes while other CUs multiply; then
+// come the longer tiles' rest and the shorter ones'.
+template <class GA, int EPI_A, class GB, int EPI_B, int TYPE>
+__global__ __launch_bounds__(GA::THREADS, 2) void k_ffn_pair(const FfnOperands oa,
+                                                             const FfnEpilogue ea,
+                                                             const FfnOperands ob,
+                                                             const FfnEpilogue eb, int na, int nb,
+                                                             int mixed, int b_leads) {
+  static_assert(GA::THREADS == GB::THREADS, "one shape of workgroup");
+  __shared__ __attribute__((aligned(1024))) char smem[GA::LDS > GB::LDS ? GA::LDS : GB::LDS];
+  int b = blockIdx.x;
+  bool lead;
+  if (b < 16 * mixed) {
+    lead = b / 8 % 2 == 0;
+    b = b / 16 * 8 + b % 8;
+  } else {
+    b -= 8 * mixed;
+    const int n = b_leads ? nb : na;
+    lead = b < n;
+    if (!lead) b -= n - 8 * mixed;
+  }
+  if (lead != (b_leads != 0)) ffn_tile<GA, TYPE, EPI_A>(smem, oa, ea, b);
+  else ffn_tile<GB, TYPE, EPI_B>(smem, ob, eb, b);
+}
+
 // The parts of a split product, added in order, and its epilogue: a wave takes
 // a fragment.
 template <int TYPE, int EPI>
@@ -461,23 +496,40 @@ __global__ __launch_bounds__(256) void k_ffn_join(const FfnEpilogue e, int split
 }
 
 // --------------------------------------------------------- packing ---------
-// rows x cols elements with any row stride and start, as a product's operand:
-// rows of `ldo` elements (cols rounded up to 8, the rest zero), 16-byte aligned;
-// an fp32 one as three bf16 planes that add up to it.  Eight columns a thread.
+// Matrices with any row stride and start as products' operands: rows of `ldo`
+// elements (cols rounded up to 8, the rest zero), 16-byte aligned; an fp32 one as
+// three bf16 planes that add up to it.  Eight columns a thread; all matrices of a
+// pass in one launch.
+constexpr int FFN_MAX_PACK = 5;
+struct FfnPack {
+  struct Matrix {
+    const void* src;
+    void* dst;
+    int64_t ld, plane, rows;
+    int cols, ldo;
+    int64_t first;          // workgroups before this matrix
+  } m[FFN_MAX_PACK];
+  int n;
+  int64_t groups;
+};
 template <int TYPE>
-__global__ __launch_bounds__(256) void k_ffn_pack(const void* src, int64_t lds_, int64_t rows,
-                                                  int cols, void* dst, int ldo, int64_t plane) {
-  const int per = ldo / 8;
-  const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x;
-  if (i >= rows * per) return;
+__global__ __launch_bounds__(256) void k_ffn_pack(const FfnPack p) {
+  int k = 0;
+#pragma unroll
+  for (int i = 1; i < FFN_MAX_PACK; ++i)
+    if (i < p.n && (int64_t)blockIdx.x >= p.m[i].first) k = i;
+  const FfnPack::Matrix& m = p.m[k];
+  const int per = m.ldo / 8;
+  const int64_t i = ((int64_t)blockIdx.x - m.first) * 256 + threadIdx.x;
+  if (i >= m.rows * per) return;
   const int64_t r = i / per;
   const int c = (int)(i % per) * 8;
 #pragma unroll
   for (int t = 0; t < 8; t += 4) {
-    const int left = cols - c - t;
-    const v4f x = ld4(src, TYPE, r * lds_ + c + t, left >= 4,
+    const int left = m.cols - c - t;
+    const v4f x = ld4(m.src, TYPE, r * m.ld + c + t, left >= 4,
                       left >= 4 ? 15 : left <= 0 ? 0 : (1 << left) - 1);
-    put_operand<TYPE>(dst, r * ldo + c + t, plane, x);
+    put_operand<TYPE>(m.dst, r * m.ldo + c + t, m.plane, x);
   }
 }
 
@@ -490,14 +542,51 @@ enum { FFN_256x256, FFN_128x128, FFN_64x128, FFN_32x128, FFN_TILES };
 constexpr int FFN_BM[FFN_TILES] = {256, 128, 64, 32}, FFN_BN[FFN_TILES] = {256, 128, 128, 128};
 
 template <int TYPE, int TILE, int WM, int WN, int LA, int LB, int EPI>
-void launch_gemm(const FfnOperands& o, const FfnEpilogue& e, hipStream_t st) {
-  using G = Gemm<FFN_BM[TILE], FFN_BN[TILE], WM, WN, LA, LB, TYPE == SCAO_F16, EPI == EPI_GATED>;
-  const int tiles = o.tiles_m * o.tiles_n;
-  k_ffn_gemm<G, TYPE, EPI><<<tiles * o.splits, G::THREADS, 0, st>>>(o, e);
+using FfnTile =
+    Gemm<FFN_BM[TILE], FFN_BN[TILE], WM, WN, LA, LB, TYPE == SCAO_F16, EPI == EPI_GATED>;
+
+template <class G, int TYPE, int EPI>
+void launch_join(const FfnOperands& o, const FfnEpilogue& e, hipStream_t st) {
   if (o.splits == 1) return;
-  const int fi = o.tiles_m * (FFN_BM[TILE] / 16), fj = o.tiles_n * (G::COLS_N / 16);
+  const int fi = o.tiles_m * (G::BM_ / 16), fj = o.tiles_n * (G::COLS_N / 16);
   const int64_t frags = (int64_t)fi * fj;
   k_ffn_join<TYPE, EPI><<<(int)((frags + 3) / 4), 256, 0, st>>>(e, o.splits, fi, fj);
+}
+
+template <int TYPE, int TILE, int WM, int WN, int LA, int LB, int EPI>
+void launch_gemm(const FfnOperands& o, const FfnEpilogue& e, hipStream_t st) {
+  using G = FfnTile<TYPE, TILE, WM, WN, LA, LB, EPI>;
+  k_ffn_gemm<G, TYPE, EPI>
+      <<<o.tiles_m * o.tiles_n * o.splits, G::THREADS, 0, st>>>(o, e);
+  launch_join<G, TYPE, EPI>(o, e, st);
+}
+
+// the products of the backward pass that go together: dh or dx, and a dW
+template <int TYPE, int TILE, int WM, int WN, int EPI>
+void launch_pair_tile(const FfnOperands& oa, const FfnEpilogue& ea, const FfnOperands& ob,
+                      const FfnEpilogue& eb, hipStream_t st) {
+  using A = FfnTile<TYPE, TILE, WM, WN, ROWS, COLS, EPI>;
+  using B = FfnTile<TYPE, TILE, WM, WN, COLS, COLS, EPI_STORE>;
+  const int na = oa.tiles_m * oa.tiles_n * oa.splits, nb = ob.tiles_m * ob.tiles_n * ob.splits;
+  const int mixed = EPI == EPI_DACT ? (na < nb ? na : nb) / 8 : 0;
+  const int64_t sa = (int64_t)oa.nseg * ((oa.K + FFN_BK - 1) / FFN_BK) / oa.splits;
+  const int64_t sb = (int64_t)ob.nseg * ((ob.K + FFN_BK - 1) / FFN_BK) / ob.splits;
+  k_ffn_pair<A, EPI, B, EPI_STORE, TYPE>
+      <<<na + nb, A::THREADS, 0, st>>>(oa, ea, ob, eb, na, nb, mixed, sb > sa);
+  launch_join<A, TYPE, EPI>(oa, ea, st);
+  launch_join<B, TYPE, EPI_STORE>(ob, eb, st);
+}
+template <int TYPE>
+void launch_pair(int kind, int tile, const FfnOperands& oa, const FfnEpilogue& ea,
+                 const FfnOperands& ob, const FfnEpilogue& eb, hipStream_t st) {
+  if (kind == FFN_DH) {
+    if (tile == FFN_256x256) launch_pair_tile<TYPE, FFN_256x256, 2, 4, EPI_DACT>(oa, ea, ob, eb, st);
+    else launch_pair_tile<TYPE, FFN_128x128, 2, 2, EPI_DACT>(oa, ea, ob, eb, st);
+  } else {
+    if (tile == FFN_256x256)
+      launch_pair_tile<TYPE, FFN_256x256, 2, 4, EPI_STORE>(oa, ea, ob, eb, st);
+    else launch_pair_tile<TYPE, FFN_128x128, 2, 2, EPI_STORE>(oa, ea, ob, eb, st);
+  }
 }
 
 template <int TYPE, int LA, int LB, int EPI>
@@ -523,17 +612,17 @@ void launch_product(int kind, int tile, const FfnOperands& o, const FfnEpilogue&
 }
 
 template <int TYPE>
-void launch_pack(const void* src, int64_t ld, int64_t rows, int cols, void* dst, int ldo,
-                 int64_t plane, hipStream_t st) {
-  const int64_t n = rows * (ldo / 8);
-  k_ffn_pack<TYPE><<<(int)((n + 255) / 256), 256, 0, st>>>(src, ld, rows, cols, dst, ldo, plane);
+void launch_pack(const FfnPack& p, hipStream_t st) {
+  k_ffn_pack<TYPE><<<(int)p.groups, 256, 0, st>>>(p);
 }
 
 struct FfnFew;
 // instantiated in ffn_f32.hip, ffn_bf16.hip and ffn_f16.hip
 struct FfnLaunchers {
   void (*product)(int, int, const FfnOperands&, const FfnEpilogue&, hipStream_t);
-  void (*pack)(const void*, int64_t, int64_t, int, void*, int, int64_t, hipStream_t);
+  void (*pair)(int, int, const FfnOperands&, const FfnEpilogue&, const FfnOperands&,
+               const FfnEpilogue&, hipStream_t);
+  void (*pack)(const FfnPack&, hipStream_t);
   void (*few)(const FfnFew&, const FfnEpilogue&, bool, hipStream_t);
 };
 FfnLaunchers ffn_f32();

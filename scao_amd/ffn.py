@@ -101,7 +101,9 @@ class _GatedFFN(torch.autograd.Function):
 
         dx, ddown = new(need[0], x.shape[0], d), new(need[3], d, f)
         dgate, dup = new(need[1], f, d), new(need[2], f, d)
-        work = _bytes(L.lib().scao_ffn_backward_workspace(at, dy.data_ptr(), dy.stride(0)), dev)
+        grads = need[0] | need[1] << 1 | need[2] << 2 | need[3] << 3
+        work = _bytes(L.lib().scao_ffn_backward_workspace(at, dy.data_ptr(), dy.stride(0), grads),
+                      dev)
         with torch.cuda.device(dev):
             L.call("scao_ffn_backward", at, dy.data_ptr(), dy.stride(0), saved.data_ptr(),
                    *(None if t is None else t.data_ptr() for t in (dx, dgate, dup, ddown)),

@@ -120,7 +120,7 @@ def test_ffn_refuses_bad_descriptors(kw):
     assert lib.scao_ffn_backward(at, P, 16, P, P, P, P, P, P, None) == 1
     assert lib.scao_last_error().startswith(b"scao_ffn_backward:")
     assert lib.scao_ffn_forward_workspace(at, 0) == 0
-    assert lib.scao_ffn_backward_workspace(at, P, 16) == 0
+    assert lib.scao_ffn_backward_workspace(at, P, 16, 15) == 0
 
 
 def test_ffn_refuses_bad_buffers():
