@@ -222,6 +222,22 @@ def lib():
     return _lib
 
 
+_tensors = None
+
+
+def tensors():
+    """The module ``scao_amd._tensors`` (csrc/tensors.cpp)."""
+    global _tensors
+    if _tensors is None:
+        try:
+            from . import _tensors as module
+        except ImportError as e:
+            raise ScaoLibError(f"scao_amd: {HERE}/_tensors.so is missing or does not fit this "
+                               f"torch ({e}). Build it with `python -m scao_amd.build`.") from None
+        _tensors = module
+    return _tensors
+
+
 def call(name: str, *args) -> None:
     """Call a C-ABI entry point and raise on a non-zero status."""
     rc = getattr(lib(), name)(*args)
@@ -232,6 +248,21 @@ def call(name: str, *args) -> None:
 
 def stream_ptr(device: torch.device) -> int:
     return torch.cuda.current_stream(device).cuda_stream
+
+
+_raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None)
+
+
+def call_on(device: torch.device, name: str, *args) -> None:
+    """``call`` with the current stream of ``device`` as the last argument, on
+    that device.  Where it is the current one already, as almost always, neither
+    a device guard nor a stream object is made (6 us of a short call)."""
+    index = device.index
+    if _raw_stream is not None and index == torch.cuda.current_device():
+        call(name, *args, _raw_stream(index))
+        return
+    with torch.cuda.device(device):
+        call(name, *args, stream_ptr(device))
 
 
 def upload(arr: np.ndarray, device: torch.device) -> torch.Tensor:

@@ -5,6 +5,9 @@ parallel, and linked into one shared object exporting the C ABI declared in
 ``include/scao_amd.h``.  Arithmetic contraction is off (-ffp-contract=off):
 fused multiply-adds are written explicitly where the reference rounds once.
 Packed fp32 instructions are disabled for all device code.
+
+``csrc/tensors.cpp`` is host code against torch's headers: the Python module
+``scao_amd._tensors`` (``scao_amd/_tensors.so``), built by g++.
 """
 
 from __future__ import annotations
@@ -13,12 +16,15 @@ import concurrent.futures as cf
 import os
 import subprocess
 import sys
+import sysconfig
 
 HERE = os.path.dirname(os.path.abspath(__file__))
 ROOT = os.path.dirname(HERE)
 CSRC = os.path.join(HERE, "csrc")
 OUT_DIR = os.path.join(HERE, "_lib")
 LIB = os.path.join(OUT_DIR, "libscao_amd.so")
+TENSORS = os.path.join(HERE, "_tensors.so")
+CXX = os.environ.get("CXX", "g++")
 HIPCC = os.environ.get("HIPCC", "/opt/rocm/bin/hipcc")
 
 FLAGS = [
@@ -38,16 +44,35 @@ def _compile(src: str, obj: str) -> str:
     return "\n".join(ln for ln in r.stderr.splitlines() if noise not in ln and ln.strip())
 
 
+def _compile_tensors() -> str:
+    from torch._C import _GLIBCXX_USE_CXX11_ABI as abi
+    from torch.utils import cpp_extension
+    # (the CPU's include paths: no HIP type is used)
+    inc = [f"-I{d}" for d in (*cpp_extension.include_paths(), sysconfig.get_path("include"))]
+    lib = os.path.join(os.path.dirname(os.path.dirname(cpp_extension.__file__)), "lib")
+    tmp = TENSORS + ".tmp"
+    cmd = [CXX, "-O2", "-std=c++17", "-fPIC", "-shared", f"-D_GLIBCXX_USE_CXX11_ABI={int(abi)}",
+           *inc, os.path.join(CSRC, "tensors.cpp"), "-o", tmp, f"-L{lib}", "-ltorch_python",
+           "-ltorch_cpu", "-lc10"]
+    r = subprocess.run(cmd, capture_output=True, text=True)
+    if r.returncode != 0:
+        raise RuntimeError(f"{CXX} failed for tensors.cpp:\n{r.stderr}")
+    os.replace(tmp, TENSORS)
+    return r.stderr
+
+
 def build(verbose: bool = False) -> str:
     os.makedirs(OUT_DIR, exist_ok=True)
     srcs = sorted(f for f in os.listdir(CSRC) if f.endswith(".hip"))
     objs = [os.path.join(OUT_DIR, f[:-4] + ".o") for f in srcs]
-    with cf.ThreadPoolExecutor(max_workers=min(8, len(srcs))) as ex:
+    with cf.ThreadPoolExecutor(max_workers=8) as ex:
+        tensors = ex.submit(_compile_tensors)
         futs = {ex.submit(_compile, os.path.join(CSRC, s), o): s for s, o in zip(srcs, objs)}
         for fut in cf.as_completed(futs):
             msg = fut.result()
             if verbose and msg:
                 print(f"[{futs[fut]}]\n{msg}", file=sys.stderr)
+        tensors.result()
     tmp = LIB + ".tmp"
     cmd = [HIPCC, "--offload-arch=gfx950", "-shared", "-fPIC", "-o", tmp, *objs]
     r = subprocess.run(cmd, capture_output=True, text=True)

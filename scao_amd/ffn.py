@@ -48,7 +48,8 @@ def _check(x: Tensor, w_gate: Tensor, w_up: Tensor, w_down: Tensor, activation: 
 
 def _rows(t: Tensor) -> Tensor:
     """2-D with unit column stride and rows that do not overlap."""
-    t = t.reshape(-1, t.shape[-1])
+    if t.dim() != 2:
+        t = t.reshape(-1, t.shape[-1])
     if t.stride(1) != 1 or (t.shape[0] > 1 and t.stride(0) < t.shape[1]):
         t = t.contiguous()
     return t
@@ -73,9 +74,8 @@ def _forward(x: Tensor, w_gate: Tensor, w_up: Tensor, w_down: Tensor, act: int, 
     y = torch.empty(x.shape, dtype=x.dtype, device=dev)
     saved = _bytes(lib.scao_ffn_saved_bytes(at), dev) if save else None
     work = _bytes(lib.scao_ffn_forward_workspace(at, int(save)), dev)
-    with torch.cuda.device(dev):
-        L.call("scao_ffn_forward", at, y.data_ptr(), saved.data_ptr() if save else None,
-               work.data_ptr(), L.stream_ptr(dev))
+    L.call_on(dev, "scao_ffn_forward", at, y.data_ptr(), saved.data_ptr() if save else None,
+              work.data_ptr())
     return y, saved
 
 
@@ -90,24 +90,24 @@ class _GatedFFN(torch.autograd.Function):
     @staticmethod
     @once_differentiable
     def backward(ctx, dy):
+        # (hooks on saved tensors may have moved them: their addresses are new)
         x, w_gate, w_up, w_down, saved = ctx.saved_tensors
-        dy, dev = _rows(dy), x.device
+        dy, dev, dtype = _rows(dy), x.device, x.dtype
         (f, d), need = w_gate.shape, ctx.needs_input_grad
         desc = _desc(x, w_gate, w_up, w_down, ctx.act)
         at = desc.ctypes.data
 
         def new(want, *shape):
-            return torch.empty(shape, dtype=x.dtype, device=dev) if want else None
+            return torch.empty(shape, dtype=dtype, device=dev) if want else None
 
         dx, ddown = new(need[0], x.shape[0], d), new(need[3], d, f)
         dgate, dup = new(need[1], f, d), new(need[2], f, d)
         grads = need[0] | need[1] << 1 | need[2] << 2 | need[3] << 3
-        work = _bytes(L.lib().scao_ffn_backward_workspace(at, dy.data_ptr(), dy.stride(0), grads),
-                      dev)
-        with torch.cuda.device(dev):
-            L.call("scao_ffn_backward", at, dy.data_ptr(), dy.stride(0), saved.data_ptr(),
-                   *(None if t is None else t.data_ptr() for t in (dx, dgate, dup, ddown)),
-                   work.data_ptr(), L.stream_ptr(dev))
+        dy_at, ld = dy.data_ptr(), dy.stride(0)
+        work = _bytes(L.lib().scao_ffn_backward_workspace(at, dy_at, ld, grads), dev)
+        L.call_on(dev, "scao_ffn_backward", at, dy_at, ld, saved.data_ptr(),
+                  *[None if t is None else t.data_ptr() for t in (dx, dgate, dup, ddown)],
+                  work.data_ptr())
         return dx, dgate, dup, ddown, None
 
 
@@ -133,7 +133,7 @@ def gated_ffn(x: Tensor, w_gate: Tensor, w_up: Tensor, w_down: Tensor,
         y = _GatedFFN.apply(x2, wg, wu, wd, act)
     else:
         y = _forward(x2, wg, wu, wd, act, False)[0]
-    return y.view(x.shape)
+    return y if x.dim() == 2 else y.view(x.shape)
 
 
 class GatedFFN(nn.Module):

@@ -14,8 +14,8 @@ a host synchronisation and without a copy of the tensors' table.
 
 from __future__ import annotations
 
+import ctypes
 import math
-import operator
 from typing import Iterable, Union
 
 import numpy as np
@@ -28,34 +28,27 @@ from .engine import require_hip
 _NORM_CODE = {1.0: 1, 2.0: 2, math.inf: 0}
 
 
-def _gradients(parameters: Union[Tensor, Iterable[Tensor]]) -> list:
-    if isinstance(parameters, Tensor):
-        parameters = [parameters]
-    return [g for p in parameters if (g := p.grad) is not None]
-
-
-# A model has hundreds of gradients, and each attribute of a tensor costs about
-# 70 ns of host time: every property is read once, for all of them in one go.
-_dtype, _is_sparse = operator.attrgetter("dtype"), operator.attrgetter("is_sparse")
-
-
-def _check(grads: list, norm_type: float, scale: float) -> tuple:
-    """(the norm's code, the gradients' dtype codes, whether all are contiguous)"""
+def _check_scalars(norm_type: float, scale: float) -> int:
     code = _NORM_CODE.get(float(norm_type))
     if code is None:
         raise ValueError(f"norm_type must be 1, 2 or inf (got {norm_type})")
     if not 0.0 < scale < math.inf:
         raise ValueError(f"scale must be positive and finite (got {scale})")
-    devices = set(map(Tensor.get_device, grads))
-    if len(devices) > 1 or -1 in devices:
-        for g in grads:
-            require_hip(g, "gradient")
-        raise RuntimeError(f"all gradients must be on one device (got devices {sorted(devices)})")
-    types = list(map(L.DTYPE_CODE.get, map(_dtype, grads)))
-    if None in types or any(map(_is_sparse, grads)):
-        raise TypeError("gradients must be dense float32, bfloat16 or float16 tensors (got "
-                        f"{sorted({f'{g.dtype} {g.layout}' for g in grads})})")
-    return code, types, all(map(Tensor.is_contiguous, grads))
+    return code
+
+
+def _irregular(parameters: list) -> list:
+    """The gradients of a list that ``_lib.tensors().gradients`` does not take, checked."""
+    grads = [g for p in parameters if (g := p.grad) is not None]
+    for g in grads:
+        require_hip(g, "gradient")
+        if g.device != grads[0].device:
+            raise RuntimeError("all gradients must be on one device "
+                               f"({g.device} vs {grads[0].device})")
+        if g.layout != torch.strided or g.dtype not in L.DTYPE_CODE:
+            raise TypeError("gradients must be dense float32, bfloat16 or float16 tensors "
+                            f"(got {g.dtype}, {g.layout})")
+    return grads
 
 
 def _dense(g: Tensor) -> bool:
@@ -63,19 +56,39 @@ def _dense(g: Tensor) -> bool:
     return g.is_contiguous() or torch.ops.aten.is_non_overlapping_and_dense(g)
 
 
-def _launch(name: str, grads: list, types: list, code: int, *scalars: float) -> Tensor:
-    n = len(grads)
-    table = np.empty(n, dtype=L.TENSOR_DESC)
-    table["data"] = list(map(Tensor.data_ptr, grads))
-    table["numel"] = list(map(Tensor.numel, grads))
-    table["dtype"] = types
-    at = table.ctypes.data
-    dev = grads[0].device
-    norm = torch.empty((), dtype=torch.float32, device=dev)
-    work = torch.empty(L.lib().scao_grad_norm_workspace(at, n), dtype=torch.uint8, device=dev)
-    with torch.cuda.device(dev):
-        L.call(name, at, n, code, *scalars, norm.data_ptr(), work.data_ptr(), L.stream_ptr(dev))
-    return norm
+class _Gradients:
+    """The table of the parameters' gradients; those with gaps in their memory
+    take part through a contiguous copy."""
+
+    def __init__(self, parameters: Union[Tensor, Iterable[Tensor]]):
+        if isinstance(parameters, Tensor):
+            parameters = [parameters]
+        elif not isinstance(parameters, (list, tuple)):
+            parameters = list(parameters)
+        self.copies = []   # (gradient, its copy)
+        found = L.tensors().gradients(parameters)
+        if found is not None:
+            index, self.count, self._table = found
+            self.device = torch.device("cuda", index) if self.count else None
+            self.at = ctypes.cast(self._table, ctypes.c_void_p).value
+            return
+        grads = _irregular(parameters)
+        flat = [g if _dense(g) else g.contiguous() for g in grads]
+        self.copies = [(g, f) for g, f in zip(grads, flat) if f is not g]
+        self.count, self.device = len(flat), flat[0].device
+        self._table = np.empty(self.count, dtype=L.TENSOR_DESC)
+        for field, of in (("data", Tensor.data_ptr), ("numel", Tensor.numel),
+                          ("dtype", lambda g: L.DTYPE_CODE[g.dtype])):
+            self._table[field] = [of(g) for g in flat]
+        self.at, self._flat = self._table.ctypes.data, flat
+
+    def launch(self, name: str, code: int, *scalars: float) -> Tensor:
+        norm = torch.empty((), dtype=torch.float32, device=self.device)
+        work = torch.empty(L.lib().scao_grad_norm_workspace(self.at, self.count),
+                           dtype=torch.uint8, device=self.device)
+        L.call_on(self.device, name, self.at, self.count, code, *scalars, norm.data_ptr(),
+                  work.data_ptr())
+        return norm
 
 
 @torch.no_grad()
@@ -84,13 +97,10 @@ def global_grad_norm(parameters: Union[Tensor, Iterable[Tensor]], norm_type: flo
     """``scale`` times the ``norm_type`` norm (1, 2 or inf) of all gradients of
     ``parameters`` as one vector: a 0-dim float32 tensor on their device
     (summed in double), a zero on the CPU where no parameter has a gradient."""
-    grads = _gradients(parameters)
-    code, types, contiguous = _check(grads, norm_type, scale)
-    if not grads:
+    code, grads = _check_scalars(norm_type, scale), _Gradients(parameters)
+    if not grads.count:
         return torch.tensor(0.0)
-    if not contiguous:
-        grads = [g if _dense(g) else g.contiguous() for g in grads]
-    return _launch("scao_grad_norm", grads, types, code, float(scale))
+    return grads.launch("scao_grad_norm", code, float(scale))
 
 
 @torch.no_grad()
@@ -107,34 +117,27 @@ def clip_grad_norm_(parameters: Union[Tensor, Iterable[Tensor]], max_norm: float
 
     Gradients may have any type of float32, bfloat16 and float16, any start and
     any strides, but no two may share memory (ValueError)."""
-    grads = _gradients(parameters)
-    code, types, contiguous = _check(grads, norm_type, scale)
-    max_norm = float(max_norm)
+    code, max_norm = _check_scalars(norm_type, scale), float(max_norm)
     if not max_norm >= 0.0:
         raise ValueError(f"max_norm must be at least 0 (got {max_norm})")
-    if not grads:
+    grads = _Gradients(parameters)
+    if not grads.count:
         return torch.tensor(0.0)
-    flat = grads
-    if not contiguous:
-        flat = [g if _dense(g) else g.contiguous() for g in grads]
-        if any(f is not g and torch._debug_has_internal_overlap(g) == 1
-               for f, g in zip(flat, grads)):
-            raise ValueError("a gradient whose elements share memory (an expanded tensor) "
-                             "cannot be scaled in place")
+    if any(torch._debug_has_internal_overlap(g) == 1 for g, _ in grads.copies):
+        raise ValueError("a gradient whose elements share memory (an expanded tensor) cannot be "
+                         "scaled in place")
     if error_if_nonfinite:
-        norm = float(_launch("scao_grad_norm", flat, types, code, float(scale)))
+        norm = float(grads.launch("scao_grad_norm", code, float(scale)))
         if not math.isfinite(norm):
             raise RuntimeError(f"the gradients' norm of order {float(norm_type)} is {norm}, so "
                                "they cannot be clipped; pass error_if_nonfinite=False to scale "
                                "them by it anyway")
     try:
-        norm = _launch("scao_grad_clip", flat, types, code, float(scale), max_norm)
+        norm = grads.launch("scao_grad_clip", code, float(scale), max_norm)
     except L.ScaoLibError as e:
         if "share memory" in str(e):
             raise ValueError(str(e)) from None
         raise
-    if not contiguous:
-        for g, f in zip(grads, flat):
-            if f is not g:
-                g.copy_(f)
+    for g, copy in grads.copies:
+        g.copy_(copy)
     return norm

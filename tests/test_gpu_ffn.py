@@ -184,6 +184,18 @@ def test_shapes_of_x_and_views(hip_device):
     _compare(dict(dx=x3.grad.transpose(0, 1).reshape(60, 32)), want, torch.bfloat16)
 
 
+def test_saved_tensors_that_moved(hip_device):
+    """Hooks that keep what the backward pass needs somewhere else."""
+    x, gate, up, down, dy = _inputs(hip_device, 33, 40, 56, torch.bfloat16, packed=True, pad=8)
+    want = _run(x, gate, up, down, dy, "silu")
+    leaves = [t.detach().requires_grad_() for t in (x, gate, up, down)]
+    with torch.autograd.graph.save_on_cpu():
+        y = scao_amd.gated_ffn(*leaves)
+    grads = torch.autograd.grad(y, leaves, dy)
+    for k, g in zip(("dx", "dgate", "dup", "ddown"), grads):
+        assert torch.equal(g, want[k])
+
+
 def test_nothing_to_do(hip_device):
     for t, d, f in ((0, 8, 16), (3, 8, 0), (3, 0, 16)):
         leaves = [torch.zeros(s, device=hip_device, requires_grad=True)
