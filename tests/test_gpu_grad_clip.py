@@ -203,3 +203,24 @@ def test_refusals(hip_device):
     assert clip([], 1.0).item() == 0.0
     assert clip([torch.nn.Parameter(torch.zeros(3, device=hip_device))], 1.0).item() == 0.0
     assert clip(_params([g[:0]]), 1.0).item() == 0.0
+
+
+@pytest.mark.parametrize("dtype", list(ULP))
+def test_more_than_the_caches_hold(hip_device, dtype):
+    """Over 512 MiB, in tensors of odd sizes, one past 2^27 elements."""
+    size = torch.finfo(dtype).bits // 8
+    sizes = [1, 70001, (1 << 27) + 12345, 3, (400 << 20) // size + 1]
+    flat = torch.empty(sum(sizes), dtype=dtype, device=hip_device)
+    period = _normal(hip_device, 0, 100003, dtype=dtype)
+    for at in range(0, flat.numel(), 100003):
+        n = min(100003, flat.numel() - at)
+        flat[at:at + n] = period[:n]
+    norm = flat.double().norm().item() if size == 2 else sum(
+        c.double().square().sum().item() for c in flat.split(1 << 26)) ** 0.5
+    want = (period.double() * min(1.0, 0.5 / (norm + 1e-6)))
+    got = scao_amd.clip_grad_norm_(_params(list(flat.split(sizes))), 0.5)
+    assert abs(got.item() - norm) <= 2e-7 * norm
+    for at in range(0, flat.numel(), 100003):
+        n = min(100003, flat.numel() - at)
+        err = (flat[at:at + n].double() - want[:n]).abs()
+        assert bool((err <= want[:n].abs() * (ULP[dtype] + 1.3e-7) + TINY[dtype]).all())
