@@ -222,20 +222,23 @@ def lib():
     return _lib
 
 
-_tensors = None
+_torch_host = None
 
 
-def tensors():
-    """The module ``scao_amd._tensors`` (csrc/tensors.cpp)."""
-    global _tensors
-    if _tensors is None:
+def torch_host():
+    """The module ``scao_amd._torch_host`` (csrc/torch_host.cpp), bound to the
+    library's entry points."""
+    global _torch_host
+    if _torch_host is None:
         try:
-            from . import _tensors as module
+            from . import _torch_host as module
         except ImportError as e:
-            raise ScaoLibError(f"scao_amd: {HERE}/_tensors.so is missing or does not fit this "
+            raise ScaoLibError(f"scao_amd: {HERE}/_torch_host.so is missing or does not fit this "
                                f"torch ({e}). Build it with `python -m scao_amd.build`.") from None
-        _tensors = module
-    return _tensors
+        names = ("scao_last_error", *(n for n in TRAIN_SIGNATURES if n.startswith("scao_ffn")))
+        module.bind({n: ctypes.cast(getattr(lib(), n), _VP).value for n in names})
+        _torch_host = module
+    return _torch_host
 
 
 def call(name: str, *args) -> None:

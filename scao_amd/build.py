@@ -6,8 +6,8 @@ parallel, and linked into one shared object exporting the C ABI declared in
 fused multiply-adds are written explicitly where the reference rounds once.
 Packed fp32 instructions are disabled for all device code.
 
-``csrc/tensors.cpp`` is host code against torch's headers: the Python module
-``scao_amd._tensors`` (``scao_amd/_tensors.so``), built by g++.
+``csrc/torch_host.cpp`` is host code against torch's headers: the Python module
+``scao_amd._torch_host`` (``scao_amd/_torch_host.so``), built by g++.
 """
 
 from __future__ import annotations
@@ -23,7 +23,8 @@ ROOT = os.path.dirname(HERE)
 CSRC = os.path.join(HERE, "csrc")
 OUT_DIR = os.path.join(HERE, "_lib")
 LIB = os.path.join(OUT_DIR, "libscao_amd.so")
-TENSORS = os.path.join(HERE, "_tensors.so")
+TORCH_HOST = os.path.join(HERE, "_torch_host.so")
+ROCM = os.path.dirname(os.path.dirname(os.environ.get("HIPCC", "/opt/rocm/bin/hipcc")))
 CXX = os.environ.get("CXX", "g++")
 HIPCC = os.environ.get("HIPCC", "/opt/rocm/bin/hipcc")
 
@@ -44,20 +45,22 @@ def _compile(src: str, obj: str) -> str:
     return "\n".join(ln for ln in r.stderr.splitlines() if noise not in ln and ln.strip())
 
 
-def _compile_tensors() -> str:
+def _compile_torch_host() -> str:
     from torch._C import _GLIBCXX_USE_CXX11_ABI as abi
     from torch.utils import cpp_extension
-    # (the CPU's include paths: no HIP type is used)
-    inc = [f"-I{d}" for d in (*cpp_extension.include_paths(), sysconfig.get_path("include"))]
-    lib = os.path.join(os.path.dirname(os.path.dirname(cpp_extension.__file__)), "lib")
-    tmp = TENSORS + ".tmp"
+    root = os.path.dirname(os.path.dirname(cpp_extension.__file__))
+    inc = [f"-I{d}" for d in (os.path.join(root, "include"),
+                              os.path.join(root, "include", "torch", "csrc", "api", "include"),
+                              sysconfig.get_path("include"), os.path.join(ROCM, "include"))]
+    tmp = TORCH_HOST + ".tmp"
     cmd = [CXX, "-O2", "-std=c++17", "-fPIC", "-shared", f"-D_GLIBCXX_USE_CXX11_ABI={int(abi)}",
-           *inc, os.path.join(CSRC, "tensors.cpp"), "-o", tmp, f"-L{lib}", "-ltorch_python",
-           "-ltorch_cpu", "-lc10"]
+           "-DUSE_ROCM", "-D__HIP_PLATFORM_AMD__", *inc, os.path.join(CSRC, "torch_host.cpp"),
+           "-o", tmp, "-L" + os.path.join(root, "lib"), "-ltorch_python", "-ltorch_cpu",
+           "-lc10_hip", "-lc10"]
     r = subprocess.run(cmd, capture_output=True, text=True)
     if r.returncode != 0:
-        raise RuntimeError(f"{CXX} failed for tensors.cpp:\n{r.stderr}")
-    os.replace(tmp, TENSORS)
+        raise RuntimeError(f"{CXX} failed for torch_host.cpp:\n{r.stderr}")
+    os.replace(tmp, TORCH_HOST)
     return r.stderr
 
 
@@ -66,13 +69,13 @@ def build(verbose: bool = False) -> str:
     srcs = sorted(f for f in os.listdir(CSRC) if f.endswith(".hip"))
     objs = [os.path.join(OUT_DIR, f[:-4] + ".o") for f in srcs]
     with cf.ThreadPoolExecutor(max_workers=8) as ex:
-        tensors = ex.submit(_compile_tensors)
+        torch_host = ex.submit(_compile_torch_host)
         futs = {ex.submit(_compile, os.path.join(CSRC, s), o): s for s, o in zip(srcs, objs)}
         for fut in cf.as_completed(futs):
             msg = fut.result()
             if verbose and msg:
                 print(f"[{futs[fut]}]\n{msg}", file=sys.stderr)
-        tensors.result()
+        torch_host.result()
     tmp = LIB + ".tmp"
     cmd = [HIPCC, "--offload-arch=gfx950", "-shared", "-fPIC", "-o", tmp, *objs]
     r = subprocess.run(cmd, capture_output=True, text=True)

@@ -6,18 +6,17 @@ with the weights in ``nn.Linear``'s layout (gate and up: ``d_ff x d_model``, dow
 ``d_model x d_ff``): the three largest matrices of a layer, whose gradients are
 what ``SCAO`` preconditions.  Both projections, the activation and the product
 are one kernel, the second projection another; a backward pass is four products
-(``scao_ffn_forward``, ``scao_ffn_backward``).  Everything runs on the current
-stream; nothing is kept between calls.
+(``scao_ffn_forward``, ``scao_ffn_backward``, called from csrc/torch_host.cpp as a
+node of torch's graph).  Everything runs on the current stream; nothing is kept
+between calls.
 """
 
 from __future__ import annotations
 
 import math
 
-import numpy as np
 import torch
 from torch import Tensor, nn
-from torch.autograd.function import once_differentiable
 
 from . import _lib as L
 from .engine import require_hip
@@ -55,62 +54,6 @@ def _rows(t: Tensor) -> Tensor:
     return t
 
 
-def _desc(x: Tensor, w_gate: Tensor, w_up: Tensor, w_down: Tensor, act: int) -> np.ndarray:
-    f, d = w_gate.shape
-    return np.array([(x.data_ptr(), w_gate.data_ptr(), w_up.data_ptr(), w_down.data_ptr(),
-                      x.stride(0), w_gate.stride(0), w_up.stride(0), w_down.stride(0),
-                      x.shape[0], d, f, L.DTYPE_CODE[x.dtype], act)], dtype=L.FFN_DESC)
-
-
-def _bytes(n: int, device: torch.device) -> Tensor:
-    return torch.empty(n, dtype=torch.uint8, device=device)
-
-
-def _forward(x: Tensor, w_gate: Tensor, w_up: Tensor, w_down: Tensor, act: int, save: bool):
-    """x is 2-D and no size is zero; (y, what the backward pass needs or None)"""
-    dev = x.device
-    desc = _desc(x, w_gate, w_up, w_down, act)
-    at, lib = desc.ctypes.data, L.lib()
-    y = torch.empty(x.shape, dtype=x.dtype, device=dev)
-    saved = _bytes(lib.scao_ffn_saved_bytes(at), dev) if save else None
-    work = _bytes(lib.scao_ffn_forward_workspace(at, int(save)), dev)
-    L.call_on(dev, "scao_ffn_forward", at, y.data_ptr(), saved.data_ptr() if save else None,
-              work.data_ptr())
-    return y, saved
-
-
-class _GatedFFN(torch.autograd.Function):
-    @staticmethod
-    def forward(ctx, x, w_gate, w_up, w_down, act):
-        y, saved = _forward(x, w_gate, w_up, w_down, act, True)
-        ctx.save_for_backward(x, w_gate, w_up, w_down, saved)
-        ctx.act = act
-        return y
-
-    @staticmethod
-    @once_differentiable
-    def backward(ctx, dy):
-        # (hooks on saved tensors may have moved them: their addresses are new)
-        x, w_gate, w_up, w_down, saved = ctx.saved_tensors
-        dy, dev, dtype = _rows(dy), x.device, x.dtype
-        (f, d), need = w_gate.shape, ctx.needs_input_grad
-        desc = _desc(x, w_gate, w_up, w_down, ctx.act)
-        at = desc.ctypes.data
-
-        def new(want, *shape):
-            return torch.empty(shape, dtype=dtype, device=dev) if want else None
-
-        dx, ddown = new(need[0], x.shape[0], d), new(need[3], d, f)
-        dgate, dup = new(need[1], f, d), new(need[2], f, d)
-        grads = need[0] | need[1] << 1 | need[2] << 2 | need[3] << 3
-        dy_at, ld = dy.data_ptr(), dy.stride(0)
-        work = _bytes(L.lib().scao_ffn_backward_workspace(at, dy_at, ld, grads), dev)
-        L.call_on(dev, "scao_ffn_backward", at, dy_at, ld, saved.data_ptr(),
-                  *[None if t is None else t.data_ptr() for t in (dx, dgate, dup, ddown)],
-                  work.data_ptr())
-        return dx, dgate, dup, ddown, None
-
-
 def gated_ffn(x: Tensor, w_gate: Tensor, w_up: Tensor, w_down: Tensor,
               activation: str = "silu") -> Tensor:
     """``(f(x w_gate^T) * (x w_up^T)) w_down^T`` with f one of ``silu``, ``gelu``,
@@ -127,12 +70,7 @@ def gated_ffn(x: Tensor, w_gate: Tensor, w_up: Tensor, w_down: Tensor,
     if x.numel() == 0 or w_gate.numel() == 0:
         # no token, or a sum over nothing: zeros, with gradients that are zeros
         return ((x @ w_gate.t()) * (x @ w_up.t())) @ w_down.t()
-    x2, wg, wu, wd = _rows(x), _rows(w_gate), _rows(w_up), _rows(w_down)
-    if torch.is_grad_enabled() and (x.requires_grad or w_gate.requires_grad or w_up.requires_grad
-                                    or w_down.requires_grad):
-        y = _GatedFFN.apply(x2, wg, wu, wd, act)
-    else:
-        y = _forward(x2, wg, wu, wd, act, False)[0]
+    y = L.torch_host().gated_ffn(_rows(x), _rows(w_gate), _rows(w_up), _rows(w_down), act)
     return y if x.dim() == 2 else y.view(x.shape)
 
 

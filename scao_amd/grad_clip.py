@@ -38,7 +38,7 @@ def _check_scalars(norm_type: float, scale: float) -> int:
 
 
 def _irregular(parameters: list) -> list:
-    """The gradients of a list that ``_lib.tensors().gradients`` does not take, checked."""
+    """The gradients of a list that ``_lib.torch_host().gradients`` does not take, checked."""
     grads = [g for p in parameters if (g := p.grad) is not None]
     for g in grads:
         require_hip(g, "gradient")
@@ -66,7 +66,7 @@ class _Gradients:
         elif not isinstance(parameters, (list, tuple)):
             parameters = list(parameters)
         self.copies = []   # (gradient, its copy)
-        found = L.tensors().gradients(parameters)
+        found = L.torch_host().gradients(parameters)
         if found is not None:
             index, self.count, self._table = found
             self.device = torch.device("cuda", index) if self.count else None
