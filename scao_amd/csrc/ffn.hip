@@ -105,8 +105,8 @@ struct Block {
     // the join: a launch, 8 bytes a part and element, and the epilogue's own
     // `moved`, which a tile's end would overlap better
     double moved;
-    double join(int64_t n) const {
-      return n == 1 ? 0.0 : 2 + (8 / 7.4e6 * n * (gated ? 2 : 1) + moved / 5e6) * M * N;
+    double join(int64_t n, double share = 1.0) const {
+      return n == 1 ? 0.0 : 2 + (8 / 7.4e6 * n * (gated ? 2 : 1) + moved / 5e6) * M * N * share;
     }
     bool may_split(int t, int64_t n) const {
       return n == 1 || (n * 2 <= steps && tiles(t) * n <= 2048);
@@ -117,20 +117,32 @@ struct Block {
         {256, 1.15, 1.50, 4.9}, {512, 0.62, 1.14, 5.2}, {512, 0.56, 0.70, 3.0}, {768, 0.44, 0.96, 1.7}};
     return costs[tile];
   }
-  static double choose(const Shape& s, bool tokens, int& tile, int& splits) {
+  // How a product is cut: its tile, how many tiles run in one piece and in how
+  // many parts the others.  Either all of them are split, or those that do not
+  // fill a last round: 777 tokens, 2048 x 11008, gate and up: 344 tiles on 256
+  // CUs, the 88 of the second round in two parts.
+  struct Cut {
+    int tile = 0, whole = 0, splits = 1;
+  };
+  static double choose(const Shape& s, bool tokens, Cut& cut) {
     double best = 1e30;
     for (int t = 0; t < (tokens ? FFN_TILES : FFN_64x128); ++t) {
       const Cost& c = cost(t);
+      const int64_t tiles = s.tiles(t);
       for (int64_t n : {1, 2, 3, 4, 6, 8, 12, 16, 24, 32}) {
         if (!s.may_split(t, n)) break;
-        const int64_t per = (s.steps + n - 1) / n, groups = s.tiles(t) * n;
-        const int64_t rest = groups % c.slots;
-        double us = (groups / c.slots) * (per * c.full + c.ends) + s.join(n);
-        if (rest) us += per * c.step(rest) + c.ends;
-        if (us < best) {
-          best = us;
-          tile = t;
-          splits = (int)n;
+        const int64_t per = (s.steps + n - 1) / n;
+        for (int64_t whole : {(int64_t)0, tiles / c.slots * c.slots}) {
+          if (whole && (n == 1 || whole == tiles)) continue;
+          const int64_t groups = (tiles - whole) * n, last = groups % c.slots;
+          double us = whole / c.slots * (s.steps * c.full + c.ends) +
+                      groups / c.slots * (per * c.full + c.ends) +
+                      s.join(n, (double)(tiles - whole) / tiles);
+          if (last) us += per * c.step(last) + c.ends;
+          if (us < best) {
+            best = us;
+            cut = {t, n == 1 ? (int)tiles : (int)whole, (int)n};
+          }
         }
       }
     }
@@ -138,7 +150,7 @@ struct Block {
   }
   // two products in one launch: `a` workgroups of one length, then as many of
   // the other's as fit where these leave room
-  static double choose_pair(const Shape& x, const Shape& y, int& tile, int& nx, int& ny) {
+  static double choose_pair(const Shape& x, const Shape& y, Cut& cx, Cut& cy) {
     double best = 1e30;
     for (int t : {FFN_256x256, FFN_128x128}) {
       const Cost& c = cost(t);
@@ -164,9 +176,8 @@ struct Block {
           us += x.join(n) + y.join(m);
           if (us < best) {
             best = us;
-            tile = t;
-            nx = (int)n;
-            ny = (int)m;
+            cx = {t, 0, (int)n};
+            cy = {t, 0, (int)m};
           }
         }
       }
@@ -192,49 +203,50 @@ struct Block {
     return Shape{o.M, o.N, (int64_t)o.nseg * ((o.K + FFN_BK - 1) / FFN_BK), kind == FFN_GATE_UP,
                  s.dtype == SCAO_F32 ? 2 * bytes : bytes};
   }
-  // the tiles' counts, and room for the parts of a split product
-  void cut(int kind, int tile, FfnOperands& o, FfnEpilogue& e) {
-    const int cols = kind == FFN_GATE_UP ? FFN_BN[tile] / 2 : FFN_BN[tile];
-    o.tiles_m = (o.M + FFN_BM[tile] - 1) / FFN_BM[tile];
-    o.tiles_n = (o.N + cols - 1) / cols;
-    e.partial = nullptr;
-    if (o.splits > 1)
-      e.partial = (float*)ws.take((int64_t)o.splits * o.tiles_m * o.tiles_n * FFN_BM[tile] *
-                                  FFN_BN[tile] * 4);
-    peak = std::max(peak, ws.used);
-  }
   struct Product {
     int kind;
     FfnOperands o;
     FfnEpilogue e;
   };
+  // the tiles' counts, and room for the parts of a split product
+  void cut(Product& p, const Cut& c) {
+    FfnOperands& o = p.o;
+    const int cols = p.kind == FFN_GATE_UP ? FFN_BN[c.tile] / 2 : FFN_BN[c.tile];
+    o.tiles_m = (o.M + FFN_BM[c.tile] - 1) / FFN_BM[c.tile];
+    o.tiles_n = (o.N + cols - 1) / cols;
+    o.splits = c.splits;
+    o.whole = c.splits == 1 ? o.tiles() : c.whole;
+    p.e.partial = nullptr;
+    if (o.whole < o.tiles())
+      p.e.partial = (float*)ws.take((int64_t)o.splits * (o.tiles() - o.whole) * FFN_BM[c.tile] *
+                                    FFN_BN[c.tile] * 4);
+    peak = std::max(peak, ws.used);
+  }
   void run(Product& p) {
     const int64_t at = ws.used;   // the parts' room is given back
-    int tile = 0;
-    choose(shape(p.kind, p.o), p.kind != FFN_DW, tile, p.o.splits);
-    cut(p.kind, tile, p.o, p.e);
+    Cut c;
+    choose(shape(p.kind, p.o), p.kind != FFN_DW, c);
+    cut(p, c);
     ws.used = at;
-    if (!dry) launchers(s.dtype).product(p.kind, tile, p.o, p.e, st);
+    if (!dry) launchers(s.dtype).product(p.kind, c.tile, p.o, p.e, st);
   }
   // dh or dx, and a dW that does not need it
   void run(Product& p, Product& w) {
     const Shape x = shape(p.kind, p.o), y = shape(w.kind, w.o);
-    int tile = 0, nx = 0, ny = 0, t, n;
-    const double apart = choose(x, true, t, n) + choose(y, false, t, n) + 3;
+    Cut c, cp, cw;
+    const double apart = choose(x, true, c) + choose(y, false, c) + 3;
     // large products lose a few per cent side by side, two working sets in an L2:
     // 8192 tokens, 4096 x 14336, the whole pass 6560 us apart and 6700 in pairs
-    if (1.06 * choose_pair(x, y, tile, nx, ny) > apart) {
+    if (1.06 * choose_pair(x, y, cp, cw) > apart) {
       run(p);
       run(w);
       return;
     }
     const int64_t at = ws.used;
-    p.o.splits = nx;
-    w.o.splits = ny;
-    cut(p.kind, tile, p.o, p.e);
-    cut(w.kind, tile, w.o, w.e);
+    cut(p, cp);
+    cut(w, cw);
     ws.used = at;
-    if (!dry) launchers(s.dtype).pair(p.kind, tile, p.o, p.e, w.o, w.e, st);
+    if (!dry) launchers(s.dtype).pair(p.kind, cp.tile, p.o, p.e, w.o, w.e, st);
   }
   int64_t peak = 0;
   int64_t need() { return std::max(peak, ws.used); }

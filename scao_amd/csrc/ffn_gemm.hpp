@@ -133,11 +133,14 @@ struct FfnOperands {
   int64_t lda, ldb;
   int M, N, K;          // C's sizes (N: one projection's with GATED), k of one segment
   int nseg;
-  int splits;           // parts of the k steps of all segments
   int tiles_m, tiles_n;
+  int whole;            // tiles that run in one piece, the others in `splits`
+  int splits;           // parts of the k steps of all segments
+  __host__ __device__ int tiles() const { return tiles_m * tiles_n; }
+  __host__ __device__ int groups() const { return whole + (tiles() - whole) * splits; }
 };
 
-// The tile of workgroup `b`.  Consecutive workgroups go to different XCDs, each
+// The place of tile `b`.  Consecutive workgroups go to different XCDs, each
 // with an L2 of its own: the tiles are dealt out so that one XCD gets a
 // contiguous piece of an order that walks C in bands of 8 tile rows.
 __device__ __forceinline__ void tile_of(int b, int tm, int tn, int& m, int& n) {
@@ -155,7 +158,8 @@ __device__ __forceinline__ void tile_of(int b, int tm, int tn, int& m, int& n) {
 // up rows; each wave's fragments are half of either.
 template <int BM, int BN, int WM, int WN, int LA, int LB, bool F16, bool GATED>
 struct Gemm {
-  static constexpr int NW = WM * WN, THREADS = NW * 64, BM_ = BM;
+  static constexpr int NW = WM * WN, THREADS = NW * 64, BM_ = BM, BN_ = BN;
+  static constexpr int FRAGS = BM / 16 * (BN / 16);   // of 16 x 16 sums
   static constexpr int MI = BM / WM / 16, NJ = BN / WN / 16;
   using TA = Tile<LA, BM, NW>;
   using TB = Tile<LB, BN, NW>;

@@ -319,30 +319,27 @@ typedef __attribute__((address_space(1))) v4f gv4f_a16;
 template <class G, int TYPE, int EPI>
 __device__ __forceinline__ void ffn_tile(char* smem, const FfnOperands& o, const FfnEpilogue& e,
                                          int block) {
-  const int tiles = o.tiles_m * o.tiles_n;
-  const int part = block / tiles;
+  const bool split = block >= o.whole;
+  const int rest = o.tiles() - o.whole;
+  const int part = split ? (block - o.whole) / rest : 0;
+  const int tile = block - part * rest;
   int tm, tn;
-  tile_of(block - part * tiles, o.tiles_m, o.tiles_n, tm, tn);
+  tile_of(tile, o.tiles_m, o.tiles_n, tm, tn);
   G g(o, (lchar*)smem, tm, tn);
   const int steps = o.nseg * ((o.K + FFN_BK - 1) / FFN_BK);
-  const int per = (steps + o.splits - 1) / o.splits;
+  const int per = split ? (steps + o.splits - 1) / o.splits : steps;
   v4f acc[G::MI][G::NJ];
   g.run(part * per, min(steps, part * per + per), acc);
 
   const int lane = g.lane, dm = lane & 15, dn = 4 * (lane >> 4);
-  if (o.splits > 1) {
-    // C's fragments in order, a projection's behind the other's (GATED)
-    constexpr int H = EPI == EPI_GATED ? 2 : 1;
-    const int64_t fj = o.tiles_n * (G::COLS_N / 16), fi = o.tiles_m * (int64_t)(G::BM_ / 16);
-    gv4f_a16* to = (gv4f_a16*)e.partial + part * fi * fj * H * 64;
+  if (split) {   // a part's sums: tile after tile, a tile's fragments in order
+    gv4f_a16* to = (gv4f_a16*)e.partial +
+                   ((int64_t)part * rest + (tile - o.whole)) * (G::FRAGS * 64) + lane;
 #pragma unroll
     for (int i = 0; i < G::MI; ++i)
 #pragma unroll
-      for (int j = 0; j < G::NJ; ++j) {
-        const int half = EPI == EPI_GATED && j >= G::NJ / 2;
-        const int n = g.n0 + g.frag_n(j) - half * G::COLS_N;
-        to[(((g.m0 + g.frag_m(i)) / 16 + half * fi) * fj + n / 16) * 64 + lane] = acc[i][j];
-      }
+      for (int j = 0; j < G::NJ; ++j)
+        to[(g.frag_m(i) / 16 * (G::BN_ / 16) + g.frag_n(j) / 16) * 64] = acc[i][j];
     return;
   }
   // pairs of fragments next to each other where a wave has them
@@ -455,21 +452,28 @@ __global__ __launch_bounds__(GA::THREADS, 2) void k_ffn_pair(const FfnOperands o
   else ffn_tile<GB, TYPE, EPI_B>(smem, ob, eb, b);
 }
 
-// The parts of a split product, added in order, and its epilogue: a wave takes
-// a fragment.
-template <int TYPE, int EPI>
-__global__ __launch_bounds__(256) void k_ffn_join(const FfnEpilogue e, int splits, int fi, int fj) {
-  constexpr int H = EPI == EPI_GATED ? 2 : 1;
+// The parts of a split product's tiles, added in order, and their epilogue: a
+// wave takes a fragment (GATED: one of either projection).
+template <class G, int TYPE, int EPI>
+__global__ __launch_bounds__(256) void k_ffn_join(const FfnOperands o, const FfnEpilogue e) {
+  constexpr int FJ = G::COLS_N / 16, FRAGS = G::BM_ / 16 * FJ;   // of C in a tile
   const int64_t frag = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6);
-  if (frag >= (int64_t)fi * fj) return;
-  const int lane = threadIdx.x & 63;
-  const int m = (int)(frag / fj) * 16 + (lane & 15), n = (int)(frag % fj) * 16 + 4 * (lane >> 4);
-  const gv4f_a16* p = (const gv4f_a16*)e.partial + frag * 64 + lane;
-  const int64_t all = (int64_t)fi * fj * 64;
+  const int rest = o.tiles() - o.whole;
+  if (frag >= (int64_t)rest * FRAGS) return;
+  const int lane = threadIdx.x & 63, tile = (int)(frag / FRAGS), in = (int)(frag % FRAGS);
+  int tm, tn;
+  tile_of(o.whole + tile, o.tiles_m, o.tiles_n, tm, tn);
+  const int m = tm * G::BM_ + in / FJ * 16 + (lane & 15);
+  const int n = tn * G::COLS_N + in % FJ * 16 + 4 * (lane >> 4);
+  if (m - (lane & 15) >= o.M || n - 4 * (lane >> 4) >= e.cols) return;
+  // in the tile's own order of fragments an up fragment follows the gate's row
+  const gv4f_a16* p = (const gv4f_a16*)e.partial +
+                      ((int64_t)tile * G::FRAGS + in / FJ * (G::BN_ / 16) + in % FJ) * 64 + lane;
+  const int64_t all = (int64_t)rest * G::FRAGS * 64;
   v4f a = {0.f, 0.f, 0.f, 0.f}, b = a;
-  for (int s = 0; s < splits; ++s) {
-    a += p[s * all * H];
-    if (EPI == EPI_GATED) b += p[s * all * H + all];
+  for (int s = 0; s < o.splits; ++s) {
+    a += p[s * all];
+    if (EPI == EPI_GATED) b += p[s * all + FJ * 64];
   }
   if constexpr (EPI == EPI_STORE) {
     epi_store<TYPE>(e, m, n, a);
@@ -547,17 +551,14 @@ using FfnTile =
 
 template <class G, int TYPE, int EPI>
 void launch_join(const FfnOperands& o, const FfnEpilogue& e, hipStream_t st) {
-  if (o.splits == 1) return;
-  const int fi = o.tiles_m * (G::BM_ / 16), fj = o.tiles_n * (G::COLS_N / 16);
-  const int64_t frags = (int64_t)fi * fj;
-  k_ffn_join<TYPE, EPI><<<(int)((frags + 3) / 4), 256, 0, st>>>(e, o.splits, fi, fj);
+  const int64_t frags = (int64_t)(o.tiles() - o.whole) * (G::BM_ / 16) * (G::COLS_N / 16);
+  if (frags) k_ffn_join<G, TYPE, EPI><<<(int)((frags + 3) / 4), 256, 0, st>>>(o, e);
 }
 
 template <int TYPE, int TILE, int WM, int WN, int LA, int LB, int EPI>
 void launch_gemm(const FfnOperands& o, const FfnEpilogue& e, hipStream_t st) {
   using G = FfnTile<TYPE, TILE, WM, WN, LA, LB, EPI>;
-  k_ffn_gemm<G, TYPE, EPI>
-      <<<o.tiles_m * o.tiles_n * o.splits, G::THREADS, 0, st>>>(o, e);
+  k_ffn_gemm<G, TYPE, EPI><<<o.groups(), G::THREADS, 0, st>>>(o, e);
   launch_join<G, TYPE, EPI>(o, e, st);
 }
 
@@ -567,7 +568,7 @@ void launch_pair_tile(const FfnOperands& oa, const FfnEpilogue& ea, const FfnOpe
                       const FfnEpilogue& eb, hipStream_t st) {
   using A = FfnTile<TYPE, TILE, WM, WN, ROWS, COLS, EPI>;
   using B = FfnTile<TYPE, TILE, WM, WN, COLS, COLS, EPI_STORE>;
-  const int na = oa.tiles_m * oa.tiles_n * oa.splits, nb = ob.tiles_m * ob.tiles_n * ob.splits;
+  const int na = oa.groups(), nb = ob.groups();
   const int mixed = EPI == EPI_DACT ? (na < nb ? na : nb) / 8 : 0;
   const int64_t sa = (int64_t)oa.nseg * ((oa.K + FFN_BK - 1) / FFN_BK) / oa.splits;
   const int64_t sb = (int64_t)ob.nseg * ((ob.K + FFN_BK - 1) / FFN_BK) / ob.splits;
