@@ -282,16 +282,20 @@ struct Block {
     return e;
   }
 
-  // Whether the forward pass alone goes without tiles.  bf16, 2048 x 8192: 8
-  // tokens 30 us against 32, 16 tokens 35 against 33; 4096 x 14336: 4 tokens 73
-  // against 78, 16 tokens 93 against 79.  The tiles' operands have to be packed
-  // in fp32 and where rows begin off 16 bytes, which takes longer than the
-  // product: fp32, 4096 x 14336, 64 tokens 394 us against 789.
+  // Whether the forward pass alone goes without tiles: up to 8 tokens, and up to
+  // 64 while the block is small.  us without tiles and with them:
+  //   bf16  2048 x 8192: 8 tokens 28 and 40, 16: 36 and 40, 24: 43 and 38;
+  //         1024 x 2816, 64 tokens: 24 and 26; 4096 x 14336: 4 tokens 78 and 87,
+  //         8: 81 and 82, 12: 88 and 81
+  //   rows off 16 bytes, which tiles have to pack: 1001 x 2049, 32 tokens 32 and
+  //         32; 2049 x 8191: 8 tokens 77 and 85, 12: 86 and 82
+  //   fp32, which tiles have to split: 2048 x 8192, 64 tokens 167 and 224
   bool few() const {
-    if (s.tokens <= 8) return true;
-    return s.tokens <= FFN_FEW_TOKENS &&
-           !(direct(s.w_gate, s.ld_gate, s.f, s.d) && direct(s.w_up, s.ld_up, s.f, s.d) &&
-             direct(s.w_down, s.ld_down, s.d, s.f));
+    if (s.tokens > FFN_FEW_TOKENS) return false;
+    if (s.tokens <= 8 || s.dtype == SCAO_F32) return true;
+    const bool as_is = direct(s.w_gate, s.ld_gate, s.f, s.d) &&
+                       direct(s.w_up, s.ld_up, s.f, s.d) && direct(s.w_down, s.ld_down, s.d, s.f);
+    return s.tokens * s.d * s.f <= (int64_t)1 << (as_is ? 28 : 26);
   }
   // h in the block's type, nothing packed
   int forward_few(void* y) {

@@ -9,6 +9,18 @@
 // are independent loads, U of them in flight at a time.  Rows may start at any
 // element and have any stride; the end of k is taken element by element.  fp32
 // products are six products of bf16 parts, split in registers.
+//
+// HALVES (up to 8 tokens): the 16 rows and 16 columns of a product are 8 output
+// columns and 8 tokens twice, for two different stretches of k; the quarters of
+// the result where both belong together are added.  Twice as many workgroups
+// with half the k each, for projections with few columns (one token, 8192 to 2048
+// in bf16: 128 workgroups of 16 columns 12.0 us, 256 of 8 columns 8.3; 14336 to
+// 4096 has enough, and loses 3 us of 71 in halves).
+//
+// Measured (bf16, weights not in the caches): one token, 4096 x 14336: 72 us,
+// 4.9 TB/s of the 5.7 that a copy reaches; 2048 x 8192: 23 us of which 17.8 are
+// the bytes.  From about 8 tokens on the tokens' operands cost as much address
+// processing as the weights (16 rows of 64 bytes a load), and tiles win.
 #pragma once
 
 #include "ffn_kernels.hpp"
@@ -30,6 +42,7 @@ template <int TYPE>
 struct Few8 {
   v4u_t q;
   static constexpr int SIZE = 2;
+  __device__ void zero() { q = v4u_t{0, 0, 0, 0}; }
   __device__ void load(const char* p) { q = *(const gv4u_any*)p; }
   __device__ void load_some(const char* p, int n) {
 #pragma unroll
@@ -50,6 +63,7 @@ template <>
 struct Few8<SCAO_F32> {
   v4f a, b;
   static constexpr int SIZE = 4;
+  __device__ void zero() { a = b = v4f{0.f, 0.f, 0.f, 0.f}; }
   __device__ void load(const char* p) {
     a = gld4((const float*)p);
     b = gld4((const float*)p + 4);
@@ -68,27 +82,36 @@ struct Few8<SCAO_F32> {
 };
 
 // U: steps in flight
-template <int TYPE, int MT, int NR, int NW, int U, bool GATED>
+template <int TYPE, int MT, int NR, int NW, int U, bool GATED, bool HALVES>
 __global__ __launch_bounds__(NW * 64) void k_ffn_few(const FfnFew o, const FfnEpilogue e) {
-  constexpr int H = GATED ? 2 : 1, NF = MT * NR * H;
+  constexpr int H = GATED ? 2 : 1, NF = MT * NR * H, P = HALVES ? 2 : 1, COLS_ = NR * 16 / P;
+  static_assert(!HALVES || (MT == 1 && NR == 1), "halves: one product of 16 x 16");
   __shared__ v4f sums[NW][NF][64];
   using V = Few8<TYPE>;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63;
   const int q = lane & 15, g = lane >> 4;
-  const int c0 = blockIdx.x * NR * 16;
+  const int c0 = blockIdx.x * COLS_;
+  const int row = HALVES ? q & 7 : q, half = HALVES ? q >> 3 : 0;
+
+  // this lane's stretch of k steps, of the same length for all
+  const int steps = (o.K + 31) / 32, per = (steps + NW * P - 1) / (NW * P);
+  const int first = (wave * P + half) * per;
+  // steps that are whole for every lane of the wave
+  const int whole = min(per, o.K / 32 - (wave * P + P - 1) * per);
 
   // row starts; rows outside of the operands repeat the last one, their results
   // are never written
   const char *pw[NR * H], *px[MT];
+  const int64_t k0 = (int64_t)first * 32 + 8 * g;
 #pragma unroll
   for (int i = 0; i < NR; ++i) {
-    const int64_t r = min(c0 + i * 16 + q, o.cols - 1);
-    pw[i] = (const char*)o.w + (r * o.ldw + 8 * g) * V::SIZE;
-    if (GATED) pw[NR * (H - 1) + i] = (const char*)o.w2 + (r * o.ldw2 + 8 * g) * V::SIZE;
+    const int64_t r = min(c0 + i * 16 + row, o.cols - 1);
+    pw[i] = (const char*)o.w + (r * o.ldw + k0) * V::SIZE;
+    if (GATED) pw[NR * (H - 1) + i] = (const char*)o.w2 + (r * o.ldw2 + k0) * V::SIZE;
   }
 #pragma unroll
   for (int m = 0; m < MT; ++m)
-    px[m] = (const char*)o.x + ((int64_t)min(m * 16 + q, o.tokens - 1) * o.ldx + 8 * g) * V::SIZE;
+    px[m] = (const char*)o.x + ((int64_t)min(m * 16 + row, o.tokens - 1) * o.ldx + k0) * V::SIZE;
 
   v4f acc[NR * H][MT];
 #pragma unroll
@@ -115,11 +138,8 @@ __global__ __launch_bounds__(NW * 64) void k_ffn_few(const FfnFew o, const FfnEp
     }
   };
 
-  const int steps = (o.K + 31) / 32, whole = o.K / 32;
-  const int per = (steps + NW - 1) / NW;
-  int s = wave * per;
-  const int end = min(steps, s + per), full = min(whole, end);
-  for (; s + U <= full; s += U) {
+  int s = 0;
+  for (; s + U <= whole; s += U) {   // all lanes' steps are whole
     V w[U][NR * H], x[U][MT];
 #pragma unroll
     for (int u = 0; u < U; ++u) {
@@ -131,22 +151,31 @@ __global__ __launch_bounds__(NW * 64) void k_ffn_few(const FfnFew o, const FfnEp
 #pragma unroll
     for (int u = 0; u < U; ++u) products(w[u], x[u]);
   }
-  for (; s < end; ++s) {
-    V w[NR * H], x[MT];
-    const int left = o.K - s * 32 - 8 * g;
+  // what is left of the stretch, and the end of k
+  for (; s < per; s += U) {
+    V w[U][NR * H], x[U][MT];
 #pragma unroll
-    for (int i = 0; i < NR * H; ++i) {
-      const char* p = pw[i] + (int64_t)s * 32 * V::SIZE;
-      if (s < full) w[i].load(p);
-      else w[i].load_some(p, left);
+    for (int u = 0; u < U; ++u) {
+      const int left = s + u < per ? o.K - (first + s + u) * 32 - 8 * g : 0;
+      const int64_t at = (int64_t)(s + u) * 32 * V::SIZE;
+#pragma unroll
+      for (int i = 0; i < NR * H; ++i) w[u][i].zero();
+#pragma unroll
+      for (int m = 0; m < MT; ++m) x[u][m].zero();
+      if (left >= 8) {
+#pragma unroll
+        for (int i = 0; i < NR * H; ++i) w[u][i].load(pw[i] + at);
+#pragma unroll
+        for (int m = 0; m < MT; ++m) x[u][m].load(px[m] + at);
+      } else if (left > 0) {
+#pragma unroll
+        for (int i = 0; i < NR * H; ++i) w[u][i].load_some(pw[i] + at, left);
+#pragma unroll
+        for (int m = 0; m < MT; ++m) x[u][m].load_some(px[m] + at, left);
+      }
     }
 #pragma unroll
-    for (int m = 0; m < MT; ++m) {
-      const char* p = px[m] + (int64_t)s * 32 * V::SIZE;
-      if (s < full) x[m].load(p);
-      else x[m].load_some(p, left);
-    }
-    products(w, x);
+    for (int u = 0; u < U; ++u) products(w[u], x[u]);
   }
 
 #pragma unroll
@@ -155,12 +184,17 @@ __global__ __launch_bounds__(NW * 64) void k_ffn_few(const FfnFew o, const FfnEp
     for (int m = 0; m < MT; ++m) sums[wave][i * MT + m][lane] = acc[i][m];
   __syncthreads();
   for (int f = wave; f < NR * MT; f += NW) {
-    v4f a = sums[0][f][lane], b = sums[0][NR * MT * (H - 1) + f][lane];
+    v4f a = {0.f, 0.f, 0.f, 0.f}, b = a;
+    // HALVES: columns 4g .. 4g+3 of tokens 0 .. 7 (lanes with q < 8, g < 2) from
+    // the first stretch, and 40 lanes further from the second
+    if (HALVES && (q >= 8 || g >= 2)) return;
 #pragma unroll
-    for (int w = 1; w < NW; ++w) {
-      a += sums[w][f][lane];
-      if (GATED) b += sums[w][NR * MT + f][lane];
-    }
+    for (int w = 0; w < NW; ++w)
+#pragma unroll
+      for (int p = 0; p < P; ++p) {
+        a += sums[w][f][lane + 40 * p];
+        if (GATED) b += sums[w][NR * MT + f][lane + 40 * p];
+      }
     const int m = (f % MT) * 16 + q, n = c0 + (f / MT) * 16 + 4 * g;
     if constexpr (GATED) {
       v4f h;
@@ -184,16 +218,22 @@ constexpr int FFN_FEW_TOKENS = 64;
 
 template <int TYPE>
 void launch_few(const FfnFew& o, const FfnEpilogue& e, bool gated, hipStream_t st) {
-#define FFN_FEW(MT, NR, NW, U, G) \
-  k_ffn_few<TYPE, MT, NR, NW, U, G><<<(o.cols + NR * 16 - 1) / (NR * 16), NW * 64, 0, st>>>(o, e)
+#define FFN_FEW(MT, NW, U, G, HALVES)                                  \
+  k_ffn_few<TYPE, MT, 1, NW, U, G, HALVES>                              \
+      <<<(o.cols + (HALVES ? 7 : 15)) / (HALVES ? 8 : 16), NW * 64, 0, st>>>(o, e)
+  // halves where 16 columns a workgroup would not give every CU one
+  const bool halves = o.tokens <= 8 && o.cols < 16 * 256;
+  constexpr int U = TYPE == SCAO_F32 ? 4 : 8;
   if (gated) {
-    if (o.tokens <= 16) FFN_FEW(1, 1, 8, 4, true);
-    else if (o.tokens <= 32) FFN_FEW(2, 1, 8, 4, true);
-    else FFN_FEW(4, 1, 8, 2, true);
+    if (halves) FFN_FEW(1, 8, U, true, true);
+    else if (o.tokens <= 16) FFN_FEW(1, 8, U, true, false);
+    else if (o.tokens <= 32) FFN_FEW(2, 8, TYPE == SCAO_F32 ? 2 : 4, true, false);
+    else FFN_FEW(4, 8, 2, true, false);
   } else {
-    if (o.tokens <= 16) FFN_FEW(1, 1, 16, 4, false);
-    else if (o.tokens <= 32) FFN_FEW(2, 1, 16, 4, false);
-    else FFN_FEW(4, 1, 8, 4, false);
+    if (halves) FFN_FEW(1, 16, U, false, true);
+    else if (o.tokens <= 16) FFN_FEW(1, 16, U, false, false);
+    else if (o.tokens <= 32) FFN_FEW(2, 16, TYPE == SCAO_F32 ? 2 : 4, false, false);
+    else FFN_FEW(4, 8, TYPE == SCAO_F32 ? 2 : 4, false, false);
   }
 #undef FFN_FEW
 }
