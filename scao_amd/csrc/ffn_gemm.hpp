@@ -11,9 +11,21 @@
 //
 // A workgroup owns a BM x BN tile of C and walks k in steps of 64.  Each step's
 // two tiles go from global memory to LDS without passing registers (16 bytes a
-// lane), one step ahead of the products, into the other of two stages.  The
-// buffer descriptor's bound and an out-of-range lane offset give zeros outside
+// lane), A's into the third of three stages while two are in use, B's into the
+// other of two (a third one does not fit, and gains nothing for 256 x 256 tiles;
+// A's does 3% for 128 x 128).  The buffer descriptor's bound and an out-of-range lane offset give zeros outside
 // the operands, so no edge needs a branch.
+//
+// What bounds it: on random data the chip's power, with zeros 1810 TFLOP/s where
+// random bf16 reach 1410 (8192^3, 256 x 256 tiles; rows x rows 1410-1430, rows x
+// cols 1390, cols x cols 1400; 128 x 128 tiles 1140).  Before that it was the
+// order of issue.  A wave's loads and LDS reads queued ahead of its products left
+// the matrix cores idle (1276; with no loads at all 1716), so every row of
+// products carries its share of both (half()), and all loads in the first half
+// of the rows cost 6% again.  Four waves of 128 x 128 products instead of eight of
+// 128 x 64 halve the LDS reads, but leave one wave a SIMD (1237); 32 x 32 x 16
+// products are faster on half of the chip (930 against 890 TFLOP/s on 128 CUs)
+// and slower on all of it (1285).
 //
 // LDS layout.  The direct load writes lane l's 16 bytes at l*16, so tiles are
 // permuted by choosing which 16 bytes a lane fetches:

@@ -23,6 +23,7 @@
 // (Llama-1B's 2.47 GB in bf16: norm 421 us, 5.9 TB/s, both passes 1308, 5.7
 // TB/s; in runs through the caches 1453).
 #include <algorithm>
+#include <new>
 #include <vector>
 
 #include "../../include/scao_train.h"
@@ -261,7 +262,7 @@ int check(const char* who, const scao_tensor_desc* t, int n, int norm_type, doub
 }
 
 // No element may be scaled twice, nor by two workgroups at once.
-int check_apart(const scao_tensor_desc* t, int n) {
+int check_apart(const scao_tensor_desc* t, int n) try {
   std::vector<std::pair<uintptr_t, uintptr_t>> r;
   r.reserve(n);
   for (int i = 0; i < n; ++i)
@@ -272,6 +273,9 @@ int check_apart(const scao_tensor_desc* t, int n) {
   for (size_t i = 1; i < r.size(); ++i)
     SCAO_CHECK_ARG(r[i].first >= r[i - 1].second, "scao_grad_clip: two gradients share memory");
   return SCAO_OK;
+} catch (const std::bad_alloc&) {
+  scao_set_error("scao_grad_clip: no host memory for %d tensors", n);
+  return SCAO_ERR_INVALID;
 }
 
 // more than the last-level cache can keep a good part of

@@ -162,6 +162,28 @@ def test_gradients_against_differences(hip_device):
             assert abs(num - ana) <= 1e-3 * got[k].double().norm().item() + 1e-4 * scale, (name, k)
 
 
+def test_offsets_past_32_bits(hip_device):
+    """More than 2^31 elements of h: the last tokens' outputs and gradients are
+    those of the last tokens alone, the weights' gradients the sums over pieces
+    (fp32 sums of bf16 results: the pieces' roundings, 2^-8 of each)."""
+    tokens, d, f = 270_001, 64, 8192
+    x, gate, up, down, dy = _inputs(hip_device, tokens, d, f, torch.bfloat16)
+    got = _run(x, gate, up, down, dy, "silu")
+    tail = slice(tokens - 999, tokens)
+    part = _run(x[tail], gate, up, down, dy[tail], "silu")
+    want = reference(x[tail], gate, up, down, dy[tail], "silu")
+    for k in ("y", "dx"):
+        _compare({k: got[k][tail]}, want, torch.bfloat16, "tail")
+        _compare({k: part[k]}, want, torch.bfloat16, "alone")
+    for k in ("dgate", "dup", "ddown"):
+        total, size = 0.0, 0.0
+        for at in range(0, tokens, 54_001):
+            piece = _run(x[at:at + 54_001], gate, up, down, dy[at:at + 54_001], "silu")[k].float()
+            total, size = total + piece, size + piece.abs()
+        err = (got[k].float() - total).abs()
+        assert bool((err <= 2.0 ** -8 * (size + total.abs()) + 1e-3).all()), k
+
+
 def test_shapes_of_x_and_views(hip_device):
     x, gate, up, down, dy = _inputs(hip_device, 60, 32, 48, torch.bfloat16)
     flat = scao_amd.gated_ffn(x, gate, up, down)

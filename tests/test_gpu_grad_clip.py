@@ -224,3 +224,17 @@ def test_more_than_the_caches_hold(hip_device, dtype):
         n = min(100003, flat.numel() - at)
         err = (flat[at:at + n].double() - want[:n]).abs()
         assert bool((err <= want[:n].abs() * (ULP[dtype] + 1.3e-7) + TINY[dtype]).all())
+
+
+def test_a_tensor_past_2_31_elements(hip_device):
+    n = (1 << 31) + 70_003
+    g = torch.zeros(n, dtype=torch.bfloat16, device=hip_device)
+    g[::1 << 16] = 3.0
+    g[-1] = 4.0
+    count = (n + (1 << 16) - 1) >> 16
+    norm = (9.0 * count + 16.0) ** 0.5
+    got = scao_amd.clip_grad_norm_(_params([g]), 1.0)
+    assert abs(got.item() - norm) <= 1.2e-7 * norm
+    for i, v in ((0, 3.0), (((n - 2) >> 16) << 16, 3.0), (n - 1, 4.0)):
+        assert abs(g[i].item() - v / norm) <= 2.0 ** -8 * v / norm
+    assert int((g != 0).sum()) == count + 1
