@@ -13,8 +13,8 @@
 // two tiles go from global memory to LDS without passing registers (16 bytes a
 // lane), A's into the third of three stages while two are in use, B's into the
 // other of two (a third one does not fit, and gains nothing for 256 x 256 tiles;
-// A's does 3% for 128 x 128).  The buffer descriptor's bound and an out-of-range lane offset give zeros outside
-// the operands, so no edge needs a branch.
+// A's does 3% for 128 x 128).  The buffer descriptor's bound and an out-of-range
+// lane offset give zeros outside the operands, so no edge needs a branch.
 //
 // What bounds it: on random data the chip's power, with zeros 1810 TFLOP/s where
 // random bf16 reach 1410 (8192^3, 256 x 256 tiles; rows x rows 1410-1430, rows x
@@ -67,9 +67,14 @@ __device__ __forceinline__ v4f mma(v8s p, v8s q, v4f c) {
 }
 
 // 16 bytes a lane from global memory to LDS at lds + 16*lane.  The compiler
-// neither counts this load nor waits for it: wait_loads does, which it cannot pass.
+// neither counts this load nor waits for it: wait_loads does, which it cannot
+// pass.  Nor does it look into the block for the waits that the instructions
+// need of each other: one after m0 is written before a load uses it, five after a
+// vector instruction (readfirstlane) has written an operand's scalar register.
+// (m0 cannot be listed as changed; the compiler itself has no use for it here:
+// gfx950's LDS instructions do not read it.)
 __device__ __forceinline__ void load_lds(v4i rsrc, uint32_t lds, uint32_t voff) {
-  asm volatile("s_mov_b32 m0, %0\n\tbuffer_load_dwordx4 %1, %2, 0 offen lds" ::"s"(
+  asm volatile("s_mov_b32 m0, %0\n\ts_nop 3\n\tbuffer_load_dwordx4 %1, %2, 0 offen lds" ::"s"(
                    __builtin_amdgcn_readfirstlane(lds)),
                "v"(voff), "s"(rsrc));
 }
