@@ -369,6 +369,7 @@ struct Gemm {
       b0_ = b1_;
       b1_ = b;
     }
+    wait_loads<0>();   // LDS belongs to the next workgroup once this one has ended
   }
 };
 
