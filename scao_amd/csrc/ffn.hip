@@ -208,11 +208,12 @@ struct Block {
     FfnOperands o;
     FfnEpilogue e;
   };
-  // the tiles' counts, and room for the parts of a split product
-  void cut(Product& p, const Cut& c) {
+  // the counts of the tiles of C's rows row0 .. to-1, and room for the parts of a
+  // split product
+  void cut(Product& p, const Cut& c, int64_t to) {
     FfnOperands& o = p.o;
     const int cols = p.kind == FFN_GATE_UP ? FFN_BN[c.tile] / 2 : FFN_BN[c.tile];
-    o.tiles_m = (o.M + FFN_BM[c.tile] - 1) / FFN_BM[c.tile];
+    o.tiles_m = (int)((to - o.row0 + FFN_BM[c.tile] - 1) / FFN_BM[c.tile]);
     o.tiles_n = (o.N + cols - 1) / cols;
     o.splits = c.splits;
     o.whole = c.splits == 1 ? o.tiles() : c.whole;
@@ -222,13 +223,35 @@ struct Block {
                                     FFN_BN[c.tile] * 4);
     peak = std::max(peak, ws.used);
   }
-  void run(Product& p) {
+  void run(Product& p, const Cut& c, int64_t from, int64_t to) {
     const int64_t at = ws.used;   // the parts' room is given back
-    Cut c;
-    choose(shape(p.kind, p.o), p.kind != FFN_DW, c);
-    cut(p, c);
+    p.o.row0 = (int)from;
+    cut(p, c, to);
     ws.used = at;
     if (!dry) launchers(s.dtype).product(p.kind, c.tile, p.o, p.e, st);
+  }
+  // With few rows left over behind whole tiles of 256 these may go by themselves,
+  // on narrow tiles, at the price of reading the weights again: 1030 tokens of
+  // 2048 x 8192 128 us against 139, where 1024 fill one round exactly.
+  void run(Product& p) {
+    const Shape all = shape(p.kind, p.o);
+    Cut c, head, tail;
+    const double us = choose(all, p.kind != FFN_DW, c);
+    const int64_t rows = all.M / 256 * 256, left = all.M - rows;
+    if (p.kind != FFN_DW && rows && left && left <= 128) {
+      Shape a = all, b = all;
+      a.M = rows;
+      b.M = left;
+      const double again = 2.0 * parts * all.N * p.o.K * p.o.nseg / 4.5e6 * (all.gated ? 2 : 1) /
+                           (parts == 3 ? 6 : 1);
+      const double apart = choose(a, true, head) + std::max(choose(b, true, tail), again + 3) + 3;
+      if (1.03 * apart < us) {
+        run(p, head, 0, rows);
+        run(p, tail, rows, all.M);
+        return;
+      }
+    }
+    run(p, c, 0, all.M);
   }
   // dh or dx, and a dW that does not need it
   void run(Product& p, Product& w) {
@@ -243,8 +266,8 @@ struct Block {
       return;
     }
     const int64_t at = ws.used;
-    cut(p, cp);
-    cut(w, cw);
+    cut(p, cp, x.M);
+    cut(w, cw, y.M);
     ws.used = at;
     if (!dry) launchers(s.dtype).pair(p.kind, cp.tile, p.o, p.e, w.o, w.e, st);
   }

@@ -150,6 +150,7 @@ struct FfnOperands {
   int64_t lda, ldb;
   int M, N, K;          // C's sizes (N: one projection's with GATED), k of one segment
   int nseg;
+  int row0;             // the first tile's row: the others belong to another launch
   int tiles_m, tiles_n;
   int whole;            // tiles that run in one piece, the others in `splits`
   int splits;           // parts of the k steps of all segments
@@ -195,7 +196,7 @@ struct Gemm {
     lane = threadIdx.x & 63;
     wm = wave / WN;
     wn = wave % WN;
-    m0 = tm * BM;
+    m0 = o.row0 + tm * BM;
     n0 = tn * COLS_N;
 #pragma unroll
     for (int i = 0; i < TA::LOADS; ++i) {

@@ -463,7 +463,7 @@ __global__ __launch_bounds__(256) void k_ffn_join(const FfnOperands o, const Ffn
   const int lane = threadIdx.x & 63, tile = (int)(frag / FRAGS), in = (int)(frag % FRAGS);
   int tm, tn;
   tile_of(o.whole + tile, o.tiles_m, o.tiles_n, tm, tn);
-  const int m = tm * G::BM_ + in / FJ * 16 + (lane & 15);
+  const int m = o.row0 + tm * G::BM_ + in / FJ * 16 + (lane & 15);
   const int n = tn * G::COLS_N + in % FJ * 16 + 4 * (lane >> 4);
   if (m - (lane & 15) >= o.M || n - 4 * (lane >> 4) >= e.cols) return;
   // in the tile's own order of fragments an up fragment follows the gate's row

@@ -67,7 +67,8 @@ def _check(dev, tokens, d, f, dtype, name="silu", **kw):
 
 SIZES = [(1, 1, 1), (1, 64, 128), (2, 8, 8), (3, 7, 5), (17, 40, 24), (64, 64, 64), (65, 63, 129),
          (130, 72, 200), (129, 257, 131), (256, 256, 256), (257, 264, 520), (33, 1001, 67),
-         (700, 96, 1000)]
+         (700, 96, 1000), (257, 512, 384), (300, 520, 1030), (521, 264, 2056), (777, 256, 512),
+         (1030, 2048, 8192)]
 
 
 @pytest.mark.parametrize("dtype", TYPES)
