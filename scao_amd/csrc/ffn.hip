@@ -135,10 +135,15 @@ struct Block {
         for (int64_t whole : {(int64_t)0, tiles / c.slots * c.slots}) {
           if (whole && (n == 1 || whole == tiles)) continue;
           const int64_t groups = (tiles - whole) * n, last = groups % c.slots;
-          double us = whole / c.slots * (s.steps * c.full + c.ends) +
-                      groups / c.slots * (per * c.full + c.ends) +
+          // a narrow gated tile's epilogue stores single fragments: 300 tokens,
+          // 4096 x 11008 bf16, 120 us on 64 x 128 tiles, 90 without this term and
+          // 95 on 256 x 256 tiles
+          const double end = c.ends + (s.gated && t == FFN_64x128 ? 8 : 0);
+          const double part_end = n == 1 ? end : c.ends;
+          double us = whole / c.slots * (s.steps * c.full + end) +
+                      groups / c.slots * (per * c.full + part_end) +
                       s.join(n, (double)(tiles - whole) / tiles);
-          if (last) us += per * c.step(last) + c.ends;
+          if (last) us += per * c.step(last) + part_end;
           if (us < best) {
             best = us;
             cut = {t, n == 1 ? (int)tiles : (int)whole, (int)n};
@@ -174,6 +179,7 @@ struct Block {
                      (int64_t)((us - hi) / b + 1e-9) * rest < gb)
             us += 0.25 * b;
           us += x.join(n) + y.join(m);
+          if (x.moved && t == FFN_256x256) us *= 1.2;   // see run()
           if (us < best) {
             best = us;
             cx = {t, 0, (int)n};
@@ -232,7 +238,10 @@ struct Block {
   }
   // With few rows left over behind whole tiles of 256 these may go by themselves,
   // on narrow tiles, at the price of reading the weights again: 1030 tokens of
-  // 2048 x 8192 128 us against 139, where 1024 fill one round exactly.
+  // 2048 x 8192 128 us against 139, where 1024 fill one round exactly.  Not
+  // behind rows that are split many times themselves: 300 tokens of 4096 x 11008
+  // fp32 951 us, 256 of them in 8 and 16 parts and 44 apart 1061.  (Over 165
+  // forward passes of up to 128 rows left 0.8% behind the better of both choices.)
   void run(Product& p) {
     const Shape all = shape(p.kind, p.o);
     Cut c, head, tail;
@@ -244,8 +253,9 @@ struct Block {
       b.M = left;
       const double again = 2.0 * parts * all.N * p.o.K * p.o.nseg / 4.5e6 * (all.gated ? 2 : 1) /
                            (parts == 3 ? 6 : 1);
-      const double apart = choose(a, true, head) + std::max(choose(b, true, tail), again + 3) + 3;
-      if (1.03 * apart < us) {
+      const double apart =
+          choose(a, true, head) + 1.15 * std::max(choose(b, true, tail), again + 3) + 3;
+      if (head.splits <= 6 && 1.03 * apart < us) {
         run(p, head, 0, rows);
         run(p, tail, rows, all.M);
         return;
@@ -257,10 +267,16 @@ struct Block {
   void run(Product& p, Product& w) {
     const Shape x = shape(p.kind, p.o), y = shape(w.kind, w.o);
     Cut c, cp, cw;
+    // dx goes with its dW where the estimates say so.  dh's epilogue moves bytes:
+    // two 128 x 128 tiles on a CU hide half of them behind dWd's products, one 256
+    // x 256 tile none, and large tiles lose in an L2 that holds two working sets.
+    // With these terms and without, of the best of apart and both tiles on 118
+    // backward passes (300 to 8192 tokens, 768 x 2048 to 4096 x 11008): dh 1.1%
+    // slower on average and 1.7%, dx 0.6%.  2048 tokens, 768 x 2048 fp32: dh and
+    // dWd apart 285 us, on 128 x 128 tiles 266; 8192 tokens, 2048 x 8192 bf16:
+    // apart 1328, on 256 x 256 tiles 1369.
     const double apart = choose(x, true, c) + choose(y, false, c) + 3;
-    // large products lose a few per cent side by side, two working sets in an L2:
-    // 8192 tokens, 4096 x 14336, the whole pass 6560 us apart and 6700 in pairs
-    if (1.06 * choose_pair(x, y, cp, cw) > apart) {
+    if (choose_pair(x, y, cp, cw) > apart + 0.5 * x.moved / 5e6 * x.M * x.N) {
       run(p);
       run(w);
       return;
