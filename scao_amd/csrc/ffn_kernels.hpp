@@ -453,11 +453,12 @@ __global__ __launch_bounds__(GA::THREADS, 2) void k_ffn_pair(const FfnOperands o
 }
 
 // The parts of a split product's tiles, added in order, and their epilogue: a
-// wave takes a fragment (GATED: one of either projection).
+// wave takes a fragment (GATED: one of either projection).  Four parts are under
+// way at a time, since few workgroups wait for memory here.
 template <class G, int TYPE, int EPI>
-__global__ __launch_bounds__(256) void k_ffn_join(const FfnOperands o, const FfnEpilogue e) {
+__device__ __forceinline__ void ffn_join(const FfnOperands& o, const FfnEpilogue& e, int block) {
   constexpr int FJ = G::COLS_N / 16, FRAGS = G::BM_ / 16 * FJ;   // of C in a tile
-  const int64_t frag = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6);
+  const int64_t frag = (int64_t)block * 4 + (threadIdx.x >> 6);
   const int rest = o.tiles() - o.whole;
   if (frag >= (int64_t)rest * FRAGS) return;
   const int lane = threadIdx.x & 63, tile = (int)(frag / FRAGS), in = (int)(frag % FRAGS);
@@ -470,16 +471,28 @@ __global__ __launch_bounds__(256) void k_ffn_join(const FfnOperands o, const Ffn
   const gv4f_a16* p = (const gv4f_a16*)e.partial +
                       ((int64_t)tile * G::FRAGS + in / FJ * (G::BN_ / 16) + in % FJ) * 64 + lane;
   const int64_t all = (int64_t)rest * G::FRAGS * 64;
+  Kept<TYPE> k;
+  if (EPI == EPI_DACT) k.load(e.ab, (int64_t)e.fi * e.fj, kept_at(e, m, n), lane);
   v4f a = {0.f, 0.f, 0.f, 0.f}, b = a;
-  for (int s = 0; s < o.splits; ++s) {
-    a += p[s * all];
-    if (EPI == EPI_GATED) b += p[s * all + FJ * 64];
+  constexpr int BATCH = 4;
+  for (int s = 0; s < o.splits; s += BATCH) {
+    v4f pa[BATCH], pb[BATCH];
+#pragma unroll
+    for (int i = 0; i < BATCH; ++i)
+      if (s + i < o.splits) {
+        pa[i] = p[(s + i) * all];
+        if (EPI == EPI_GATED) pb[i] = p[(s + i) * all + FJ * 64];
+      }
+#pragma unroll
+    for (int i = 0; i < BATCH; ++i)
+      if (s + i < o.splits) {
+        a += pa[i];
+        if (EPI == EPI_GATED) b += pb[i];
+      }
   }
   if constexpr (EPI == EPI_STORE) {
     epi_store<TYPE>(e, m, n, a);
   } else {
-    Kept<TYPE> k;
-    if (EPI == EPI_DACT) k.load(e.ab, (int64_t)e.fi * e.fj, kept_at(e, m, n), lane);
     const bool in = m < e.rows && n < e.cols;
     const int64_t at = (int64_t)m * e.ldo + n;
     for_activation(e.act, [&](auto act) {
@@ -499,6 +512,19 @@ __global__ __launch_bounds__(256) void k_ffn_join(const FfnOperands o, const Ffn
   }
 }
 
+template <class G, int TYPE, int EPI>
+__global__ __launch_bounds__(256) void k_ffn_join(const FfnOperands o, const FfnEpilogue e) {
+  ffn_join<G, TYPE, EPI>(o, e, blockIdx.x);
+}
+// of both products of a pair; na: workgroups of the first's
+template <class GA, int EPI_A, class GB, int EPI_B, int TYPE>
+__global__ __launch_bounds__(256) void k_ffn_join_pair(const FfnOperands oa, const FfnEpilogue ea,
+                                                       const FfnOperands ob, const FfnEpilogue eb,
+                                                       int na) {
+  if ((int)blockIdx.x < na) ffn_join<GA, TYPE, EPI_A>(oa, ea, blockIdx.x);
+  else ffn_join<GB, TYPE, EPI_B>(ob, eb, blockIdx.x - na);
+}
+
 // --------------------------------------------------------- packing ---------
 // Matrices with any row stride and start as products' operands: rows of `ldo`
 // elements (cols rounded up to 8, the rest zero), 16-byte aligned; an fp32 one as
@@ -516,6 +542,8 @@ struct FfnPack {
   int n;
   int64_t groups;
 };
+typedef v4f v4f_a4 __attribute__((aligned(4)));
+typedef __attribute__((address_space(1))) v4f_a4 gv4f_a4;
 template <int TYPE>
 __global__ __launch_bounds__(256) void k_ffn_pack(const FfnPack p) {
   int k = 0;
@@ -524,16 +552,40 @@ __global__ __launch_bounds__(256) void k_ffn_pack(const FfnPack p) {
     if (i < p.n && (int64_t)blockIdx.x >= p.m[i].first) k = i;
   const FfnPack::Matrix& m = p.m[k];
   const int per = m.ldo / 8;
-  const int64_t i = ((int64_t)blockIdx.x - m.first) * 256 + threadIdx.x;
-  if (i >= m.rows * per) return;
-  const int64_t r = i / per;
-  const int c = (int)(i % per) * 8;
+  const int64_t i0 = ((int64_t)blockIdx.x - m.first) * 256;
+  const int at = (int)(i0 % per) + threadIdx.x;
+  const int64_t r = i0 / per + at / per;
+  if (r >= m.rows) return;
+  const int c = at % per * 8, left = m.cols - c;
+  uint16_t* dst = (uint16_t*)m.dst + r * m.ldo + c;
+  if constexpr (TYPE == SCAO_F32) {
+    const gfloat* src = (const gfloat*)m.src + r * m.ld + c;
+    v4f x[2] = {{0.f, 0.f, 0.f, 0.f}, {0.f, 0.f, 0.f, 0.f}};
+    if (left >= 8) {
+      x[0] = ((const gv4f_a4*)src)[0];
+      x[1] = ((const gv4f_a4*)src)[1];
+    } else {
 #pragma unroll
-  for (int t = 0; t < 8; t += 4) {
-    const int left = m.cols - c - t;
-    const v4f x = ld4(m.src, TYPE, r * m.ld + c + t, left >= 4,
-                      left >= 4 ? 15 : left <= 0 ? 0 : (1 << left) - 1);
-    put_operand<TYPE>(m.dst, r * m.ldo + c + t, m.plane, x);
+      for (int t = 0; t < 8; ++t)
+        if (t < left) x[t / 4][t % 4] = src[t];
+    }
+    v2u w[2][3];
+    operand_words<SCAO_F32>(x[0], w[0]);
+    operand_words<SCAO_F32>(x[1], w[1]);
+#pragma unroll
+    for (int i = 0; i < 3; ++i)
+      *(gv4u_a16*)(dst + i * m.plane) = v4u_t{w[0][i][0], w[0][i][1], w[1][i][0], w[1][i][1]};
+  } else {
+    const gu16* src = (const gu16*)m.src + r * m.ld + c;
+    v4u_t w = {0, 0, 0, 0};
+    if (left >= 8) {
+      w = *(const gv4u_a2*)src;
+    } else {
+#pragma unroll
+      for (int t = 0; t < 8; ++t)
+        if (t < left) w[t / 2] |= (uint32_t)src[t] << (16 * (t % 2));
+    }
+    *(gv4u_a16*)dst = w;
   }
 }
 
@@ -549,10 +601,14 @@ template <int TYPE, int TILE, int WM, int WN, int LA, int LB, int EPI>
 using FfnTile =
     Gemm<FFN_BM[TILE], FFN_BN[TILE], WM, WN, LA, LB, TYPE == SCAO_F16, EPI == EPI_GATED>;
 
+template <class G>
+int join_groups(const FfnOperands& o) {
+  const int64_t frags = (int64_t)(o.tiles() - o.whole) * (G::BM_ / 16) * (G::COLS_N / 16);
+  return (int)((frags + 3) / 4);
+}
 template <class G, int TYPE, int EPI>
 void launch_join(const FfnOperands& o, const FfnEpilogue& e, hipStream_t st) {
-  const int64_t frags = (int64_t)(o.tiles() - o.whole) * (G::BM_ / 16) * (G::COLS_N / 16);
-  if (frags) k_ffn_join<G, TYPE, EPI><<<(int)((frags + 3) / 4), 256, 0, st>>>(o, e);
+  if (const int n = join_groups<G>(o)) k_ffn_join<G, TYPE, EPI><<<n, 256, 0, st>>>(o, e);
 }
 
 template <int TYPE, int TILE, int WM, int WN, int LA, int LB, int EPI>
@@ -574,8 +630,13 @@ void launch_pair_tile(const FfnOperands& oa, const FfnEpilogue& ea, const FfnOpe
   const int64_t sb = (int64_t)ob.nseg * ((ob.K + FFN_BK - 1) / FFN_BK) / ob.splits;
   k_ffn_pair<A, EPI, B, EPI_STORE, TYPE>
       <<<na + nb, A::THREADS, 0, st>>>(oa, ea, ob, eb, na, nb, mixed, sb > sa);
-  launch_join<A, TYPE, EPI>(oa, ea, st);
-  launch_join<B, TYPE, EPI_STORE>(ob, eb, st);
+  const int ja = join_groups<A>(oa), jb = join_groups<B>(ob);
+  if (ja && jb)
+    k_ffn_join_pair<A, EPI, B, EPI_STORE, TYPE><<<ja + jb, 256, 0, st>>>(oa, ea, ob, eb, ja);
+  else if (ja)
+    k_ffn_join<A, TYPE, EPI><<<ja, 256, 0, st>>>(oa, ea);
+  else if (jb)
+    k_ffn_join<B, TYPE, EPI_STORE><<<jb, 256, 0, st>>>(ob, eb);
 }
 template <int TYPE>
 void launch_pair(int kind, int tile, const FfnOperands& oa, const FfnEpilogue& ea,
