@@ -138,7 +138,7 @@ struct Block {
           // a narrow gated tile's epilogue stores single fragments: 300 tokens,
           // 4096 x 11008 bf16, 120 us on 64 x 128 tiles, 90 without this term and
           // 95 on 256 x 256 tiles
-          const double end = c.ends + (s.gated && t == FFN_64x128 ? 8 : 0);
+          const double end = c.ends + (s.gated && t >= FFN_64x128 ? 2.5 : 0);
           const double part_end = n == 1 ? end : c.ends;
           double us = whole / c.slots * (s.steps * c.full + end) +
                       groups / c.slots * (per * c.full + part_end) +
