@@ -79,11 +79,32 @@ def test_views_at_any_start_leave_their_neighbours(hip_device, dtype, start):
 
 
 def test_many_tensors_of_mixed_types(hip_device):
-    """More tensors than one launch's table holds (190), empty ones among them."""
+    """More tensors than one launch's table holds (336), empty ones among them."""
     types = list(ULP)
     grads = [_normal(hip_device, i, (i * 37) % 501, dtype=types[i % 3]) for i in range(431)]
     _check(grads, 1.0)
     _check(grads, 0.01, math.inf, 0.5)
+
+
+def test_a_large_tensor_in_two_tables(hip_device):
+    """More than 2^31 elements, which take two entries of a table: the first in
+    one launch's last place, the second in the next launch."""
+    small = [_normal(hip_device, i, i % 50 + 1, dtype=torch.bfloat16) for i in range(340)]
+    n = (1 << 31) + 9
+    big = torch.zeros(n, dtype=torch.bfloat16, device=hip_device)
+    big[::1 << 20] = 2.0
+    big[-1] = 4.0
+    count = (n + (1 << 20) - 1) >> 20
+    kept = [g.double() for g in small]
+    norm = (sum(g.square().sum().item() for g in kept) + 4.0 * count + 16.0) ** 0.5
+    got = scao_amd.clip_grad_norm_(_params(small[:335] + [big] + small[335:]), 1.0)
+    assert abs(got.item() - norm) <= 1.2e-7 * norm
+    for g, k in zip(small, kept):
+        assert bool(((g.double() - k / norm).abs()
+                     <= k.abs() / norm * (ULP[torch.bfloat16] + 1.3e-7) + TINY[torch.bfloat16]).all())
+    for i, v in ((0, 2.0), (1 << 31, 2.0), (n - 1, 4.0)):
+        assert abs(big[i].item() - v / norm) <= 2.0 ** -8 * v / norm
+    assert int((big != 0).sum()) == count + 1
 
 
 def test_strides(hip_device):

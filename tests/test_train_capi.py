@@ -88,7 +88,7 @@ def test_workspace_holds_every_launch():
     t = _table(*GOOD * 400)
     assert lib.scao_grad_norm_workspace(t.ctypes.data, 0) == 0
     assert lib.scao_grad_norm_workspace(t.ctypes.data, 1) == 2048 * 8
-    assert lib.scao_grad_norm_workspace(t.ctypes.data, 400) == 3 * 2048 * 8
+    assert lib.scao_grad_norm_workspace(t.ctypes.data, 400) == 2 * 2048 * 8
 
 
 def _ffn(**kw):
