@@ -80,8 +80,8 @@ struct Block {
   // Estimated us of products on tiles: us of a k step with one workgroup a CU
   // and with all a CU holds, and of a tile's beginning and end, fitted to the
   // times of every tile and part count of 225 products (8 to 4096 tokens, 256 x
-  // 704 to 4096 x 14336): the choice is 1.7% slower than the best on the
-  // geometric average, 17% at most.  For example dx of 24 tokens, 2048 x 8192: 32
+  // 704 to 4096 x 14336; 256 x 128 tiles: to 66 forward passes): the choice is 1.7%
+  // slower than the best on the geometric average, 17% at most.  For example dx of 24 tokens, 2048 x 8192: 32
   // x 128 tiles in one part 116 us, in 16 parts 21.8; of 4096 tokens: 256 x 256
   // in one part 285, in two 183, 128 x 128 in one 251.
   struct Cost {
@@ -96,6 +96,7 @@ struct Block {
     }
   };
   struct Shape {
+    int kind;
     int64_t M, N, steps;
     bool gated;
     int64_t tiles(int t) const {
@@ -114,7 +115,8 @@ struct Block {
   };
   static const Cost& cost(int tile) {
     static const Cost costs[FFN_TILES] = {
-        {256, 1.15, 1.50, 4.9}, {512, 0.62, 1.14, 5.2}, {512, 0.56, 0.70, 3.0}, {768, 0.44, 0.96, 1.7}};
+        {256, 1.15, 1.50, 4.9}, {256, 0.68, 0.89, 5.5}, {512, 0.62, 1.14, 5.2},
+        {512, 0.56, 0.70, 3.0}, {768, 0.44, 0.96, 1.7}};
     return costs[tile];
   }
   // How a product is cut: its tile, how many tiles run in one piece and in how
@@ -124,9 +126,14 @@ struct Block {
   struct Cut {
     int tile = 0, whole = 0, splits = 1;
   };
-  static double choose(const Shape& s, bool tokens, Cut& cut) {
+  static double choose(const Shape& s, Cut& cut) {
     double best = 1e30;
-    for (int t = 0; t < (tokens ? FFN_TILES : FFN_64x128); ++t) {
+    for (int t = 0; t < (s.kind == FFN_DW ? FFN_64x128 : FFN_TILES); ++t) {
+      // 256 x 128 tiles for DOWN: 1024 tokens, 2048 x 8192 bf16, 64 of them in four
+      // parts, the forward pass 106 us, with 128 x 128 tiles 112.  In the backward
+      // pass they change nothing on average (0.1%), and an epilogue that moves bytes
+      // gains from the other 128 x 128 tile on its CU.
+      if (t == FFN_256x128 && s.kind != FFN_DOWN) continue;
       const Cost& c = cost(t);
       const int64_t tiles = s.tiles(t);
       for (int64_t n : {1, 2, 3, 4, 6, 8, 12, 16, 24, 32}) {
@@ -206,7 +213,7 @@ struct Block {
 
   Shape shape(int kind, const FfnOperands& o) const {
     const double bytes = kind == FFN_GATE_UP ? 8 : kind == FFN_DH ? 10 : 0;
-    return Shape{o.M, o.N, (int64_t)o.nseg * ((o.K + FFN_BK - 1) / FFN_BK), kind == FFN_GATE_UP,
+    return Shape{kind, o.M, o.N, (int64_t)o.nseg * ((o.K + FFN_BK - 1) / FFN_BK), kind == FFN_GATE_UP,
                  s.dtype == SCAO_F32 ? 2 * bytes : bytes};
   }
   struct Product {
@@ -245,7 +252,7 @@ struct Block {
   void run(Product& p) {
     const Shape all = shape(p.kind, p.o);
     Cut c, head, tail;
-    const double us = choose(all, p.kind != FFN_DW, c);
+    const double us = choose(all, c);
     const int64_t rows = all.M / 256 * 256, left = all.M - rows;
     if (p.kind != FFN_DW && rows && left && left <= 128) {
       Shape a = all, b = all;
@@ -254,7 +261,7 @@ struct Block {
       const double again = 2.0 * parts * all.N * p.o.K * p.o.nseg / 4.5e6 * (all.gated ? 2 : 1) /
                            (parts == 3 ? 6 : 1);
       const double apart =
-          choose(a, true, head) + 1.15 * std::max(choose(b, true, tail), again + 3) + 3;
+          choose(a, head) + 1.15 * std::max(choose(b, tail), again + 3) + 3;
       if (head.splits <= 6 && 1.03 * apart < us) {
         run(p, head, 0, rows);
         run(p, tail, rows, all.M);
@@ -275,7 +282,7 @@ struct Block {
     // slower on average and 1.7%, dx 0.6%.  2048 tokens, 768 x 2048 fp32: dh and
     // dWd apart 285 us, on 128 x 128 tiles 266; 8192 tokens, 2048 x 8192 bf16:
     // apart 1328, on 256 x 256 tiles 1369.
-    const double apart = choose(x, true, c) + choose(y, false, c) + 3;
+    const double apart = choose(x, c) + choose(y, c) + 3;
     if (choose_pair(x, y, cp, cw) > apart + 0.5 * x.moved / 5e6 * x.M * x.N) {
       run(p);
       run(w);

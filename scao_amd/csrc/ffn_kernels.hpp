@@ -593,9 +593,11 @@ __global__ __launch_bounds__(256) void k_ffn_pack(const FfnPack p) {
 // The products by the layouts of their operands and their epilogue.
 enum { FFN_GATE_UP, FFN_DOWN, FFN_DH, FFN_DX, FFN_DW };
 
-// The tiles, and how many columns of C one covers: half of BN for GATE_UP.
-enum { FFN_256x256, FFN_128x128, FFN_64x128, FFN_32x128, FFN_TILES };
-constexpr int FFN_BM[FFN_TILES] = {256, 128, 64, 32}, FFN_BN[FFN_TILES] = {256, 128, 128, 128};
+// The tiles, and how many columns of C one covers: half of BN for GATE_UP.  256 x
+// 128 is for DOWN.
+enum { FFN_256x256, FFN_256x128, FFN_128x128, FFN_64x128, FFN_32x128, FFN_TILES };
+constexpr int FFN_BM[FFN_TILES] = {256, 256, 128, 64, 32};
+constexpr int FFN_BN[FFN_TILES] = {256, 128, 128, 128, 128};
 
 template <int TYPE, int TILE, int WM, int WN, int LA, int LB, int EPI>
 using FfnTile =
@@ -655,9 +657,11 @@ template <int TYPE, int LA, int LB, int EPI>
 void launch_tile(int tile, const FfnOperands& o, const FfnEpilogue& e, hipStream_t st) {
   if (tile == FFN_256x256) launch_gemm<TYPE, FFN_256x256, 2, 4, LA, LB, EPI>(o, e, st);
   else if (tile == FFN_128x128) launch_gemm<TYPE, FFN_128x128, 2, 2, LA, LB, EPI>(o, e, st);
-  else if constexpr (LA == ROWS) {   // A's rows are tokens: there may be few
+  if constexpr (LA == ROWS) {   // A's rows are tokens: there may be few
     if (tile == FFN_64x128) launch_gemm<TYPE, FFN_64x128, 1, 4, LA, LB, EPI>(o, e, st);
-    else launch_gemm<TYPE, FFN_32x128, 1, 4, LA, LB, EPI>(o, e, st);
+    else if (tile == FFN_32x128) launch_gemm<TYPE, FFN_32x128, 1, 4, LA, LB, EPI>(o, e, st);
+    if constexpr (LB == ROWS && EPI == EPI_STORE)
+      if (tile == FFN_256x128) launch_gemm<TYPE, FFN_256x128, 4, 2, LA, LB, EPI>(o, e, st);
   }
 }
 
