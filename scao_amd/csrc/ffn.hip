@@ -81,9 +81,9 @@ struct Block {
   // and with all a CU holds, and of a tile's beginning and end, fitted to the
   // times of every tile and part count of 225 products (8 to 4096 tokens, 256 x
   // 704 to 4096 x 14336; 256 x 128 tiles: to 66 forward passes): the choice is 1.7%
-  // slower than the best on the geometric average, 17% at most.  For example dx of 24 tokens, 2048 x 8192: 32
-  // x 128 tiles in one part 116 us, in 16 parts 21.8; of 4096 tokens: 256 x 256
-  // in one part 285, in two 183, 128 x 128 in one 251.
+  // slower than the best on the geometric average, 17% at most.  For example dx
+  // of 24 tokens, 2048 x 8192: 32 x 128 tiles in one part 116 us, in 16 parts 21.8;
+  // of 4096 tokens: 256 x 256 in one part 285, in two 183, 128 x 128 in one 251.
   struct Cost {
     int slots;
     double lone, full, ends;

@@ -18,13 +18,16 @@
 // whatever the tensor's start is: the first and the last vector of a tensor are
 // taken element by element.
 //
-// Gradients that the last-level cache (256 MiB) can hold a good part of: each
-// workgroup takes a run of chunks, and the scaling begins with what was read
-// last (GPT-2-small's 268 MB in fp32: 128 us for 3 x 268 MB, 6.3 TB/s; in turns
-// past the caches 139).  Larger ones: the workgroups take chunks in turns, so
-// that all of them read near each other, and the scaling goes past the caches
-// (Llama-1B's 2.47 GB in bf16: norm 421 us, 5.9 TB/s, both passes 1308, 5.7
-// TB/s; in runs through the caches 1453).
+// Gradients that the last-level cache (256 MiB) holds: each workgroup takes a run
+// of chunks, and the scaling begins with what was read last and writes through
+// the caches.  Larger ones: the workgroups take chunks in turns, so that all of
+// them read near each other, and the scaling goes past the caches, which would
+// write the rest back while the next kernels read.  Gradients written, clipped
+// and added to the parameters, runs through the caches against turns past them:
+// 128 MB 196 us and 201, 200 MB 302 and 304, 268 MB 428 and 416, 400 MB 632 and
+// 604; the clipping alone among others of its size, 268 MB 162 and 132 (6.1 TB/s
+// for 3 x 268 MB).  Llama-1B's 2.47 GB in bf16: norm 419 us, 5.9 TB/s, both passes
+// 1293, 5.7 TB/s; in runs through the caches 1453.
 #include <algorithm>
 #include <new>
 #include <vector>
@@ -316,11 +319,11 @@ int check_apart(const scao_tensor_desc* t, int n) try {
   return SCAO_ERR_INVALID;
 }
 
-// more than the last-level cache can keep a good part of
+// more than the last-level cache can keep beside what else a step moves
 bool large(const scao_tensor_desc* t, int n) {
   int64_t bytes = 0;
   for (int i = 0; i < n; ++i) bytes += t[i].numel * size_of(t[i].dtype);
-  return bytes > ((int64_t)512 << 20);
+  return bytes > ((int64_t)192 << 20);
 }
 
 template <class F>
