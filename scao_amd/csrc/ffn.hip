@@ -115,7 +115,7 @@ struct Block {
   };
   static const Cost& cost(int tile) {
     static const Cost costs[FFN_TILES] = {
-        {256, 1.15, 1.50, 4.9}, {256, 0.68, 0.89, 5.5}, {512, 0.62, 1.14, 5.2},
+        {256, 1.15, 1.50, 4.9}, {256, 0.76, 0.93, 4.5}, {512, 0.62, 1.14, 5.2},
         {512, 0.56, 0.70, 3.0}, {768, 0.44, 0.96, 1.7}};
     return costs[tile];
   }
@@ -274,16 +274,17 @@ struct Block {
   void run(Product& p, Product& w) {
     const Shape x = shape(p.kind, p.o), y = shape(w.kind, w.o);
     Cut c, cp, cw;
-    // dx goes with its dW where the estimates say so.  dh's epilogue moves bytes:
-    // two 128 x 128 tiles on a CU hide half of them behind dWd's products, one 256
-    // x 256 tile none, and large tiles lose in an L2 that holds two working sets.
-    // With these terms and without, of the best of apart and both tiles on 118
-    // backward passes (300 to 8192 tokens, 768 x 2048 to 4096 x 11008): dh 1.1%
-    // slower on average and 1.7%, dx 0.6%.  2048 tokens, 768 x 2048 fp32: dh and
-    // dWd apart 285 us, on 128 x 128 tiles 266; 8192 tokens, 2048 x 8192 bf16:
-    // apart 1328, on 256 x 256 tiles 1369.
+    // dx goes with its dW where the estimates say so by more than a launch's share
+    // (8192 tokens, 4096 x 14336 bf16, the whole pass: 6560 us apart, 6650 in
+    // pairs).  dh's epilogue moves bytes: two 128 x 128 tiles on a CU hide half of
+    // them behind dWd's products, one 256 x 256 tile none, and large tiles lose in
+    // an L2 that holds two working sets.  Of the best of apart and both tiles on
+    // 118 backward passes (300 to 8192 tokens, 768 x 2048 to 4096 x 11008) dh is
+    // 1.1% slower on average, dx 0.6%.  2048 tokens, 768 x 2048 fp32: dh and dWd
+    // apart 285 us, on 128 x 128 tiles 266; 8192 tokens, 2048 x 8192 bf16: apart
+    // 1328, on 256 x 256 tiles 1369.
     const double apart = choose(x, c) + choose(y, c) + 3;
-    if (choose_pair(x, y, cp, cw) > apart + 0.5 * x.moved / 5e6 * x.M * x.N) {
+    if (1.005 * choose_pair(x, y, cp, cw) > apart + 0.5 * x.moved / 5e6 * x.M * x.N) {
       run(p);
       run(w);
       return;
