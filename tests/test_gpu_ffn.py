@@ -108,6 +108,13 @@ def test_many_tiles(hip_device, dtype):
 
 
 @pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("tokens,d,f", [(1000, 129, 4099), (1023, 777, 2049), (1490, 1537, 4097)])
+def test_down_projections_between(hip_device, dtype, tokens, d, f):
+    """Too few columns for 256 x 256 tiles, rows enough for 256 x 128, in parts."""
+    _check(hip_device, tokens, d, f, dtype)
+
+
+@pytest.mark.parametrize("dtype", TYPES)
 @pytest.mark.parametrize("kw", [dict(pad=8), dict(pad=3), dict(skip=1), dict(pad=64, skip=8),
                                 dict(packed=True), dict(packed=True, pad=5, skip=3)])
 @pytest.mark.parametrize("d,f", [(96, 144), (97, 141)])

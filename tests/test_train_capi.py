@@ -54,6 +54,7 @@ BAD_CLIP = [
     ([(4097, 10, 1)], 2, 1.0, 1.0, P, P),
     ([(4096, -1, 0)], 2, 1.0, 1.0, P, P),
     ([(4096, 10, 3)], 2, 1.0, 1.0, P, P),
+    ([(1 << 57, 10, 0)], 2, 1.0, 1.0, P, P),   # no address
 ]
 
 
