@@ -65,6 +65,8 @@ class _Gradients:
             parameters = [parameters]
         elif not isinstance(parameters, (list, tuple)):
             parameters = list(parameters)
+        # until the kernels are queued: an iterator's parameters may live here alone
+        self._parameters = parameters
         self.copies = []   # (gradient, its copy)
         found = L.torch_host().gradients(parameters)
         if found is not None:
