@@ -53,7 +53,7 @@ enum scao_activation {
   SCAO_ACT_SILU = 0,        /* a / (1 + exp(-a))                                 */
   SCAO_ACT_GELU = 1,        /* a (1 + erf(a / sqrt 2)) / 2                       */
   SCAO_ACT_GELU_TANH = 2,   /* a (1 + tanh(sqrt(2/pi) (a + 0.044715 a^3))) / 2   */
-  SCAO_ACT_RELU = 3,        /* a where a > 0, else 0                             */
+  SCAO_ACT_RELU = 3,        /* a where a > 0 or a is NaN, else 0                  */
   SCAO_ACT_SIGMOID = 4      /* 1 / (1 + exp(-a))                                 */
 };
 typedef struct scao_ffn_desc {   /* HOST */

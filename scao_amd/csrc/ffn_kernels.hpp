@@ -67,8 +67,7 @@ __device__ __forceinline__ void activation(float a, float& f, float& g) {
     f = s;
     g = s * (1.f - s);
   } else if (ACT == SCAO_ACT_RELU) {
-    // a NaN stays one, as in a product with (a > 0)
-    f = a > 0.f ? a : a * 0.f;
+    f = a > 0.f || a != a ? a : 0.f;   // a NaN stays one, minus infinity does not become one
     g = a > 0.f ? 1.f : 0.f;
   } else if (ACT == SCAO_ACT_GELU) {
     // erfc(z) = t (a1 + t (a2 + ... )) exp(-z^2), t = 1 / (1 + 0.3275911 z), z >= 0,

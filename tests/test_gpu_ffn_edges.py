@@ -1,0 +1,65 @@
+"""The feed-forward block at the ends of what it takes: infinite
+pre-activations, rows of any stride, sizes of one, tracing, forward mode.
+
+Where a call is compared with the same call on contiguous copies the bits have
+to be equal; everything else has an exact result (zero or NaN)."""
+
+from __future__ import annotations
+
+import math
+
+import pytest
+import torch
+
+import scao_amd
+
+pytestmark = pytest.mark.gpu
+
+TYPES = [torch.bfloat16, torch.float16, torch.float32]
+
+
+def _normal(dev, seed, *shape, dtype=torch.bfloat16, std=1.0):
+    g = torch.Generator(device=dev).manual_seed(seed)
+    return (torch.randn(*shape, generator=g, device=dev) * std).to(dtype)
+
+
+def _inputs(dev, tokens, d, f, dtype=torch.bfloat16):
+    return [_normal(dev, 0, tokens, d, dtype=dtype),
+            _normal(dev, 1, f, d, dtype=dtype, std=d ** -0.5),
+            _normal(dev, 2, f, d, dtype=dtype, std=d ** -0.5),
+            _normal(dev, 3, d, f, dtype=dtype, std=f ** -0.5),
+            _normal(dev, 4, tokens, d, dtype=dtype)]
+
+
+def _run(x, gate, up, down, dy, name="silu"):
+    leaves = [t.detach().requires_grad_() for t in (x, gate, up, down)]
+    y = scao_amd.gated_ffn(*leaves, activation=name)
+    grads = torch.autograd.grad(y, leaves, dy)
+    return dict(y=y.detach(), **dict(zip(("dx", "dgate", "dup", "ddown"), grads)))
+
+
+def _same(got, want):
+    for k in want:
+        assert torch.equal(got[k], want[k]), k
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("tokens,d,f", [(5, 8, 16), (33, 41, 53), (300, 72, 130)])
+def test_relu_of_minus_infinity_is_zero(hip_device, dtype, tokens, d, f):
+    """Every pre-activation is minus infinity: from a sum that overflows (fp32,
+    bf16; powers of two, whose split parts are zero) or from a weight (16-bit)."""
+    x, gate, up, down, dy = _inputs(hip_device, tokens, d, f, dtype)
+    up[:, 0] = 0
+    for large in ([2.0 ** 80] if dtype != torch.float16 else []) + \
+                 ([math.inf] if dtype != torch.float32 else []):
+        x[:, 0] = 1.0 if math.isinf(large) else large
+        gate[:, 0] = -large
+        got = _run(x, gate, up, down, dy, "relu")
+        got["forward"] = scao_amd.gated_ffn(x, gate, up, down, "relu")
+        if math.isinf(large):
+            del got["dx"]   # 0 * infinity
+        for k, v in got.items():
+            assert bool(v.eq(0).all()), (k, large)
+    x[tokens // 2, 1] = math.nan
+    y = scao_amd.gated_ffn(x, gate, up, down, "relu")
+    assert bool(y[tokens // 2].isnan().all()) and int(y.isnan().sum()) == d
