@@ -41,8 +41,9 @@ int scao_grad_clip(const scao_tensor_desc* tensors, int n, int norm_type, double
 
 /* ---- gated feed-forward block ---------------------------------------------
  * a = x Wg^T, b = x Wu^T, h = f(a) * b, y = h Wd^T, all row-major: x tokens x d,
- * Wg and Wu f x d, Wd d x f, y tokens x d, with unit column stride and any row
- * stride of at least a row; fp32, bf16 or fp16, one type for all.  Sums are
+ * Wg and Wu f x d, Wd d x f, y tokens x d, with unit column stride and a row
+ * stride of at least a row and less than 2^21 elements (that of a single row is
+ * not looked at); fp32, bf16 or fp16, one type for all.  Sums are
  * fp32.  With `saved` (scao_ffn_saved_bytes() bytes) the forward pass keeps h, a
  * and b for scao_ffn_backward: dh = dy Wd, da = dh * b * f'(a), db = dh * f(a),
  * dx = da Wg + db Wu, dWg = da^T x, dWu = db^T x, dWd = dy^T h, each written

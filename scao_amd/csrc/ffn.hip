@@ -477,7 +477,8 @@ int check_matrix(const char* who, const char* name, const void* p, int64_t ld, i
                  int64_t cols, int dtype) {
   SCAO_CHECK_ARG(p && (uintptr_t)p % size_of(dtype) == 0,
                  "%s: %s is null or not aligned to its elements", who, name);
-  SCAO_CHECK_ARG((rows == 1 || ld >= cols) && ld < ((int64_t)1 << 21),
+  // (a single row's stride is never used)
+  SCAO_CHECK_ARG(rows == 1 || (ld >= cols && ld < ((int64_t)1 << 21)),
                  "%s: row stride %lld of %s (%lld columns; at most 2^21 - 1)", who, (long long)ld,
                  name, (long long)cols);
   return SCAO_OK;

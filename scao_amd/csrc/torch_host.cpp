@@ -55,6 +55,8 @@ Tensor bytes(int64_t n, const Tensor& like) {
 }
 
 // ------------------------------------------------------------- gated_ffn ---
+constexpr int64_t MAX_STRIDE = (int64_t)1 << 21;   // of rows that scao_ffn_* take
+
 // x, w_gate, w_up, w_down: 2-D, unit column stride, rows that do not overlap,
 // matching sizes, type and device (the caller has checked them)
 scao_ffn_desc describe(const Tensor& x, const Tensor& g, const Tensor& u, const Tensor& d,
@@ -98,7 +100,9 @@ struct GatedFFN : torch::autograd::Function<GatedFFN> {
       const at::NoGradGuard no_grad;
       const c10::DeviceGuard guard(x.device());
       Tensor dy = grads[0];
-      if (dy.stride(1) != 1 || (dy.size(0) > 1 && dy.stride(0) < dy.size(1))) dy = dy.contiguous();
+      if (dy.stride(1) != 1 ||
+          (dy.size(0) > 1 && (dy.stride(0) < dy.size(1) || dy.stride(0) >= MAX_STRIDE)))
+        dy = dy.contiguous();
       const scao_ffn_desc desc = describe(x, g, u, d, ctx->saved_data["act"].toInt());
       int want = 0;
       const Tensor* like[4] = {&x, &g, &u, &d};

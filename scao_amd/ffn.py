@@ -45,11 +45,14 @@ def _check(x: Tensor, w_gate: Tensor, w_up: Tensor, w_down: Tensor, activation: 
     return act
 
 
+_MAX_STRIDE = 1 << 21   # of rows, in elements: what scao_ffn_forward takes
+
+
 def _rows(t: Tensor) -> Tensor:
     """2-D with unit column stride and rows that do not overlap."""
     if t.dim() != 2:
         t = t.reshape(-1, t.shape[-1])
-    if t.stride(1) != 1 or (t.shape[0] > 1 and t.stride(0) < t.shape[1]):
+    if t.stride(1) != 1 or (t.shape[0] > 1 and not t.shape[1] <= t.stride(0) < _MAX_STRIDE):
         t = t.contiguous()
     return t
 
@@ -62,10 +65,11 @@ def gated_ffn(x: Tensor, w_gate: Tensor, w_up: Tensor, w_down: Tensor,
     x: ``(..., d_model)``; w_gate, w_up: ``(d_ff, d_model)``; w_down: ``(d_model,
     d_ff)``, all float32, bfloat16 or float16 on one ROCm device.  Rows may have
     any stride (the halves of a packed gate-and-up weight, a slice of a wider
-    input) and start at any element; columns of another stride are copied first.
-    Sums are float32; the 16-bit types round h, and in the backward pass the
-    gradients of both projections, once to the type before the next product.
-    Differentiable once, in any of the four arguments."""
+    input) and start at any element; columns of another stride, and rows 2^21
+    elements and more apart, are copied first.  Sums are float32; the 16-bit
+    types round h, and in the backward pass the gradients of both projections,
+    once to the type before the next product.  Differentiable once, in any of
+    the four arguments."""
     act = _check(x, w_gate, w_up, w_down, activation)
     if x.numel() == 0 or w_gate.numel() == 0:
         # no token, or a sum over nothing: zeros, with gradients that are zeros

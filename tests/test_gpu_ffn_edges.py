@@ -63,3 +63,41 @@ def test_relu_of_minus_infinity_is_zero(hip_device, dtype, tokens, d, f):
     x[tokens // 2, 1] = math.nan
     y = scao_amd.gated_ffn(x, gate, up, down, "relu")
     assert bool(y[tokens // 2].isnan().all()) and int(y.isnan().sum()) == d
+
+
+def _wide(t, stride):
+    """t's values in rows that begin `stride` elements apart"""
+    out = torch.zeros(t.shape[0] * stride, dtype=t.dtype, device=t.device).view(-1, stride)
+    out[:, :t.shape[1]] = t
+    return out[:, :t.shape[1]]
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("tokens,d,f", [(1, 64, 24), (3, 64, 24), (70, 33, 9)])
+def test_rows_of_any_stride(hip_device, dtype, tokens, d, f):
+    """Rows 2^21 elements and more apart, in every matrix and in dy, and the
+    last token of a long prompt."""
+    ins = _inputs(hip_device, tokens, d, f, dtype)
+    want, forward = _run(*ins), scao_amd.gated_ffn(*ins[:4])
+    for i in range(5):
+        moved = list(ins)
+        moved[i] = _wide(ins[i], (1 << 21) + 8 * i)
+        _same(_run(*moved), want)
+        if i < 4:
+            assert torch.equal(scao_amd.gated_ffn(*moved[:4]), forward)
+    hidden = torch.zeros(tokens, (1 << 21) // 64, 64, dtype=dtype, device=hip_device)[:, :, :d]
+    hidden[:, -1] = ins[0]
+    assert torch.equal(scao_amd.gated_ffn(hidden[:, -1], *ins[1:4]), forward)
+
+
+def test_outputs_taken_from_a_long_sequence(hip_device):
+    """The gradient of the output arrives as rows of a much larger one."""
+    ins = _inputs(hip_device, 3, 64, 24)
+    want = _run(*ins)
+    leaves = [t.detach().requires_grad_() for t in ins[:4]]
+    y = scao_amd.gated_ffn(*leaves)
+    long = torch.zeros(3, (1 << 21) // 64, 64, dtype=y.dtype, device=hip_device)
+    grads = torch.autograd.grad(torch.cat([y[:, None], long], 1), leaves,
+                                torch.cat([ins[4][:, None], long], 1))
+    _same(dict(zip(("dx", "dgate", "dup", "ddown"), grads)),
+          {k: v for k, v in want.items() if k != "y"})
