@@ -100,7 +100,7 @@ struct GatedFFN : torch::autograd::Function<GatedFFN> {
       const at::NoGradGuard no_grad;
       const c10::DeviceGuard guard(x.device());
       Tensor dy = grads[0];
-      if (dy.stride(1) != 1 ||
+      if ((dy.stride(1) != 1 && dy.size(1) != 1) ||
           (dy.size(0) > 1 && (dy.stride(0) < dy.size(1) || dy.stride(0) >= MAX_STRIDE)))
         dy = dy.contiguous();
       const scao_ffn_desc desc = describe(x, g, u, d, ctx->saved_data["act"].toInt());
@@ -147,7 +147,7 @@ PyObject* gated_ffn(PyObject*, PyObject* const* args, Py_ssize_t n) {
   const Tensor &x = THPVariable_Unpack(args[0]), &g = THPVariable_Unpack(args[1]),
                &u = THPVariable_Unpack(args[2]), &d = THPVariable_Unpack(args[3]);
   for (const Tensor* t : {&x, &g, &u, &d})
-    TORCH_CHECK(t->dim() == 2 && t->stride(1) == 1, "gated_ffn() takes rows");
+    TORCH_CHECK(t->dim() == 2 && (t->stride(1) == 1 || t->size(1) == 1), "gated_ffn() takes rows");
   if (at::GradMode::is_enabled() && (x.requires_grad() || g.requires_grad() ||
                                      u.requires_grad() || d.requires_grad()))
     return THPVariable_Wrap(GatedFFN::apply(x, g, u, d, (int64_t)act));

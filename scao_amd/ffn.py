@@ -49,10 +49,12 @@ _MAX_STRIDE = 1 << 21   # of rows, in elements: what scao_ffn_forward takes
 
 
 def _rows(t: Tensor) -> Tensor:
-    """2-D with unit column stride and rows that do not overlap."""
+    """2-D with unit column stride and rows that do not overlap.  (A single column
+    may have any stride: torch calls it contiguous, and a copy would keep it.)"""
     if t.dim() != 2:
         t = t.reshape(-1, t.shape[-1])
-    if t.stride(1) != 1 or (t.shape[0] > 1 and not t.shape[1] <= t.stride(0) < _MAX_STRIDE):
+    if (t.stride(1) != 1 and t.shape[1] != 1) or \
+            (t.shape[0] > 1 and not t.shape[1] <= t.stride(0) < _MAX_STRIDE):
         t = t.contiguous()
     return t
 

@@ -101,3 +101,22 @@ def test_outputs_taken_from_a_long_sequence(hip_device):
                                 torch.cat([ins[4][:, None], long], 1))
     _same(dict(zip(("dx", "dgate", "dup", "ddown"), grads)),
           {k: v for k, v in want.items() if k != "y"})
+
+
+def _column(t):
+    """a tensor of one column whose column stride is not one"""
+    return t.t().contiguous().t() if t.shape[1] == 1 else t
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("tokens,d,f", [(5, 1, 7), (5, 7, 1), (70, 1, 9), (1, 1, 1)])
+def test_single_columns_of_any_stride(hip_device, dtype, tokens, d, f):
+    """Torch ignores the stride of a dimension of one, and calls such a tensor
+    contiguous whatever it is."""
+    ins = _inputs(hip_device, tokens, d, f, dtype)
+    want, forward = _run(*ins), scao_amd.gated_ffn(*ins[:4])
+    odd = [_column(t).as_strided(t.shape, (1, 5)) if t.shape[1] == 1 else t for t in ins]
+    assert any(t.stride(1) == 5 for t in odd)
+    assert all(torch.equal(a, b) for a, b in zip(odd, ins))
+    _same(_run(*odd), want)
+    assert torch.equal(scao_amd.gated_ffn(*odd[:4]), forward)
