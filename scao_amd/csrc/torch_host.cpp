@@ -4,18 +4,20 @@
 //   gradients   the table of a model's gradients (scao_tensor_desc): reading six
 //               properties of 332 tensors from Python takes 125 us, their norm
 //               and scaling 25
-//   gated_ffn   the feed-forward block as a node of torch's graph, its backward
-//               pass without the interpreter: a small block's training step took
-//               145 us of host time as a Python function
+//   gated_ffn   the feed-forward block as an operator of torch's dispatcher, its
+//               backward pass without the interpreter: a small block's training
+//               step took 145 us of host time as a Python function
 //   bind        the addresses of the C ABI's entry points, which the caller has
 //               loaded (so that one library is used, whichever it is)
 #include <ATen/ATen.h>
+#include <ATen/core/LegacyTypeDispatch.h>
 #include <c10/core/DeviceGuard.h>
 #include <c10/hip/HIPStream.h>
 #include <torch/csrc/Exceptions.h>
 #include <torch/csrc/autograd/custom_function.h>
 #include <torch/csrc/autograd/functions/basic_ops.h>
 #include <torch/csrc/autograd/python_variable.h>
+#include <torch/library.h>
 
 #include "../../include/scao_train.h"
 
@@ -55,10 +57,62 @@ Tensor bytes(int64_t n, const Tensor& like) {
 }
 
 // ------------------------------------------------------------- gated_ffn ---
+// Operators of torch's dispatcher, so that what follows a program by its
+// operators (tracers, dispatch modes, negated views, tensor subclasses) finds the
+// block among them, or refuses it:
+//   gated_ffn           without a gradient
+//   gated_ffn_save      the same, and what the backward pass needs
+//   gated_ffn_backward  the wanted gradients (bits SCAO_FFN_DX ...) in order
 constexpr int64_t MAX_STRIDE = (int64_t)1 << 21;   // of rows that scao_ffn_* take
 
-// x, w_gate, w_up, w_down: 2-D, unit column stride, rows that do not overlap,
-// matching sizes, type and device (the caller has checked them)
+Tensor op_gated_ffn(const Tensor& x, const Tensor& g, const Tensor& u, const Tensor& d,
+                    int64_t act) {
+  static const auto op = c10::Dispatcher::singleton()
+                             .findSchemaOrThrow("scao_amd::gated_ffn", "")
+                             .typed<decltype(op_gated_ffn)>();
+  return op.call(x, g, u, d, act);
+}
+std::tuple<Tensor, Tensor> op_gated_ffn_save(const Tensor& x, const Tensor& g, const Tensor& u,
+                                             const Tensor& d, int64_t act) {
+  static const auto op = c10::Dispatcher::singleton()
+                             .findSchemaOrThrow("scao_amd::gated_ffn_save", "")
+                             .typed<decltype(op_gated_ffn_save)>();
+  return op.call(x, g, u, d, act);
+}
+std::vector<Tensor> op_gated_ffn_backward(const Tensor& dy, const Tensor& saved, const Tensor& x,
+                                          const Tensor& g, const Tensor& u, const Tensor& d,
+                                          int64_t act, int64_t wanted) {
+  static const auto op = c10::Dispatcher::singleton()
+                             .findSchemaOrThrow("scao_amd::gated_ffn_backward", "")
+                             .typed<decltype(op_gated_ffn_backward)>();
+  return op.call(dy, saved, x, g, u, d, act, wanted);
+}
+
+// sizes, types and devices, whoever calls
+void check_block(const Tensor& x, const Tensor& g, const Tensor& u, const Tensor& d) {
+  TORCH_CHECK(lib.forward, "gated_ffn: scao_amd has not loaded its library");
+  TORCH_CHECK(x.dim() == 2 && g.dim() == 2 && u.dim() == 2 && d.dim() == 2,
+              "gated_ffn takes matrices");
+  TORCH_CHECK(x.sym_size(1) == g.sym_size(1) && u.sym_sizes() == g.sym_sizes() &&
+                  d.sym_size(0) == g.sym_size(1) && d.sym_size(1) == g.sym_size(0),
+              "gated_ffn: shape mismatch: x ", x.sym_sizes(), ", w_gate ", g.sym_sizes(),
+              ", w_up ", u.sym_sizes(), ", w_down ", d.sym_sizes());
+  for (const Tensor* t : {&x, &g, &u, &d})
+    TORCH_CHECK(code_of(t->scalar_type()) >= 0 && t->scalar_type() == x.scalar_type() &&
+                    t->device() == x.device(),
+                "gated_ffn takes float32, bfloat16 or float16 tensors of one type and device");
+}
+
+// t with unit column stride and rows that do not overlap and that scao_ffn_* take.
+// (A single column may have any stride: torch calls it contiguous, and a copy
+// would keep it.)
+Tensor rows(const Tensor& t) {
+  const bool unit = t.stride(1) == 1 || t.size(1) == 1;
+  const bool apart = t.size(0) <= 1 || (t.stride(0) >= t.size(1) && t.stride(0) < MAX_STRIDE);
+  return unit && apart ? t : t.contiguous();
+}
+
+// of matrices that rows() has made
 scao_ffn_desc describe(const Tensor& x, const Tensor& g, const Tensor& u, const Tensor& d,
                        int64_t act) {
   return scao_ffn_desc{x.data_ptr(),  g.data_ptr(),  u.data_ptr(),        d.data_ptr(),
@@ -67,11 +121,13 @@ scao_ffn_desc describe(const Tensor& x, const Tensor& g, const Tensor& u, const 
                        (int32_t)act};
 }
 
-std::pair<Tensor, Tensor> forward(const Tensor& x, const Tensor& g, const Tensor& u,
-                                  const Tensor& d, int64_t act, bool save) {
-  const c10::DeviceGuard guard(x.device());
+std::tuple<Tensor, Tensor> forward(const Tensor& x_, const Tensor& g_, const Tensor& u_,
+                                   const Tensor& d_, int64_t act, bool save) {
+  check_block(x_, g_, u_, d_);
+  const c10::DeviceGuard guard(x_.device());
+  const Tensor x = rows(x_), g = rows(g_), u = rows(u_), d = rows(d_);
   const scao_ffn_desc desc = describe(x, g, u, d, act);
-  Tensor y = at::empty({x.size(0), x.size(1)}, x.options().requires_grad(false)), saved;
+  Tensor y = at::empty({x.size(0), x.size(1)}, x.options()), saved;
   if (save) saved = bytes(lib.saved_bytes(&desc), x);
   const Tensor work = bytes(lib.forward_workspace(&desc, save), x);
   check(lib.forward(&desc, y.data_ptr(), save ? saved.data_ptr() : nullptr, work.data_ptr(),
@@ -79,11 +135,80 @@ std::pair<Tensor, Tensor> forward(const Tensor& x, const Tensor& g, const Tensor
         "scao_ffn_forward");
   return {y, saved};
 }
+Tensor gated_ffn_hip(const Tensor& x, const Tensor& g, const Tensor& u, const Tensor& d,
+                     int64_t act) {
+  return std::get<0>(forward(x, g, u, d, act, false));
+}
+std::tuple<Tensor, Tensor> gated_ffn_save_hip(const Tensor& x, const Tensor& g, const Tensor& u,
+                                              const Tensor& d, int64_t act) {
+  return forward(x, g, u, d, act, true);
+}
+
+std::vector<Tensor> gated_ffn_backward_hip(const Tensor& dy_, const Tensor& saved,
+                                           const Tensor& x_, const Tensor& g_, const Tensor& u_,
+                                           const Tensor& d_, int64_t act, int64_t wanted) {
+  check_block(x_, g_, u_, d_);
+  TORCH_CHECK(dy_.sizes() == x_.sizes() && dy_.scalar_type() == x_.scalar_type() &&
+                  dy_.device() == x_.device(),
+              "gated_ffn_backward: dy is not like x");
+  const c10::DeviceGuard guard(x_.device());
+  const Tensor x = rows(x_), g = rows(g_), u = rows(u_), d = rows(d_), dy = rows(dy_);
+  const scao_ffn_desc desc = describe(x, g, u, d, act);
+  TORCH_CHECK(saved.scalar_type() == at::kByte && saved.device() == x.device() &&
+                  saved.is_contiguous() && saved.numel() == lib.saved_bytes(&desc),
+              "gated_ffn_backward: saved is not what gated_ffn_save returned");
+  static_assert(SCAO_FFN_DX == 1 && SCAO_FFN_DGATE == 2 && SCAO_FFN_DUP == 4 &&
+                    SCAO_FFN_DDOWN == 8,
+                "the inputs' order");
+  std::vector<Tensor> out;
+  const Tensor* like[4] = {&x, &g, &u, &d};
+  void* to[4] = {};
+  for (int i = 0; i < 4; ++i) {
+    if (!(wanted >> i & 1)) continue;
+    out.push_back(at::empty({like[i]->size(0), like[i]->size(1)}, x.options()));
+    to[i] = out.back().data_ptr();
+  }
+  const Tensor work =
+      bytes(lib.backward_workspace(&desc, dy.data_ptr(), dy.stride(0), (int)wanted & 15), x);
+  check(lib.backward(&desc, dy.data_ptr(), dy.stride(0), saved.data_ptr(), to[0], to[1], to[2],
+                     to[3], work.data_ptr(), stream_of(x)),
+        "scao_ffn_backward");
+  return out;
+}
+
+// shapes alone, for tensors without memory
+Tensor like(const Tensor& t) { return at::empty_symint(t.sym_sizes(), t.options()); }
+Tensor gated_ffn_meta(const Tensor& x, const Tensor& g, const Tensor& u, const Tensor& d,
+                      int64_t) {
+  check_block(x, g, u, d);
+  return like(x);
+}
+std::tuple<Tensor, Tensor> gated_ffn_save_meta(const Tensor& x, const Tensor& g, const Tensor& u,
+                                               const Tensor& d, int64_t act) {
+  check_block(x, g, u, d);
+  scao_ffn_desc desc{};
+  desc.tokens = x.sym_size(0).guard_int(__FILE__, __LINE__);
+  desc.d = g.sym_size(1).guard_int(__FILE__, __LINE__);
+  desc.f = g.sym_size(0).guard_int(__FILE__, __LINE__);
+  desc.dtype = code_of(x.scalar_type());
+  desc.act = (int32_t)act;
+  return {like(x), bytes(lib.saved_bytes(&desc), x)};
+}
+std::vector<Tensor> gated_ffn_backward_meta(const Tensor&, const Tensor&, const Tensor& x,
+                                            const Tensor& g, const Tensor& u, const Tensor& d,
+                                            int64_t, int64_t wanted) {
+  std::vector<Tensor> out;
+  int i = 0;
+  for (const Tensor* t : {&x, &g, &u, &d})
+    if (wanted >> i++ & 1) out.push_back(like(*t));
+  return out;
+}
 
 struct GatedFFN : torch::autograd::Function<GatedFFN> {
   static Tensor forward(AutogradContext* ctx, const Tensor& x, const Tensor& g, const Tensor& u,
                         const Tensor& d, int64_t act) {
-    auto [y, saved] = ::forward(x, g, u, d, act, true);
+    const at::AutoDispatchBelowADInplaceOrView below;
+    auto [y, saved] = op_gated_ffn_save(x, g, u, d, act);
     ctx->save_for_backward({x, g, u, d, saved});
     ctx->saved_data["act"] = act;
     return y;
@@ -92,50 +217,57 @@ struct GatedFFN : torch::autograd::Function<GatedFFN> {
   static variable_list backward(AutogradContext* ctx, const variable_list& grads) {
     // (hooks on saved tensors may have moved them: their addresses are new)
     const variable_list t = ctx->get_saved_variables();
-    const Tensor &x = t[0], &g = t[1], &u = t[2], &d = t[3], &saved = t[4];
     variable_list out(5);
     if (!grads[0].defined()) return out;
-    const bool higher = at::GradMode::is_enabled();
+    int64_t wanted = 0;
+    for (int i = 0; i < 4; ++i) wanted |= (int64_t)ctx->needs_input_grad(i) << i;
+    variable_list have;
     {
-      const at::NoGradGuard no_grad;
-      const c10::DeviceGuard guard(x.device());
-      Tensor dy = grads[0];
-      if ((dy.stride(1) != 1 && dy.size(1) != 1) ||
-          (dy.size(0) > 1 && (dy.stride(0) < dy.size(1) || dy.stride(0) >= MAX_STRIDE)))
-        dy = dy.contiguous();
-      const scao_ffn_desc desc = describe(x, g, u, d, ctx->saved_data["act"].toInt());
-      int want = 0;
-      const Tensor* like[4] = {&x, &g, &u, &d};
-      void* to[4] = {};
-      for (int i = 0; i < 4; ++i) {
-        if (!ctx->needs_input_grad(i)) continue;
-        want |= 1 << i;
-        out[i] = at::empty({like[i]->size(0), like[i]->size(1)},
-                           x.options().requires_grad(false));
-        to[i] = out[i].data_ptr();
-      }
-      static_assert(SCAO_FFN_DX == 1 && SCAO_FFN_DGATE == 2 && SCAO_FFN_DUP == 4 &&
-                        SCAO_FFN_DDOWN == 8,
-                    "the inputs' order");
-      const Tensor work =
-          bytes(lib.backward_workspace(&desc, dy.data_ptr(), dy.stride(0), want), x);
-      check(lib.backward(&desc, dy.data_ptr(), dy.stride(0), saved.data_ptr(), to[0], to[1], to[2],
-                         to[3], work.data_ptr(), stream_of(x)),
-            "scao_ffn_backward");
+      const at::AutoDispatchBelowADInplaceOrView below;
+      have = op_gated_ffn_backward(grads[0], t[4], t[0], t[1], t[2], t[3],
+                                   ctx->saved_data["act"].toInt(), wanted);
     }
-    if (higher) {   // a gradient of these gradients is an error, not a zero
+    if (at::GradMode::is_enabled()) {   // a gradient of these gradients is an error, not a zero
       const auto error = std::make_shared<torch::autograd::DelayedError>(
           "gated_ffn is differentiable once", 4);
-      variable_list have;
-      for (int i = 0; i < 4; ++i)
-        if (out[i].defined()) have.push_back(out[i].requires_grad_(true));
+      for (Tensor& g : have) g.requires_grad_(true);
       have = (*error)(std::move(have));
-      for (int i = 0, k = 0; i < 4; ++i)
-        if (out[i].defined()) out[i] = have[k++];
     }
+    for (int i = 0, k = 0; i < 4; ++i)
+      if (wanted >> i & 1) out[i] = have[k++];
     return out;
   }
 };
+
+Tensor gated_ffn_autograd(const Tensor& x, const Tensor& g, const Tensor& u, const Tensor& d,
+                          int64_t act) {
+  check_block(x, g, u, d);
+  if (at::GradMode::is_enabled() && (x.requires_grad() || g.requires_grad() ||
+                                     u.requires_grad() || d.requires_grad()))
+    // (what rows() copies, it copies here once for both passes)
+    return GatedFFN::apply(rows(x), rows(g), rows(u), rows(d), act);
+  const at::AutoDispatchBelowADInplaceOrView below;
+  return op_gated_ffn(x, g, u, d, act);
+}
+
+TORCH_LIBRARY(scao_amd, m) {
+#define SCAO_BLOCK "Tensor x, Tensor w_gate, Tensor w_up, Tensor w_down, int activation"
+  m.def("gated_ffn(" SCAO_BLOCK ") -> Tensor");
+  m.def("gated_ffn_save(" SCAO_BLOCK ") -> (Tensor, Tensor)");
+  m.def("gated_ffn_backward(Tensor dy, Tensor saved, " SCAO_BLOCK ", int wanted) -> Tensor[]");
+#undef SCAO_BLOCK
+}
+TORCH_LIBRARY_IMPL(scao_amd, CUDA, m) {
+  m.impl("gated_ffn", gated_ffn_hip);
+  m.impl("gated_ffn_save", gated_ffn_save_hip);
+  m.impl("gated_ffn_backward", gated_ffn_backward_hip);
+}
+TORCH_LIBRARY_IMPL(scao_amd, Meta, m) {
+  m.impl("gated_ffn", gated_ffn_meta);
+  m.impl("gated_ffn_save", gated_ffn_save_meta);
+  m.impl("gated_ffn_backward", gated_ffn_backward_meta);
+}
+TORCH_LIBRARY_IMPL(scao_amd, Autograd, m) { m.impl("gated_ffn", gated_ffn_autograd); }
 
 PyObject* gated_ffn(PyObject*, PyObject* const* args, Py_ssize_t n) {
   HANDLE_TH_ERRORS
@@ -144,14 +276,9 @@ PyObject* gated_ffn(PyObject*, PyObject* const* args, Py_ssize_t n) {
     TORCH_CHECK_TYPE(THPVariable_Check(args[i]), "gated_ffn() takes tensors");
   const long act = PyLong_AsLong(args[4]);
   if (act == -1 && PyErr_Occurred()) return nullptr;
-  const Tensor &x = THPVariable_Unpack(args[0]), &g = THPVariable_Unpack(args[1]),
-               &u = THPVariable_Unpack(args[2]), &d = THPVariable_Unpack(args[3]);
-  for (const Tensor* t : {&x, &g, &u, &d})
-    TORCH_CHECK(t->dim() == 2 && (t->stride(1) == 1 || t->size(1) == 1), "gated_ffn() takes rows");
-  if (at::GradMode::is_enabled() && (x.requires_grad() || g.requires_grad() ||
-                                     u.requires_grad() || d.requires_grad()))
-    return THPVariable_Wrap(GatedFFN::apply(x, g, u, d, (int64_t)act));
-  return THPVariable_Wrap(forward(x, g, u, d, act, false).first);
+  return THPVariable_Wrap(op_gated_ffn(THPVariable_Unpack(args[0]), THPVariable_Unpack(args[1]),
+                                       THPVariable_Unpack(args[2]), THPVariable_Unpack(args[3]),
+                                       act));
   END_HANDLE_TH_ERRORS
 }
 

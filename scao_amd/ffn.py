@@ -6,8 +6,8 @@ with the weights in ``nn.Linear``'s layout (gate and up: ``d_ff x d_model``, dow
 ``d_model x d_ff``): the three largest matrices of a layer, whose gradients are
 what ``SCAO`` preconditions.  Both projections, the activation and the product
 are one kernel, the second projection another; a backward pass is four products
-(``scao_ffn_forward``, ``scao_ffn_backward``, called from csrc/torch_host.cpp as a
-node of torch's graph).  Everything runs on the current stream; nothing is kept
+(``scao_ffn_forward``, ``scao_ffn_backward``, called from csrc/torch_host.cpp as
+operators of torch's dispatcher).  Everything runs on the current stream; nothing is kept
 between calls.
 """
 
@@ -45,20 +45,6 @@ def _check(x: Tensor, w_gate: Tensor, w_up: Tensor, w_down: Tensor, activation: 
     return act
 
 
-_MAX_STRIDE = 1 << 21   # of rows, in elements: what scao_ffn_forward takes
-
-
-def _rows(t: Tensor) -> Tensor:
-    """2-D with unit column stride and rows that do not overlap.  (A single column
-    may have any stride: torch calls it contiguous, and a copy would keep it.)"""
-    if t.dim() != 2:
-        t = t.reshape(-1, t.shape[-1])
-    if (t.stride(1) != 1 and t.shape[1] != 1) or \
-            (t.shape[0] > 1 and not t.shape[1] <= t.stride(0) < _MAX_STRIDE):
-        t = t.contiguous()
-    return t
-
-
 def gated_ffn(x: Tensor, w_gate: Tensor, w_up: Tensor, w_down: Tensor,
               activation: str = "silu") -> Tensor:
     """``(f(x w_gate^T) * (x w_up^T)) w_down^T`` with f one of ``silu``, ``gelu``,
@@ -76,8 +62,10 @@ def gated_ffn(x: Tensor, w_gate: Tensor, w_up: Tensor, w_down: Tensor,
     if x.numel() == 0 or w_gate.numel() == 0:
         # no token, or a sum over nothing: zeros, with gradients that are zeros
         return ((x @ w_gate.t()) * (x @ w_up.t())) @ w_down.t()
-    y = L.torch_host().gated_ffn(_rows(x), _rows(w_gate), _rows(w_up), _rows(w_down), act)
-    return y if x.dim() == 2 else y.view(x.shape)
+    if x.dim() == 2:
+        return L.torch_host().gated_ffn(x, w_gate, w_up, w_down, act)
+    return L.torch_host().gated_ffn(x.reshape(-1, x.shape[-1]), w_gate, w_up, w_down,
+                                    act).view(x.shape)
 
 
 class GatedFFN(nn.Module):

@@ -120,3 +120,92 @@ def test_single_columns_of_any_stride(hip_device, dtype, tokens, d, f):
     assert all(torch.equal(a, b) for a, b in zip(odd, ins))
     _same(_run(*odd), want)
     assert torch.equal(scao_amd.gated_ffn(*odd[:4]), forward)
+
+
+def test_traces_hold_the_block(hip_device):
+    """A trace computes the block of the inputs that it is called with."""
+    from torch.fx.experimental.proxy_tensor import make_fx
+    x, gate, up, down, dy = _inputs(hip_device, 20, 24, 40)
+    new = _normal(hip_device, 7, 20, 24)
+
+    def forward(x):
+        return scao_amd.gated_ffn(x, gate, up, down)
+
+    def training(x, dy):
+        leaves = [t.detach().requires_grad_() for t in (x, gate, up, down)]
+        return torch.autograd.grad(scao_amd.gated_ffn(*leaves), leaves, dy)
+
+    for traced in (torch.jit.trace(forward, (x,)), make_fx(forward)(x)):
+        assert torch.equal(traced(new), forward(new))
+    traced = make_fx(training)(x, dy)
+    for got, want in zip(traced(new, 2 * dy), training(new, 2 * dy)):
+        assert torch.equal(got, want)
+
+
+def test_dispatch_modes_see_the_block(hip_device):
+    from torch.utils._python_dispatch import TorchDispatchMode
+    seen = []
+
+    class Log(TorchDispatchMode):
+        def __torch_dispatch__(self, func, types, args=(), kwargs=None):
+            seen.append(str(func))
+            return func(*args, **(kwargs or {}))
+
+    ins = _inputs(hip_device, 20, 24, 40)
+    want = _run(*ins)
+    with Log():
+        scao_amd.gated_ffn(*ins[:4])
+        got = _run(*ins)
+    _same(got, want)
+    assert {s.split(".")[1] for s in seen if s.startswith("scao_amd.")} == {
+        "gated_ffn", "gated_ffn_save", "gated_ffn_backward"}
+
+
+def test_operators_check_their_arguments(hip_device):
+    """Called by their names, past the Python function's own checks."""
+    x, gate, up, down, dy = _inputs(hip_device, 20, 24, 40)
+    scao_amd.gated_ffn(x, gate, up, down)
+    op = torch.ops.scao_amd.gated_ffn
+    assert torch.equal(op(x, gate, up, down, 0), scao_amd.gated_ffn(x, gate, up, down))
+    for bad in ((x, gate, up[:-1], down, 0), (x[:, :-1], gate, up, down, 0),
+                (x, gate, up, down.t(), 0), (x[0], gate, up, down, 0),
+                (x.float(), gate, up, down, 0), (x, gate, up, down, 5),
+                (x, gate, up, down.cpu(), 0), (x.double(),) * 4 + (0,)):
+        with pytest.raises(RuntimeError):
+            op(*bad)
+    y, saved = torch.ops.scao_amd.gated_ffn_save(x, gate, up, down, 0)
+    back = torch.ops.scao_amd.gated_ffn_backward
+    assert len(back(dy, saved, x, gate, up, down, 0, 15)) == 4
+    for bad in ((dy[:-1], saved), (dy, saved[:-1]), (dy, saved.cpu()), (dy.float(), saved)):
+        with pytest.raises(RuntimeError):
+            back(*bad, x, gate, up, down, 0, 15)
+
+
+def test_negated_views(hip_device):
+    """Tensors that hold their values negated, as the imaginary part of a
+    conjugate does."""
+    ins = _inputs(hip_device, 20, 24, 40)
+    want, forward = _run(*ins), scao_amd.gated_ffn(*ins[:4])
+    for i in range(5):
+        moved = list(ins)
+        moved[i] = torch._neg_view(-ins[i])
+        assert moved[i].is_neg()
+        _same(_run(*moved), want)
+        if i < 4:
+            assert torch.equal(scao_amd.gated_ffn(*moved[:4]), forward)
+
+
+def test_traces_without_memory(hip_device):
+    """A trace of shapes alone, and its run on real tensors."""
+    from torch.fx.experimental.proxy_tensor import make_fx
+    ins = _inputs(hip_device, 20, 24, 40)
+
+    def training(x, gate, up, down, dy):
+        leaves = [t.detach().requires_grad_() for t in (x, gate, up, down)]
+        y = scao_amd.gated_ffn(*leaves)
+        return y.detach(), *torch.autograd.grad(y, leaves, dy)
+
+    traced = make_fx(training, tracing_mode="fake")(*ins)
+    want = _run(*ins)
+    for got, k in zip(traced(*ins), want):
+        assert torch.equal(got, want[k])
