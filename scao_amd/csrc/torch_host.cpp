@@ -16,6 +16,7 @@
 #include <torch/csrc/Exceptions.h>
 #include <torch/csrc/autograd/custom_function.h>
 #include <torch/csrc/autograd/functions/basic_ops.h>
+#include <torch/csrc/autograd/functions/utils.h>
 #include <torch/csrc/autograd/python_variable.h>
 #include <torch/library.h>
 
@@ -242,6 +243,9 @@ struct GatedFFN : torch::autograd::Function<GatedFFN> {
 Tensor gated_ffn_autograd(const Tensor& x, const Tensor& g, const Tensor& u, const Tensor& d,
                           int64_t act) {
   check_block(x, g, u, d);
+  for (const Tensor* t : {&x, &g, &u, &d})   // a tangent would be lost
+    TORCH_CHECK_NOT_IMPLEMENTED(!torch::autograd::isFwGradDefined(*t),
+                                "gated_ffn has no forward-mode derivative");
   if (at::GradMode::is_enabled() && (x.requires_grad() || g.requires_grad() ||
                                      u.requires_grad() || d.requires_grad()))
     // (what rows() copies, it copies here once for both passes)

@@ -57,7 +57,7 @@ def gated_ffn(x: Tensor, w_gate: Tensor, w_up: Tensor, w_down: Tensor,
     elements and more apart, are copied first.  Sums are float32; the 16-bit
     types round h, and in the backward pass the gradients of both projections,
     once to the type before the next product.  Differentiable once, in any of
-    the four arguments."""
+    the four arguments, not in forward mode."""
     act = _check(x, w_gate, w_up, w_down, activation)
     if x.numel() == 0 or w_gate.numel() == 0:
         # no token, or a sum over nothing: zeros, with gradients that are zeros

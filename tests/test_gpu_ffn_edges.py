@@ -209,3 +209,16 @@ def test_traces_without_memory(hip_device):
     want = _run(*ins)
     for got, k in zip(traced(*ins), want):
         assert torch.equal(got, want[k])
+
+
+@pytest.mark.parametrize("which", range(4))
+@pytest.mark.parametrize("grad", [False, True])
+def test_forward_mode_is_refused(hip_device, which, grad):
+    import torch.autograd.forward_ad as fwd
+    ins = [t.requires_grad_(grad) for t in _inputs(hip_device, 20, 24, 40)[:4]]
+    with fwd.dual_level():
+        ins[which] = fwd.make_dual(ins[which], torch.ones_like(ins[which]))
+        with pytest.raises(RuntimeError, match="forward"):
+            scao_amd.gated_ffn(*ins)
+        with torch.no_grad(), pytest.raises(RuntimeError, match="forward"):
+            scao_amd.gated_ffn(*ins)
