@@ -23,7 +23,8 @@ extern "C" {
  * order, into *norm (device fp32).  scao_grad_clip then multiplies every
  * gradient by f = fp32(scale * min(1, max_norm / (N + 1e-6))), rounding once
  * to its type; with f = 1 nothing is written.  A NaN anywhere makes N and,
- * through f, every gradient NaN; an infinity makes N infinite and f zero.
+ * through f, every gradient NaN; an infinity makes N infinite and f zero, or
+ * scale where max_norm is infinite (which clips nothing).
  * Tensors start at any multiple of their element size and must not overlap
  * when they are clipped (SCAO_ERR_INVALID).  workspace:
  * scao_grad_norm_workspace() bytes. */

@@ -267,8 +267,9 @@ __global__ __launch_bounds__(THREADS) void k_scale(const Table tab, const double
   __shared__ double lds[4];
   const double n = total_norm<P>(parts, nparts, scale, lds);
   if (norm && blockIdx.x == 0 && threadIdx.x == 0) *norm = (float)n;
+  // (max_norm infinite: the factor is scale, with an infinite norm too)
   const double c = max_norm / (n + 1e-6);
-  const float factor = (float)(c < 1.0 || c != c ? scale * c : scale);
+  const float factor = (float)(c < 1.0 || n != n ? scale * c : scale);
   if (factor == 1.0f) return;
   walk<true, PAST>(tab, gridDim.x - 1 - blockIdx.x, [&](float x) { return x * factor; });
 }

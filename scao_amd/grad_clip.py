@@ -113,7 +113,8 @@ def clip_grad_norm_(parameters: Union[Tensor, Iterable[Tensor]], max_norm: float
     1e-6))`` with N = ``global_grad_norm(parameters, norm_type, scale)``, and
     return N (0-dim float32).  Each gradient is rounded once, to its type; with
     a factor of exactly 1 nothing is written.  A NaN in any gradient makes N and
-    all gradients NaN, an infinity makes N infinite and the factor 0, unless
+    all gradients NaN, an infinity makes N infinite and the factor 0 (``scale``
+    with a max_norm of infinity, which clips nothing), unless
     ``error_if_nonfinite``: then N is read back (the host waits for it) and a
     RuntimeError is raised with the gradients as they were.
 

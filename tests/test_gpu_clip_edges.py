@@ -43,3 +43,20 @@ def test_gradients_that_only_an_iterator_holds(hip_device):
 
         torch.cuda.synchronize()
         assert entry(temporaries()).item() == 2000.0
+
+
+@pytest.mark.parametrize("p", [1.0, 2.0, math.inf])
+@pytest.mark.parametrize("scale", [1.0, 0.5])
+def test_a_bound_of_infinity_clips_nothing(hip_device, p, scale):
+    """max_norm = inf measures: the factor is `scale`, with an infinite norm too."""
+    for bad in (None, math.inf, -math.inf):
+        g, h = _normal(hip_device, 4, 20000), _normal(hip_device, 5, 7, dtype=torch.bfloat16)
+        if bad is not None:
+            g[12345] = bad
+        want = [t * scale for t in (g, h)]
+        norm = scao_amd.clip_grad_norm_(_params([g, h]), math.inf, norm_type=p, scale=scale)
+        assert norm.item() == math.inf if bad is not None else math.isfinite(norm.item())
+        assert torch.equal(g, want[0]) and torch.equal(h, want[1])
+    g[3] = math.nan
+    norm = scao_amd.clip_grad_norm_(_params([g, h]), math.inf, norm_type=p)
+    assert math.isnan(norm.item()) and bool(g.isnan().all()) and bool(h.isnan().all())
