@@ -235,7 +235,7 @@ def torch_host():
         except ImportError as e:
             raise ScaoLibError(f"scao_amd: {HERE}/_torch_host.so is missing or does not fit this "
                                f"torch ({e}). Build it with `python -m scao_amd.build`.") from None
-        names = ("scao_last_error", *(n for n in TRAIN_SIGNATURES if n.startswith("scao_ffn")))
+        names = ("scao_last_error", *TRAIN_SIGNATURES)
         module.bind({n: ctypes.cast(getattr(lib(), n), _VP).value for n in names})
         _torch_host = module
     return _torch_host
@@ -251,21 +251,6 @@ def call(name: str, *args) -> None:
 
 def stream_ptr(device: torch.device) -> int:
     return torch.cuda.current_stream(device).cuda_stream
-
-
-_raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None)
-
-
-def call_on(device: torch.device, name: str, *args) -> None:
-    """``call`` with the current stream of ``device`` as the last argument, on
-    that device.  Where it is the current one already, as almost always, neither
-    a device guard nor a stream object is made (6 us of a short call)."""
-    index = device.index
-    if _raw_stream is not None and index == torch.cuda.current_device():
-        call(name, *args, _raw_stream(index))
-        return
-    with torch.cuda.device(device):
-        call(name, *args, stream_ptr(device))
 
 
 def upload(arr: np.ndarray, device: torch.device) -> torch.Tensor:

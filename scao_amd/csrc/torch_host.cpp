@@ -1,15 +1,17 @@
 // The Python module scao_amd._torch_host: what would cost more host time in
 // Python than the kernels take.
 //
-//   gradients   the table of a model's gradients (scao_tensor_desc): reading six
-//               properties of 332 tensors from Python takes 125 us, their norm
-//               and scaling 25
+//   grad_norm, grad_clip
+//               the norm of a model's gradients and their clipping as operators of
+//               torch's dispatcher: reading six properties of 332 tensors from
+//               Python takes 125 us, their norm and scaling 25
 //   gated_ffn   the feed-forward block as an operator of torch's dispatcher, its
 //               backward pass without the interpreter: a small block's training
 //               step took 145 us of host time as a Python function
 //   bind        the addresses of the C ABI's entry points, which the caller has
 //               loaded (so that one library is used, whichever it is)
 #include <ATen/ATen.h>
+#include <ATen/MemoryOverlap.h>
 #include <ATen/core/LegacyTypeDispatch.h>
 #include <c10/core/DeviceGuard.h>
 #include <c10/hip/HIPStream.h>
@@ -18,7 +20,10 @@
 #include <torch/csrc/autograd/functions/basic_ops.h>
 #include <torch/csrc/autograd/functions/utils.h>
 #include <torch/csrc/autograd/python_variable.h>
+#include <torch/csrc/utils/object_ptr.h>
 #include <torch/library.h>
+
+#include <cstring>
 
 #include "../../include/scao_train.h"
 
@@ -35,6 +40,9 @@ struct Entries {
   decltype(&scao_ffn_forward) forward;
   decltype(&scao_ffn_backward_workspace) backward_workspace;
   decltype(&scao_ffn_backward) backward;
+  decltype(&scao_grad_norm_workspace) grad_norm_workspace;
+  decltype(&scao_grad_norm) grad_norm;
+  decltype(&scao_grad_clip) grad_clip;
 } lib;
 
 void check(int rc, const char* who) {
@@ -286,50 +294,151 @@ PyObject* gated_ffn(PyObject*, PyObject* const* args, Py_ssize_t n) {
   END_HANDLE_TH_ERRORS
 }
 
-// ------------------------------------------------------------- gradients ---
-// gradients(parameters) -> (device index, count, table) or None.
-// The gradients of a list or tuple of tensors, those that have one, as an array
-// of scao_tensor_desc in a bytes object; None where any of them is not a dense
-// fp32, bf16 or fp16 tensor on the first one's GPU whose elements fill their
-// memory (in any order): those are for the caller to refuse or to copy.
-PyObject* gradients(PyObject*, PyObject* arg) {
-  PyObject* seq = PySequence_Fast(arg, "gradients() takes a list or a tuple");
-  if (!seq) return nullptr;
-  const Py_ssize_t n = PySequence_Fast_GET_SIZE(seq);
-  PyObject* out = PyBytes_FromStringAndSize(nullptr, n * (Py_ssize_t)sizeof(scao_tensor_desc));
-  if (!out) {
-    Py_DECREF(seq);
-    return nullptr;
-  }
-  auto* t = reinterpret_cast<scao_tensor_desc*>(PyBytes_AS_STRING(out));
-  Py_ssize_t count = 0;
-  int device = -1;
-  bool plain = true;
-  try {
-    for (Py_ssize_t i = 0; i < n && plain; ++i) {
-      PyObject* o = PySequence_Fast_GET_ITEM(seq, i);
-      if (!THPVariable_Check(o)) {
-        plain = false;
-        break;
-      }
-      const Tensor& g = THPVariable_Unpack(o).grad();
-      if (!g.defined()) continue;
-      const int code = g.layout() == at::kStrided && g.is_cuda() ? code_of(g.scalar_type()) : -1;
-      plain = code >= 0 && (device < 0 || g.device().index() == device) &&
-              g.is_non_overlapping_and_dense();
-      if (!plain) break;
-      device = g.device().index();
-      t[count++] = scao_tensor_desc{g.data_ptr(), g.numel(), code, 0};
+// ------------------------------------------------- gradient norm, clipping ---
+// Operators of the dispatcher, as the block is:
+//   grad_norm   the norm of a list of gradients, a 0-dim fp32 tensor
+//   grad_clip_  the same, and the gradients scaled in place
+// norm types as in scao_train.h
+Tensor op_grad_norm(at::TensorList grads, int64_t norm_type, double scale) {
+  static const auto op = c10::Dispatcher::singleton()
+                             .findSchemaOrThrow("scao_amd::grad_norm", "")
+                             .typed<decltype(op_grad_norm)>();
+  return op.call(grads, norm_type, scale);
+}
+Tensor op_grad_clip_(at::TensorList grads, int64_t norm_type, double scale, double max_norm) {
+  static const auto op = c10::Dispatcher::singleton()
+                             .findSchemaOrThrow("scao_amd::grad_clip_", "")
+                             .typed<decltype(op_grad_clip_)>();
+  return op.call(grads, norm_type, scale, max_norm);
+}
+
+bool regular(const Tensor& g, c10::Device on) {
+  return g.layout() == at::kStrided && code_of(g.scalar_type()) >= 0 && g.device() == on;
+}
+void check_gradients(at::TensorList grads) {
+  TORCH_CHECK(lib.grad_clip, "clip_grad_norm_: scao_amd has not loaded its library");
+  TORCH_CHECK(!grads.empty(), "clip_grad_norm_: no gradients");
+  const c10::Device on = grads[0].device();
+  for (const Tensor& g : grads)
+    TORCH_CHECK(regular(g, on), "gradients must be dense float32, bfloat16 or "
+                "float16 tensors on one device (got ", g.scalar_type(), ", ", g.layout(), ")");
+}
+
+// The table of the gradients; those with gaps in their memory take part through
+// a contiguous copy.
+struct Gradients {
+  std::vector<scao_tensor_desc> table;
+  std::vector<std::pair<Tensor, Tensor>> copies;   // gradient, copy
+  Tensor norm, work;
+
+  explicit Gradients(at::TensorList grads) {
+    table.reserve(grads.size());
+    for (const Tensor& g : grads) {
+      // every element of its memory range once, in any order
+      const bool dense = g.is_non_overlapping_and_dense();
+      if (!dense) copies.emplace_back(g, g.contiguous());
+      const Tensor& t = dense ? g : copies.back().second;
+      table.push_back({t.data_ptr(), t.numel(), code_of(t.scalar_type()), 0});
     }
-  } catch (const std::exception&) {
-    plain = false;   // the caller's way through Python says what is wrong
+    norm = at::empty({}, grads[0].options().dtype(at::kFloat));
+    work = bytes(lib.grad_norm_workspace(table.data(), (int)table.size()), grads[0]);
   }
-  Py_DECREF(seq);
-  if (!plain) {
-    Py_DECREF(out);
-    Py_RETURN_NONE;
+};
+
+Tensor grad_norm_hip(at::TensorList grads, int64_t norm_type, double scale) {
+  check_gradients(grads);
+  const c10::DeviceGuard guard(grads[0].device());
+  const Gradients g(grads);
+  check(lib.grad_norm(g.table.data(), (int)g.table.size(), (int)norm_type, scale,
+                      (float*)g.norm.data_ptr(), g.work.data_ptr(), stream_of(g.norm)),
+        "scao_grad_norm");
+  return g.norm;
+}
+
+Tensor grad_clip_hip_(at::TensorList grads, int64_t norm_type, double scale, double max_norm) {
+  check_gradients(grads);
+  const c10::DeviceGuard guard(grads[0].device());
+  const Gradients g(grads);
+  for (const auto& [to, copy] : g.copies)
+    TORCH_CHECK_VALUE(at::has_internal_overlap(to) != at::MemOverlap::Yes,
+                      "a gradient whose elements share memory (an expanded tensor) cannot be "
+                      "scaled in place");
+  const int rc = lib.grad_clip(g.table.data(), (int)g.table.size(), (int)norm_type, scale, max_norm,
+                               (float*)g.norm.data_ptr(), g.work.data_ptr(), stream_of(g.norm));
+  TORCH_CHECK_VALUE(rc == SCAO_OK || !strstr(lib.last_error(), "share memory"), lib.last_error());
+  check(rc, "scao_grad_clip");
+  for (const auto& [to, copy] : g.copies) to.copy_(copy);
+  return g.norm;
+}
+
+Tensor grad_norm_meta(at::TensorList grads, int64_t, double) {
+  check_gradients(grads);
+  return at::empty({}, grads[0].options().dtype(at::kFloat));
+}
+Tensor grad_clip_meta_(at::TensorList grads, int64_t norm_type, double scale, double) {
+  return grad_norm_meta(grads, norm_type, scale);
+}
+
+TORCH_LIBRARY_FRAGMENT(scao_amd, m) {
+  m.def("grad_norm(Tensor[] grads, int norm_type, float scale) -> Tensor");
+  m.def("grad_clip_(Tensor(a!)[] grads, int norm_type, float scale, float max_norm) -> Tensor");
+}
+TORCH_LIBRARY_IMPL(scao_amd, CUDA, m) {
+  m.impl("grad_norm", grad_norm_hip);
+  m.impl("grad_clip_", grad_clip_hip_);
+}
+TORCH_LIBRARY_IMPL(scao_amd, Meta, m) {
+  m.impl("grad_norm", grad_norm_meta);
+  m.impl("grad_clip_", grad_clip_meta_);
+}
+// neither depends on the sign of what is held
+TORCH_LIBRARY_IMPL(scao_amd, Negative, m) {
+  m.impl("grad_norm", torch::CppFunction::makeFallthrough());
+  m.impl("grad_clip_", torch::CppFunction::makeFallthrough());
+}
+
+// The gradients of a list or tuple of tensors, those that have one; false where
+// any of them is not a dense fp32, bf16 or fp16 tensor on the first one's GPU,
+// for the caller to refuse.
+bool collect(PyObject* parameters, std::vector<Tensor>& grads) {
+  const THPObjectPtr seq(PySequence_Fast(parameters, "a list or a tuple of parameters"));
+  if (!seq) throw python_error();
+  const Py_ssize_t n = PySequence_Fast_GET_SIZE(seq.get());
+  grads.reserve(n);
+  for (Py_ssize_t i = 0; i < n; ++i) {
+    PyObject* o = PySequence_Fast_GET_ITEM(seq.get(), i);
+    if (!THPVariable_Check(o)) return false;
+    const Tensor& g = THPVariable_Unpack(o).grad();
+    if (!g.defined()) continue;
+    if (!g.is_cuda() || !regular(g, grads.empty() ? g.device() : grads[0].device())) return false;
+    grads.push_back(g);
   }
-  return Py_BuildValue("inN", device, count, out);
+  return true;
+}
+
+// grad_norm(parameters, norm_type, scale), grad_clip(parameters, norm_type, scale,
+// max_norm) -> the norm; None where there is no gradient, False where one is not
+// as collect() says
+PyObject* call_on_gradients(PyObject* const* args, Py_ssize_t n, bool clip) {
+  HANDLE_TH_ERRORS
+  TORCH_CHECK_TYPE(n == (clip ? 4 : 3), "wrong number of arguments");
+  std::vector<Tensor> grads;
+  if (!collect(args[0], grads)) Py_RETURN_FALSE;
+  const long norm_type = PyLong_AsLong(args[1]);
+  const double scale = PyFloat_AsDouble(args[2]);
+  const double max_norm = clip ? PyFloat_AsDouble(args[3]) : 0;
+  if (PyErr_Occurred()) return nullptr;
+  if (grads.empty()) Py_RETURN_NONE;
+  const at::AutoDispatchBelowADInplaceOrView below;
+  return THPVariable_Wrap(clip ? op_grad_clip_(grads, norm_type, scale, max_norm)
+                               : op_grad_norm(grads, norm_type, scale));
+  END_HANDLE_TH_ERRORS
+}
+PyObject* grad_norm(PyObject*, PyObject* const* args, Py_ssize_t n) {
+  return call_on_gradients(args, n, false);
+}
+PyObject* grad_clip(PyObject*, PyObject* const* args, Py_ssize_t n) {
+  return call_on_gradients(args, n, true);
 }
 
 // bind({name: address})
@@ -345,15 +454,20 @@ PyObject* bind(PyObject*, PyObject* arg) {
         at("scao_ffn_forward_workspace", lib.forward_workspace) &&
         at("scao_ffn_forward", lib.forward) &&
         at("scao_ffn_backward_workspace", lib.backward_workspace) &&
-        at("scao_ffn_backward", lib.backward)))
+        at("scao_ffn_backward", lib.backward) &&
+        at("scao_grad_norm_workspace", lib.grad_norm_workspace) &&
+        at("scao_grad_norm", lib.grad_norm) && at("scao_grad_clip", lib.grad_clip)))
     return nullptr;
   Py_RETURN_NONE;
 }
 
 PyMethodDef methods[] = {
-    {"gradients", gradients, METH_O, nullptr},
-    {"gated_ffn", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(gated_ffn)),
-     METH_FASTCALL, nullptr},
+#define SCAO_FASTCALL(f) \
+  {#f, reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(f)), METH_FASTCALL, nullptr}
+    SCAO_FASTCALL(gated_ffn),
+    SCAO_FASTCALL(grad_norm),
+    SCAO_FASTCALL(grad_clip),
+#undef SCAO_FASTCALL
     {"bind", bind, METH_O, nullptr},
     {nullptr, nullptr, 0, nullptr}};
 PyModuleDef module = {PyModuleDef_HEAD_INIT, "_torch_host", nullptr, -1, methods,

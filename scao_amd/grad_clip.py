@@ -8,17 +8,16 @@ training loop does between ``loss.backward()`` and ``SCAO.step()``.
 The call forms are ``torch.nn.utils.clip_grad_norm_``'s, with ``scale`` for
 gradients that are a sum of micro-batches or carry a loss scale: it multiplies
 every gradient in the same pass.  The gradients of all tensors go through two
-kernels (``scao_grad_norm`` / ``scao_grad_clip``) on the current stream, without
-a host synchronisation and without a copy of the tensors' table.
+kernels (``scao_grad_norm`` / ``scao_grad_clip``, called from csrc/torch_host.cpp
+as operators of torch's dispatcher) on the current stream, without a host
+synchronisation and without a copy of the tensors' table.
 """
 
 from __future__ import annotations
 
-import ctypes
 import math
 from typing import Iterable, Union
 
-import numpy as np
 import torch
 from torch import Tensor
 
@@ -37,8 +36,8 @@ def _check_scalars(norm_type: float, scale: float) -> int:
     return code
 
 
-def _irregular(parameters: list) -> list:
-    """The gradients of a list that ``_lib.torch_host().gradients`` does not take, checked."""
+def _checked(parameters: list) -> list:
+    """The gradients of a list that _torch_host does not take."""
     grads = [g for p in parameters if (g := p.grad) is not None]
     for g in grads:
         require_hip(g, "gradient")
@@ -51,46 +50,19 @@ def _irregular(parameters: list) -> list:
     return grads
 
 
-def _dense(g: Tensor) -> bool:
-    """Every element of the gradient's memory range once, in any order."""
-    return g.is_contiguous() or torch.ops.aten.is_non_overlapping_and_dense(g)
+def _as_list(parameters: Union[Tensor, Iterable[Tensor]]) -> list:
+    """(an iterator's parameters may live in this list alone)"""
+    if isinstance(parameters, Tensor):
+        return [parameters]
+    return parameters if isinstance(parameters, (list, tuple)) else list(parameters)
 
 
-class _Gradients:
-    """The table of the parameters' gradients; those with gaps in their memory
-    take part through a contiguous copy."""
-
-    def __init__(self, parameters: Union[Tensor, Iterable[Tensor]]):
-        if isinstance(parameters, Tensor):
-            parameters = [parameters]
-        elif not isinstance(parameters, (list, tuple)):
-            parameters = list(parameters)
-        # until the kernels are queued: an iterator's parameters may live here alone
-        self._parameters = parameters
-        self.copies = []   # (gradient, its copy)
-        found = L.torch_host().gradients(parameters)
-        if found is not None:
-            index, self.count, self._table = found
-            self.device = torch.device("cuda", index) if self.count else None
-            self.at = ctypes.cast(self._table, ctypes.c_void_p).value
-            return
-        grads = _irregular(parameters)
-        flat = [g if _dense(g) else g.contiguous() for g in grads]
-        self.copies = [(g, f) for g, f in zip(grads, flat) if f is not g]
-        self.count, self.device = len(flat), flat[0].device
-        self._table = np.empty(self.count, dtype=L.TENSOR_DESC)
-        for field, of in (("data", Tensor.data_ptr), ("numel", Tensor.numel),
-                          ("dtype", lambda g: L.DTYPE_CODE[g.dtype])):
-            self._table[field] = [of(g) for g in flat]
-        self.at, self._flat = self._table.ctypes.data, flat
-
-    def launch(self, name: str, code: int, *scalars: float) -> Tensor:
-        norm = torch.empty((), dtype=torch.float32, device=self.device)
-        work = torch.empty(L.lib().scao_grad_norm_workspace(self.at, self.count),
-                           dtype=torch.uint8, device=self.device)
-        L.call_on(self.device, name, self.at, self.count, code, *scalars, norm.data_ptr(),
-                  work.data_ptr())
-        return norm
+def _call(host, operator: str, parameters: list, *scalars) -> Tensor:
+    norm = host(parameters, *scalars)
+    if norm is False:
+        grads = _checked(parameters)
+        norm = getattr(torch.ops.scao_amd, operator)(grads, *scalars) if grads else None
+    return torch.tensor(0.0) if norm is None else norm
 
 
 @torch.no_grad()
@@ -99,10 +71,8 @@ def global_grad_norm(parameters: Union[Tensor, Iterable[Tensor]], norm_type: flo
     """``scale`` times the ``norm_type`` norm (1, 2 or inf) of all gradients of
     ``parameters`` as one vector: a 0-dim float32 tensor on their device
     (summed in double), a zero on the CPU where no parameter has a gradient."""
-    code, grads = _check_scalars(norm_type, scale), _Gradients(parameters)
-    if not grads.count:
-        return torch.tensor(0.0)
-    return grads.launch("scao_grad_norm", code, float(scale))
+    code = _check_scalars(norm_type, scale)
+    return _call(L.torch_host().grad_norm, "grad_norm", _as_list(parameters), code, float(scale))
 
 
 @torch.no_grad()
@@ -123,24 +93,11 @@ def clip_grad_norm_(parameters: Union[Tensor, Iterable[Tensor]], max_norm: float
     code, max_norm = _check_scalars(norm_type, scale), float(max_norm)
     if not max_norm >= 0.0:
         raise ValueError(f"max_norm must be at least 0 (got {max_norm})")
-    grads = _Gradients(parameters)
-    if not grads.count:
-        return torch.tensor(0.0)
-    if any(torch._debug_has_internal_overlap(g) == 1 for g, _ in grads.copies):
-        raise ValueError("a gradient whose elements share memory (an expanded tensor) cannot be "
-                         "scaled in place")
+    parameters, host = _as_list(parameters), L.torch_host()
     if error_if_nonfinite:
-        norm = float(grads.launch("scao_grad_norm", code, float(scale)))
+        norm = float(_call(host.grad_norm, "grad_norm", parameters, code, float(scale)))
         if not math.isfinite(norm):
             raise RuntimeError(f"the gradients' norm of order {float(norm_type)} is {norm}, so "
                                "they cannot be clipped; pass error_if_nonfinite=False to scale "
                                "them by it anyway")
-    try:
-        norm = grads.launch("scao_grad_clip", code, float(scale), max_norm)
-    except L.ScaoLibError as e:
-        if "share memory" in str(e):
-            raise ValueError(str(e)) from None
-        raise
-    for g, copy in grads.copies:
-        g.copy_(copy)
-    return norm
+    return _call(host.grad_clip, "grad_clip_", parameters, code, float(scale), max_norm)

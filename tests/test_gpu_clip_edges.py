@@ -60,3 +60,66 @@ def test_a_bound_of_infinity_clips_nothing(hip_device, p, scale):
     g[3] = math.nan
     norm = scao_amd.clip_grad_norm_(_params([g, h]), math.inf, norm_type=p)
     assert math.isnan(norm.item()) and bool(g.isnan().all()) and bool(h.isnan().all())
+
+
+def test_traces_hold_the_clipping(hip_device):
+    from torch.fx.experimental.proxy_tensor import make_fx
+    params = _params([_normal(hip_device, 8, 33), _normal(hip_device, 9, 5, 7)])
+
+    def clip(a, b):
+        params[0].grad, params[1].grad = a * 2, b * 2
+        norm = scao_amd.clip_grad_norm_(params, 0.5)
+        return norm, scao_amd.global_grad_norm(params), params[0].grad, params[1].grad
+
+    first = [p.grad for p in params]
+    new = [_normal(hip_device, 10, 33), _normal(hip_device, 11, 5, 7)]
+    want = [t.clone() for t in clip(*new)]
+    assert abs(want[1].item() - 0.5) < 1e-5
+    for traced in (torch.jit.trace(clip, first), make_fx(clip)(*first)):
+        for got, w in zip(traced(*new), want):
+            assert torch.equal(got, w)
+
+
+def test_dispatch_modes_see_the_clipping(hip_device):
+    from torch.utils._python_dispatch import TorchDispatchMode
+    seen = []
+
+    class Log(TorchDispatchMode):
+        def __torch_dispatch__(self, func, types, args=(), kwargs=None):
+            seen.append(str(func))
+            return func(*args, **(kwargs or {}))
+
+    g = torch.ones(100, device=hip_device)
+    with Log():
+        assert scao_amd.global_grad_norm(_params([g])).item() == 10.0
+        assert scao_amd.clip_grad_norm_(_params([g]), 20.0).item() == 10.0
+    assert {s.split(".")[1] for s in seen if s.startswith("scao_amd.")} == {"grad_norm",
+                                                                          "grad_clip_"}
+
+
+def test_operators_check_their_arguments(hip_device):
+    """Called by their names, past the Python functions' own checks."""
+    g = torch.ones(100, device=hip_device)
+    scao_amd.global_grad_norm(_params([g]))
+    norm, clip = torch.ops.scao_amd.grad_norm, torch.ops.scao_amd.grad_clip_
+    assert norm([g, g], 1, 1.0).item() == 200.0
+    for grads in ([g.double()], [g, g.cpu()], [g.to_sparse()]):
+        with pytest.raises((RuntimeError, NotImplementedError)):
+            norm(grads, 2, 1.0)
+        with pytest.raises((RuntimeError, NotImplementedError)):
+            clip(grads, 2, 1.0, 0.1)
+    with pytest.raises(ValueError, match="share memory"):
+        clip([g, g], 2, 1.0, 0.1)
+    with pytest.raises(RuntimeError):
+        clip([g], 3, 1.0, 0.1)
+    assert bool(g.eq(1).all())
+
+
+def test_negated_views(hip_device):
+    """A gradient that holds its values negated is scaled in place all the same."""
+    g = _normal(hip_device, 12, 500)
+    want = g.double() * 0.25
+    neg = torch._neg_view(-g)
+    assert neg.is_neg()
+    scao_amd.clip_grad_norm_(_params([neg]), math.inf, scale=0.25)
+    assert torch.equal(neg.double(), want)

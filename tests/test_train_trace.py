@@ -29,7 +29,21 @@ def test_a_trace_holds_the_block():
             scao_amd.gated_ffn(x, gate, up[:3], down)
 
 
+def test_a_trace_holds_the_clipping():
+    with FakeTensorMode():
+        params = [torch.nn.Parameter(torch.empty(n, device="cuda")) for n in (7, 33)]
+
+        def clip(*grads):
+            for p, g in zip(params, grads):
+                p.grad = g * 2
+            norm = scao_amd.clip_grad_norm_(params, 0.5)
+            return norm + scao_amd.global_grad_norm(params)
+
+        graph = make_fx(clip)(*(torch.empty(n, device="cuda") for n in (7, 33)))
+        assert _ops(graph) == ["scao_amd.grad_clip_.default", "scao_amd.grad_norm.default"]
+
+
 def test_the_names_of_the_operators():
     scao_amd._lib.torch_host()
-    for name in ("gated_ffn", "gated_ffn_save", "gated_ffn_backward"):
+    for name in ("gated_ffn", "gated_ffn_save", "gated_ffn_backward", "grad_norm", "grad_clip_"):
         assert hasattr(torch.ops.scao_amd, name)
