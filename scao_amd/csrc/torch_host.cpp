@@ -371,6 +371,18 @@ Tensor grad_clip_hip_(at::TensorList grads, int64_t norm_type, double scale, dou
   return g.norm;
 }
 
+// a graph that holds a gradient has to see that it changed
+Tensor grad_clip_version_(at::TensorList grads, int64_t norm_type, double scale, double max_norm) {
+  Tensor norm;
+  {
+    const at::AutoDispatchBelowADInplaceOrView below;
+    norm = op_grad_clip_(grads, norm_type, scale, max_norm);
+  }
+  for (const Tensor& g : grads)
+    if (!g.is_inference()) torch::autograd::impl::bump_version(g);
+  return norm;
+}
+
 Tensor grad_norm_meta(at::TensorList grads, int64_t, double) {
   check_gradients(grads);
   return at::empty({}, grads[0].options().dtype(at::kFloat));
@@ -391,6 +403,7 @@ TORCH_LIBRARY_IMPL(scao_amd, Meta, m) {
   m.impl("grad_norm", grad_norm_meta);
   m.impl("grad_clip_", grad_clip_meta_);
 }
+TORCH_LIBRARY_IMPL(scao_amd, ADInplaceOrView, m) { m.impl("grad_clip_", grad_clip_version_); }
 // neither depends on the sign of what is held
 TORCH_LIBRARY_IMPL(scao_amd, Negative, m) {
   m.impl("grad_norm", torch::CppFunction::makeFallthrough());
@@ -429,7 +442,7 @@ PyObject* call_on_gradients(PyObject* const* args, Py_ssize_t n, bool clip) {
   const double max_norm = clip ? PyFloat_AsDouble(args[3]) : 0;
   if (PyErr_Occurred()) return nullptr;
   if (grads.empty()) Py_RETURN_NONE;
-  const at::AutoDispatchBelowADInplaceOrView below;
+  const at::AutoDispatchBelowAutograd below;
   return THPVariable_Wrap(clip ? op_grad_clip_(grads, norm_type, scale, max_norm)
                                : op_grad_norm(grads, norm_type, scale));
   END_HANDLE_TH_ERRORS

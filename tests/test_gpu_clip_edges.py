@@ -123,3 +123,28 @@ def test_negated_views(hip_device):
     assert neg.is_neg()
     scao_amd.clip_grad_norm_(_params([neg]), math.inf, scale=0.25)
     assert torch.equal(neg.double(), want)
+
+
+def test_versions_count_the_clipping(hip_device):
+    buf = _normal(hip_device, 0, 40, 30)
+    grads = [_normal(hip_device, 1, 100), buf[:, 3:20], _normal(hip_device, 2, 7, 5).t()]
+    params = _params(grads)
+    before = [g._version for g in grads]
+    scao_amd.global_grad_norm(params)
+    assert [g._version for g in grads] == before
+    scao_amd.clip_grad_norm_(params, 0.1)
+    assert all(g._version > v for g, v in zip(grads, before))
+    with torch.inference_mode():
+        g = torch.ones(10, device=hip_device)
+        scao_amd.clip_grad_norm_(_params([g]), 1.0)
+    assert abs(g[0].item() - 10 ** -0.5) < 1e-6
+
+
+def test_a_clipped_gradient_that_a_graph_holds(hip_device):
+    """Its later backward pass must not use the scaled values."""
+    p = torch.nn.Parameter(_normal(hip_device, 3, 50))
+    (p ** 3).sum().backward(create_graph=True)
+    again = (p.grad ** 2).sum()
+    scao_amd.clip_grad_norm_([p], 0.1)
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+        again.backward()
