@@ -23,6 +23,7 @@
 #include <torch/csrc/utils/object_ptr.h>
 #include <torch/library.h>
 
+#include <algorithm>
 #include <cstring>
 
 #include "../../include/scao_train.h"
@@ -355,6 +356,98 @@ Tensor grad_norm_hip(at::TensorList grads, int64_t norm_type, double scale) {
   return g.norm;
 }
 
+// Where the bytes of a tensor lie: begin + sum of i_k stride_k, 0 <= i_k < size_k.
+struct Bytes {
+  int64_t begin, end;
+  std::vector<std::pair<int64_t, int64_t>> dims;   // size, stride
+  explicit Bytes(const Tensor& t) : begin((int64_t)(uintptr_t)t.data_ptr()) {
+    const int64_t item = (int64_t)t.element_size();
+    if (t.is_non_overlapping_and_dense()) {
+      dims = {{t.numel() * item, 1}};
+    } else {
+      for (int64_t k = 0; k < t.dim(); ++k)
+        if (t.size(k) > 1) dims.emplace_back(t.size(k), t.stride(k) * item);
+      dims.emplace_back(item, 1);
+    }
+    end = begin + 1;
+    for (const auto& [size, stride] : dims) end += (size - 1) * stride;
+  }
+};
+// Solutions of sum t_k stride_k = to with lo_k <= t_k <= hi_k, up to `enough`: term
+// by term from the largest stride on, taking only what the others can make up
+// for. That is one or two values of t where the strides are those of one buffer's
+// parts; with others it may take too long to tell, which counts as enough.
+struct Sums {
+  struct Term {
+    int64_t stride, lo, hi;
+  };
+  std::vector<Term> terms;
+  int enough, found = 0, steps = 0;
+  explicit Sums(int n) : enough(n) {}
+  void add(int64_t stride, int64_t lo, int64_t hi) {
+    for (Term& t : terms)
+      if (t.stride == stride) {
+        t.lo += lo;
+        t.hi += hi;
+        return;
+      }
+    terms.push_back({stride, lo, hi});
+  }
+  bool reach(int64_t to) {
+    std::sort(terms.begin(), terms.end(),
+              [](const Term& a, const Term& b) { return a.stride > b.stride; });
+    walk(0, to);
+    return found >= enough;
+  }
+  void walk(size_t k, int64_t to) {
+    if (++steps > 1 << 16) found = enough;
+    if (found >= enough) return;
+    if (k == terms.size()) {
+      found += to == 0;
+      return;
+    }
+    int64_t low = 0, high = 0;   // what the terms behind this one can add up to
+    for (size_t j = k + 1; j < terms.size(); ++j) {
+      low += terms[j].lo * terms[j].stride;
+      high += terms[j].hi * terms[j].stride;
+    }
+    const auto [stride, lo, hi] = terms[k];
+    auto floor = [s = stride](int64_t x) { return x / s - (x % s < 0); };
+    const int64_t last = std::min(hi, floor(to - low));
+    for (int64_t t = std::max(lo, -floor(high - to)); t <= last && found < enough; ++t)
+      walk(k + 1, to - t * stride);
+  }
+};
+bool share_memory(const Bytes& a, const Bytes& b) {
+  if (a.end <= b.begin || b.end <= a.begin) return false;
+  Sums s(1);
+  for (const auto& [size, stride] : a.dims) s.add(stride, 0, size - 1);
+  for (const auto& [size, stride] : b.dims) s.add(stride, 1 - size, 0);
+  return s.reach(b.begin - a.begin);
+}
+// two elements of one tensor: all t_k zero is one solution (and each term stands
+// for itself, so that two of one stride have others)
+bool share_memory(const Bytes& a) {
+  Sums s(2);
+  for (const auto& [size, stride] : a.dims) s.terms.push_back({stride, 1 - size, size - 1});
+  return s.reach(0);
+}
+// Gradients with gaps: scao_grad_clip sees their copies and cannot tell.
+void check_apart(at::TensorList grads, const std::vector<std::pair<Tensor, Tensor>>& copies) {
+  if (copies.empty()) return;
+  std::vector<Bytes> gaps, all;
+  for (const Tensor& g : grads) {
+    if (g.numel() == 0) continue;
+    (g.is_non_overlapping_and_dense() ? all : gaps).emplace_back(g);
+  }
+  for (size_t i = 0; i < gaps.size(); ++i) {
+    TORCH_CHECK_VALUE(!share_memory(gaps[i]), "elements of a gradient share memory");
+    for (const Bytes& b : all)
+      TORCH_CHECK_VALUE(!share_memory(gaps[i], b), "two gradients share memory");
+    all.push_back(gaps[i]);
+  }
+}
+
 Tensor grad_clip_hip_(at::TensorList grads, int64_t norm_type, double scale, double max_norm) {
   check_gradients(grads);
   const c10::DeviceGuard guard(grads[0].device());
@@ -363,6 +456,7 @@ Tensor grad_clip_hip_(at::TensorList grads, int64_t norm_type, double scale, dou
     TORCH_CHECK_VALUE(at::has_internal_overlap(to) != at::MemOverlap::Yes,
                       "a gradient whose elements share memory (an expanded tensor) cannot be "
                       "scaled in place");
+  check_apart(grads, g.copies);
   const int rc = lib.grad_clip(g.table.data(), (int)g.table.size(), (int)norm_type, scale, max_norm,
                                (float*)g.norm.data_ptr(), g.work.data_ptr(), stream_of(g.norm));
   TORCH_CHECK_VALUE(rc == SCAO_OK || !strstr(lib.last_error(), "share memory"), lib.last_error());

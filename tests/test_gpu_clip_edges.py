@@ -148,3 +148,58 @@ def test_a_clipped_gradient_that_a_graph_holds(hip_device):
     scao_amd.clip_grad_norm_([p], 0.1)
     with pytest.raises(RuntimeError, match="modified by an inplace operation"):
         again.backward()
+
+
+def _shared():
+    """names of layouts of two gradients in one buffer of 40 x 30 that share an element"""
+    return {
+        "columns": lambda b: (b[:, 0:10], b[:, 9:20]),
+        "columns of another order": lambda b: (b[:, 9:20], b[:, 0:10]),
+        "one twice": lambda b: (b[:, 0:10], b[:, 0:10]),
+        "a row and columns": lambda b: (b[7], b[:, 29:]),
+        "every second and every third": lambda b: (b.view(-1)[::2], b.view(-1)[1::3]),
+        "a corner": lambda b: (b[:20, :16], b[19:, 15:]),
+        "the buffer's last element": lambda b: (b[:, 20:], b[39, 29:]),
+        "another type's bytes": lambda b: (b[:, :4], b.view(torch.bfloat16)[:, 7:9]),
+        "a window on itself": lambda b: (b.as_strided((30, 9), (4, 1)),),
+        "two dimensions of one stride": lambda b: (b.as_strided((4, 4), (2, 2)),),
+    }
+
+
+@pytest.mark.parametrize("name", _shared())
+def test_gradients_with_gaps_that_share_memory(hip_device, name):
+    b = _normal(hip_device, 6, 40, 30)
+    kept = b.clone()
+    with pytest.raises(ValueError, match="share memory"):
+        scao_amd.clip_grad_norm_(_params(_shared()[name](b)), 0.1)
+    assert torch.equal(b, kept)
+
+
+APART = {
+    "columns": lambda b: (b[:, 0:10], b[:, 10:20], b[:, 25:]),
+    "every second": lambda b: (b[:, ::2], b[:, 1::2]),
+    "rows between columns": lambda b: (b[::2, :], b[1::2, :7], b[1::2, 7:]),
+    "corners": lambda b: (b[:20, :16], b[:20, 16:], b[20:, :9], b[20:, 9:]),
+    "a block and its frame": lambda b: (b[10:20, 10:20], b[:10], b[20:], b[10:20, :10],
+                                       b[10:20, 20:]),
+    "another type's bytes": lambda b: (b[:, :4], b.view(torch.bfloat16)[:, 8:11]),
+    "transposed": lambda b: (b[:, :10].t(), b[:, 10:20].t()),
+    "strides of 3 and 2": lambda b: (b.as_strided((2, 3), (3, 2)), b[1:]),
+}
+
+
+@pytest.mark.parametrize("name", APART)
+def test_gradients_with_gaps_beside_each_other(hip_device, name):
+    """Those that only lie between each other's elements are scaled once each."""
+    b = _normal(hip_device, 7, 40, 30)
+    if "type" in name:
+        b.view(torch.bfloat16)[:, 8:11] = 1.0
+    grads = APART[name](b)
+    wide = [g.double() for g in grads]
+    norm = math.sqrt(sum(w.square().sum().item() for w in wide))
+    got = scao_amd.clip_grad_norm_(_params(grads), 0.25)
+    assert abs(got.item() - norm) <= 1.2e-7 * norm
+    for g, w in zip(grads, wide):
+        want = w * (0.25 / (norm + 1e-6))
+        ulp = 2.0 ** -24 if g.dtype == torch.float32 else 2.0 ** -8
+        assert bool(((g.double() - want).abs() <= want.abs() * (ulp + 1.3e-7)).all())
