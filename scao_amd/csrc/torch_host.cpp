@@ -18,7 +18,6 @@
 #include <torch/csrc/Exceptions.h>
 #include <torch/csrc/autograd/custom_function.h>
 #include <torch/csrc/autograd/functions/basic_ops.h>
-#include <torch/csrc/autograd/functions/utils.h>
 #include <torch/csrc/autograd/python_variable.h>
 #include <torch/csrc/utils/object_ptr.h>
 #include <torch/library.h>
@@ -253,7 +252,7 @@ Tensor gated_ffn_autograd(const Tensor& x, const Tensor& g, const Tensor& u, con
                           int64_t act) {
   check_block(x, g, u, d);
   for (const Tensor* t : {&x, &g, &u, &d})   // a tangent would be lost
-    TORCH_CHECK_NOT_IMPLEMENTED(!torch::autograd::isFwGradDefined(*t),
+    TORCH_CHECK_NOT_IMPLEMENTED(!t->_fw_grad(0).defined(),
                                 "gated_ffn has no forward-mode derivative");
   if (at::GradMode::is_enabled() && (x.requires_grad() || g.requires_grad() ||
                                      u.requires_grad() || d.requires_grad()))
@@ -316,13 +315,13 @@ Tensor op_grad_clip_(at::TensorList grads, int64_t norm_type, double scale, doub
 bool regular(const Tensor& g, c10::Device on) {
   return g.layout() == at::kStrided && code_of(g.scalar_type()) >= 0 && g.device() == on;
 }
-void check_gradients(at::TensorList grads) {
+void check_gradient(const Tensor& g, c10::Device on) {
+  TORCH_CHECK(regular(g, on), "gradients must be dense float32, bfloat16 or float16 tensors on "
+              "one device (got ", g.scalar_type(), ", ", g.layout(), ", ", g.device(), ")");
+}
+void check_call(at::TensorList grads) {
   TORCH_CHECK(lib.grad_clip, "clip_grad_norm_: scao_amd has not loaded its library");
   TORCH_CHECK(!grads.empty(), "clip_grad_norm_: no gradients");
-  const c10::Device on = grads[0].device();
-  for (const Tensor& g : grads)
-    TORCH_CHECK(regular(g, on), "gradients must be dense float32, bfloat16 or "
-                "float16 tensors on one device (got ", g.scalar_type(), ", ", g.layout(), ")");
 }
 
 // The table of the gradients; those with gaps in their memory take part through
@@ -334,7 +333,9 @@ struct Gradients {
 
   explicit Gradients(at::TensorList grads) {
     table.reserve(grads.size());
+    const c10::Device on = grads[0].device();
     for (const Tensor& g : grads) {
+      check_gradient(g, on);
       // every element of its memory range once, in any order
       const bool dense = g.is_non_overlapping_and_dense();
       if (!dense) copies.emplace_back(g, g.contiguous());
@@ -347,7 +348,7 @@ struct Gradients {
 };
 
 Tensor grad_norm_hip(at::TensorList grads, int64_t norm_type, double scale) {
-  check_gradients(grads);
+  check_call(grads);
   const c10::DeviceGuard guard(grads[0].device());
   const Gradients g(grads);
   check(lib.grad_norm(g.table.data(), (int)g.table.size(), (int)norm_type, scale,
@@ -449,7 +450,7 @@ void check_apart(at::TensorList grads, const std::vector<std::pair<Tensor, Tenso
 }
 
 Tensor grad_clip_hip_(at::TensorList grads, int64_t norm_type, double scale, double max_norm) {
-  check_gradients(grads);
+  check_call(grads);
   const c10::DeviceGuard guard(grads[0].device());
   const Gradients g(grads);
   for (const auto& [to, copy] : g.copies)
@@ -473,12 +474,13 @@ Tensor grad_clip_version_(at::TensorList grads, int64_t norm_type, double scale,
     norm = op_grad_clip_(grads, norm_type, scale, max_norm);
   }
   for (const Tensor& g : grads)
-    if (!g.is_inference()) torch::autograd::impl::bump_version(g);
+    if (!g.is_inference()) g.unsafeGetTensorImpl()->bump_version();
   return norm;
 }
 
 Tensor grad_norm_meta(at::TensorList grads, int64_t, double) {
-  check_gradients(grads);
+  check_call(grads);
+  for (const Tensor& g : grads) check_gradient(g, grads[0].device());
   return at::empty({}, grads[0].options().dtype(at::kFloat));
 }
 Tensor grad_clip_meta_(at::TensorList grads, int64_t norm_type, double scale, double) {
@@ -536,6 +538,9 @@ PyObject* call_on_gradients(PyObject* const* args, Py_ssize_t n, bool clip) {
   const double max_norm = clip ? PyFloat_AsDouble(args[3]) : 0;
   if (PyErr_Occurred()) return nullptr;
   if (grads.empty()) Py_RETURN_NONE;
+  for (const Tensor& g : grads)   // a tangent would be lost
+    TORCH_CHECK_NOT_IMPLEMENTED(!g._fw_grad(0).defined(),
+                                "the gradients' norm has no forward-mode derivative");
   const at::AutoDispatchBelowAutograd below;
   return THPVariable_Wrap(clip ? op_grad_clip_(grads, norm_type, scale, max_norm)
                                : op_grad_norm(grads, norm_type, scale));

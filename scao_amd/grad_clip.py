@@ -61,11 +61,11 @@ def _call(host, operator: str, parameters: list, *scalars) -> Tensor:
     norm = host(parameters, *scalars)
     if norm is False:
         grads = _checked(parameters)
-        norm = getattr(torch.ops.scao_amd, operator)(grads, *scalars) if grads else None
+        with torch.no_grad():
+            norm = getattr(torch.ops.scao_amd, operator)(grads, *scalars) if grads else None
     return torch.tensor(0.0) if norm is None else norm
 
 
-@torch.no_grad()
 def global_grad_norm(parameters: Union[Tensor, Iterable[Tensor]], norm_type: float = 2.0,
                      scale: float = 1.0) -> Tensor:
     """``scale`` times the ``norm_type`` norm (1, 2 or inf) of all gradients of
@@ -75,7 +75,6 @@ def global_grad_norm(parameters: Union[Tensor, Iterable[Tensor]], norm_type: flo
     return _call(L.torch_host().grad_norm, "grad_norm", _as_list(parameters), code, float(scale))
 
 
-@torch.no_grad()
 def clip_grad_norm_(parameters: Union[Tensor, Iterable[Tensor]], max_norm: float,
                     norm_type: float = 2.0, error_if_nonfinite: bool = False,
                     scale: float = 1.0) -> Tensor:

@@ -203,3 +203,17 @@ def test_gradients_with_gaps_beside_each_other(hip_device, name):
         want = w * (0.25 / (norm + 1e-6))
         ulp = 2.0 ** -24 if g.dtype == torch.float32 else 2.0 ** -8
         assert bool(((g.double() - want).abs() <= want.abs() * (ulp + 1.3e-7)).all())
+
+
+def test_forward_mode_is_refused(hip_device):
+    import torch.autograd.forward_ad as fwd
+    g = _normal(hip_device, 13, 50)
+    kept = g.clone()
+    p = torch.nn.Parameter(torch.zeros(50, device=hip_device))
+    with fwd.dual_level():
+        p.grad = fwd.make_dual(g, torch.ones_like(g))
+        with pytest.raises(RuntimeError, match="forward"):
+            scao_amd.clip_grad_norm_([p], 0.1)
+        with pytest.raises(RuntimeError, match="forward"):
+            scao_amd.global_grad_norm([p])
+    assert torch.equal(g, kept)
