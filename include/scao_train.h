@@ -27,7 +27,7 @@ extern "C" {
  * scale where max_norm is infinite (which clips nothing).
  * Tensors start at any multiple of their element size and must not overlap
  * when they are clipped (SCAO_ERR_INVALID).  workspace:
- * scao_grad_norm_workspace() bytes. */
+ * scao_grad_norm_workspace() bytes, aligned to 8. */
 typedef struct scao_tensor_desc {
   void* data;               /* numel elements of dtype, contiguous               */
   int64_t numel;
@@ -50,7 +50,7 @@ int scao_grad_clip(const scao_tensor_desc* tensors, int n, int norm_type, double
  * dx = da Wg + db Wu, dWg = da^T x, dWu = db^T x, dWd = dy^T h, each written
  * densely (row strides d, d, d, f) unless its pointer is null.  No atomics: the
  * same call gives the same bits.  workspace: the *_workspace() bytes for the
- * same descriptor, aligned to 256, as is `saved`. */
+ * same descriptor, aligned to 16, as is `saved`. */
 enum scao_activation {
   SCAO_ACT_SILU = 0,        /* a / (1 + exp(-a))                                 */
   SCAO_ACT_GELU = 1,        /* a (1 + erf(a / sqrt 2)) / 2                       */

@@ -304,6 +304,13 @@ int check(const char* who, const scao_tensor_desc* t, int n, int norm_type, doub
   return SCAO_OK;
 }
 
+int check_buffers(const char* who, int n, const float* norm, const void* workspace) {
+  SCAO_CHECK_ARG(norm && (workspace || n == 0), "%s: null pointer", who);
+  SCAO_CHECK_ARG((uintptr_t)norm % 4 == 0 && (uintptr_t)workspace % 8 == 0,
+                 "%s: norm or workspace is not aligned", who);
+  return SCAO_OK;
+}
+
 // No element may be scaled twice, nor by two workgroups at once.  Tensors in the
 // order of their addresses, or against it, as a backward pass often allocates
 // them, need no sorting (332 tensors: 16 us).
@@ -400,7 +407,7 @@ extern "C" int64_t scao_grad_norm_workspace(const scao_tensor_desc* tensors, int
 extern "C" int scao_grad_norm(const scao_tensor_desc* tensors, int n, int norm_type, double scale,
                               float* norm, void* workspace, void* stream) {
   if (int rc = check("scao_grad_norm", tensors, n, norm_type, scale)) return rc;
-  SCAO_CHECK_ARG(norm && (workspace || n == 0), "scao_grad_norm: null pointer");
+  if (int rc = check_buffers("scao_grad_norm", n, norm, workspace)) return rc;
   hipStream_t st = (hipStream_t)stream;
   double* parts = (double*)workspace;
   int np = 0;
@@ -416,7 +423,7 @@ extern "C" int scao_grad_clip(const scao_tensor_desc* tensors, int n, int norm_t
                               double max_norm, float* norm, void* workspace, void* stream) {
   if (int rc = check("scao_grad_clip", tensors, n, norm_type, scale)) return rc;
   SCAO_CHECK_ARG(max_norm >= 0.0, "scao_grad_clip: max_norm %g is negative or no number", max_norm);
-  SCAO_CHECK_ARG(norm && (workspace || n == 0), "scao_grad_clip: null pointer");
+  if (int rc = check_buffers("scao_grad_clip", n, norm, workspace)) return rc;
   if (int rc = check_apart(tensors, n)) return rc;
   hipStream_t st = (hipStream_t)stream;
   double* parts = (double*)workspace;

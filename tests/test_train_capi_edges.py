@@ -28,3 +28,15 @@ def test_the_stride_of_a_single_row_is_not_looked_at():
             many = _ffn(**{k: v for k, v in kw.items() if k.startswith("ld")})
             assert lib.scao_ffn_forward_workspace(many.ctypes.data, 0) == 0
             assert b"row stride" in lib.scao_last_error()
+
+
+def test_buffers_off_their_alignment_are_refused():
+    from scao_amd import _lib as L
+    lib = L.lib()
+    t = np.zeros(1, dtype=L.TENSOR_DESC)
+    t[0] = (4096, 10, 0, 0)
+    for norm, work in ((4, 4), (4, 12), (2, 8), (5, 16)):
+        assert lib.scao_grad_norm(t.ctypes.data, 1, 2, 1.0, norm, work, None) == 1
+        assert b"not aligned" in lib.scao_last_error()
+        assert lib.scao_grad_clip(t.ctypes.data, 1, 2, 1.0, 1.0, norm, work, None) == 1
+        assert b"not aligned" in lib.scao_last_error()
