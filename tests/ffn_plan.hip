@@ -1,0 +1,58 @@
+// The launches that the feed-forward block plans, without a GPU: csrc/ffn.hip with
+// launchers that write them down. Built for the host alone by tests/test_ffn_plan.py.
+#include "../scao_amd/csrc/ffn.hip"
+
+#include <vector>
+
+namespace {
+
+struct Launch {   // mirrored in tests/test_ffn_plan.py
+  int32_t kind, tile, type, whole, tiles, splits, row0, paired;
+};
+std::vector<Launch> launches;
+
+template <int TYPE>
+void put(int kind, int tile, const FfnOperands& o, bool paired) {
+  launches.push_back({kind, tile, TYPE, o.whole, o.tiles(), o.splits, o.row0, paired});
+}
+template <int TYPE>
+FfnLaunchers recorders() {
+  return {[](int kind, int tile, const FfnOperands& o, const FfnEpilogue&, hipStream_t) {
+            put<TYPE>(kind, tile, o, false);
+          },
+          [](int kind, int tile, const FfnOperands& a, const FfnEpilogue&, const FfnOperands& b,
+             const FfnEpilogue&, hipStream_t) {
+            put<TYPE>(kind, tile, a, true);
+            put<TYPE>(FFN_DW, tile, b, true);
+          },
+          [](const FfnPack&, hipStream_t) {},
+          [](const FfnFew& o, const FfnEpilogue&, bool gated, hipStream_t) {
+            launches.push_back({gated ? -1 : -2, 0, TYPE, 0, o.tokens, o.cols, 0, 0});
+          }};
+}
+
+}  // namespace
+
+namespace scao {
+FfnLaunchers ffn_f32() { return recorders<SCAO_F32>(); }
+FfnLaunchers ffn_bf16() { return recorders<SCAO_BF16>(); }
+FfnLaunchers ffn_f16() { return recorders<SCAO_F16>(); }
+}  // namespace scao
+
+void scao_set_error(const char*, ...) {}
+
+// the forward pass (train: with what it saves, and the backward pass of all
+// gradients); how many launches there are, the first `cap` of them in out
+extern "C" int ffn_plan(const scao_ffn_desc* d, int train, int64_t ld_dy, int32_t* out, int cap) {
+  launches.clear();
+  alignas(16) static char at[16];
+  Block f(*d, at, nullptr, false);
+  f.forward(at, train ? at : nullptr, train);
+  if (train) {
+    Block b(*d, at, nullptr, false);
+    b.backward(at, ld_dy, at, at, at, at, at, 15);
+  }
+  for (int i = 0; i < (int)launches.size() && i < cap; ++i)
+    __builtin_memcpy(out + 8 * i, &launches[i], sizeof(Launch));
+  return (int)launches.size();
+}
