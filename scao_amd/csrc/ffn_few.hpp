@@ -1,8 +1,8 @@
 // The gated feed-forward block's forward products for few tokens (serving):
 // bound by reading the weights once.
 //
-// A workgroup owns NR x 16 output columns (with GATED those of both projections)
-// for all tokens; its NW waves share k, and their sums meet in LDS in a fixed
+// A workgroup owns 16 output columns (with GATED those of both projections) for
+// all tokens; its NW waves share k, and their sums meet in LDS in a fixed
 // order.  The weights go from global memory straight into the matrix cores'
 // operand registers, 16 bytes (fp32: 32) a lane and step of 32 k: each byte is
 // used once, so staging them would only add a trip.  All steps of a wave's run
@@ -82,11 +82,11 @@ struct Few8<SCAO_F32> {
 };
 
 // U: steps in flight
-template <int TYPE, int MT, int NR, int NW, int U, bool GATED, bool HALVES>
+template <int TYPE, int MT, int NW, int U, bool GATED, bool HALVES>
 __global__ __launch_bounds__(NW * 64) void k_ffn_few(const FfnFew o, const FfnEpilogue e) {
-  constexpr int H = GATED ? 2 : 1, NF = MT * NR * H, P = HALVES ? 2 : 1, COLS_ = NR * 16 / P;
-  static_assert(!HALVES || (MT == 1 && NR == 1), "halves: one product of 16 x 16");
-  __shared__ v4f sums[NW][NF][64];
+  constexpr int H = GATED ? 2 : 1, P = HALVES ? 2 : 1, COLS_ = 16 / P;
+  static_assert(!HALVES || MT == 1, "halves: one product of 16 x 16");
+  __shared__ v4f sums[NW][H * MT][64];
   using V = Few8<TYPE>;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63;
   const int q = lane & 15, g = lane >> 4;
@@ -101,38 +101,35 @@ __global__ __launch_bounds__(NW * 64) void k_ffn_few(const FfnFew o, const FfnEp
 
   // row starts; rows outside of the operands repeat the last one, their results
   // are never written
-  const char *pw[NR * H], *px[MT];
+  const char *pw[H], *px[MT];
   const int64_t k0 = (int64_t)first * 32 + 8 * g;
-#pragma unroll
-  for (int i = 0; i < NR; ++i) {
-    const int64_t r = min(c0 + i * 16 + row, o.cols - 1);
-    pw[i] = (const char*)o.w + (r * o.ldw + k0) * V::SIZE;
-    if (GATED) pw[NR * (H - 1) + i] = (const char*)o.w2 + (r * o.ldw2 + k0) * V::SIZE;
-  }
+  const int64_t r = min(c0 + row, o.cols - 1);
+  pw[0] = (const char*)o.w + (r * o.ldw + k0) * V::SIZE;
+  if (GATED) pw[H - 1] = (const char*)o.w2 + (r * o.ldw2 + k0) * V::SIZE;
 #pragma unroll
   for (int m = 0; m < MT; ++m)
     px[m] = (const char*)o.x + ((int64_t)min(m * 16 + row, o.tokens - 1) * o.ldx + k0) * V::SIZE;
 
-  v4f acc[NR * H][MT];
+  v4f acc[H][MT];
 #pragma unroll
-  for (int i = 0; i < NR * H; ++i)
+  for (int i = 0; i < H; ++i)
 #pragma unroll
     for (int m = 0; m < MT; ++m) acc[i][m] = v4f{0.f, 0.f, 0.f, 0.f};
 
-  auto products = [&](const V (&w)[NR * H], const V (&x)[MT]) {
+  auto products = [&](const V (&w)[H], const V (&x)[MT]) {
     if constexpr (TYPE == SCAO_F32) {
       bf3 xs[MT];
 #pragma unroll
       for (int m = 0; m < MT; ++m) xs[m] = x[m].split();
 #pragma unroll
-      for (int i = 0; i < NR * H; ++i) {
+      for (int i = 0; i < H; ++i) {
         const bf3 ws = w[i].split();
 #pragma unroll
         for (int m = 0; m < MT; ++m) acc[i][m] = mfma_x6(ws, xs[m], acc[i][m]);
       }
     } else {
 #pragma unroll
-      for (int i = 0; i < NR * H; ++i)
+      for (int i = 0; i < H; ++i)
 #pragma unroll
         for (int m = 0; m < MT; ++m) acc[i][m] = V::product(w[i], x[m], acc[i][m]);
     }
@@ -140,11 +137,11 @@ __global__ __launch_bounds__(NW * 64) void k_ffn_few(const FfnFew o, const FfnEp
 
   int s = 0;
   for (; s + U <= whole; s += U) {   // all lanes' steps are whole
-    V w[U][NR * H], x[U][MT];
+    V w[U][H], x[U][MT];
 #pragma unroll
     for (int u = 0; u < U; ++u) {
 #pragma unroll
-      for (int i = 0; i < NR * H; ++i) w[u][i].load(pw[i] + (int64_t)(s + u) * 32 * V::SIZE);
+      for (int i = 0; i < H; ++i) w[u][i].load(pw[i] + (int64_t)(s + u) * 32 * V::SIZE);
 #pragma unroll
       for (int m = 0; m < MT; ++m) x[u][m].load(px[m] + (int64_t)(s + u) * 32 * V::SIZE);
     }
@@ -153,23 +150,23 @@ __global__ __launch_bounds__(NW * 64) void k_ffn_few(const FfnFew o, const FfnEp
   }
   // what is left of the stretch, and the end of k
   for (; s < per; s += U) {
-    V w[U][NR * H], x[U][MT];
+    V w[U][H], x[U][MT];
 #pragma unroll
     for (int u = 0; u < U; ++u) {
       const int left = s + u < per ? o.K - (first + s + u) * 32 - 8 * g : 0;
       const int64_t at = (int64_t)(s + u) * 32 * V::SIZE;
 #pragma unroll
-      for (int i = 0; i < NR * H; ++i) w[u][i].zero();
+      for (int i = 0; i < H; ++i) w[u][i].zero();
 #pragma unroll
       for (int m = 0; m < MT; ++m) x[u][m].zero();
       if (left >= 8) {
 #pragma unroll
-        for (int i = 0; i < NR * H; ++i) w[u][i].load(pw[i] + at);
+        for (int i = 0; i < H; ++i) w[u][i].load(pw[i] + at);
 #pragma unroll
         for (int m = 0; m < MT; ++m) x[u][m].load(px[m] + at);
       } else if (left > 0) {
 #pragma unroll
-        for (int i = 0; i < NR * H; ++i) w[u][i].load_some(pw[i] + at, left);
+        for (int i = 0; i < H; ++i) w[u][i].load_some(pw[i] + at, left);
 #pragma unroll
         for (int m = 0; m < MT; ++m) x[u][m].load_some(px[m] + at, left);
       }
@@ -179,11 +176,11 @@ __global__ __launch_bounds__(NW * 64) void k_ffn_few(const FfnFew o, const FfnEp
   }
 
 #pragma unroll
-  for (int i = 0; i < NR * H; ++i)
+  for (int i = 0; i < H; ++i)
 #pragma unroll
     for (int m = 0; m < MT; ++m) sums[wave][i * MT + m][lane] = acc[i][m];
   __syncthreads();
-  for (int f = wave; f < NR * MT; f += NW) {
+  for (int f = wave; f < MT; f += NW) {
     v4f a = {0.f, 0.f, 0.f, 0.f}, b = a;
     // HALVES: columns 4g .. 4g+3 of tokens 0 .. 7 (lanes with q < 8, g < 2) from
     // the first stretch, and 40 lanes further from the second
@@ -193,9 +190,9 @@ __global__ __launch_bounds__(NW * 64) void k_ffn_few(const FfnFew o, const FfnEp
 #pragma unroll
       for (int p = 0; p < P; ++p) {
         a += sums[w][f][lane + 40 * p];
-        if (GATED) b += sums[w][NR * MT + f][lane + 40 * p];
+        if (GATED) b += sums[w][MT + f][lane + 40 * p];
       }
-    const int m = (f % MT) * 16 + q, n = c0 + (f / MT) * 16 + 4 * g;
+    const int m = f * 16 + q, n = c0 + 4 * g;
     if constexpr (GATED) {
       v4f h;
       for_activation(e.act, [&](auto act) {
@@ -219,7 +216,7 @@ constexpr int FFN_FEW_TOKENS = 64;
 template <int TYPE>
 void launch_few(const FfnFew& o, const FfnEpilogue& e, bool gated, hipStream_t st) {
 #define FFN_FEW(MT, NW, U, G, HALVES)                                  \
-  k_ffn_few<TYPE, MT, 1, NW, U, G, HALVES>                              \
+  k_ffn_few<TYPE, MT, NW, U, G, HALVES>                                 \
       <<<(o.cols + (HALVES ? 7 : 15)) / (HALVES ? 8 : 16), NW * 64, 0, st>>>(o, e)
   // halves where 16 columns a workgroup would not give every CU one
   const bool halves = o.tokens <= 8 && o.cols < 16 * 256;
