@@ -92,7 +92,7 @@ class GatedFFN(nn.Module):
     @torch.no_grad()
     def reset_parameters(self) -> None:
         for p in self.parameters():
-            bound = 1.0 / math.sqrt(p.shape[1])
+            bound = 1.0 / math.sqrt(p.shape[1]) if p.shape[1] else 0.0
             p.uniform_(-bound, bound)
 
     def forward(self, x: Tensor) -> Tensor:
