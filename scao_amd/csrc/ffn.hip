@@ -80,10 +80,11 @@ struct Block {
   // Estimated us of products on tiles: us of a k step with one workgroup a CU
   // and with all a CU holds, and of a tile's beginning and end, fitted to the
   // times of every tile and part count of 225 products (8 to 4096 tokens, 256 x
-  // 704 to 4096 x 14336; 256 x 128 tiles: to 66 forward passes): the choice is 1.7%
-  // slower than the best on the geometric average, 17% at most.  For example dx
-  // of 24 tokens, 2048 x 8192: 32 x 128 tiles in one part 116 us, in 16 parts 21.8;
-  // of 4096 tokens: 256 x 256 in one part 285, in two 183, 128 x 128 in one 251.
+  // 704 to 4096 x 14336; 256 x 128 tiles: to 66 forward passes).  On the present
+  // kernels the choice is 3.2% slower than the best on the geometric average, 44%
+  // (9.2 us for 6.4) at most.  For example dx of 24 tokens, 2048 x 8192: 32 x 128
+  // tiles in one part 120 us, in 16 parts 20.0; of 4096 tokens: 256 x 256 in one
+  // part 286, in two 185, 128 x 128 in one 248.
   struct Cost {
     int slots;
     double lone, full, ends;
@@ -245,10 +246,11 @@ struct Block {
   }
   // With few rows left over behind whole tiles of 256 these may go by themselves,
   // on narrow tiles, at the price of reading the weights again: 1030 tokens of
-  // 2048 x 8192 128 us against 139, where 1024 fill one round exactly.  Not
+  // 2048 x 8192 119 us against 129, where 1024 fill one round exactly.  Not
   // behind rows that are split many times themselves: 300 tokens of 4096 x 11008
-  // fp32 951 us, 256 of them in 8 and 16 parts and 44 apart 1061.  (Over 165
-  // forward passes of up to 128 rows left 0.8% behind the better of both choices.)
+  // fp32 886 us, 256 of them in 8 and 16 parts and 44 apart 973.  (Over 141
+  // forward passes of up to 128 rows left gate + up 0.8% and down 0.4% behind the
+  // better of both choices.)
   void run(Product& p) {
     const Shape all = shape(p.kind, p.o);
     Cut c, head, tail;
@@ -275,14 +277,14 @@ struct Block {
     const Shape x = shape(p.kind, p.o), y = shape(w.kind, w.o);
     Cut c, cp, cw;
     // dx goes with its dW where the estimates say so by more than a launch's share
-    // (8192 tokens, 4096 x 14336 bf16, the whole pass: 6560 us apart, 6650 in
+    // (8192 tokens, 4096 x 14336 bf16, the whole pass: 6580 us apart, 6760 in
     // pairs).  dh's epilogue moves bytes: two 128 x 128 tiles on a CU hide half of
     // them behind dWd's products, one 256 x 256 tile none, and large tiles lose in
     // an L2 that holds two working sets.  Of the best of apart and both tiles on
-    // 118 backward passes (300 to 8192 tokens, 768 x 2048 to 4096 x 11008) dh is
-    // 1.1% slower on average, dx 0.6%.  2048 tokens, 768 x 2048 fp32: dh and dWd
-    // apart 285 us, on 128 x 128 tiles 266; 8192 tokens, 2048 x 8192 bf16: apart
-    // 1328, on 256 x 256 tiles 1369.
+    // 89 backward passes (300 to 8192 tokens, 768 x 2048 to 4096 x 11008) dh is
+    // 1.3% slower on average, dx 0.8%.  2048 tokens, 768 x 2048 fp32: dh and dWd
+    // apart 276 us, on 128 x 128 tiles 260; 8192 tokens, 2048 x 8192 bf16: apart
+    // 1378, on 256 x 256 tiles 1439.
     const double apart = choose(x, c) + choose(y, c) + 3;
     if (1.005 * choose_pair(x, y, cp, cw) > apart + 0.5 * x.moved / 5e6 * x.M * x.N) {
       run(p);

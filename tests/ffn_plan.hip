@@ -56,3 +56,25 @@ extern "C" int ffn_plan(const scao_ffn_desc* d, int train, int64_t ld_dy, int32_
     __builtin_memcpy(out + 8 * i, &launches[i], sizeof(Launch));
   return (int)launches.size();
 }
+
+// the choice for one product alone: tile, tiles in one piece, parts of the others,
+// tiles in all; the estimate in us
+extern "C" double ffn_choose(int kind, int64_t tokens, int64_t d, int64_t f, int32_t* out) {
+  scao_ffn_desc s{};
+  s.dtype = SCAO_BF16;
+  const Block b(s, nullptr, nullptr, true);
+  FfnOperands o{};
+  const bool over_f = kind == FFN_DOWN || kind == FFN_DX;
+  o.M = (int)(kind == FFN_DW ? 2 * f : tokens);
+  o.N = (int)(kind == FFN_GATE_UP || kind == FFN_DH ? f : d);
+  o.K = (int)(kind == FFN_DW ? tokens : over_f ? f : d);
+  o.nseg = kind == FFN_DX ? 2 : 1;
+  Block::Cut c;
+  const Block::Shape shape = b.shape(kind, o);
+  const double us = Block::choose(shape, c);
+  out[0] = c.tile;
+  out[1] = c.whole;
+  out[2] = c.splits;
+  out[3] = (int32_t)shape.tiles(c.tile);
+  return us;
+}

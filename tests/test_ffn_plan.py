@@ -36,6 +36,8 @@ def plan(tmp_path_factory):
     lib = ctypes.CDLL(so)
     lib.ffn_plan.argtypes = [ctypes.c_void_p, ctypes.c_int, ctypes.c_int64, ctypes.c_void_p,
                              ctypes.c_int]
+    lib.ffn_choose.restype = ctypes.c_double
+    lib.ffn_choose.argtypes = [ctypes.c_int] + 3 * [ctypes.c_int64] + [ctypes.c_void_p]
     desc = np.zeros(1, dtype=L.FFN_DESC)
     for k in ("x", "w_gate", "w_up", "w_down"):
         desc[k] = 4096
@@ -49,6 +51,7 @@ def plan(tmp_path_factory):
         assert 0 < n <= len(out)
         return out[:n].tolist()
 
+    call.lib = lib
     return call
 
 
@@ -88,3 +91,25 @@ def test_both_16_bit_types_take_the_same_paths(plan):
     for size in SIZES + PATHS_16:
         a, b = (plan(*size, dtype, True) for dtype in (1, 2))
         assert [row[:2] + row[3:] for row in a] == [row[:2] + row[3:] for row in b]
+
+
+def test_choice_of_tiles_against_measured_products(plan):
+    """perf/ffn_fit.py's model is the one that chooses (a last round split alone
+    aside, which it does not know), and stays near the best of what was measured."""
+    import importlib.util
+    spec = importlib.util.spec_from_file_location("ffn_fit", os.path.join(ROOT, "perf", "ffn_fit.py"))
+    fit = importlib.util.module_from_spec(spec)
+    spec.loader.exec_module(fit)
+    forms = fit.Forms(fit.read(os.path.join(ROOT, "profiles", "ffn_tiles.csv")))
+    slots, c = fit.constants()
+    out = (ctypes.c_int32 * 4)()
+    alone = 0
+    for (kind, *size), at in zip(forms.products, forms.chosen(slots, c)):
+        plan.lib.ffn_choose(KINDS.index(kind), *size, out)
+        tile, whole, parts, tiles = out
+        if 0 < whole < tiles:
+            alone += 1
+        else:
+            assert (tile, parts) == (forms.tile[at], forms.parts[at]), (kind, size)
+    assert alone < 10 and len(forms.products) == 225
+    assert np.exp(np.log(forms.behind(slots, c)).mean()) < 1.04
