@@ -17,6 +17,7 @@
 #include <c10/hip/HIPStream.h>
 #include <torch/csrc/Exceptions.h>
 #include <torch/csrc/autograd/custom_function.h>
+#include <torch/csrc/autograd/forward_grad.h>
 #include <torch/csrc/autograd/functions/basic_ops.h>
 #include <torch/csrc/autograd/python_variable.h>
 #include <torch/csrc/utils/object_ptr.h>
@@ -64,6 +65,9 @@ void* stream_of(const Tensor& t) {
 Tensor bytes(int64_t n, const Tensor& like) {
   return at::empty({n}, like.options().dtype(at::kByte));
 }
+
+// whether any tensor may have a tangent (asking a view takes a lock)
+bool forward_mode() { return torch::autograd::ForwardADLevel::try_get_by_idx(0) != nullptr; }
 
 // ------------------------------------------------------------- gated_ffn ---
 // Operators of torch's dispatcher, so that what follows a program by its
@@ -251,9 +255,10 @@ struct GatedFFN : torch::autograd::Function<GatedFFN> {
 Tensor gated_ffn_autograd(const Tensor& x, const Tensor& g, const Tensor& u, const Tensor& d,
                           int64_t act) {
   check_block(x, g, u, d);
-  for (const Tensor* t : {&x, &g, &u, &d})   // a tangent would be lost
-    TORCH_CHECK_NOT_IMPLEMENTED(!t->_fw_grad(0).defined(),
-                                "gated_ffn has no forward-mode derivative");
+  if (forward_mode())   // a tangent would be lost
+    for (const Tensor* t : {&x, &g, &u, &d})
+      TORCH_CHECK_NOT_IMPLEMENTED(!t->_fw_grad(0).defined(),
+                                  "gated_ffn has no forward-mode derivative");
   if (at::GradMode::is_enabled() && (x.requires_grad() || g.requires_grad() ||
                                      u.requires_grad() || d.requires_grad()))
     // (what rows() copies, it copies here once for both passes)
@@ -538,9 +543,10 @@ PyObject* call_on_gradients(PyObject* const* args, Py_ssize_t n, bool clip) {
   const double max_norm = clip ? PyFloat_AsDouble(args[3]) : 0;
   if (PyErr_Occurred()) return nullptr;
   if (grads.empty()) Py_RETURN_NONE;
-  for (const Tensor& g : grads)   // a tangent would be lost
-    TORCH_CHECK_NOT_IMPLEMENTED(!g._fw_grad(0).defined(),
-                                "the gradients' norm has no forward-mode derivative");
+  if (forward_mode())   // a tangent would be lost
+    for (const Tensor& g : grads)
+      TORCH_CHECK_NOT_IMPLEMENTED(!g._fw_grad(0).defined(),
+                                  "the gradients' norm has no forward-mode derivative");
   const at::AutoDispatchBelowAutograd below;
   return THPVariable_Wrap(clip ? op_grad_clip_(grads, norm_type, scale, max_norm)
                                : op_grad_norm(grads, norm_type, scale));
