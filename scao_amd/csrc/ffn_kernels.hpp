@@ -9,11 +9,12 @@
 // Roundings of the 16-bit types: h, da and db, which enter further products on
 // the matrix cores, to the type itself, once each; nothing else before the
 // outputs.  a and b, which only enter f' and elementwise products, are kept for
-// the backward pass with 16 significant bits (24 of a float's 32): rounded to 8
-// (bf16) they would add as much error to da and db as those' own rounding.  In
-// fp32 nothing is rounded below it: h, da and db are kept as three bf16 parts
-// that add up to them, and a product of two such sums is six products of parts
-// (see mfma_x6) run as six segments of one bf16 product.
+// the backward pass with 16 significant bits (a float without its lowest byte):
+// rounded to 8 (bf16) they would add as much error to da and db as those' own
+// rounding.  In fp32 nothing is rounded below it (GELU's polynomial aside, which
+// is good to 1.5e-7 of erfc): h, da and db are kept as three bf16 parts that add
+// up to them, and a product of two such sums is six products of parts (see
+// mfma_x6) run as six segments of one bf16 product.
 #pragma once
 
 #include "ffn_gemm.hpp"

@@ -12,7 +12,7 @@
 // The tensors' table travels in the kernel's arguments, so a call copies
 // nothing to the device and waits for nothing: at most TABLE tensors a launch.
 // Each workgroup adds up for itself where a tensor's chunks begin, so that a
-// tensor takes 12 bytes of it and not 20: 332 tensors of 76 MB in one table
+// tensor takes 12 bytes of it and not 20: 332 tensors of 25.5 MB in one table
 // 25.5 us, in two tables of 190 40.2.  A tensor is cut into chunks of 32 KiB
 // (eight 16-byte loads in flight a thread).  Vectors are aligned to 16 bytes
 // whatever the tensor's start is: the first and the last vector of a tensor are

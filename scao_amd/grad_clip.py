@@ -5,12 +5,12 @@ training loop does between ``loss.backward()`` and ``SCAO.step()``.
     norm = scao_amd.clip_grad_norm_(model.parameters(), 1.0, scale=scale)
     opt.step()
 
-The call forms are ``torch.nn.utils.clip_grad_norm_``'s, with ``scale`` for
-gradients that are a sum of micro-batches or carry a loss scale: it multiplies
-every gradient in the same pass.  The gradients of all tensors go through two
-kernels (``scao_grad_norm`` / ``scao_grad_clip``, called from csrc/torch_host.cpp
-as operators of torch's dispatcher) on the current stream, without a host
-synchronisation and without a copy of the tensors' table.
+The call forms are ``torch.nn.utils.clip_grad_norm_``'s (without ``foreach``),
+with ``scale`` for gradients that are a sum of micro-batches or carry a loss
+scale: it multiplies every gradient in the same pass.  The gradients of all
+tensors go through two kernels (``scao_grad_norm`` / ``scao_grad_clip``, called
+from csrc/torch_host.cpp as operators of torch's dispatcher) on the current
+stream, without a host synchronisation and without a copy of the tensors' table.
 """
 
 from __future__ import annotations
