@@ -48,9 +48,11 @@ int scao_grad_clip(const scao_tensor_desc* tensors, int n, int norm_type, double
  * fp32.  With `saved` (scao_ffn_saved_bytes() bytes) the forward pass keeps h, a
  * and b for scao_ffn_backward: dh = dy Wd, da = dh * b * f'(a), db = dh * f(a),
  * dx = da Wg + db Wu, dWg = da^T x, dWu = db^T x, dWd = dy^T h, each written
- * densely (row strides d, d, d, f) unless its pointer is null.  No atomics: the
- * same call gives the same bits.  workspace: the *_workspace() bytes for the
- * same descriptor, aligned to 16, as is `saved`. */
+ * densely (row strides d, d, d, f) unless its pointer is null.  A NaN or an
+ * infinity in a token's row of x or dy reaches that token's y and dx (as NaN also
+ * where the exact result would be infinite) and the weights' gradients, and no
+ * other token.  No atomics: the same call gives the same bits.  workspace: the
+ * *_workspace() bytes for the same descriptor, aligned to 16, as is `saved`. */
 enum scao_activation {
   SCAO_ACT_SILU = 0,        /* a / (1 + exp(-a))                                 */
   SCAO_ACT_GELU = 1,        /* a (1 + erf(a / sqrt 2)) / 2                       */

@@ -205,10 +205,11 @@ def test_traces_without_memory(hip_device):
         y = scao_amd.gated_ffn(*leaves)
         return y.detach(), *torch.autograd.grad(y, leaves, dy)
 
-    traced = make_fx(training, tracing_mode="fake")(*ins)
     want = _run(*ins)
-    for got, k in zip(traced(*ins), want):
-        assert torch.equal(got, want[k])
+    for mode in ("fake", "symbolic"):
+        traced = make_fx(training, tracing_mode=mode)(*ins)
+        for got, k in zip(traced(*ins), want):
+            assert torch.equal(got, want[k]), mode
 
 
 @pytest.mark.parametrize("which", range(4))
