@@ -85,6 +85,55 @@ int scao_ffn_backward(const scao_ffn_desc* desc, const void* dy, int64_t ld_dy, 
                       void* dx, void* dw_gate, void* dw_up, void* dw_down, void* workspace,
                       void* stream);
 
+/* ---- orthogonalised updates --------------------------------------------------
+ * Newton-Schulz products: X = G / (|G|_F + eps), then `steps` times, with the
+ * step's coefficients (a, b, c) = coefficients[3k .. 3k+2] (host doubles),
+ *   A = X X^T,  X <- a X + (b A + c A A) X     (rows <= cols, else on X^T)
+ * which sends every singular value s of G / (|G|_F + eps) through the odd
+ * polynomials a s + b s^3 + c s^5.  The matrices of a HOST table may differ in
+ * shape and type; all of them share the launches.  Rows have unit column stride
+ * and a row stride of at least a row; src and dst may differ in type.
+ *   SCAO_ORTHO_FAST  products of fp16 words with fp32 sums, X, A and B rounded to
+ *                    11 significant bits once a step (results about 5e-4 off);
+ *   SCAO_ORTHO_FP32  words of 22 bits, three products each: fp32's accuracy.
+ * A matrix with a NaN or an infinity (or with a sum of squares beyond double's
+ * range) gives NaN throughout, and no other matrix; one of zeros gives zeros.
+ * Coefficients that may take a singular value of [0, 1] beyond 1024 are refused.
+ * The norm is summed in double, no atomics: the same call gives the same bits.
+ *
+ * scao_muon_step: with the momentum m (fp32) and the gradient g
+ *   m <- mu m + (1 - mu) g,  G = nesterov ? mu m + (1 - mu) g : m,
+ *   p <- decay p - rate orthogonalised(G)
+ * p, g and m contiguous; p and g may have different types; p is rounded once.
+ *
+ * Written memory may not overlap with anything else of the table
+ * (SCAO_ERR_INVALID).  workspace: the *_workspace() bytes for the same table,
+ * steps and precision, aligned to 16, contents of no meaning. */
+enum scao_ortho_precision { SCAO_ORTHO_FAST = 0, SCAO_ORTHO_FP32 = 1 };
+typedef struct scao_ortho_desc {   /* HOST */
+  const void* src;
+  void* dst;
+  int64_t rows, cols;              /* below 2^20, the smaller one up to 2^15     */
+  int64_t ld_src, ld_dst;          /* row strides in elements                    */
+  int32_t src_dtype, dst_dtype;    /* enum scao_dtype                            */
+} scao_ortho_desc;
+int64_t scao_orthogonalize_workspace(const scao_ortho_desc* matrices, int n, int steps,
+                                     int precision);
+int scao_orthogonalize(const scao_ortho_desc* matrices, int n, const double* coefficients, int steps,
+                       double eps, int precision, void* workspace, void* stream);
+typedef struct scao_muon_desc {    /* HOST */
+  void* p;
+  const void* g;
+  float* m;
+  int64_t rows, cols;
+  int32_t dtype, grad_dtype;       /* of p, of g                                 */
+  float rate, decay;
+} scao_muon_desc;
+int64_t scao_muon_workspace(const scao_muon_desc* matrices, int n, int steps, int precision);
+int scao_muon_step(const scao_muon_desc* matrices, int n, double momentum, int nesterov,
+                   const double* coefficients, int steps, double eps, int precision,
+                   void* workspace, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

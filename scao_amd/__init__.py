@@ -11,6 +11,7 @@ from .preconditioner import SparsePreconditioner
 from .utils import matrix_power_neg_quarter, adaptive_rank
 from .ffn import GatedFFN, gated_ffn
 from .grad_clip import clip_grad_norm_, global_grad_norm
+from .ortho import Muon, orthogonalize
 from . import logging as scao_logging
 
 __version__ = "0.2.0"
@@ -25,6 +26,8 @@ __all__ = [
     "gated_ffn",
     "clip_grad_norm_",
     "global_grad_norm",
+    "Muon",
+    "orthogonalize",
     "scao_logging",
     "__version__",
 ]

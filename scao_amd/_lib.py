@@ -103,6 +103,15 @@ FFN_DESC = np.dtype([
     ("ld_gate", "i8"), ("ld_up", "i8"), ("ld_down", "i8"), ("tokens", "i8"), ("d", "i8"),
     ("f", "i8"), ("dtype", "i4"), ("act", "i4"),
 ], align=True)
+ORTHO_DESC = np.dtype([
+    ("src", "u8"), ("dst", "u8"), ("rows", "i8"), ("cols", "i8"), ("ld_src", "i8"),
+    ("ld_dst", "i8"), ("src_dtype", "i4"), ("dst_dtype", "i4"),
+], align=True)
+MUON_DESC = np.dtype([
+    ("p", "u8"), ("g", "u8"), ("m", "u8"), ("rows", "i8"), ("cols", "i8"), ("dtype", "i4"),
+    ("grad_dtype", "i4"), ("rate", "f4"), ("decay", "f4"),
+], align=True)
+ORTHO_FAST, ORTHO_FP32 = 0, 1
 FILTER_WORK_WORDS = 2 * 2048 + 16
 FILTER_COMPACT_WORD = 2 * 2048 + 11   # 1 when the refinement passes read the candidates
 FILTER_REGION = 2048                  # candidate slots per chunk (SCAO_FLAT_CHUNK / 2)
@@ -116,7 +125,9 @@ STRUCTS = {0: (PARAM_DESC, [n for n in PARAM_DESC.names if n != "pad0"]),
            6: (FILTER_DESC, list(FILTER_DESC.names)),
            7: (LOOKAHEAD_DESC, [n for n in LOOKAHEAD_DESC.names if n != "pad0"]),
            8: (TENSOR_DESC, [n for n in TENSOR_DESC.names if n != "pad0"]),
-           9: (FFN_DESC, list(FFN_DESC.names))}
+           9: (FFN_DESC, list(FFN_DESC.names)),
+           10: (ORTHO_DESC, list(ORTHO_DESC.names)),
+           11: (MUON_DESC, list(MUON_DESC.names))}
 
 _VP, _I, _I64, _D = ctypes.c_void_p, ctypes.c_int, ctypes.c_int64, ctypes.c_double
 
@@ -175,6 +186,10 @@ TRAIN_SIGNATURES = {
     "scao_ffn_forward": (_I, [_VP, _VP, _VP, _VP, _VP]),
     "scao_ffn_backward_workspace": (_I64, [_VP, _VP, _I64, _I]),
     "scao_ffn_backward": (_I, [_VP, _VP, _I64, _VP, _VP, _VP, _VP, _VP, _VP, _VP]),
+    "scao_orthogonalize_workspace": (_I64, [_VP, _I, _I, _I]),
+    "scao_orthogonalize": (_I, [_VP, _I, _VP, _I, _D, _I, _VP, _VP]),
+    "scao_muon_workspace": (_I64, [_VP, _I, _I, _I]),
+    "scao_muon_step": (_I, [_VP, _I, _D, _I, _VP, _I, _D, _I, _VP, _VP]),
 }
 
 

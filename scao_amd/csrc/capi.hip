@@ -122,6 +122,22 @@ extern "C" int scao_struct_layout(int which, int64_t* out, int cap) {
       PUT(offsetof(S, d)); PUT(offsetof(S, f)); PUT(offsetof(S, dtype)); PUT(offsetof(S, act));
       break;
     }
+    case 10: {
+      typedef scao_ortho_desc S;
+      PUT(sizeof(S));
+      PUT(offsetof(S, src)); PUT(offsetof(S, dst)); PUT(offsetof(S, rows)); PUT(offsetof(S, cols));
+      PUT(offsetof(S, ld_src)); PUT(offsetof(S, ld_dst)); PUT(offsetof(S, src_dtype));
+      PUT(offsetof(S, dst_dtype));
+      break;
+    }
+    case 11: {
+      typedef scao_muon_desc S;
+      PUT(sizeof(S));
+      PUT(offsetof(S, p)); PUT(offsetof(S, g)); PUT(offsetof(S, m)); PUT(offsetof(S, rows));
+      PUT(offsetof(S, cols)); PUT(offsetof(S, dtype)); PUT(offsetof(S, grad_dtype));
+      PUT(offsetof(S, rate)); PUT(offsetof(S, decay));
+      break;
+    }
     default:
       return 0;
   }

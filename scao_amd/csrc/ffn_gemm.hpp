@@ -173,8 +173,10 @@ __device__ __forceinline__ void tile_of(int b, int tm, int tn, int& m, int& n) {
 }
 
 // GATED: B's tile rows 0 .. BN/2-1 are gate rows, the others the same columns'
-// up rows; each wave's fragments are half of either.
-template <int BM, int BN, int WM, int WN, int LA, int LB, bool F16, bool GATED>
+// up rows; each wave's fragments are half of either.  OPS: FfnOperands, or what
+// has its a[segment], b[segment], strides and sizes.
+template <int BM, int BN, int WM, int WN, int LA, int LB, bool F16, bool GATED,
+          class OPS = FfnOperands>
 struct Gemm {
   static constexpr int NW = WM * WN, THREADS = NW * 64, BM_ = BM, BN_ = BN;
   static constexpr int FRAGS = BM / 16 * (BN / 16);   // of 16 x 16 sums
@@ -185,13 +187,13 @@ struct Gemm {
   static constexpr int COLS_N = GATED ? BN / 2 : BN;   // of C
   static_assert(!GATED || LB == ROWS, "gated products have weights in rows");
 
-  const FfnOperands& o;
+  const OPS& o;
   lchar* lds;
   int wave, lane, wm, wn, m0, n0;
   uint32_t offa[TA::LOADS], offb[TB::LOADS];
   int ina[TA::LOADS], inb[TB::LOADS];
 
-  __device__ __forceinline__ Gemm(const FfnOperands& ops, lchar* l, int tm, int tn) : o(ops), lds(l) {
+  __device__ __forceinline__ Gemm(const OPS& ops, lchar* l, int tm, int tn) : o(ops), lds(l) {
     wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     lane = threadIdx.x & 63;
     wm = wave / WN;

@@ -1,0 +1,525 @@
+// Newton-Schulz orthogonalisation of matrix updates, and the step of the optimiser
+// that is built on it: argument checks, memory plans and the order of the launches.
+// The kernels are in ortho_norm.hpp and ortho_kernels.hpp.
+#include <algorithm>
+#include <cmath>
+#include <new>
+#include <vector>
+
+#include "ortho_norm.hpp"
+
+using namespace scao;
+
+namespace {
+
+constexpr int MAX_STEPS = 64;
+constexpr int64_t MAX_SIDE = (int64_t)1 << 20, MAX_SMALLER = (int64_t)1 << 15;
+
+int64_t round_up(int64_t x, int64_t to) { return (x + to - 1) / to * to; }
+int size_of(int dt) { return dt == SCAO_F32 ? 4 : 2; }
+
+struct Matrix {
+  const void* src;
+  float* buf;
+  void* dst;
+  int64_t rows, cols, ld_src, ld_dst;
+  int src_dtype, dst_dtype;
+  float rate, decay;
+  int64_t smaller() const { return std::min(rows, cols); }
+  int64_t larger() const { return std::max(rows, cols); }
+  // C's tiles of 256 x 256 in an update
+  int64_t tiles() const { return ((rows + 255) / 256) * ((cols + 255) / 256); }
+};
+
+// ------------------------------------------------- what the words can hold ---
+// The largest |f| on [0, u] of an odd polynomial a x + b x^3 + c x^5.
+double largest(double a, double b, double c, double u) {
+  auto at = [&](double x) { return std::fabs(x * (a + x * x * (b + x * x * c))); };
+  double most = at(u);
+  // a + 3 b t + 5 c t^2 = 0, t = x^2
+  double t[2] = {-1, -1};
+  const double p = 5 * c, q = 3 * b, disc = q * q - 4 * p * a;
+  if (p == 0) {
+    if (q != 0) t[0] = -a / q;
+  } else if (disc >= 0) {
+    const double z = -0.5 * (q + std::copysign(std::sqrt(disc), q));
+    t[0] = z / p;
+    if (z != 0) t[1] = a / z;
+  }
+  for (double x : t)
+    if (x > 0 && x < u * u) most = std::max(most, at(std::sqrt(x)));
+  return most;
+}
+// of b t + c t^2 on [0, t0]
+double largest2(double b, double c, double t0) {
+  auto at = [&](double t) { return std::fabs(t * (b + t * c)); };
+  double most = at(t0);
+  if (c != 0) {
+    const double t = -b / (2 * c);
+    if (t > 0 && t < t0) most = std::max(most, at(t));
+  }
+  return most;
+}
+// a power of two that takes values up to `most` to at most 16384, a quarter of
+// fp16's range: what the roundings before it have added finds room
+double power_for(double most, int limit) {
+  if (!(most > 0)) return std::ldexp(1.0, limit);
+  return std::ldexp(1.0, std::min(limit, (int)std::floor(std::log2(16384.0 / most))));
+}
+struct Scales {
+  double first;                       // of the first X
+  float gram[MAX_STEPS], square[MAX_STEPS], square_keep[MAX_STEPS];
+  float update[MAX_STEPS], update_keep[MAX_STEPS];
+};
+// false: some singular value may grow past what the words hold
+bool scales_of(const double* co, int steps, Scales& s) {
+  double u = 1.0, sx = power_for(u, 14);
+  s.first = sx;
+  for (int k = 0; k < steps; ++k) {
+    const double a = co[3 * k], b = co[3 * k + 1], c = co[3 * k + 2];
+    const double sa = power_for(u * u, 14), sb = power_for(largest2(b, c, u * u), 20);
+    const double next = largest(a, b, c, u) * 1.01;
+    if (!(next <= 1024.0) || !(sb >= 1.0 / 65536)) return false;
+    const double to = k + 1 < steps ? power_for(next, 14) : 1.0;
+    s.gram[k] = (float)(sa / (sx * sx));
+    s.square[k] = (float)(c * sb / (sa * sa));
+    s.square_keep[k] = (float)(b * sb / sa);
+    s.update[k] = (float)(to / (sb * sx));
+    s.update_keep[k] = (float)(a * to / sx);
+    u = next;
+    sx = to;
+  }
+  return true;
+}
+
+// -------------------------------------------------------------- one pass ---
+// us of a k step with one workgroup a CU and with all a CU holds, and of a tile's
+// beginning and end: those of the feed-forward block's products on the same tiles
+struct Cost {
+  int side, slots;
+  double lone, full, ends;
+  double step(int64_t groups) const {
+    const double crowd = groups >= slots  ? 1.0
+                         : slots == 256   ? groups / 256.0
+                         : groups <= 256  ? 0.0
+                                          : (groups - 256.0) / (slots - 256.0);
+    return lone + (full - lone) * crowd;
+  }
+};
+const Cost COSTS[2] = {{128, 512, 0.62, 1.14, 5.2}, {256, 256, 1.15, 1.50, 4.9}};
+
+struct Plan {
+  int big = 0;
+  OrthoPhase ph{};
+};
+
+struct Pass {
+  const Matrix* m;
+  const int* order;          // the pass's entries
+  int n, words;
+  char* base;
+  std::vector<OrthoGroup> groups;
+  double* norms = nullptr;
+  int64_t used = 0, peak = 0;
+
+  int64_t take(int64_t bytes) {
+    const int64_t at = used;
+    used += round_up(bytes, 256);
+    peak = std::max(peak, used);
+    return at;
+  }
+  const Matrix& entry(int i) const { return m[order[i]]; }
+
+  Pass(const Matrix* matrices, const int* order_, int n_, int words_, char* base_, bool again)
+      : m(matrices), order(order_), n(n_), words(words_), base(base_) {
+    norms = (double*)(base + take((int64_t)ORTHO_MATRICES * ORTHO_PARTS * 8));
+    for (int i = 0; i < n;) {
+      OrthoGroup g{};
+      g.first = i;
+      g.rows = (int)entry(i).rows;
+      g.cols = (int)entry(i).cols;
+      while (i < n && entry(i).rows == g.rows && entry(i).cols == g.cols) ++i;
+      g.count = i - g.first;
+      const int64_t s = std::min(g.rows, g.cols);
+      g.ldx = (int)round_up(g.cols, 8);
+      g.lda = (int)round_up(s, 8);
+      g.x_step = round_up((int64_t)words * g.rows * g.ldx * 2, 256);
+      g.a_step = round_up(words * s * g.lda * 2, 256);
+      g.x = take(g.count * g.x_step);
+      g.y = again ? take(g.count * g.x_step) : g.x;   // (one step writes the result alone)
+      g.a = take(g.count * g.a_step);
+      g.b = take(g.count * g.a_step);
+      groups.push_back(g);
+    }
+  }
+
+  static int64_t sum_of(int phase, const OrthoGroup& g) {
+    return phase == ORTHO_GRAM ? std::max(g.rows, g.cols) : std::min(g.rows, g.cols);
+  }
+  // The groups' tiles of `side`, the longest sums first.
+  void lay(int phase, int side, OrthoPhase& ph) const {
+    std::vector<OrthoGroup> g = groups;
+    std::stable_sort(g.begin(), g.end(), [&](const OrthoGroup& a, const OrthoGroup& b) {
+      return sum_of(phase, a) > sum_of(phase, b);
+    });
+    int64_t tiles = 0;
+    for (size_t i = 0; i < g.size(); ++i) {
+      OrthoGroup& q = g[i];
+      if (phase == ORTHO_UPDATE) {
+        q.tiles_m = (q.rows + side - 1) / side;
+        q.tiles_n = (q.cols + side - 1) / side;
+        q.per = q.tiles_m * q.tiles_n;
+      } else {
+        q.tiles_m = q.tiles_n = (int)((std::min(q.rows, q.cols) + side - 1) / side);
+        q.per = q.tiles_m * (q.tiles_m + 1) / 2;
+      }
+      q.tile0 = (int)tiles;
+      tiles += (int64_t)q.count * q.per;
+      ph.g[i] = q;
+    }
+    ph.groups = (int)g.size();
+    ph.tiles = (int)tiles;
+  }
+  // Estimated us of the tiles from `begin` on, each in n parts: rounds of as many
+  // workgroups as the chip holds, as long as their first.
+  double rounds(int phase, const OrthoPhase& ph, const Cost& c, int begin, int end, int n) const {
+    double us = 0;
+    int k = 0;
+    const int64_t all = (int64_t)(end - begin) * n;
+    for (int64_t at = 0; at < all; at += c.slots) {
+      const int tile = begin + (int)(at / n);
+      while (k + 1 < ph.groups && ph.g[k + 1].tile0 <= tile) ++k;
+      const int64_t steps = steps_of(phase, ph.g[k]);
+      us += (steps + n - 1) / n * c.step(std::min<int64_t>(c.slots, all - at)) + c.ends;
+    }
+    return us;
+  }
+  int64_t steps_of(int phase, const OrthoGroup& g) const {
+    return (words == 2 ? 3 : 1) * ((sum_of(phase, g) + FFN_BK - 1) / FFN_BK);
+  }
+  // Which tile, how many of them run in one piece and in how many parts the others:
+  // all of them, or those that do not fill a last round.  The join: a launch, and 8
+  // bytes a part and element.
+  Plan plan(int phase) {
+    Plan best;
+    double least = 1e30;
+    for (int big = 0; big < 2; ++big) {
+      const Cost& c = COSTS[big];
+      OrthoPhase ph{};
+      lay(phase, c.side, ph);
+      const int whole_rounds = ph.tiles / c.slots * c.slots;
+      for (int n : {1, 2, 3, 4, 6, 8, 12, 16})
+        for (int whole : {0, whole_rounds}) {
+          if (n == 1 ? whole != 0 : whole == ph.tiles) continue;
+          const int rest = ph.tiles - whole;
+          if (n > 1 && ((int64_t)rest * n > (big ? 1024 : 2048) ||
+                        2 * n > steps_of(phase, ph.g[ph.groups - 1])))
+            continue;
+          double us = n == 1 ? rounds(phase, ph, c, 0, ph.tiles, 1)
+                             : rounds(phase, ph, c, 0, whole, 1) +
+                                   rounds(phase, ph, c, whole, ph.tiles, n) + 3 +
+                                   (8 / 7.4e6 * n + 4 / 5e6) * rest * c.side * c.side;
+          if (us < least) {
+            least = us;
+            best.big = big;
+            best.ph = ph;
+            best.ph.splits = n;
+            best.ph.whole = n == 1 ? ph.tiles : whole;
+          }
+        }
+    }
+    const int64_t rest = best.ph.tiles - best.ph.whole;
+    best.ph.base = base;
+    if (rest) {   // the parts' room is given back
+      const int64_t at = used, side = COSTS[best.big].side;
+      best.ph.partial = (float*)(base + take(rest * best.ph.splits * side * side * 4));
+      used = at;
+    }
+    return best;
+  }
+
+  void prep(OrthoPrep& p, int& blocks) const {
+    blocks = 0;
+    for (size_t i = 0; i < groups.size(); ++i) {
+      const OrthoGroup& g = groups[i];
+      OrthoSource& s = p.g[i];
+      s.rows = g.rows;
+      s.cols = g.cols;
+      s.ldx = g.ldx;
+      s.first = g.first;
+      s.x = g.x;
+      s.x_step = g.x_step;
+      s.vecs = 1;
+      while (s.vecs < 256 && s.vecs * 8 < g.ldx) s.vecs *= 2;
+      s.across = (g.ldx / 8 + s.vecs - 1) / s.vecs;
+      const int64_t down = (g.rows + 256 / s.vecs - 1) / (256 / s.vecs), units = down * s.across;
+      s.per = (int)std::max<int64_t>(8, (units + ORTHO_PARTS - 1) / ORTHO_PARTS);
+      s.parts = (int)((units + s.per - 1) / s.per);
+      s.block0 = blocks;
+      blocks += s.parts * g.count;
+    }
+    for (int i = 0; i < n; ++i) {
+      const Matrix& e = entry(i);
+      p.src[i] = e.src;
+      p.buf[i] = e.buf;
+      p.ld[i] = (int)e.ld_src;
+      p.dt[i] = (uint8_t)e.src_dtype;
+    }
+    p.groups = (int)groups.size();
+    p.base = base;
+    p.norms = norms;
+  }
+
+  int run(const char* who, const Scales& sc, int steps, double eps, double momentum, bool nesterov,
+          int dest, hipStream_t st) {
+    Plan plans[3] = {plan(ORTHO_GRAM), plan(ORTHO_SQUARE), plan(ORTHO_UPDATE)};
+    OrthoPrep p{};
+    int blocks;
+    prep(p, blocks);
+    p.eps = eps;
+    p.scale = sc.first;
+    p.momentum = (float)momentum;
+    p.rest = (float)(1.0 - momentum);
+    p.nesterov = nesterov;
+    k_ortho_norm<<<blocks, 256, 0, st>>>(p);
+    if (words == 2) k_ortho_scale<2><<<blocks, 256, 0, st>>>(p);
+    else k_ortho_scale<1><<<blocks, 256, 0, st>>>(p);
+    SCAO_LAUNCH_CHECK(who);
+    OrthoOut out{};
+    for (int i = 0; i < n; ++i) {
+      out.p[i] = entry(i).dst;
+      out.ld[i] = (int)entry(i).ld_dst;
+      out.dt[i] = (uint8_t)entry(i).dst_dtype;
+      out.rate[i] = entry(i).rate;
+      out.decay[i] = entry(i).decay;
+    }
+    const auto product = words == 2 ? ortho_product2 : ortho_product1;
+    for (int k = 0; k < steps; ++k) {
+      plans[ORTHO_GRAM].ph.by = sc.gram[k];
+      plans[ORTHO_SQUARE].ph.by = sc.square[k];
+      plans[ORTHO_SQUARE].ph.keep = sc.square_keep[k];
+      plans[ORTHO_UPDATE].ph.by = sc.update[k];
+      plans[ORTHO_UPDATE].ph.keep = sc.update_keep[k];
+      for (int phase = 0; phase < 3; ++phase) {
+        product(plans[phase].big, phase,
+                phase == ORTHO_UPDATE && k + 1 == steps ? dest : ORTHO_NEXT, plans[phase].ph, out,
+                st);
+        SCAO_LAUNCH_CHECK(who);
+      }
+      for (Plan& q : plans)
+        for (int i = 0; i < q.ph.groups; ++i) std::swap(q.ph.g[i].x, q.ph.g[i].y);
+    }
+    return SCAO_OK;
+  }
+};
+
+// The matrices in passes, those of one shape together, larger ones first.  A pass
+// ends at eight rounds of tiles, so that the workspace does not grow with the model.
+constexpr int64_t PASS_TILES = 2048;
+template <class F>
+int for_passes(const std::vector<Matrix>& m, F&& f) {
+  std::vector<int> order;
+  for (int i = 0; i < (int)m.size(); ++i)
+    if (m[i].rows && m[i].cols) order.push_back(i);
+  std::stable_sort(order.begin(), order.end(), [&](int i, int j) {
+    const Matrix &a = m[i], &b = m[j];
+    if (a.smaller() != b.smaller()) return a.smaller() > b.smaller();
+    return a.rows != b.rows ? a.rows > b.rows : a.cols > b.cols;
+  });
+  for (size_t i = 0; i < order.size();) {
+    const size_t begin = i;
+    int64_t tiles = 0;
+    int groups = 0;
+    while (i < order.size() && i - begin < ORTHO_MATRICES && tiles < PASS_TILES) {
+      const Matrix& e = m[order[i]];
+      if (i == begin || e.rows != m[order[i - 1]].rows || e.cols != m[order[i - 1]].cols)
+        if (++groups > ORTHO_GROUPS) break;
+      tiles += e.tiles();
+      ++i;
+    }
+    if (const int rc = f(&order[begin], (int)(i - begin))) return rc;
+  }
+  return SCAO_OK;
+}
+
+int64_t workspace_of(const std::vector<Matrix>& m, int words, int steps) {
+  int64_t most = 0;
+  for_passes(m, [&](const int* order, int n) {
+    Pass p(m.data(), order, n, words, nullptr, steps > 1);
+    for (int phase = 0; phase < 3; ++phase) p.plan(phase);
+    most = std::max(most, p.peak);
+    return SCAO_OK;
+  });
+  return most;
+}
+
+int run_all(const char* who, const std::vector<Matrix>& m, const double* coefficients, int steps,
+            double eps, int words, double momentum, bool nesterov, int dest, void* workspace,
+            void* stream) {
+  Scales sc;
+  SCAO_CHECK_ARG(scales_of(coefficients, steps, sc),
+                 "%s: with these coefficients singular values may grow beyond 1024", who);
+  SCAO_CHECK_ARG((uintptr_t)workspace % 16 == 0, "%s: workspace is not aligned", who);
+  return for_passes(m, [&](const int* order, int n) -> int {
+    SCAO_CHECK_ARG(workspace, "%s: null workspace", who);
+    Pass p(m.data(), order, n, words, (char*)workspace, steps > 1);
+    return p.run(who, sc, steps, eps, momentum, nesterov, dest, (hipStream_t)stream);
+  });
+}
+
+int check_scheme(const char* who, int n, const void* table, const double* coefficients, int steps,
+                 double eps, int precision) {
+  SCAO_CHECK_ARG(n >= 0 && (n == 0 || table), "%s: null table or negative count", who);
+  SCAO_CHECK_ARG(steps >= 1 && steps <= MAX_STEPS, "%s: %d steps (1 to %d)", who, steps, MAX_STEPS);
+  SCAO_CHECK_ARG(coefficients, "%s: null coefficients", who);
+  for (int i = 0; i < 3 * steps; ++i)
+    SCAO_CHECK_ARG(std::isfinite(coefficients[i]), "%s: coefficient %d is no finite number", who, i);
+  SCAO_CHECK_ARG(eps > 0 && std::isfinite(eps), "%s: eps %g is not positive and finite", who, eps);
+  SCAO_CHECK_ARG(precision == SCAO_ORTHO_FAST || precision == SCAO_ORTHO_FP32, "%s: precision %d",
+                 who, precision);
+  return SCAO_OK;
+}
+int check_sizes(const char* who, int i, int64_t rows, int64_t cols) {
+  SCAO_CHECK_ARG(rows >= 0 && cols >= 0 && std::max(rows, cols) < MAX_SIDE &&
+                     std::min(rows, cols) <= MAX_SMALLER,
+                 "%s: matrix %d is %lld x %lld (sides below 2^20, the smaller one up to 2^15)", who,
+                 i, (long long)rows, (long long)cols);
+  return SCAO_OK;
+}
+int check_matrix(const char* who, int i, const char* name, const void* p, int64_t rows, int64_t cols,
+                 int64_t ld, int dtype) {
+  SCAO_CHECK_ARG(dtype >= 0 && dtype <= SCAO_F16, "%s: dtype %d of matrix %d", who, dtype, i);
+  SCAO_CHECK_ARG(p && (uintptr_t)p % size_of(dtype) == 0,
+                 "%s: %s of matrix %d is null or not aligned to its elements", who, name, i);
+  SCAO_CHECK_ARG(rows == 1 || (ld >= cols && ld <= 0x7fffffff),
+                 "%s: row stride %lld of %s of matrix %d (%lld columns)", who, (long long)ld, name,
+                 i, (long long)cols);
+  return SCAO_OK;
+}
+
+// what a call writes may not be what it writes or reads elsewhere
+struct Range {
+  uintptr_t begin, end;
+  bool written;
+};
+int check_apart(const char* who, std::vector<Range>& r) {
+  std::sort(r.begin(), r.end(), [](const Range& a, const Range& b) { return a.begin < b.begin; });
+  // the furthest end so far of what is written, and of anything
+  uintptr_t wrote = 0, any = 0;
+  for (const Range& x : r) {
+    SCAO_CHECK_ARG(x.begin >= wrote && (!x.written || x.begin >= any),
+                   "%s: two matrices share memory that is written", who);
+    any = std::max(any, x.end);
+    if (x.written) wrote = std::max(wrote, x.end);
+  }
+  return SCAO_OK;
+}
+Range range_of(const void* p, int64_t rows, int64_t cols, int64_t ld, int dtype, bool written) {
+  const uintptr_t at = (uintptr_t)p;
+  return {at, at + ((rows - 1) * (rows == 1 ? 0 : ld) + cols) * size_of(dtype), written};
+}
+
+int collect(const char* who, const scao_ortho_desc* t, int n, bool pointers, std::vector<Matrix>& m) {
+  std::vector<Range> r;
+  for (int i = 0; i < n; ++i) {
+    if (int rc = check_sizes(who, i, t[i].rows, t[i].cols)) return rc;
+    if (pointers && t[i].rows && t[i].cols) {
+      if (int rc = check_matrix(who, i, "src", t[i].src, t[i].rows, t[i].cols, t[i].ld_src,
+                                t[i].src_dtype))
+        return rc;
+      if (int rc = check_matrix(who, i, "dst", t[i].dst, t[i].rows, t[i].cols, t[i].ld_dst,
+                                t[i].dst_dtype))
+        return rc;
+      r.push_back(range_of(t[i].src, t[i].rows, t[i].cols, t[i].ld_src, t[i].src_dtype, false));
+      r.push_back(range_of(t[i].dst, t[i].rows, t[i].cols, t[i].ld_dst, t[i].dst_dtype, true));
+    }
+    const int64_t one = t[i].cols;   // a single row's stride is never used
+    m.push_back({t[i].src, nullptr, t[i].dst, t[i].rows, t[i].cols,
+                 t[i].rows == 1 ? one : t[i].ld_src, t[i].rows == 1 ? one : t[i].ld_dst,
+                 t[i].src_dtype, t[i].dst_dtype, 0.f, 0.f});
+  }
+  return check_apart(who, r);
+}
+int collect(const char* who, const scao_muon_desc* t, int n, bool pointers, std::vector<Matrix>& m) {
+  std::vector<Range> r;
+  for (int i = 0; i < n; ++i) {
+    const auto [rows, cols] = std::pair(t[i].rows, t[i].cols);
+    if (int rc = check_sizes(who, i, rows, cols)) return rc;
+    if (pointers && rows && cols) {
+      if (int rc = check_matrix(who, i, "p", t[i].p, rows, cols, cols, t[i].dtype)) return rc;
+      if (int rc = check_matrix(who, i, "g", t[i].g, rows, cols, cols, t[i].grad_dtype)) return rc;
+      if (int rc = check_matrix(who, i, "m", t[i].m, rows, cols, cols, SCAO_F32)) return rc;
+      SCAO_CHECK_ARG(std::isfinite(t[i].rate) && std::isfinite(t[i].decay),
+                     "%s: rate or decay of matrix %d is no finite number", who, i);
+      r.push_back(range_of(t[i].g, rows, cols, cols, t[i].grad_dtype, false));
+      r.push_back(range_of(t[i].p, rows, cols, cols, t[i].dtype, true));
+      r.push_back(range_of(t[i].m, rows, cols, cols, SCAO_F32, true));
+    }
+    m.push_back({t[i].g, t[i].m, t[i].p, rows, cols, cols, cols, t[i].grad_dtype, t[i].dtype,
+                 t[i].rate, t[i].decay});
+  }
+  return check_apart(who, r);
+}
+int words_of(int precision) { return precision == SCAO_ORTHO_FP32 ? 2 : 1; }
+
+}  // namespace
+
+namespace {
+// no C++ exception leaves a C entry
+template <class T, class F>
+T guarded(const char* who, int n, T failed, F&& f) {
+  try {
+    return f();
+  } catch (const std::bad_alloc&) {
+    scao_set_error("%s: no host memory for %d matrices", who, n);
+    return failed;
+  }
+}
+}  // namespace
+
+extern "C" int64_t scao_orthogonalize_workspace(const scao_ortho_desc* matrices, int n, int steps,
+                                                int precision) {
+  const char* who = "scao_orthogonalize_workspace";
+  return guarded<int64_t>(who, n, 0, [&]() -> int64_t {
+    std::vector<Matrix> m;
+    if (n <= 0 || !matrices || collect(who, matrices, n, false, m)) return 0;
+    return workspace_of(m, words_of(precision), steps);
+  });
+}
+
+extern "C" int scao_orthogonalize(const scao_ortho_desc* matrices, int n,
+                                  const double* coefficients, int steps, double eps, int precision,
+                                  void* workspace, void* stream) {
+  const char* who = "scao_orthogonalize";
+  return guarded<int>(who, n, SCAO_ERR_INVALID, [&]() -> int {
+    if (int rc = check_scheme(who, n, matrices, coefficients, steps, eps, precision)) return rc;
+    std::vector<Matrix> m;
+    if (int rc = collect(who, matrices, n, true, m)) return rc;
+    return run_all(who, m, coefficients, steps, eps, words_of(precision), 0.0, false, ORTHO_RESULT,
+                   workspace, stream);
+  });
+}
+
+extern "C" int64_t scao_muon_workspace(const scao_muon_desc* matrices, int n, int steps,
+                                       int precision) {
+  const char* who = "scao_muon_workspace";
+  return guarded<int64_t>(who, n, 0, [&]() -> int64_t {
+    std::vector<Matrix> m;
+    if (n <= 0 || !matrices || collect(who, matrices, n, false, m)) return 0;
+    return workspace_of(m, words_of(precision), steps);
+  });
+}
+
+extern "C" int scao_muon_step(const scao_muon_desc* matrices, int n, double momentum, int nesterov,
+                              const double* coefficients, int steps, double eps, int precision,
+                              void* workspace, void* stream) {
+  const char* who = "scao_muon_step";
+  return guarded<int>(who, n, SCAO_ERR_INVALID, [&]() -> int {
+    if (int rc = check_scheme(who, n, matrices, coefficients, steps, eps, precision)) return rc;
+    SCAO_CHECK_ARG(momentum >= 0 && momentum < 1, "%s: momentum %g is not in [0, 1)", who, momentum);
+    std::vector<Matrix> m;
+    if (int rc = collect(who, matrices, n, true, m)) return rc;
+    return run_all(who, m, coefficients, steps, eps, words_of(precision), momentum, nesterov != 0,
+                   ORTHO_PARAMETER, workspace, stream);
+  });
+}

@@ -1,0 +1,473 @@
+// The kernels of the Newton-Schulz orthogonalisation.
+//
+//   X = G / (|G| + eps), then for every step, on the smaller side of X:
+//   A = X X^T, B = b A + c A A, X <- a X + B X      (wide: rows <= cols)
+//   A = X^T X, B = b A + c A A, X <- a X + X B      (tall)
+//
+// Nothing is transposed in memory: the tiled product reads an operand with k or
+// with its rows contiguous.  A and B are symmetric, so only the tiles on and below
+// the diagonal are computed and the others stored as their mirror image.
+//
+// Words of the products.  X, A and B are fp16 (or, P = 2, a sum of two fp16 words,
+// 22 significant bits, multiplied as three products of words), scaled by powers of
+// two that the host chooses from what the polynomial can reach, so that neither end
+// of fp16's range matters: |X|, |A| and |B| are bounded by their largest singular
+// value.  fp16 has three bits more than bf16 at the same rate; each of the three is
+// rounded once a step.  Sums, a X and b A are fp32.
+//
+// All matrices of a call go through the same launches, whatever their shapes: a
+// launch's tiles are those of up to ORTHO_GROUPS groups of one shape each, the ones
+// with the longest sums first.
+#pragma once
+
+#include "ffn_kernels.hpp"
+
+namespace scao {
+
+constexpr int ORTHO_GROUPS = 16;     // shapes a pass
+constexpr int ORTHO_MATRICES = 64;   // matrices a pass
+constexpr int ORTHO_PARTS = 256;     // sums of squares a matrix
+
+enum { ORTHO_GRAM, ORTHO_SQUARE, ORTHO_UPDATE };
+// where an update goes: the next X, the result, or (the optimiser) the parameter
+enum { ORTHO_NEXT, ORTHO_RESULT, ORTHO_PARAMETER };
+
+// Matrices of one shape, with their buffers in the workspace one after the other.
+struct OrthoGroup {
+  int64_t x, y, a, b;        // bytes from the workspace's start: X, the next X, A, B
+  int64_t x_step, a_step;    // bytes from a matrix's X to the next one's; of A and B
+  int rows, cols, ldx, lda;
+  int first, count;          // entries of the pass's tables
+  int per, tiles_m, tiles_n; // tiles of a matrix
+  int tile0;                 // tiles of the groups before
+};
+struct OrthoPhase {
+  OrthoGroup g[ORTHO_GROUPS];
+  char* base;
+  float* partial;            // parts of split tiles
+  int groups, tiles, whole, splits;
+  float by, keep;            // of the product; of what is added to it
+};
+struct OrthoOut {
+  void* p[ORTHO_MATRICES];
+  int ld[ORTHO_MATRICES];
+  float rate[ORTHO_MATRICES], decay[ORTHO_MATRICES];   // p <- decay p - rate update
+  uint8_t dt[ORTHO_MATRICES];
+};
+
+// a matrix's words: segment `low` takes the lower ones
+struct OrthoWords {
+  const uint16_t* p;
+  int64_t plane;
+  int low;
+  __device__ __forceinline__ const void* operator[](int seg) const {
+    return p + (seg == low ? plane : 0);
+  }
+};
+struct OrthoOperands {
+  OrthoWords a, b;
+  int64_t lda, ldb;
+  int M, N, K, nseg, row0;
+};
+// P = 2: low x high, high x low, high x high
+template <int P>
+__device__ __forceinline__ OrthoOperands ortho_operands(const char* a, int64_t plane_a, int lda,
+                                                        const char* b, int64_t plane_b, int ldb,
+                                                        int M, int N, int K) {
+  return OrthoOperands{{(const uint16_t*)a, plane_a, P == 2 ? 0 : -1},
+                       {(const uint16_t*)b, plane_b, P == 2 ? 1 : -1},
+                       lda, ldb, M, N, K, P == 2 ? 3 : 1, 0};
+}
+
+// four values as fp16 words: rounded, or with the rest in a second word
+template <int P>
+__device__ __forceinline__ void ortho_words(v4f x, v2u (&w)[P]) {
+  w[0] = v4f_to_halves(SCAO_F16, x);
+  if constexpr (P == 2) w[1] = v4f_to_halves(SCAO_F16, x - halves_to_v4f(SCAO_F16, w[0]));
+}
+
+// ---------------------------------------------------------- products -------
+// The tile of place t of a group's tiles.  As tile_of does it, one XCD gets a
+// contiguous piece of them.
+__device__ __forceinline__ void ortho_tile_of(const OrthoGroup& g, bool lower, int t, int& matrix,
+                                              int& tm, int& tn) {
+  const int total = g.count * g.per, each = total / 8, rest = total % 8;
+  const int x = t % 8, at = x * each + (x < rest ? x : rest) + t / 8;
+  matrix = at / g.per;
+  const int in = at - matrix * g.per;
+  if (lower) {   // row tm's tiles 0 .. tm behind those of the rows before
+    tm = (int)((sqrtf(8.f * in + 1.f) - 1.f) * 0.5f);
+    if (tm * (tm + 1) / 2 > in) --tm;
+    if ((tm + 1) * (tm + 2) / 2 <= in) ++tm;
+    tn = in - tm * (tm + 1) / 2;
+    return;
+  }
+  constexpr int BAND = 8;
+  const int band = in / (BAND * g.tiles_n), rows = min(BAND, g.tiles_m - band * BAND);
+  const int rem = in - band * BAND * g.tiles_n;
+  tm = band * BAND + rem % rows;
+  tn = rem / rows;
+}
+__device__ __forceinline__ int ortho_group_of(const OrthoPhase& ph, int tile) {
+  int k = 0;
+  for (int i = 1; i < ph.groups; ++i)
+    if (tile >= ph.g[i].tile0) k = i;
+  return k;
+}
+
+// where the phase's product is stored, and what is added to it
+struct OrthoTarget {
+  uint16_t* to;
+  const uint16_t* add;
+  int64_t plane;
+  int ld, M, N, cols;      // cols: with the padding, N rounded up to 8
+  bool mirror;             // a tile below the diagonal
+};
+template <int PHASE>
+__device__ __forceinline__ OrthoTarget ortho_target(const OrthoPhase& ph, const OrthoGroup& g,
+                                                    int matrix, bool mirror) {
+  char* x = ph.base + matrix * g.x_step;
+  char* a = ph.base + matrix * g.a_step;
+  OrthoTarget t;
+  t.mirror = PHASE != ORTHO_UPDATE && mirror;
+  if (PHASE == ORTHO_UPDATE) {
+    t.to = (uint16_t*)(x + g.y);
+    t.add = (const uint16_t*)(x + g.x);
+    t.plane = (int64_t)g.rows * g.ldx;
+    t.ld = g.ldx;
+    t.M = g.rows;
+    t.N = g.cols;
+  } else {
+    t.to = (uint16_t*)(a + (PHASE == ORTHO_GRAM ? g.a : g.b));
+    t.add = (const uint16_t*)(a + g.a);
+    t.M = t.N = min(g.rows, g.cols);
+    t.plane = (int64_t)t.M * g.lda;
+    t.ld = g.lda;
+  }
+  t.cols = (t.N + 7) & ~7;
+  return t;
+}
+
+// the inverse of join_pair
+__device__ __forceinline__ void part_pair(v4u_t w, v2u& p, v2u& q) {
+  const auto a = __builtin_amdgcn_permlane16_swap(w[0], w[2], false, false);
+  const auto b = __builtin_amdgcn_permlane16_swap(w[1], w[3], false, false);
+  p = v2u{a[0], b[0]};
+  q = v2u{a[1], b[1]};
+}
+// Four lanes next to each other hold four columns of a row each; each gets one of
+// these columns' four rows instead.
+__device__ __forceinline__ v2u turn4(v2u w, int lane) {
+  const uint32_t sel = lane & 1 ? 0x03020706u : 0x05040100u;
+  uint32_t n[2];
+#pragma unroll
+  for (int i = 0; i < 2; ++i)
+    n[i] = __builtin_amdgcn_perm(__builtin_amdgcn_mov_dpp((int)w[i], 0xB1, 15, 15, true), w[i], sel);
+  const bool up = lane & 2;
+  const uint32_t own = up ? n[1] : n[0];
+  const uint32_t other = __builtin_amdgcn_mov_dpp((int)(up ? n[0] : n[1]), 0x4E, 15, 15, true);
+  return up ? v2u{other, own} : v2u{own, other};
+}
+
+// Two fragments next to each other, the first at row m (this lane's) and column n.
+template <int P, int PHASE>
+struct OrthoPair {
+  v4u_t w[P];
+  __device__ __forceinline__ void load(const OrthoTarget& t, int m, int n, int lane) {
+    if (PHASE == ORTHO_GRAM) return;
+    n += pair_column(lane);
+    const bool in = m < t.M && n < t.cols;
+#pragma unroll
+    for (int i = 0; i < P; ++i)
+      w[i] = in ? (v4u_t) * (const gv4u_a16*)(t.add + (int64_t)m * t.ld + n + i * t.plane)
+                : v4u_t{0, 0, 0, 0};
+  }
+  // by c + keep (what is added), likewise d
+  __device__ __forceinline__ void sum(float by, float keep, v4f& c, v4f& d) const {
+    c *= by;
+    d *= by;
+    if (PHASE == ORTHO_GRAM) return;
+#pragma unroll
+    for (int i = 0; i < P; ++i) {
+      v2u p, q;
+      part_pair(w[i], p, q);
+      const v4f x = halves_to_v4f(SCAO_F16, p), y = halves_to_v4f(SCAO_F16, q);
+#pragma unroll
+      for (int t = 0; t < 4; ++t) {
+        c[t] = fmaf(keep, x[t], c[t]);
+        d[t] = fmaf(keep, y[t], d[t]);
+      }
+    }
+  }
+};
+
+template <int P>
+__device__ __forceinline__ void ortho_store(const OrthoTarget& t, int m, int n, int lane, v4f c,
+                                            v4f d) {
+  v2u p[P], q[P];
+  ortho_words<P>(c, p);
+  ortho_words<P>(d, q);
+  const int at = n + pair_column(lane);
+  const bool in = m < t.M && at < t.cols;
+#pragma unroll
+  for (int i = 0; i < P; ++i) {
+    const v4u_t w = join_pair(p[i], q[i]);
+    if (in) *(gv4u_a16*)(t.to + (int64_t)m * t.ld + at + i * t.plane) = w;
+  }
+  if (!t.mirror) return;
+  // (a row of C is a column of the image, so C's padding rows are stored as the
+  // image's padding columns; a tile below the diagonal has no padding columns)
+  const int dm = lane & 15, row = n + 4 * (lane >> 4) + (dm & 3), col = m - (dm & 3);
+#pragma unroll
+  for (int i = 0; i < P; ++i) {
+    const v2u a = turn4(p[i], lane), b = turn4(q[i], lane);
+    if (col < t.cols) {
+      uint16_t* to = t.to + (int64_t)row * t.ld + col + i * t.plane;
+      typedef __attribute__((address_space(1))) v2u gv2u_a8;
+      *(gv2u_a8*)to = a;
+      *(gv2u_a8*)(to + (int64_t)16 * t.ld) = b;
+    }
+  }
+}
+
+// the last update: four columns from n of row m, in the type and place of the result
+struct OrthoPlace {
+  void* p;
+  int ld, dt;
+  float rate, decay;
+};
+template <int DEST>
+__device__ __forceinline__ void ortho_put4(const OrthoPlace& o, const OrthoTarget& t, int m, int n,
+                                           v4f c) {
+  const int left = t.N - n;
+  if (m >= t.M || left <= 0) return;
+  const int64_t at = (int64_t)m * o.ld + n;
+  const int mask = left >= 4 ? 15 : (1 << left) - 1;
+  if (DEST == ORTHO_PARAMETER) {
+    const v4f p = ld4(o.p, SCAO_F32, at, left >= 4, mask);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) c[i] = fmaf(-o.rate, c[i], o.decay * p[i]);
+  }
+  st4(o.p, SCAO_F32, at, c, left >= 4, mask);
+}
+template <int DEST>
+__device__ __forceinline__ void ortho_put(const OrthoPlace& o, const OrthoTarget& t, int m, int n,
+                                          int lane, v4f c, v4f d) {
+  const int dt = o.dt;
+  if (dt == SCAO_F32) {
+    n += 4 * (lane >> 4);
+    ortho_put4<DEST>(o, t, m, n, c);
+    ortho_put4<DEST>(o, t, m, n + 16, d);
+    return;
+  }
+  const int at = n + pair_column(lane);
+  uint16_t* to = (uint16_t*)o.p + (int64_t)m * o.ld + at;
+  const bool in = m < t.M && at < t.N, full = in && at + 8 <= t.N;
+  if (DEST == ORTHO_PARAMETER) {
+    v4u_t w = {0, 0, 0, 0};
+    if (full) {
+      w = *(const gv4u_a2*)to;
+    } else if (in) {
+#pragma unroll
+      for (int i = 0; i < 8; ++i)
+        if (at + i < t.N) w[i / 2] |= (uint32_t)((const gu16*)to)[i] << (16 * (i & 1));
+    }
+    v2u p, q;
+    part_pair(w, p, q);
+    const v4f x = halves_to_v4f(dt, p), y = halves_to_v4f(dt, q);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      c[i] = fmaf(-o.rate, c[i], o.decay * x[i]);
+      d[i] = fmaf(-o.rate, d[i], o.decay * y[i]);
+    }
+  }
+  v2u p, q;
+  if (dt == SCAO_BF16) {
+    p = v2u{pk_bf16(c[0], c[1]), pk_bf16(c[2], c[3])};
+    q = v2u{pk_bf16(d[0], d[1]), pk_bf16(d[2], d[3])};
+  } else {
+    p = v4f_to_halves(SCAO_F16, c);
+    q = v4f_to_halves(SCAO_F16, d);
+  }
+  const v4u_t w = join_pair(p, q);
+  if (full) {
+    *(gv4u_a2*)to = w;
+  } else if (in) {
+#pragma unroll
+    for (int i = 0; i < 8; ++i)
+      if (at + i < t.N) ((gu16*)to)[i] = (uint16_t)(w[i / 2] >> (16 * (i & 1)));
+  }
+}
+
+template <int P, int PHASE, int DEST>
+__device__ __forceinline__ void ortho_finish(const OrthoPhase& ph, const OrthoPlace& o,
+                                             const OrthoTarget& t, const OrthoPair<P, PHASE>& add,
+                                             int m, int n, int lane, v4f c, v4f d) {
+  add.sum(ph.by, ph.keep, c, d);
+  if constexpr (DEST == ORTHO_NEXT) ortho_store<P>(t, m, n, lane, c, d);
+  else ortho_put<DEST>(o, t, m, n, lane, c, d);
+}
+template <int DEST>
+__device__ __forceinline__ OrthoPlace ortho_place(const OrthoOut& o, int e) {
+  if (DEST == ORTHO_NEXT) return OrthoPlace{};
+  return OrthoPlace{o.p[e], o.ld[e], o.dt[e], o.rate[e], o.decay[e]};
+}
+
+template <int BM, int LA, int LB>
+using OrthoGemm = Gemm<BM, BM, 2, BM == 256 ? 4 : 2, LA, LB, true, false, OrthoOperands>;
+
+template <class G, int P, int PHASE, int DEST>
+__device__ __forceinline__ void ortho_tile(char* smem, const OrthoPhase& ph, const OrthoOut& out,
+                                           const OrthoGroup& g, const OrthoOperands& o, int matrix,
+                                           int tm, int tn, int tile, int part) {
+  G gm(o, (lchar*)smem, tm, tn);
+  const int steps = o.nseg * ((o.K + FFN_BK - 1) / FFN_BK);
+  const bool split = part >= 0;
+  const int per = split ? (steps + ph.splits - 1) / ph.splits : steps;
+  const int begin = split ? part * per : 0;
+  v4f acc[G::MI][G::NJ];
+  gm.run(begin, min(steps, begin + per), acc);
+  const int lane = gm.lane;
+  if (split) {
+    gv4f_a16* to = (gv4f_a16*)ph.partial +
+                   ((int64_t)part * (ph.tiles - ph.whole) + (tile - ph.whole)) * (G::FRAGS * 64) +
+                   lane;
+#pragma unroll
+    for (int i = 0; i < G::MI; ++i)
+#pragma unroll
+      for (int j = 0; j < G::NJ; ++j)
+        to[(gm.frag_m(i) / 16 * (G::BN_ / 16) + gm.frag_n(j) / 16) * 64] = acc[i][j];
+    return;
+  }
+  const OrthoTarget t = ortho_target<PHASE>(ph, g, matrix, tm > tn);
+  const OrthoPlace to = ortho_place<DEST>(out, g.first + matrix);
+  // what is added is loaded for several rows of fragments at a time, as a wait for
+  // loads also waits for the stores before them
+  constexpr int BATCH = G::MI / P / (G::MI > 4 ? 2 : 1);
+#pragma unroll
+  for (int i0 = 0; i0 < G::MI; i0 += BATCH) {
+    OrthoPair<P, PHASE> add[BATCH][G::NJ / 2];
+#pragma unroll
+    for (int i = 0; i < BATCH; ++i)
+#pragma unroll
+      for (int j = 0; j < G::NJ; j += 2)
+        add[i][j / 2].load(t, gm.m0 + gm.frag_m(i0 + i) + (lane & 15), gm.n0 + gm.frag_n(j), lane);
+    __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+    for (int i = 0; i < BATCH; ++i)
+#pragma unroll
+      for (int j = 0; j < G::NJ; j += 2)
+        ortho_finish<P, PHASE, DEST>(ph, to, t, add[i][j / 2],
+                                     gm.m0 + gm.frag_m(i0 + i) + (lane & 15), gm.n0 + gm.frag_n(j),
+                                     lane, acc[i0 + i][j], acc[i0 + i][j + 1]);
+    __builtin_amdgcn_sched_barrier(0);
+  }
+}
+
+template <int P, int BM, int PHASE, int DEST>
+__global__ __launch_bounds__(BM * 2, 2) void k_ortho(const OrthoPhase ph, const OrthoOut out) {
+  using RR = OrthoGemm<BM, ROWS, ROWS>;
+  using RC = OrthoGemm<BM, ROWS, COLS>;
+  using CC = OrthoGemm<BM, COLS, COLS>;
+  static_assert(RR::THREADS == BM * 2, "a wave for every 32 rows");
+  __shared__ __attribute__((aligned(1024))) char smem[RR::LDS];
+  const int b = blockIdx.x, rest = ph.tiles - ph.whole;
+  const int part = b < ph.whole ? -1 : (b - ph.whole) / rest;
+  const int tile = part < 0 ? b : ph.whole + (b - ph.whole) % rest;
+  const OrthoGroup& g = ph.g[ortho_group_of(ph, tile)];
+  int matrix, tm, tn;
+  ortho_tile_of(g, PHASE != ORTHO_UPDATE, tile - g.tile0, matrix, tm, tn);
+  const char* x = ph.base + matrix * g.x_step + g.x;
+  const char* a = ph.base + matrix * g.a_step + (PHASE == ORTHO_SQUARE ? g.a : g.b);
+  const bool wide = g.rows <= g.cols;
+  const int s = wide ? g.rows : g.cols;
+  const int64_t px = (int64_t)g.rows * g.ldx, pa = (int64_t)s * g.lda;
+  if constexpr (PHASE == ORTHO_SQUARE) {
+    const OrthoOperands o = ortho_operands<P>(a, pa, g.lda, a, pa, g.lda, s, s, s);
+    ortho_tile<RR, P, PHASE, DEST>(smem, ph, out, g, o, matrix, tm, tn, tile, part);
+  } else if constexpr (PHASE == ORTHO_GRAM) {
+    const OrthoOperands o =
+        ortho_operands<P>(x, px, g.ldx, x, px, g.ldx, s, s, wide ? g.cols : g.rows);
+    if (wide) ortho_tile<RR, P, PHASE, DEST>(smem, ph, out, g, o, matrix, tm, tn, tile, part);
+    else ortho_tile<CC, P, PHASE, DEST>(smem, ph, out, g, o, matrix, tm, tn, tile, part);
+  } else if (wide) {
+    const OrthoOperands o = ortho_operands<P>(a, pa, g.lda, x, px, g.ldx, g.rows, g.cols, s);
+    ortho_tile<RC, P, PHASE, DEST>(smem, ph, out, g, o, matrix, tm, tn, tile, part);
+  } else {
+    const OrthoOperands o = ortho_operands<P>(x, px, g.ldx, a, pa, g.lda, g.rows, g.cols, s);
+    ortho_tile<RR, P, PHASE, DEST>(smem, ph, out, g, o, matrix, tm, tn, tile, part);
+  }
+}
+
+// The parts of split tiles, added in order: a wave takes two fragments.
+template <int P, int BM, int PHASE, int DEST>
+__global__ __launch_bounds__(256) void k_ortho_join(const OrthoPhase ph, const OrthoOut out) {
+  constexpr int F = BM / 16, PAIRS = F * F / 2;   // of a tile
+  const int64_t at = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6);
+  const int rest = ph.tiles - ph.whole, lane = threadIdx.x & 63;
+  if (at >= (int64_t)rest * PAIRS) return;
+  const int tile = ph.whole + (int)(at / PAIRS), in = (int)(at % PAIRS);
+  const OrthoGroup& g = ph.g[ortho_group_of(ph, tile)];
+  int matrix, tm, tn;
+  ortho_tile_of(g, PHASE != ORTHO_UPDATE, tile - g.tile0, matrix, tm, tn);
+  const OrthoTarget t = ortho_target<PHASE>(ph, g, matrix, tm > tn);
+  const OrthoPlace to = ortho_place<DEST>(out, g.first + matrix);
+  const int fm = in / (F / 2), fn = in % (F / 2) * 2;
+  const int m = tm * BM + fm * 16 + (lane & 15), n = tn * BM + fn * 16;
+  // (whole fragments outside; the mirror image's padding columns are C's rows)
+  if (tm * BM + fm * 16 >= ((t.M + 7) & ~7) || n >= t.cols) return;
+  OrthoPair<P, PHASE> add;
+  add.load(t, m, n, lane);
+  const gv4f_a16* p = (const gv4f_a16*)ph.partial +
+                      ((int64_t)(tile - ph.whole) * F * F + fm * F + fn) * 64 + lane;
+  const int64_t all = (int64_t)rest * F * F * 64;
+  v4f c = {0.f, 0.f, 0.f, 0.f}, d = c;
+  constexpr int BATCH = 4;
+  for (int s = 0; s < ph.splits; s += BATCH) {
+    v4f pc[BATCH], pd[BATCH];
+#pragma unroll
+    for (int i = 0; i < BATCH; ++i)
+      if (s + i < ph.splits) {
+        pc[i] = p[(s + i) * all];
+        pd[i] = p[(s + i) * all + 64];
+      }
+#pragma unroll
+    for (int i = 0; i < BATCH; ++i)
+      if (s + i < ph.splits) {
+        c += pc[i];
+        d += pd[i];
+      }
+  }
+  ortho_finish<P, PHASE, DEST>(ph, to, t, add, m, n, lane, c, d);
+}
+
+// --------------------------------------------------------- launches --------
+template <int P, int BM, int PHASE, int DEST>
+void ortho_launch(const OrthoPhase& ph, const OrthoOut& out, hipStream_t st) {
+  const int rest = ph.tiles - ph.whole;
+  k_ortho<P, BM, PHASE, DEST><<<ph.whole + rest * ph.splits, BM * 2, 0, st>>>(ph, out);
+  if (rest)
+    k_ortho_join<P, BM, PHASE, DEST>
+        <<<(int)(((int64_t)rest * (BM / 16) * (BM / 16) / 2 + 3) / 4), 256, 0, st>>>(ph, out);
+}
+template <int P, int BM>
+void ortho_launch(int phase, int dest, const OrthoPhase& ph, const OrthoOut& out, hipStream_t st) {
+  if (phase == ORTHO_GRAM) ortho_launch<P, BM, ORTHO_GRAM, ORTHO_NEXT>(ph, out, st);
+  else if (phase == ORTHO_SQUARE) ortho_launch<P, BM, ORTHO_SQUARE, ORTHO_NEXT>(ph, out, st);
+  else if (dest == ORTHO_NEXT) ortho_launch<P, BM, ORTHO_UPDATE, ORTHO_NEXT>(ph, out, st);
+  else if (dest == ORTHO_RESULT) ortho_launch<P, BM, ORTHO_UPDATE, ORTHO_RESULT>(ph, out, st);
+  else ortho_launch<P, BM, ORTHO_UPDATE, ORTHO_PARAMETER>(ph, out, st);
+}
+template <int P>
+void ortho_product(int big, int phase, int dest, const OrthoPhase& ph, const OrthoOut& out,
+                   hipStream_t st) {
+  if (big) ortho_launch<P, 256>(phase, dest, ph, out, st);
+  else ortho_launch<P, 128>(phase, dest, ph, out, st);
+}
+// instantiated in ortho_words1.hip and ortho_words2.hip
+void ortho_product1(int big, int phase, int dest, const OrthoPhase& ph, const OrthoOut& out,
+                    hipStream_t st);
+void ortho_product2(int big, int phase, int dest, const OrthoPhase& ph, const OrthoOut& out,
+                    hipStream_t st);
+
+}  // namespace scao

@@ -8,6 +8,9 @@
 //   gated_ffn   the feed-forward block as an operator of torch's dispatcher, its
 //               backward pass without the interpreter: a small block's training
 //               step took 145 us of host time as a Python function
+//   orthogonalize, muon_step
+//               matrix updates orthogonalised, and the step of the optimiser that is
+//               built on it, as operators of the dispatcher over lists of tensors
 //   bind        the addresses of the C ABI's entry points, which the caller has
 //               loaded (so that one library is used, whichever it is)
 #include <ATen/ATen.h>
@@ -44,6 +47,10 @@ struct Entries {
   decltype(&scao_grad_norm_workspace) grad_norm_workspace;
   decltype(&scao_grad_norm) grad_norm;
   decltype(&scao_grad_clip) grad_clip;
+  decltype(&scao_orthogonalize_workspace) orthogonalize_workspace;
+  decltype(&scao_orthogonalize) orthogonalize;
+  decltype(&scao_muon_workspace) muon_workspace;
+  decltype(&scao_muon_step) muon_step;
 } lib;
 
 void check(int rc, const char* who) {
@@ -559,6 +566,245 @@ PyObject* grad_clip(PyObject*, PyObject* const* args, Py_ssize_t n) {
   return call_on_gradients(args, n, true);
 }
 
+// -------------------------------------------------- orthogonalised updates ---
+// Operators of the dispatcher over lists of matrices and stacks of matrices:
+//   orthogonalize  fresh results of one type
+//   muon_step_     parameters and momenta written in place
+std::vector<Tensor> op_orthogonalize(at::TensorList updates, at::ArrayRef<double> coefficients,
+                                     double eps, at::ScalarType dtype, int64_t precision) {
+  static const auto op = c10::Dispatcher::singleton()
+                             .findSchemaOrThrow("scao_amd::orthogonalize", "")
+                             .typed<decltype(op_orthogonalize)>();
+  return op.call(updates, coefficients, eps, dtype, precision);
+}
+void op_muon_step_(at::TensorList params, at::TensorList grads, at::TensorList momenta,
+                   at::ArrayRef<double> rates, at::ArrayRef<double> decays, double momentum,
+                   bool nesterov, at::ArrayRef<double> coefficients, double eps,
+                   int64_t precision) {
+  static const auto op = c10::Dispatcher::singleton()
+                             .findSchemaOrThrow("scao_amd::muon_step_", "")
+                             .typed<decltype(op_muon_step_)>();
+  op.call(params, grads, momenta, rates, decays, momentum, nesterov, coefficients, eps, precision);
+}
+
+void check_matrices(at::TensorList list, const char* name, c10::Device on) {
+  for (const Tensor& t : list) {
+    TORCH_CHECK(t.layout() == at::kStrided && code_of(t.scalar_type()) >= 0 && t.device() == on,
+                name, " must be dense float32, bfloat16 or float16 tensors on one device (got ",
+                t.scalar_type(), ", ", t.layout(), ", ", t.device(), ")");
+    TORCH_CHECK(t.dim() >= 2, name, " must be matrices or stacks of matrices (got ",
+                t.sym_sizes(), ")");
+  }
+}
+void check_scheme(at::ArrayRef<double> coefficients) {
+  TORCH_CHECK(lib.orthogonalize, "orthogonalize: scao_amd has not loaded its library");
+  TORCH_CHECK(!coefficients.empty() && coefficients.size() % 3 == 0,
+              "orthogonalize: three coefficients a step");
+}
+
+// the matrices of a stack, whose rows are unit-strided and apart
+template <class F>
+void for_matrices(const Tensor& t, F&& f) {
+  const int64_t n = t.dim(), rows = t.size(n - 2), cols = t.size(n - 1);
+  int64_t many = 1;
+  for (int64_t k = 0; k < n - 2; ++k) many *= t.size(k);
+  if (many * rows * cols == 0) return;
+  char* base = (char*)t.data_ptr();
+  for (int64_t i = 0; i < many; ++i) {
+    int64_t at = 0, left = i;
+    for (int64_t k = n - 3; k >= 0; --k) {
+      at += left % t.size(k) * t.stride(k);
+      left /= t.size(k);
+    }
+    f(base + at * (int64_t)t.element_size(), rows, cols, t.stride(n - 2));
+  }
+}
+Tensor row_strided(const Tensor& t) {
+  const int64_t n = t.dim();
+  const bool unit = t.stride(n - 1) == 1 || t.size(n - 1) == 1;
+  return unit && (t.size(n - 2) <= 1 || (t.stride(n - 2) >= t.size(n - 1) &&
+                                         t.stride(n - 2) <= 0x7fffffff))
+             ? t
+             : t.contiguous();
+}
+
+std::vector<Tensor> orthogonalize_hip(at::TensorList updates, at::ArrayRef<double> coefficients,
+                                      double eps, at::ScalarType dtype, int64_t precision) {
+  check_scheme(coefficients);
+  std::vector<Tensor> out;
+  if (updates.empty()) return out;
+  check_matrices(updates, "updates", updates[0].device());
+  TORCH_CHECK(code_of(dtype) >= 0, "orthogonalize: no result of type ", dtype);
+  const c10::DeviceGuard guard(updates[0].device());
+  std::vector<Tensor> in;
+  std::vector<scao_ortho_desc> table;
+  for (const Tensor& t : updates) {
+    in.push_back(row_strided(t.resolve_neg()));
+    out.push_back(at::empty(t.sizes(), t.options().dtype(dtype)));
+    char* to = (char*)out.back().data_ptr();
+    for_matrices(in.back(), [&](char* p, int64_t rows, int64_t cols, int64_t ld) {
+      table.push_back({p, to, rows, cols, ld, cols, code_of(t.scalar_type()), code_of(dtype)});
+      to += rows * cols * (int64_t)out.back().element_size();
+    });
+  }
+  const int steps = (int)coefficients.size() / 3, n = (int)table.size();
+  const Tensor work =
+      bytes(lib.orthogonalize_workspace(table.data(), n, steps, (int)precision), updates[0]);
+  check(lib.orthogonalize(table.data(), n, coefficients.data(), steps, eps, (int)precision,
+                          work.data_ptr(), stream_of(updates[0])),
+        "scao_orthogonalize");
+  return out;
+}
+
+void muon_step_hip_(at::TensorList params, at::TensorList grads, at::TensorList momenta,
+                    at::ArrayRef<double> rates, at::ArrayRef<double> decays, double momentum,
+                    bool nesterov, at::ArrayRef<double> coefficients, double eps,
+                    int64_t precision) {
+  check_scheme(coefficients);
+  const size_t n = params.size();
+  TORCH_CHECK(grads.size() == n && momenta.size() == n && rates.size() == n && decays.size() == n,
+              "muon_step_: lists of different lengths");
+  if (!n) return;
+  const c10::Device on = params[0].device();
+  check_matrices(params, "parameters", on);
+  check_matrices(grads, "gradients", on);
+  const c10::DeviceGuard guard(on);
+  std::vector<Tensor> copies;
+  std::vector<scao_muon_desc> table;
+  for (size_t i = 0; i < n; ++i) {
+    const Tensor &p = params[i], &m = momenta[i];
+    TORCH_CHECK(p.is_contiguous() && !p.is_neg() && m.is_contiguous() && !m.is_neg() && m.scalar_type() == at::kFloat &&
+                    m.device() == on && m.sizes() == p.sizes() && grads[i].sizes() == p.sizes(),
+                "muon_step_: a parameter and its momentum must be contiguous, the momentum "
+                "float32, and both and the gradient of one shape");
+    copies.push_back(grads[i].resolve_neg().contiguous());
+    const char* g = (const char*)copies.back().data_ptr();
+    float* buf = (float*)m.data_ptr();
+    const int64_t g_size = (int64_t)copies.back().element_size();
+    for_matrices(p, [&](char* at, int64_t rows, int64_t cols, int64_t) {
+      table.push_back({at, g, buf, rows, cols, code_of(p.scalar_type()),
+                       code_of(copies.back().scalar_type()), (float)rates[i], (float)decays[i]});
+      g += rows * cols * g_size;
+      buf += rows * cols;
+    });
+  }
+  const int steps = (int)coefficients.size() / 3, many = (int)table.size();
+  const Tensor work = bytes(lib.muon_workspace(table.data(), many, steps, (int)precision), params[0]);
+  check(lib.muon_step(table.data(), many, momentum, nesterov, coefficients.data(), steps, eps,
+                      (int)precision, work.data_ptr(), stream_of(params[0])),
+        "scao_muon_step");
+}
+// a graph that holds a parameter has to see that it changed
+void muon_step_version_(at::TensorList params, at::TensorList grads, at::TensorList momenta,
+                        at::ArrayRef<double> rates, at::ArrayRef<double> decays, double momentum,
+                        bool nesterov, at::ArrayRef<double> coefficients, double eps,
+                        int64_t precision) {
+  {
+    const at::AutoDispatchBelowADInplaceOrView below;
+    op_muon_step_(params, grads, momenta, rates, decays, momentum, nesterov, coefficients, eps,
+                  precision);
+  }
+  for (const at::TensorList list : {params, momenta})
+    for (const Tensor& t : list)
+      if (!t.is_inference()) t.unsafeGetTensorImpl()->bump_version();
+}
+
+std::vector<Tensor> orthogonalize_meta(at::TensorList updates, at::ArrayRef<double> coefficients,
+                                       double, at::ScalarType dtype, int64_t) {
+  check_scheme(coefficients);
+  std::vector<Tensor> out;
+  if (!updates.empty()) check_matrices(updates, "updates", updates[0].device());
+  for (const Tensor& t : updates)
+    out.push_back(at::empty_symint(t.sym_sizes(), t.options().dtype(dtype)));
+  return out;
+}
+void muon_step_meta_(at::TensorList params, at::TensorList, at::TensorList, at::ArrayRef<double>,
+                     at::ArrayRef<double>, double, bool, at::ArrayRef<double> coefficients, double,
+                     int64_t) {
+  check_scheme(coefficients);
+  if (!params.empty()) check_matrices(params, "parameters", params[0].device());
+}
+
+bool tangent(at::TensorList list) {
+  if (forward_mode())
+    for (const Tensor& t : list)
+      if (t._fw_grad(0).defined()) return true;
+  return false;
+}
+std::vector<Tensor> orthogonalize_autograd(at::TensorList updates,
+                                           at::ArrayRef<double> coefficients, double eps,
+                                           at::ScalarType dtype, int64_t precision) {
+  bool wanted = tangent(updates);
+  if (at::GradMode::is_enabled())
+    for (const Tensor& t : updates) wanted = wanted || t.requires_grad();
+  TORCH_CHECK_NOT_IMPLEMENTED(!wanted, "orthogonalize has no derivative: detach the updates");
+  const at::AutoDispatchBelowADInplaceOrView below;
+  return op_orthogonalize(updates, coefficients, eps, dtype, precision);
+}
+
+TORCH_LIBRARY_FRAGMENT(scao_amd, m) {
+  m.def("orthogonalize(Tensor[] updates, float[] coefficients, float eps, ScalarType dtype, "
+        "int precision) -> Tensor[]");
+  m.def("muon_step_(Tensor(a!)[] params, Tensor[] grads, Tensor(b!)[] momenta, float[] rates, "
+        "float[] decays, float momentum, bool nesterov, float[] coefficients, float eps, "
+        "int precision) -> ()");
+}
+TORCH_LIBRARY_IMPL(scao_amd, CUDA, m) {
+  m.impl("orthogonalize", orthogonalize_hip);
+  m.impl("muon_step_", muon_step_hip_);
+}
+TORCH_LIBRARY_IMPL(scao_amd, Meta, m) {
+  m.impl("orthogonalize", orthogonalize_meta);
+  m.impl("muon_step_", muon_step_meta_);
+}
+TORCH_LIBRARY_IMPL(scao_amd, Autograd, m) { m.impl("orthogonalize", orthogonalize_autograd); }
+TORCH_LIBRARY_IMPL(scao_amd, ADInplaceOrView, m) { m.impl("muon_step_", muon_step_version_); }
+// (torch's fallback does not look into lists; the kernels above do)
+TORCH_LIBRARY_IMPL(scao_amd, Negative, m) {
+  m.impl("orthogonalize", torch::CppFunction::makeFallthrough());
+  m.impl("muon_step_", torch::CppFunction::makeFallthrough());
+}
+
+std::vector<Tensor> tensors(PyObject* list) {
+  const THPObjectPtr seq(PySequence_Fast(list, "a list of tensors"));
+  if (!seq) throw python_error();
+  std::vector<Tensor> out;
+  for (Py_ssize_t i = 0; i < PySequence_Fast_GET_SIZE(seq.get()); ++i) {
+    PyObject* o = PySequence_Fast_GET_ITEM(seq.get(), i);
+    TORCH_CHECK_TYPE(THPVariable_Check(o), "a list of tensors");
+    out.push_back(THPVariable_Unpack(o));
+  }
+  return out;
+}
+std::vector<double> numbers(PyObject* list) {
+  const THPObjectPtr seq(PySequence_Fast(list, "a list of numbers"));
+  if (!seq) throw python_error();
+  std::vector<double> out;
+  for (Py_ssize_t i = 0; i < PySequence_Fast_GET_SIZE(seq.get()); ++i)
+    out.push_back(PyFloat_AsDouble(PySequence_Fast_GET_ITEM(seq.get(), i)));
+  if (PyErr_Occurred()) throw python_error();
+  return out;
+}
+// muon_step(parameters, gradients, momenta, rates, decays, momentum, nesterov,
+// coefficients, eps, precision)
+PyObject* muon_step(PyObject*, PyObject* const* args, Py_ssize_t n) {
+  HANDLE_TH_ERRORS
+  TORCH_CHECK_TYPE(n == 10, "muon_step() takes ten arguments");
+  const std::vector<Tensor> params = tensors(args[0]), grads = tensors(args[1]),
+                            momenta = tensors(args[2]);
+  const std::vector<double> rates = numbers(args[3]), decays = numbers(args[4]),
+                            coefficients = numbers(args[7]);
+  const double momentum = PyFloat_AsDouble(args[5]), eps = PyFloat_AsDouble(args[8]);
+  const int nesterov = PyObject_IsTrue(args[6]);
+  const long precision = PyLong_AsLong(args[9]);
+  if (PyErr_Occurred()) return nullptr;
+  const at::AutoDispatchBelowAutograd below;
+  op_muon_step_(params, grads, momenta, rates, decays, momentum, nesterov != 0, coefficients, eps,
+                precision);
+  Py_RETURN_NONE;
+  END_HANDLE_TH_ERRORS
+}
+
 // bind({name: address})
 PyObject* bind(PyObject*, PyObject* arg) {
   auto at = [&](const char* name, auto& entry) {
@@ -574,7 +820,10 @@ PyObject* bind(PyObject*, PyObject* arg) {
         at("scao_ffn_backward_workspace", lib.backward_workspace) &&
         at("scao_ffn_backward", lib.backward) &&
         at("scao_grad_norm_workspace", lib.grad_norm_workspace) &&
-        at("scao_grad_norm", lib.grad_norm) && at("scao_grad_clip", lib.grad_clip)))
+        at("scao_grad_norm", lib.grad_norm) && at("scao_grad_clip", lib.grad_clip) &&
+        at("scao_orthogonalize_workspace", lib.orthogonalize_workspace) &&
+        at("scao_orthogonalize", lib.orthogonalize) &&
+        at("scao_muon_workspace", lib.muon_workspace) && at("scao_muon_step", lib.muon_step)))
     return nullptr;
   Py_RETURN_NONE;
 }
@@ -585,6 +834,7 @@ PyMethodDef methods[] = {
     SCAO_FASTCALL(gated_ffn),
     SCAO_FASTCALL(grad_norm),
     SCAO_FASTCALL(grad_clip),
+    SCAO_FASTCALL(muon_step),
 #undef SCAO_FASTCALL
     {"bind", bind, METH_O, nullptr},
     {nullptr, nullptr, 0, nullptr}};
