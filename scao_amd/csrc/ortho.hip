@@ -50,10 +50,10 @@ double largest(double a, double b, double c, double u) {
     if (x > 0 && x < u * u) most = std::max(most, at(std::sqrt(x)));
   return most;
 }
-// of b t + c t^2 on [0, t0]
-double largest2(double b, double c, double t0) {
-  auto at = [&](double t) { return std::fabs(t * (b + t * c)); };
-  double most = at(t0);
+// of a + b t + c t^2 on [0, t0]
+double largest2(double a, double b, double c, double t0) {
+  auto at = [&](double t) { return std::fabs(a + t * (b + t * c)); };
+  double most = std::max(at(0), at(t0));
   if (c != 0) {
     const double t = -b / (2 * c);
     if (t > 0 && t < t0) most = std::max(most, at(t));
@@ -69,7 +69,7 @@ double power_for(double most, int limit) {
 struct Scales {
   double first;                       // of the first X
   float gram[MAX_STEPS], square[MAX_STEPS], square_keep[MAX_STEPS];
-  float update[MAX_STEPS], update_keep[MAX_STEPS];
+  float diagonal[MAX_STEPS], update[MAX_STEPS];
 };
 // false: some singular value may grow past what the words hold
 bool scales_of(const double* co, int steps, Scales& s) {
@@ -77,15 +77,15 @@ bool scales_of(const double* co, int steps, Scales& s) {
   s.first = sx;
   for (int k = 0; k < steps; ++k) {
     const double a = co[3 * k], b = co[3 * k + 1], c = co[3 * k + 2];
-    const double sa = power_for(u * u, 14), sb = power_for(largest2(b, c, u * u), 20);
+    const double sa = power_for(u * u, 14), sb = power_for(largest2(a, b, c, u * u), 20);
     const double next = largest(a, b, c, u) * 1.01;
     if (!(next <= 1024.0) || !(sb >= 1.0 / 65536)) return false;
     const double to = k + 1 < steps ? power_for(next, 14) : 1.0;
     s.gram[k] = (float)(sa / (sx * sx));
     s.square[k] = (float)(c * sb / (sa * sa));
     s.square_keep[k] = (float)(b * sb / sa);
+    s.diagonal[k] = (float)(a * sb);
     s.update[k] = (float)(to / (sb * sx));
-    s.update_keep[k] = (float)(a * to / sx);
     u = next;
     sx = to;
   }
@@ -298,8 +298,8 @@ struct Pass {
       plans[ORTHO_GRAM].ph.by = sc.gram[k];
       plans[ORTHO_SQUARE].ph.by = sc.square[k];
       plans[ORTHO_SQUARE].ph.keep = sc.square_keep[k];
+      plans[ORTHO_SQUARE].ph.diagonal = sc.diagonal[k];
       plans[ORTHO_UPDATE].ph.by = sc.update[k];
-      plans[ORTHO_UPDATE].ph.keep = sc.update_keep[k];
       for (int phase = 0; phase < 3; ++phase) {
         product(plans[phase].big, phase,
                 phase == ORTHO_UPDATE && k + 1 == steps ? dest : ORTHO_NEXT, plans[phase].ph, out,

@@ -1,8 +1,8 @@
 // The kernels of the Newton-Schulz orthogonalisation.
 //
 //   X = G / (|G| + eps), then for every step, on the smaller side of X:
-//   A = X X^T, B = b A + c A A, X <- a X + B X      (wide: rows <= cols)
-//   A = X^T X, B = b A + c A A, X <- a X + X B      (tall)
+//   A = X X^T, B = a + b A + c A A, X <- B X      (wide: rows <= cols)
+//   A = X^T X, B = a + b A + c A A, X <- X B      (tall)
 //
 // Nothing is transposed in memory: the tiled product reads an operand with k or
 // with its rows contiguous.  A and B are symmetric, so only the tiles on and below
@@ -26,7 +26,7 @@ namespace scao {
 
 constexpr int ORTHO_GROUPS = 16;     // shapes a pass
 constexpr int ORTHO_MATRICES = 64;   // matrices a pass
-constexpr int ORTHO_PARTS = 256;     // sums of squares a matrix
+constexpr int ORTHO_PARTS = 1024;    // sums of squares a matrix
 
 enum { ORTHO_GRAM, ORTHO_SQUARE, ORTHO_UPDATE };
 // where an update goes: the next X, the result, or (the optimiser) the parameter
@@ -41,12 +41,17 @@ struct OrthoGroup {
   int per, tiles_m, tiles_n; // tiles of a matrix
   int tile0;                 // tiles of the groups before
 };
+// A phase's tiles in order.  The first `whole` go one to a workgroup, the others' k
+// steps in `splits` parts.  (Parts of one length for every tile, and not shares of
+// all steps wherever a tile ends: those balance 136 tiles on 256 CUs, but then no two
+// workgroups of an XCD read the same k at a time, and its L2 serves nobody: 14336 x
+// 4096's Gram matrix 269 us, with three parts a tile 251.)
 struct OrthoPhase {
   OrthoGroup g[ORTHO_GROUPS];
   char* base;
   float* partial;            // parts of split tiles
   int groups, tiles, whole, splits;
-  float by, keep;            // of the product; of what is added to it
+  float by, keep, diagonal;  // of the product; of A; added to B's diagonal
 };
 struct OrthoOut {
   void* p[ORTHO_MATRICES];
@@ -114,7 +119,6 @@ __device__ __forceinline__ int ortho_group_of(const OrthoPhase& ph, int tile) {
     if (tile >= ph.g[i].tile0) k = i;
   return k;
 }
-
 // where the phase's product is stored, and what is added to it
 struct OrthoTarget {
   uint16_t* to;
@@ -132,7 +136,7 @@ __device__ __forceinline__ OrthoTarget ortho_target(const OrthoPhase& ph, const 
   t.mirror = PHASE != ORTHO_UPDATE && mirror;
   if (PHASE == ORTHO_UPDATE) {
     t.to = (uint16_t*)(x + g.y);
-    t.add = (const uint16_t*)(x + g.x);
+    t.add = nullptr;
     t.plane = (int64_t)g.rows * g.ldx;
     t.ld = g.ldx;
     t.M = g.rows;
@@ -174,7 +178,7 @@ template <int P, int PHASE>
 struct OrthoPair {
   v4u_t w[P];
   __device__ __forceinline__ void load(const OrthoTarget& t, int m, int n, int lane) {
-    if (PHASE == ORTHO_GRAM) return;
+    if (PHASE != ORTHO_SQUARE) return;
     n += pair_column(lane);
     const bool in = m < t.M && n < t.cols;
 #pragma unroll
@@ -182,11 +186,12 @@ struct OrthoPair {
       w[i] = in ? (v4u_t) * (const gv4u_a16*)(t.add + (int64_t)m * t.ld + n + i * t.plane)
                 : v4u_t{0, 0, 0, 0};
   }
-  // by c + keep (what is added), likewise d
-  __device__ __forceinline__ void sum(float by, float keep, v4f& c, v4f& d) const {
-    c *= by;
-    d *= by;
-    if (PHASE == ORTHO_GRAM) return;
+  // by c, of a square by c + keep A + diagonal, likewise d
+  __device__ __forceinline__ void sum(const OrthoPhase& ph, int m, int n, int lane, v4f& c,
+                                      v4f& d) const {
+    c *= ph.by;
+    d *= ph.by;
+    if (PHASE != ORTHO_SQUARE) return;
 #pragma unroll
     for (int i = 0; i < P; ++i) {
       v2u p, q;
@@ -194,9 +199,15 @@ struct OrthoPair {
       const v4f x = halves_to_v4f(SCAO_F16, p), y = halves_to_v4f(SCAO_F16, q);
 #pragma unroll
       for (int t = 0; t < 4; ++t) {
-        c[t] = fmaf(keep, x[t], c[t]);
-        d[t] = fmaf(keep, y[t], d[t]);
+        c[t] = fmaf(ph.keep, x[t], c[t]);
+        d[t] = fmaf(ph.keep, y[t], d[t]);
       }
+    }
+    n += 4 * (lane >> 4);
+#pragma unroll
+    for (int t = 0; t < 4; ++t) {
+      if (n + t == m) c[t] += ph.diagonal;
+      if (n + 16 + t == m) d[t] += ph.diagonal;
     }
   }
 };
@@ -303,7 +314,7 @@ template <int P, int PHASE, int DEST>
 __device__ __forceinline__ void ortho_finish(const OrthoPhase& ph, const OrthoPlace& o,
                                              const OrthoTarget& t, const OrthoPair<P, PHASE>& add,
                                              int m, int n, int lane, v4f c, v4f d) {
-  add.sum(ph.by, ph.keep, c, d);
+  add.sum(ph, m, n, lane, c, d);
   if constexpr (DEST == ORTHO_NEXT) ortho_store<P>(t, m, n, lane, c, d);
   else ortho_put<DEST>(o, t, m, n, lane, c, d);
 }

@@ -55,29 +55,38 @@ __device__ __forceinline__ OrthoVector ortho_load(const void* p, int64_t ld, int
   }
   return v;
 }
-// the update of momentum and gradient (and, NORM, the momentum's own step)
-template <bool NORM>
-__device__ __forceinline__ void ortho_momentum(const OrthoPrep& p, float* buf, int r, int c, int cols,
-                                               OrthoVector& g) {
-  const int64_t at = (int64_t)r * cols + c;
+__device__ __forceinline__ OrthoVector ortho_load_momentum(const float* buf, int cols, int r, int c) {
+  OrthoVector v;
 #pragma unroll
   for (int h = 0; h < 2; ++h) {
-    const int n = cols - c - 4 * h, mask = n >= 4 ? 15 : n <= 0 ? 0 : (1 << n) - 1;
-    v4f m = ldf4(buf, at + 4 * h, n >= 4, mask);
+    const int n = cols - c - 4 * h;
+    v.x[h] = ldf4(buf, (int64_t)r * cols + c + 4 * h, n >= 4, n <= 0 ? 0 : (1 << n) - 1);
+  }
+  return v;
+}
+// g becomes the update of momentum and gradient; NORM: the momentum takes its step
+template <bool NORM>
+__device__ __forceinline__ void ortho_momentum(const OrthoPrep& p, float* buf, int r, int c, int cols,
+                                               OrthoVector& g, OrthoVector& m) {
+#pragma unroll
+  for (int h = 0; h < 2; ++h) {
 #pragma unroll
     for (int t = 0; t < 4; ++t) {
       const float s = p.rest * g.x[h][t];
-      if (NORM) m[t] = fmaf(p.momentum, m[t], s);
-      g.x[h][t] = p.nesterov ? fmaf(p.momentum, m[t], s) : m[t];
+      if (NORM) m.x[h][t] = fmaf(p.momentum, m.x[h][t], s);
+      g.x[h][t] = p.nesterov ? fmaf(p.momentum, m.x[h][t], s) : m.x[h][t];
     }
-    if (NORM) stf4(buf, at + 4 * h, m, n >= 4, mask);
+    const int n = cols - c - 4 * h;
+    if (NORM)
+      stf4(buf, (int64_t)r * cols + c + 4 * h, m.x[h], n >= 4, n <= 0 ? 0 : (1 << n) - 1);
   }
 }
 
-// f(row, column, vector) for the vectors of this thread
+// f(row, column, vector) for the vectors of this thread, four of them loaded at a time
 template <int DT, bool NORM, class F>
 __device__ __forceinline__ void ortho_walk(const OrthoPrep& p, const OrthoSource& g, int matrix,
                                            int part, int width, F&& f) {
+  constexpr int AHEAD = 4;
   const int rows_a_unit = 256 / g.vecs;
   const int units = (g.rows + rows_a_unit - 1) / rows_a_unit * g.across;
   const int begin = part * g.per, end = min(units, begin + g.per);
@@ -85,14 +94,25 @@ __device__ __forceinline__ void ortho_walk(const OrthoPrep& p, const OrthoSource
   const void* src = p.src[g.first + matrix];
   float* buf = p.buf[g.first + matrix];
   const int64_t ld = p.ld[g.first + matrix];
-  for (int u = begin; u < end; ++u) {
-    const int r = u / g.across * rows_a_unit + rr;
-    const int c = (u % g.across * g.vecs + v) * 8;
-    if (r < g.rows && c < width) {
-      OrthoVector x = ortho_load<DT>(src, ld, r, c, g.cols);
-      if (buf) ortho_momentum<NORM>(p, buf, r, c, g.cols, x);
-      f(r, c, x);
+  for (int u = begin; u < end; u += AHEAD) {
+    OrthoVector x[AHEAD], m[AHEAD];
+    int r[AHEAD], c[AHEAD];
+#pragma unroll
+    for (int i = 0; i < AHEAD; ++i) {
+      r[i] = (u + i) / g.across * rows_a_unit + rr;
+      c[i] = ((u + i) % g.across * g.vecs + v) * 8;
+      if (u + i >= end || r[i] >= g.rows) c[i] = width;
+      if (c[i] < width) {
+        x[i] = ortho_load<DT>(src, ld, r[i], c[i], g.cols);
+        if (buf) m[i] = ortho_load_momentum(buf, g.cols, r[i], c[i]);
+      }
     }
+#pragma unroll
+    for (int i = 0; i < AHEAD; ++i)
+      if (c[i] < width) {
+        if (buf) ortho_momentum<NORM>(p, buf, r[i], c[i], g.cols, x[i], m[i]);
+        f(r[i], c[i], x[i]);
+      }
   }
 }
 template <bool NORM, class F>
@@ -138,7 +158,8 @@ __global__ __launch_bounds__(256) void k_ortho_scale(const OrthoPrep p) {
   int matrix, part;
   const OrthoSource& g = ortho_source(p, matrix, part);
   double s[1] = {0.0};
-  if ((int)threadIdx.x < g.parts) s[0] = p.norms[(g.first + matrix) * ORTHO_PARTS + threadIdx.x];
+  for (int i = threadIdx.x; i < g.parts; i += 256)
+    s[0] += p.norms[(g.first + matrix) * ORTHO_PARTS + i];
   block_sum(s, lds);
   if (threadIdx.x == 0) total = s[0];
   __syncthreads();
