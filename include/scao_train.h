@@ -134,6 +134,41 @@ int scao_muon_step(const scao_muon_desc* matrices, int n, double momentum, int n
                    const double* coefficients, int steps, double eps, int precision,
                    void* workspace, void* stream);
 
+/* ---- norms of queries and keys with their rotation ---------------------------
+ * For every token and head of q ([0]) and k ([1]), of `dim` columns x with unit
+ * stride:  y = x w / sqrt(mean x^2 + eps), and of y's first `rotary` columns the
+ * pairs (i, i + rotary/2), or interleaved (2i, 2i + 1), turned by the token's angles:
+ *   y'_i = y_i cos[p][i] - y_j sin[p][i],  y'_j = y_j cos[p][i] + y_i sin[p][i]
+ * in fp32, rounded once to dtype.  p: positions[sequence][token], or null: the
+ * token's place in its sequence; a p outside of the tables gives NaN in the rotated
+ * columns.  w null: ones.  backward: dx (p null: not wanted) and dw (null: not
+ * wanted), summed in a fixed order without atomics; the angles have no gradient.
+ * Batch, token and head strides of any tensor are free; outputs may not overlap.
+ * workspace: scao_qk_rope_backward_workspace() bytes, aligned to 16; needed for
+ * the weights' gradients. */
+typedef struct scao_rope_tensor {  /* HOST; strides in elements                  */
+  void* p;
+  int64_t batch, token, head;
+} scao_rope_tensor;
+typedef struct scao_rope_desc {    /* HOST */
+  scao_rope_tensor x[2];
+  const void* w[2];
+  const float* cos;                /* table_rows x rotary/2, ld_table apart      */
+  const float* sin;
+  const void* positions;           /* int64 (wide_positions) or int32            */
+  int64_t position_strides[2];     /* of sequence and token                      */
+  int64_t batch, seq, table_rows, ld_table;
+  int32_t heads[2], w_dtype[2];
+  int32_t dim, rotary;             /* 1 to 512; even, up to dim                  */
+  int32_t dtype, wide_positions, interleaved;
+  float eps;
+} scao_rope_desc;
+int scao_qk_rope_forward(const scao_rope_desc* desc, const scao_rope_tensor* y, void* stream);
+int64_t scao_qk_rope_backward_workspace(const scao_rope_desc* desc);
+int scao_qk_rope_backward(const scao_rope_desc* desc, const scao_rope_tensor* dy,
+                          const scao_rope_tensor* dx, void* dw_q, void* dw_k, void* workspace,
+                          void* stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -12,6 +12,7 @@ from .utils import matrix_power_neg_quarter, adaptive_rank
 from .ffn import GatedFFN, gated_ffn
 from .grad_clip import clip_grad_norm_, global_grad_norm
 from .ortho import Muon, orthogonalize
+from .qk_rope import QKNormRope, qk_norm_rope, rotary_table
 from . import logging as scao_logging
 
 __version__ = "0.2.0"
@@ -28,6 +29,9 @@ __all__ = [
     "global_grad_norm",
     "Muon",
     "orthogonalize",
+    "QKNormRope",
+    "qk_norm_rope",
+    "rotary_table",
     "scao_logging",
     "__version__",
 ]

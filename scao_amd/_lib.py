@@ -111,6 +111,13 @@ MUON_DESC = np.dtype([
     ("p", "u8"), ("g", "u8"), ("m", "u8"), ("rows", "i8"), ("cols", "i8"), ("dtype", "i4"),
     ("grad_dtype", "i4"), ("rate", "f4"), ("decay", "f4"),
 ], align=True)
+ROPE_TENSOR = np.dtype([("p", "u8"), ("batch", "i8"), ("token", "i8"), ("head", "i8")], align=True)
+ROPE_DESC = np.dtype([
+    ("x", ROPE_TENSOR, 2), ("w", "u8", 2), ("cos", "u8"), ("sin", "u8"), ("positions", "u8"),
+    ("position_strides", "i8", 2), ("batch", "i8"), ("seq", "i8"), ("table_rows", "i8"),
+    ("ld_table", "i8"), ("heads", "i4", 2), ("w_dtype", "i4", 2), ("dim", "i4"), ("rotary", "i4"),
+    ("dtype", "i4"), ("wide_positions", "i4"), ("interleaved", "i4"), ("eps", "f4"),
+], align=True)
 ORTHO_FAST, ORTHO_FP32 = 0, 1
 FILTER_WORK_WORDS = 2 * 2048 + 16
 FILTER_COMPACT_WORD = 2 * 2048 + 11   # 1 when the refinement passes read the candidates
@@ -127,7 +134,9 @@ STRUCTS = {0: (PARAM_DESC, [n for n in PARAM_DESC.names if n != "pad0"]),
            8: (TENSOR_DESC, [n for n in TENSOR_DESC.names if n != "pad0"]),
            9: (FFN_DESC, list(FFN_DESC.names)),
            10: (ORTHO_DESC, list(ORTHO_DESC.names)),
-           11: (MUON_DESC, list(MUON_DESC.names))}
+           11: (MUON_DESC, list(MUON_DESC.names)),
+           12: (ROPE_TENSOR, list(ROPE_TENSOR.names)),
+           13: (ROPE_DESC, list(ROPE_DESC.names))}
 
 _VP, _I, _I64, _D = ctypes.c_void_p, ctypes.c_int, ctypes.c_int64, ctypes.c_double
 
@@ -190,6 +199,9 @@ TRAIN_SIGNATURES = {
     "scao_orthogonalize": (_I, [_VP, _I, _VP, _I, _D, _I, _VP, _VP]),
     "scao_muon_workspace": (_I64, [_VP, _I, _I, _I]),
     "scao_muon_step": (_I, [_VP, _I, _D, _I, _VP, _I, _D, _I, _VP, _VP]),
+    "scao_qk_rope_forward": (_I, [_VP, _VP, _VP]),
+    "scao_qk_rope_backward_workspace": (_I64, [_VP]),
+    "scao_qk_rope_backward": (_I, [_VP, _VP, _VP, _VP, _VP, _VP, _VP]),
 }
 
 

@@ -138,6 +138,23 @@ extern "C" int scao_struct_layout(int which, int64_t* out, int cap) {
       PUT(offsetof(S, rate)); PUT(offsetof(S, decay));
       break;
     }
+    case 12: {
+      typedef scao_rope_tensor S;
+      PUT(sizeof(S));
+      PUT(offsetof(S, p)); PUT(offsetof(S, batch)); PUT(offsetof(S, token)); PUT(offsetof(S, head));
+      break;
+    }
+    case 13: {
+      typedef scao_rope_desc S;
+      PUT(sizeof(S));
+      PUT(offsetof(S, x)); PUT(offsetof(S, w)); PUT(offsetof(S, cos)); PUT(offsetof(S, sin));
+      PUT(offsetof(S, positions)); PUT(offsetof(S, position_strides)); PUT(offsetof(S, batch));
+      PUT(offsetof(S, seq)); PUT(offsetof(S, table_rows)); PUT(offsetof(S, ld_table));
+      PUT(offsetof(S, heads)); PUT(offsetof(S, w_dtype)); PUT(offsetof(S, dim));
+      PUT(offsetof(S, rotary)); PUT(offsetof(S, dtype)); PUT(offsetof(S, wide_positions));
+      PUT(offsetof(S, interleaved)); PUT(offsetof(S, eps));
+      break;
+    }
     default:
       return 0;
   }

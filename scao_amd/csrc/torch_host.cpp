@@ -11,6 +11,8 @@
 //   orthogonalize, muon_step
 //               matrix updates orthogonalised, and the step of the optimiser that is
 //               built on it, as operators of the dispatcher over lists of tensors
+//   qk_norm_rope
+//               norms of queries and keys with their rotation, forward and backward
 //   bind        the addresses of the C ABI's entry points, which the caller has
 //               loaded (so that one library is used, whichever it is)
 #include <ATen/ATen.h>
@@ -51,6 +53,9 @@ struct Entries {
   decltype(&scao_orthogonalize) orthogonalize;
   decltype(&scao_muon_workspace) muon_workspace;
   decltype(&scao_muon_step) muon_step;
+  decltype(&scao_qk_rope_forward) rope_forward;
+  decltype(&scao_qk_rope_backward_workspace) rope_backward_workspace;
+  decltype(&scao_qk_rope_backward) rope_backward;
 } lib;
 
 void check(int rc, const char* who) {
@@ -805,6 +810,267 @@ PyObject* muon_step(PyObject*, PyObject* const* args, Py_ssize_t n) {
   END_HANDLE_TH_ERRORS
 }
 
+// ---------------------------------------- norms of queries and keys, rotation ---
+//   qk_norm_rope           both outputs
+//   qk_norm_rope_backward  dq, dk, dw_q, dw_k: the wanted ones (bits 1, 2, 4, 8) in order
+#define ROPE_PARAMS                                                                    \
+  const Tensor &q, const Tensor &k, const std::optional<Tensor>&wq,                    \
+      const std::optional<Tensor>&wk, const Tensor &cos, const Tensor &sin,            \
+      const std::optional<Tensor>&positions, double eps, bool interleaved
+#define ROPE_ARGS q, k, wq, wk, cos, sin, positions, eps, interleaved
+
+std::tuple<Tensor, Tensor> op_qk_norm_rope(ROPE_PARAMS) {
+  static const auto op = c10::Dispatcher::singleton()
+                             .findSchemaOrThrow("scao_amd::qk_norm_rope", "")
+                             .typed<decltype(op_qk_norm_rope)>();
+  return op.call(ROPE_ARGS);
+}
+std::vector<Tensor> op_qk_norm_rope_backward(const Tensor& dq, const Tensor& dk, ROPE_PARAMS,
+                                             int64_t wanted) {
+  static const auto op = c10::Dispatcher::singleton()
+                             .findSchemaOrThrow("scao_amd::qk_norm_rope_backward", "")
+                             .typed<decltype(op_qk_norm_rope_backward)>();
+  return op.call(dq, dk, ROPE_ARGS, wanted);
+}
+
+// q and k: batch x tokens x heads x columns
+void check_rope(ROPE_PARAMS) {
+  TORCH_CHECK(lib.rope_forward, "qk_norm_rope: scao_amd has not loaded its library");
+  TORCH_CHECK(q.dim() == 4 && k.dim() == 4 && q.sym_size(0) == k.sym_size(0) &&
+                  q.sym_size(1) == k.sym_size(1) && q.sym_size(3) == k.sym_size(3),
+              "qk_norm_rope: shape mismatch: q ", q.sym_sizes(), ", k ", k.sym_sizes());
+  auto on = [&](const Tensor& t) { return t.layout() == at::kStrided && t.device() == q.device(); };
+  TORCH_CHECK(on(q) && on(k) && code_of(q.scalar_type()) >= 0 && k.scalar_type() == q.scalar_type(),
+              "qk_norm_rope takes q and k of one type of float32, bfloat16 and float16 on one device");
+  for (const auto* w : {&wq, &wk})
+    TORCH_CHECK(!*w || (on(**w) && code_of((*w)->scalar_type()) >= 0 && (*w)->dim() == 1 &&
+                        (*w)->sym_size(0) == q.sym_size(3)),
+                "qk_norm_rope: a weight is not a vector of a head's size on q's device");
+  TORCH_CHECK(on(cos) && on(sin) && cos.scalar_type() == at::kFloat &&
+                  sin.scalar_type() == at::kFloat && cos.dim() == 2 &&
+                  cos.sym_sizes() == sin.sym_sizes() && cos.sym_size(1) * 2 <= q.sym_size(3),
+              "qk_norm_rope: cos and sin must be float32 tables of at most half a head's columns "
+              "on q's device");
+  TORCH_CHECK(!positions || (on(*positions) && positions->dim() == 2 &&
+                             (positions->scalar_type() == at::kLong ||
+                              positions->scalar_type() == at::kInt) &&
+                             positions->sym_size(0) == q.sym_size(0) &&
+                             positions->sym_size(1) == q.sym_size(1)),
+              "qk_norm_rope: positions must be int64 or int32, one a token, on q's device");
+}
+
+Tensor unit_columns(const Tensor& t) {
+  return t.stride(-1) == 1 || t.size(-1) <= 1 ? t : t.contiguous();
+}
+scao_rope_tensor rope_tensor(const Tensor& t) {
+  return {t.data_ptr(), t.stride(0), t.stride(1), t.stride(2)};
+}
+struct Rope {
+  Tensor q, k, wq, wk, cos, sin, at;
+  scao_rope_desc d{};
+  Rope(const Tensor& q_, const Tensor& k_, const std::optional<Tensor>& wq_,
+       const std::optional<Tensor>& wk_, const Tensor& cos_, const Tensor& sin_,
+       const std::optional<Tensor>& positions, double eps, bool interleaved)
+      : q(unit_columns(q_)), k(unit_columns(k_)) {
+    // rows of one stride for both tables
+    const bool same = cos_.stride(1) == 1 && sin_.stride(1) == 1 && cos_.stride(0) == sin_.stride(0) &&
+                      cos_.stride(0) >= cos_.size(1);
+    cos = same ? cos_ : cos_.contiguous();
+    sin = same ? sin_ : sin_.contiguous();
+    if (wq_) wq = wq_->contiguous();
+    if (wk_) wk = wk_->contiguous();
+    d.x[0] = rope_tensor(q);
+    d.x[1] = rope_tensor(k);
+    int i = 0;
+    for (const Tensor* w : {&wq, &wk}) {
+      if (w->defined()) {
+        d.w[i] = w->data_ptr();
+        d.w_dtype[i] = code_of(w->scalar_type());
+      }
+      ++i;
+    }
+    d.cos = (const float*)cos.data_ptr();
+    d.sin = (const float*)sin.data_ptr();
+    if (positions) {
+      at = *positions;
+      d.positions = at.data_ptr();
+      d.wide_positions = at.scalar_type() == at::kLong;
+      d.position_strides[0] = at.stride(0);
+      d.position_strides[1] = at.stride(1);
+    }
+    d.batch = q.size(0);
+    d.seq = q.size(1);
+    d.table_rows = cos.size(0);
+    d.ld_table = cos.stride(0);
+    d.heads[0] = (int32_t)q.size(2);
+    d.heads[1] = (int32_t)k.size(2);
+    d.dim = (int32_t)q.size(3);
+    d.rotary = (int32_t)cos.size(1) * 2;
+    d.dtype = code_of(q.scalar_type());
+    d.interleaved = interleaved;
+    d.eps = (float)eps;
+  }
+};
+
+std::tuple<Tensor, Tensor> qk_norm_rope_hip(ROPE_PARAMS) {
+  check_rope(ROPE_ARGS);
+  const c10::DeviceGuard guard(q.device());
+  const Rope r(ROPE_ARGS);
+  const Tensor yq = at::empty_like(r.q), yk = at::empty_like(r.k);
+  const scao_rope_tensor y[2] = {rope_tensor(yq), rope_tensor(yk)};
+  check(lib.rope_forward(&r.d, y, stream_of(q)), "scao_qk_rope_forward");
+  return {yq, yk};
+}
+
+std::vector<Tensor> qk_norm_rope_backward_hip(const Tensor& dq_, const Tensor& dk_, ROPE_PARAMS,
+                                              int64_t wanted) {
+  check_rope(ROPE_ARGS);
+  TORCH_CHECK(dq_.sizes() == q.sizes() && dk_.sizes() == k.sizes() &&
+                  dq_.scalar_type() == q.scalar_type() && dk_.scalar_type() == k.scalar_type() &&
+                  dq_.device() == q.device() && dk_.device() == q.device(),
+              "qk_norm_rope_backward: the gradients are not like q and k");
+  TORCH_CHECK((wq || !(wanted & 4)) && (wk || !(wanted & 8)),
+              "qk_norm_rope_backward: no weight, no gradient");
+  const c10::DeviceGuard guard(q.device());
+  const Rope r(ROPE_ARGS);
+  const Tensor dq = unit_columns(dq_), dk = unit_columns(dk_);
+  std::vector<Tensor> out;
+  scao_rope_tensor dx[2] = {};
+  void* dw[2] = {};
+  for (int i = 0; i < 2; ++i)
+    if (wanted >> i & 1) {
+      out.push_back(at::empty_like(i ? r.k : r.q));
+      dx[i] = rope_tensor(out.back());
+    }
+  for (int i = 0; i < 2; ++i)
+    if (wanted >> i & 4) {
+      out.push_back(at::empty_like(i ? r.wk : r.wq));
+      dw[i] = out.back().data_ptr();
+    }
+  const scao_rope_tensor dy[2] = {rope_tensor(dq), rope_tensor(dk)};
+  const Tensor work = bytes(wanted & 12 ? lib.rope_backward_workspace(&r.d) : 0, q);
+  check(lib.rope_backward(&r.d, dy, dx, dw[0], dw[1], work.data_ptr(), stream_of(q)),
+        "scao_qk_rope_backward");
+  return out;
+}
+
+std::tuple<Tensor, Tensor> qk_norm_rope_meta(ROPE_PARAMS) {
+  check_rope(ROPE_ARGS);
+  return {at::empty_like(q), at::empty_like(k)};
+}
+std::vector<Tensor> qk_norm_rope_backward_meta(const Tensor&, const Tensor&, ROPE_PARAMS,
+                                               int64_t wanted) {
+  std::vector<Tensor> out;
+  if (wanted & 1) out.push_back(at::empty_like(q));
+  if (wanted & 2) out.push_back(at::empty_like(k));
+  if (wanted & 4) out.push_back(at::empty_like(*wq));
+  if (wanted & 8) out.push_back(at::empty_like(*wk));
+  return out;
+}
+
+struct QkNormRope : torch::autograd::Function<QkNormRope> {
+  static variable_list forward(AutogradContext* ctx, const Tensor& q, const Tensor& k,
+                               const std::optional<Tensor>& wq, const std::optional<Tensor>& wk,
+                               const Tensor& cos, const Tensor& sin,
+                               const std::optional<Tensor>& positions, double eps,
+                               bool interleaved) {
+    const at::AutoDispatchBelowADInplaceOrView below;
+    auto [yq, yk] = op_qk_norm_rope(ROPE_ARGS);
+    ctx->save_for_backward({q, k, wq.value_or(Tensor()), wk.value_or(Tensor()), cos, sin,
+                            positions.value_or(Tensor())});
+    ctx->saved_data["eps"] = eps;
+    ctx->saved_data["interleaved"] = interleaved;
+    return {yq, yk};
+  }
+  static variable_list backward(AutogradContext* ctx, const variable_list& grads) {
+    const variable_list t = ctx->get_saved_variables();
+    variable_list out(9);
+    auto given = [](const Tensor& x) { return x.defined() ? std::optional<Tensor>(x) : std::nullopt; };
+    int64_t wanted = 0;
+    for (int i = 0; i < 4; ++i) wanted |= (int64_t)(ctx->needs_input_grad(i) && t[i].defined()) << i;
+    variable_list have;
+    {
+      const at::AutoDispatchBelowADInplaceOrView below;
+      have = op_qk_norm_rope_backward(
+          grads[0].defined() ? grads[0] : at::zeros_like(t[0]),
+          grads[1].defined() ? grads[1] : at::zeros_like(t[1]), t[0], t[1], given(t[2]), given(t[3]),
+          t[4], t[5], given(t[6]), ctx->saved_data["eps"].toDouble(),
+          ctx->saved_data["interleaved"].toBool(), wanted);
+    }
+    if (at::GradMode::is_enabled()) {   // a gradient of these gradients is an error, not a zero
+      const auto error = std::make_shared<torch::autograd::DelayedError>(
+          "qk_norm_rope is differentiable once", (int64_t)have.size());
+      for (Tensor& g : have) g.requires_grad_(true);
+      have = (*error)(std::move(have));
+    }
+    for (int i = 0, n = 0; i < 4; ++i)
+      if (wanted >> i & 1) out[i] = have[n++];
+    return out;
+  }
+};
+
+std::tuple<Tensor, Tensor> qk_norm_rope_autograd(ROPE_PARAMS) {
+  check_rope(ROPE_ARGS);
+  const Tensor none;
+  const Tensor* inputs[6] = {&q, &k, wq ? &*wq : &none, wk ? &*wk : &none, &cos, &sin};
+  bool wanted = false;
+  for (int i = 0; i < 6; ++i) {
+    if (!inputs[i]->defined()) continue;
+    if (forward_mode())   // a tangent would be lost
+      TORCH_CHECK_NOT_IMPLEMENTED(!inputs[i]->_fw_grad(0).defined(),
+                                  "qk_norm_rope has no forward-mode derivative");
+    if (!at::GradMode::is_enabled() || !inputs[i]->requires_grad()) continue;
+    TORCH_CHECK_NOT_IMPLEMENTED(i < 4, "qk_norm_rope: cos and sin have no gradient");
+    wanted = true;
+  }
+  if (wanted) {
+    const variable_list y = QkNormRope::apply(unit_columns(q), unit_columns(k), wq, wk, cos, sin,
+                                              positions, eps, interleaved);
+    return {y[0], y[1]};
+  }
+  const at::AutoDispatchBelowADInplaceOrView below;
+  return op_qk_norm_rope(ROPE_ARGS);
+}
+
+TORCH_LIBRARY_FRAGMENT(scao_amd, m) {
+#define SCAO_ROPE                                                                       \
+  "Tensor q, Tensor k, Tensor? q_weight, Tensor? k_weight, Tensor cos, Tensor sin, "    \
+  "Tensor? positions, float eps, bool interleaved"
+  m.def("qk_norm_rope(" SCAO_ROPE ") -> (Tensor, Tensor)");
+  m.def("qk_norm_rope_backward(Tensor dq, Tensor dk, " SCAO_ROPE ", int wanted) -> Tensor[]");
+#undef SCAO_ROPE
+}
+TORCH_LIBRARY_IMPL(scao_amd, CUDA, m) {
+  m.impl("qk_norm_rope", qk_norm_rope_hip);
+  m.impl("qk_norm_rope_backward", qk_norm_rope_backward_hip);
+}
+TORCH_LIBRARY_IMPL(scao_amd, Meta, m) {
+  m.impl("qk_norm_rope", qk_norm_rope_meta);
+  m.impl("qk_norm_rope_backward", qk_norm_rope_backward_meta);
+}
+TORCH_LIBRARY_IMPL(scao_amd, Autograd, m) { m.impl("qk_norm_rope", qk_norm_rope_autograd); }
+
+// qk_norm_rope(q, k, q_weight, k_weight, cos, sin, positions, eps, interleaved), tensors
+// or None
+PyObject* qk_norm_rope(PyObject*, PyObject* const* args, Py_ssize_t n) {
+  HANDLE_TH_ERRORS
+  TORCH_CHECK_TYPE(n == 9, "qk_norm_rope() takes nine arguments");
+  std::optional<Tensor> t[7];
+  for (int i = 0; i < 7; ++i) {
+    if (args[i] == Py_None && (i == 2 || i == 3 || i == 6)) continue;
+    TORCH_CHECK_TYPE(THPVariable_Check(args[i]), "qk_norm_rope() takes tensors");
+    t[i] = THPVariable_Unpack(args[i]);
+  }
+  const double eps = PyFloat_AsDouble(args[7]);
+  const int interleaved = PyObject_IsTrue(args[8]);
+  if (PyErr_Occurred()) return nullptr;
+  auto [yq, yk] = op_qk_norm_rope(*t[0], *t[1], t[2], t[3], *t[4], *t[5], t[6], eps, interleaved != 0);
+  const THPObjectPtr a(THPVariable_Wrap(yq)), b(THPVariable_Wrap(yk));
+  if (!a || !b) return nullptr;
+  return PyTuple_Pack(2, a.get(), b.get());
+  END_HANDLE_TH_ERRORS
+}
+
 // bind({name: address})
 PyObject* bind(PyObject*, PyObject* arg) {
   auto at = [&](const char* name, auto& entry) {
@@ -823,7 +1089,10 @@ PyObject* bind(PyObject*, PyObject* arg) {
         at("scao_grad_norm", lib.grad_norm) && at("scao_grad_clip", lib.grad_clip) &&
         at("scao_orthogonalize_workspace", lib.orthogonalize_workspace) &&
         at("scao_orthogonalize", lib.orthogonalize) &&
-        at("scao_muon_workspace", lib.muon_workspace) && at("scao_muon_step", lib.muon_step)))
+        at("scao_muon_workspace", lib.muon_workspace) && at("scao_muon_step", lib.muon_step) &&
+        at("scao_qk_rope_forward", lib.rope_forward) &&
+        at("scao_qk_rope_backward_workspace", lib.rope_backward_workspace) &&
+        at("scao_qk_rope_backward", lib.rope_backward)))
     return nullptr;
   Py_RETURN_NONE;
 }
@@ -835,6 +1104,7 @@ PyMethodDef methods[] = {
     SCAO_FASTCALL(grad_norm),
     SCAO_FASTCALL(grad_clip),
     SCAO_FASTCALL(muon_step),
+    SCAO_FASTCALL(qk_norm_rope),
 #undef SCAO_FASTCALL
     {"bind", bind, METH_O, nullptr},
     {nullptr, nullptr, 0, nullptr}};
