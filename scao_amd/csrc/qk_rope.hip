@@ -32,7 +32,7 @@ int size_of(int dt) { return dt == SCAO_F32 ? 4 : 2; }
 
 constexpr int THREADS = 256;
 constexpr int MAX_DIM = 512;
-constexpr int MAX_BLOCKS = 1024;    // of a backward pass, with a partial sum each
+constexpr int MAX_BLOCKS = 768;     // of a backward pass, with a partial sum each
 
 // one of the two tensors
 struct Side {
@@ -67,27 +67,31 @@ typedef v4u_t v4u_a2 __attribute__((aligned(2)));
 typedef float v2f_a4 __attribute__((ext_vector_type(2), aligned(4)));
 #define GLOBAL(T) __attribute__((address_space(1))) T
 
-// V elements in a row; they start at any element
+// V elements in a row, which start at any element: as they are in memory, and as
+// numbers.  (They are held as they are until they are needed.)
 template <int DT, int V>
-__device__ __forceinline__ void load(const void* p, int64_t at, float (&x)[V]) {
-  if constexpr (V == 1) {
-    x[0] = ld1(p, DT, at);
-  } else if constexpr (DT == SCAO_F32) {
-    if constexpr (V == 2) {
-      const v2f_a4 w = *(const GLOBAL(v2f_a4)*)((const float*)p + at);
-      x[0] = w[0];
-      x[1] = w[1];
-    } else {
+struct Words {
+  static constexpr int N = DT == SCAO_F32 ? V : V > 1 ? V / 2 : 1;
+  uint32_t w[N];
+  __device__ __forceinline__ void load(const void* p, int64_t at) {
+    if constexpr (DT == SCAO_F32) {
+      if constexpr (V == 1) {
+        w[0] = __float_as_uint(gld1((const float*)p + at));
+      } else if constexpr (V == 2) {
+        const v2f_a4 v = *(const GLOBAL(v2f_a4)*)((const float*)p + at);
+        w[0] = __float_as_uint(v[0]);
+        w[1] = __float_as_uint(v[1]);
+      } else {
 #pragma unroll
-      for (int h = 0; h < V; h += 4) {
-        const v4f w = gld4((const float*)p + at + h);
+        for (int h = 0; h < V; h += 4) {
+          const v4f v = gld4((const float*)p + at + h);
 #pragma unroll
-        for (int t = 0; t < 4; ++t) x[h + t] = w[t];
+          for (int t = 0; t < 4; ++t) w[h + t] = __float_as_uint(v[t]);
+        }
       }
-    }
-  } else {
-    uint32_t w[V / 2];
-    if constexpr (V == 2) {
+    } else if constexpr (V == 1) {
+      w[0] = ((const gu16*)p)[at];
+    } else if constexpr (V == 2) {
       w[0] = *(const GLOBAL(v1u_a2)*)((const uint16_t*)p + at);
     } else if constexpr (V == 4) {
       const v2u v = gld2w((const uint16_t*)p + at);
@@ -98,14 +102,24 @@ __device__ __forceinline__ void load(const void* p, int64_t at, float (&x)[V]) {
 #pragma unroll
       for (int t = 0; t < 4; ++t) w[t] = v[t];
     }
+  }
+  __device__ __forceinline__ void get(float (&x)[V]) const {
 #pragma unroll
     for (int t = 0; t < V; ++t) {
-      if (DT == SCAO_BF16)
+      if (DT == SCAO_F32)
+        x[t] = __uint_as_float(w[t % N]);
+      else if (DT == SCAO_BF16)
         x[t] = __uint_as_float(t & 1 ? w[t / 2] & 0xffff0000u : w[t / 2] << 16);
       else
         x[t] = f16_to_f((uint16_t)(w[t / 2] >> (16 * (t & 1))));
     }
   }
+};
+template <int DT, int V>
+__device__ __forceinline__ void load(const void* p, int64_t at, float (&x)[V]) {
+  Words<DT, V> w;
+  w.load(p, at);
+  w.get(x);
 }
 template <int DT, int V>
 __device__ __forceinline__ void store(void* p, int64_t at, const float (&x)[V]) {
@@ -168,21 +182,16 @@ struct Lane {
         else load<SCAO_F16, V>(s.w, at[k][h], w[k][h]);
       }
   }
-  // of token t of sequence b; a position outside of the tables: NaN
-  __device__ __forceinline__ void angles(const Args& a, uint32_t b, uint32_t t) {
-    int64_t p = t;
-    if (a.positions) {
-      const int64_t i = b * a.pb + t * a.pt;
-      p = a.wide_positions ? ((gi64*)a.positions)[i] : ((gi32*)a.positions)[i];
-    }
+  // those of position p; one outside of the tables: NaN
+  __device__ __forceinline__ void angles(const Args& a, int64_t p) {
     const bool in = p >= 0 && p < a.table;
     const int64_t row = in ? p * a.ld_table : 0;
 #pragma unroll
     for (int k = 0; k < N; ++k) {
 #pragma unroll
-      for (int t2 = 0; t2 < V; ++t2) {
-        cos[k][t2] = in ? 1.f : __uint_as_float(0x7fc00000u);
-        sin[k][t2] = 0.f;
+      for (int t = 0; t < V; ++t) {
+        cos[k][t] = in ? 1.f : __uint_as_float(0x7fc00000u);
+        sin[k][t] = 0.f;
       }
       if (turns[k] && in) {
         const int64_t c = row + at[k][0] / (BESIDE ? 2 : 1);
@@ -191,15 +200,22 @@ struct Lane {
       }
     }
   }
-  __device__ __forceinline__ void get(const void* p, int64_t head, float (&x)[N][2][V]) const {
+  using Head = Words<DT, V>[N][2];
+  __device__ __forceinline__ void fetch(const void* p, int64_t head, Head& x) const {
 #pragma unroll
     for (int k = 0; k < N; ++k)
 #pragma unroll
       for (int h = 0; h < 2; ++h) {
 #pragma unroll
-        for (int t = 0; t < V; ++t) x[k][h][t] = 0.f;
-        if (at[k][h] >= 0) load<DT, V>(p, head + at[k][h], x[k][h]);
+        for (int t = 0; t < Words<DT, V>::N; ++t) x[k][h].w[t] = 0;
+        if (at[k][h] >= 0) x[k][h].load(p, head + at[k][h]);
       }
+  }
+  static __device__ __forceinline__ void get(const Head& w, float (&x)[N][2][V]) {
+#pragma unroll
+    for (int k = 0; k < N; ++k)
+#pragma unroll
+      for (int h = 0; h < 2; ++h) w[k][h].get(x[k][h]);
   }
   __device__ __forceinline__ void put(void* p, int64_t head, const float (&x)[N][2][V]) const {
 #pragma unroll
@@ -235,6 +251,12 @@ struct Lane {
   }
 };
 
+// the position of token t of sequence b
+__device__ __forceinline__ int64_t position_of(const Args& a, uint32_t b, uint32_t t) {
+  if (!a.positions) return t;
+  const int64_t i = b * a.pb + t * a.pt;
+  return a.wide_positions ? ((gi64*)a.positions)[i] : ((gi32*)a.positions)[i];
+}
 // of a head's lanes
 __device__ __forceinline__ float over_lanes(float x, int lanes) {
   for (int o = lanes / 2; o > 0; o >>= 1) x += __shfl_xor(x, o, SCAO_WAVE);
@@ -277,21 +299,23 @@ __global__ __launch_bounds__(THREADS) void k_rope_forward(const Args a) {
   const uint32_t b = token / a.seq, t = token % a.seq;
   Lane<DT, V, BESIDE> l(a, lane);
   const int64_t xs = b * s.xb + t * s.xt + run.head * s.xh;
-  float x[R][N][2][V];
+  typename Lane<DT, V, BESIDE>::Head heads[R];
 #pragma unroll
   for (int r = 0; r < R; ++r)
-    if (r < run.heads) l.get(s.x, xs + r * s.xh, x[r]);
+    if (r < run.heads) l.fetch(s.x, xs + r * s.xh, heads[r]);
   l.weights(s);
-  l.angles(a, b, t);
+  l.angles(a, position_of(a, b, t));
   const int64_t os = b * s.ob + t * s.ot + run.head * s.oh;
 #pragma unroll
   for (int r = 0; r < R; ++r) {
-    float sum = 0.f;
-    if (r < run.heads)
+    float x[N][2][V], sum = 0.f;
+    if (r < run.heads) {
+      l.get(heads[r], x);
 #pragma unroll
       for (int k = 0; k < N; ++k)
 #pragma unroll
-        for (int e = 0; e < 2 * V; ++e) sum = fmaf(x[r][k][e / V][e % V], x[r][k][e / V][e % V], sum);
+        for (int e = 0; e < 2 * V; ++e) sum = fmaf(x[k][e / V][e % V], x[k][e / V][e % V], sum);
+    }
     sum = over_lanes(sum, a.lanes);
     const float rms = 1.f / sqrtf(sum / a.dim + a.eps);
     if (r >= run.heads) continue;
@@ -299,29 +323,31 @@ __global__ __launch_bounds__(THREADS) void k_rope_forward(const Args a) {
     for (int k = 0; k < N; ++k)
 #pragma unroll
       for (int e = 0; e < 2 * V; ++e) {
-        float& y = x[r][k][e / V][e % V];
+        float& y = x[k][e / V][e % V];
         y = y * rms * l.w[k][e / V][e % V];
       }
-    l.template rotate<false>(x[r]);
-    l.put(s.out, os + r * s.oh, x[r]);
+    l.template rotate<false>(x);
+    l.put(s.out, os + r * s.oh, x);
   }
 }
 
-// A group keeps its run of heads from token to token, so that a lane adds up its
-// columns of one weight's gradient; a workgroup's groups are added in order.
-constexpr int BACKWARD_HEADS = 2;
+// A group keeps its head from token to token, so that a lane adds up its columns of
+// one weight's gradient; a workgroup's groups are added in order.  The next token's
+// head and position are under way, as they are in memory, while one is worked on: 8192
+// tokens of 32 + 8 heads of 128 in bf16 54 us (4.7 TB/s); with two heads a group 55 on
+// two thirds of the waves and 111 on as many (registers), without the next head 76.
+constexpr int BACKWARD_HEADS = 1;
 template <int DT, int V, bool BESIDE>
-__global__ __launch_bounds__(THREADS) void k_rope_backward(const Args a) {
-  constexpr int N = PAIRS<V>, R = BACKWARD_HEADS;
+__global__ __launch_bounds__(THREADS, 3) void k_rope_backward(const Args a) {
+  constexpr int N = PAIRS<V>;
   __shared__ float sums[THREADS * 2 * V * N];
   const int groups = THREADS / a.lanes, own = threadIdx.x / a.lanes;
   const int lane = threadIdx.x & (a.lanes - 1), runs = a.s[0].runs + a.s[1].runs;
   const uint32_t group = blockIdx.x * groups + own, tracks = gridDim.x * groups / runs;
-  const int which = group % runs;
   uint32_t token = group / runs;
-  if (token >= tracks) token = a.tokens;   // none: the last few groups
-  const Run run = run_of<R>(a, which);
+  const Run run = run_of<BACKWARD_HEADS>(a, group % runs);
   const Side s = side_of(a, run.side);
+  if (token >= tracks) token = a.tokens;   // none: the last few groups
   Lane<DT, V, BESIDE> l(a, lane);
   l.weights(s);
   float dw[N][2][V];
@@ -329,53 +355,53 @@ __global__ __launch_bounds__(THREADS) void k_rope_backward(const Args a) {
   for (int k = 0; k < N; ++k)
 #pragma unroll
     for (int e = 0; e < 2 * V; ++e) dw[k][e / V][e % V] = 0.f;
-  // (every lane goes round as often as the first group of the workgroup, which has
-  // the earliest token)
+
+  typename Lane<DT, V, BESIDE>::Head xn = {}, dn = {};
+  int64_t position = 0, on = 0;   // and where dx goes
+  auto begin = [&](uint32_t i) {
+    if (i >= a.tokens) return;
+    const uint32_t b = i / a.seq, t = i % a.seq;
+    position = position_of(a, b, t);
+    l.fetch(s.x, b * s.xb + t * s.xt + run.head * s.xh, xn);
+    l.fetch(s.dy, b * s.yb + t * s.yt + run.head * s.yh, dn);
+    on = b * s.ob + t * s.ot + run.head * s.oh;
+  };
+  begin(token);
+  // (every lane goes round as often as the one with the most tokens)
   const uint32_t rounds = (a.tokens + tracks - 1) / tracks;
   for (uint32_t i = 0; i < rounds; ++i, token += tracks) {
     const bool in = token < a.tokens;
-    const uint32_t b = in ? token / a.seq : 0, t = in ? token % a.seq : 0;
-    const int heads = in ? run.heads : 0;
-    const int64_t xs = b * s.xb + t * s.xt + run.head * s.xh;
-    const int64_t ys = b * s.yb + t * s.yt + run.head * s.yh;
-    const int64_t os = b * s.ob + t * s.ot + run.head * s.oh;
-    float x[R][N][2][V], d[R][N][2][V];
-#pragma unroll
-    for (int r = 0; r < R; ++r)
-      if (r < heads) {
-        l.get(s.x, xs + r * s.xh, x[r]);
-        l.get(s.dy, ys + r * s.yh, d[r]);
-      }
-    l.angles(a, b, t);
-#pragma unroll
-    for (int r = 0; r < R; ++r) {
-      float square = 0.f, product = 0.f;
-      if (r < heads) {
-        l.template rotate<true>(d[r]);
-#pragma unroll
-        for (int k = 0; k < N; ++k)
-#pragma unroll
-          for (int e = 0; e < 2 * V; ++e) {
-            const float v = x[r][k][e / V][e % V];
-            square = fmaf(v, v, square);
-            product = fmaf(d[r][k][e / V][e % V] * l.w[k][e / V][e % V], v, product);
-          }
-      }
-      square = over_lanes(square, a.lanes);
-      product = over_lanes(product, a.lanes);
-      if (r >= heads) continue;
-      const float rms = 1.f / sqrtf(square / a.dim + a.eps);
-      const float mean = product * rms / a.dim;
+    const int64_t os = on;
+    float x[N][2][V], d[N][2][V], square = 0.f, product = 0.f;
+    if (in) {
+      l.angles(a, position);
+      l.get(xn, x);
+      l.get(dn, d);
+      begin(token + tracks);
+      l.template rotate<true>(d);
 #pragma unroll
       for (int k = 0; k < N; ++k)
 #pragma unroll
         for (int e = 0; e < 2 * V; ++e) {
-          const float u = x[r][k][e / V][e % V] * rms, g = d[r][k][e / V][e % V];
-          dw[k][e / V][e % V] = fmaf(g, u, dw[k][e / V][e % V]);
-          x[r][k][e / V][e % V] = rms * fmaf(-u, mean, g * l.w[k][e / V][e % V]);
+          const float v = x[k][e / V][e % V];
+          square = fmaf(v, v, square);
+          product = fmaf(d[k][e / V][e % V] * l.w[k][e / V][e % V], v, product);
         }
-      if (s.out) l.put(s.out, os + r * s.oh, x[r]);
     }
+    square = over_lanes(square, a.lanes);
+    product = over_lanes(product, a.lanes);
+    if (!in) continue;
+    const float rms = 1.f / sqrtf(square / a.dim + a.eps);
+    const float mean = product * rms / a.dim;
+#pragma unroll
+    for (int k = 0; k < N; ++k)
+#pragma unroll
+      for (int e = 0; e < 2 * V; ++e) {
+        const float u = x[k][e / V][e % V] * rms, g = d[k][e / V][e % V];
+        dw[k][e / V][e % V] = fmaf(g, u, dw[k][e / V][e % V]);
+        x[k][e / V][e % V] = rms * fmaf(-u, mean, g * l.w[k][e / V][e % V]);
+      }
+    if (s.out) l.put(s.out, os, x);
   }
   if (!a.parts) return;
   // [group][column]: dim columns of lanes * 2 V N at most
@@ -399,26 +425,40 @@ __global__ __launch_bounds__(THREADS) void k_rope_backward(const Args a) {
   }
 }
 
-// The workgroups' sums, added in order in double: 16 columns a workgroup, 16 threads
-// a column.
+// The workgroups' sums, added in order in double: 16 columns a workgroup, 64 threads
+// a column, each with eight loads under way.
+constexpr int JOIN_ROWS = 64;
 struct JoinArgs {
   const float* parts;
   void* dw[2];
   int w_dtype[2];
   int blocks, dim;
 };
-__global__ __launch_bounds__(THREADS) void k_rope_join(const JoinArgs a) {
-  __shared__ double sums[16][17];
+__global__ __launch_bounds__(16 * JOIN_ROWS) void k_rope_join(const JoinArgs a) {
+  __shared__ double sums[JOIN_ROWS][17];
   const int c = threadIdx.x % 16, row = threadIdx.x / 16, i = blockIdx.x * 16 + c;
   double x = 0.0;
+  constexpr int AHEAD = 8;
   if (i < 2 * a.dim)
-    for (int b = row; b < a.blocks; b += 16) x += gld1(a.parts + (int64_t)b * 2 * a.dim + i);
+    for (int b = row; b < a.blocks; b += JOIN_ROWS * AHEAD) {
+      float p[AHEAD];
+#pragma unroll
+      for (int t = 0; t < AHEAD; ++t)
+        p[t] = b + t * JOIN_ROWS < a.blocks
+                   ? gld1(a.parts + (int64_t)(b + t * JOIN_ROWS) * 2 * a.dim + i)
+                   : 0.f;
+#pragma unroll
+      for (int t = 0; t < AHEAD; ++t) x += p[t];
+    }
   sums[row][c] = x;
   __syncthreads();
+  for (int half = JOIN_ROWS / 2; half > 0; half /= 2) {
+    if (row < half) sums[row][c] += sums[row + half][c];
+    __syncthreads();
+  }
   if (row || i >= 2 * a.dim) return;
-  for (int r = 1; r < 16; ++r) x += sums[r][c];
   const int side = i >= a.dim;
-  if (a.dw[side]) st1(a.dw[side], a.w_dtype[side], i - side * a.dim, (float)x);
+  if (a.dw[side]) st1(a.dw[side], a.w_dtype[side], i - side * a.dim, (float)sums[0][c]);
 }
 
 // ------------------------------------------------------------------ host ---
@@ -536,9 +576,9 @@ void for_variant(int dt, int v, bool beside, F&& f) {
 int backward_blocks(const Args& a) {
   const int groups = THREADS / a.lanes, runs = a.s[0].runs + a.s[1].runs;
   const int64_t all = ((int64_t)a.tokens * runs + groups - 1) / groups;
-  // at least one track of every run
-  const int64_t least = (runs + groups - 1) / groups;
-  return (int)std::max(least, std::min<int64_t>(all, MAX_BLOCKS));
+  // at least one track of every run, and as many tokens for each
+  const int64_t least = (runs + groups - 1) / groups, rounds = (all + MAX_BLOCKS - 1) / MAX_BLOCKS;
+  return (int)std::max(least, (all + rounds - 1) / rounds);
 }
 
 }  // namespace
@@ -609,7 +649,7 @@ extern "C" int scao_qk_rope_backward(const scao_rope_desc* d, const scao_rope_te
     });
   }
   // (no token: the weights' gradients are zeros)
-  if (dw_q || dw_k) k_rope_join<<<(2 * d->dim + 15) / 16, THREADS, 0, st>>>(j);
+  if (dw_q || dw_k) k_rope_join<<<(2 * d->dim + 15) / 16, 16 * JOIN_ROWS, 0, st>>>(j);
   SCAO_LAUNCH_CHECK(who);
   return SCAO_OK;
 }
