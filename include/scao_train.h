@@ -91,10 +91,12 @@ int scao_ffn_backward(const scao_ffn_desc* desc, const void* dy, int64_t ld_dy, 
  *   A = X X^T,  X <- a X + (b A + c A A) X     (rows <= cols, else on X^T)
  * which sends every singular value s of G / (|G|_F + eps) through the odd
  * polynomials a s + b s^3 + c s^5.  The matrices of a HOST table may differ in
- * shape and type; all of them share the launches.  Rows have unit column stride
- * and a row stride of at least a row; src and dst may differ in type.
+ * shape, type and precision; all of them share the launches.  Rows have unit column
+ * stride and a row stride of at least a row; src and dst may differ in type.
  *   SCAO_ORTHO_FAST  products of fp16 words with fp32 sums, X, A and B rounded to
- *                    11 significant bits once a step (results about 5e-4 off);
+ *                    11 significant bits once a step (the published five steps:
+ *                    results about 1.2e-3 off, a bf16's own rounding 1.7e-3;
+ *                    with up to 128 rows or columns as SCAO_ORTHO_FP32);
  *   SCAO_ORTHO_FP32  words of 22 bits, three products each: fp32's accuracy.
  * A matrix with a NaN or an infinity (or with a sum of squares beyond double's
  * range) gives NaN throughout, and no other matrix; one of zeros gives zeros.
@@ -107,8 +109,8 @@ int scao_ffn_backward(const scao_ffn_desc* desc, const void* dy, int64_t ld_dy, 
  * p, g and m contiguous; p and g may have different types; p is rounded once.
  *
  * Written memory may not overlap with anything else of the table
- * (SCAO_ERR_INVALID).  workspace: the *_workspace() bytes for the same table,
- * steps and precision, aligned to 16, contents of no meaning. */
+ * (SCAO_ERR_INVALID).  workspace: the *_workspace() bytes for the same table and
+ * steps, aligned to 16, contents of no meaning. */
 enum scao_ortho_precision { SCAO_ORTHO_FAST = 0, SCAO_ORTHO_FP32 = 1 };
 typedef struct scao_ortho_desc {   /* HOST */
   const void* src;
@@ -116,11 +118,11 @@ typedef struct scao_ortho_desc {   /* HOST */
   int64_t rows, cols;              /* below 2^20, the smaller one up to 2^15     */
   int64_t ld_src, ld_dst;          /* row strides in elements                    */
   int32_t src_dtype, dst_dtype;    /* enum scao_dtype                            */
+  int32_t precision, pad0;         /* enum scao_ortho_precision                  */
 } scao_ortho_desc;
-int64_t scao_orthogonalize_workspace(const scao_ortho_desc* matrices, int n, int steps,
-                                     int precision);
+int64_t scao_orthogonalize_workspace(const scao_ortho_desc* matrices, int n, int steps);
 int scao_orthogonalize(const scao_ortho_desc* matrices, int n, const double* coefficients, int steps,
-                       double eps, int precision, void* workspace, void* stream);
+                       double eps, void* workspace, void* stream);
 typedef struct scao_muon_desc {    /* HOST */
   void* p;
   const void* g;
@@ -128,11 +130,12 @@ typedef struct scao_muon_desc {    /* HOST */
   int64_t rows, cols;
   int32_t dtype, grad_dtype;       /* of p, of g                                 */
   float rate, decay;
+  int32_t precision, pad0;
 } scao_muon_desc;
-int64_t scao_muon_workspace(const scao_muon_desc* matrices, int n, int steps, int precision);
+int64_t scao_muon_workspace(const scao_muon_desc* matrices, int n, int steps);
 int scao_muon_step(const scao_muon_desc* matrices, int n, double momentum, int nesterov,
-                   const double* coefficients, int steps, double eps, int precision,
-                   void* workspace, void* stream);
+                   const double* coefficients, int steps, double eps, void* workspace,
+                   void* stream);
 
 /* ---- norms of queries and keys with their rotation ---------------------------
  * For every token and head of q ([0]) and k ([1]), of `dim` columns x with unit

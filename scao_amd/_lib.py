@@ -105,11 +105,11 @@ FFN_DESC = np.dtype([
 ], align=True)
 ORTHO_DESC = np.dtype([
     ("src", "u8"), ("dst", "u8"), ("rows", "i8"), ("cols", "i8"), ("ld_src", "i8"),
-    ("ld_dst", "i8"), ("src_dtype", "i4"), ("dst_dtype", "i4"),
+    ("ld_dst", "i8"), ("src_dtype", "i4"), ("dst_dtype", "i4"), ("precision", "i4"), ("pad0", "i4"),
 ], align=True)
 MUON_DESC = np.dtype([
     ("p", "u8"), ("g", "u8"), ("m", "u8"), ("rows", "i8"), ("cols", "i8"), ("dtype", "i4"),
-    ("grad_dtype", "i4"), ("rate", "f4"), ("decay", "f4"),
+    ("grad_dtype", "i4"), ("rate", "f4"), ("decay", "f4"), ("precision", "i4"), ("pad0", "i4"),
 ], align=True)
 ROPE_TENSOR = np.dtype([("p", "u8"), ("batch", "i8"), ("token", "i8"), ("head", "i8")], align=True)
 ROPE_DESC = np.dtype([
@@ -133,8 +133,8 @@ STRUCTS = {0: (PARAM_DESC, [n for n in PARAM_DESC.names if n != "pad0"]),
            7: (LOOKAHEAD_DESC, [n for n in LOOKAHEAD_DESC.names if n != "pad0"]),
            8: (TENSOR_DESC, [n for n in TENSOR_DESC.names if n != "pad0"]),
            9: (FFN_DESC, list(FFN_DESC.names)),
-           10: (ORTHO_DESC, list(ORTHO_DESC.names)),
-           11: (MUON_DESC, list(MUON_DESC.names)),
+           10: (ORTHO_DESC, [n for n in ORTHO_DESC.names if n != "pad0"]),
+           11: (MUON_DESC, [n for n in MUON_DESC.names if n != "pad0"]),
            12: (ROPE_TENSOR, list(ROPE_TENSOR.names)),
            13: (ROPE_DESC, list(ROPE_DESC.names))}
 
@@ -195,10 +195,10 @@ TRAIN_SIGNATURES = {
     "scao_ffn_forward": (_I, [_VP, _VP, _VP, _VP, _VP]),
     "scao_ffn_backward_workspace": (_I64, [_VP, _VP, _I64, _I]),
     "scao_ffn_backward": (_I, [_VP, _VP, _I64, _VP, _VP, _VP, _VP, _VP, _VP, _VP]),
-    "scao_orthogonalize_workspace": (_I64, [_VP, _I, _I, _I]),
-    "scao_orthogonalize": (_I, [_VP, _I, _VP, _I, _D, _I, _VP, _VP]),
-    "scao_muon_workspace": (_I64, [_VP, _I, _I, _I]),
-    "scao_muon_step": (_I, [_VP, _I, _D, _I, _VP, _I, _D, _I, _VP, _VP]),
+    "scao_orthogonalize_workspace": (_I64, [_VP, _I, _I]),
+    "scao_orthogonalize": (_I, [_VP, _I, _VP, _I, _D, _VP, _VP]),
+    "scao_muon_workspace": (_I64, [_VP, _I, _I]),
+    "scao_muon_step": (_I, [_VP, _I, _D, _I, _VP, _I, _D, _VP, _VP]),
     "scao_qk_rope_forward": (_I, [_VP, _VP, _VP]),
     "scao_qk_rope_backward_workspace": (_I64, [_VP]),
     "scao_qk_rope_backward": (_I, [_VP, _VP, _VP, _VP, _VP, _VP, _VP]),

@@ -127,7 +127,7 @@ extern "C" int scao_struct_layout(int which, int64_t* out, int cap) {
       PUT(sizeof(S));
       PUT(offsetof(S, src)); PUT(offsetof(S, dst)); PUT(offsetof(S, rows)); PUT(offsetof(S, cols));
       PUT(offsetof(S, ld_src)); PUT(offsetof(S, ld_dst)); PUT(offsetof(S, src_dtype));
-      PUT(offsetof(S, dst_dtype));
+      PUT(offsetof(S, dst_dtype)); PUT(offsetof(S, precision));
       break;
     }
     case 11: {
@@ -135,7 +135,7 @@ extern "C" int scao_struct_layout(int which, int64_t* out, int cap) {
       PUT(sizeof(S));
       PUT(offsetof(S, p)); PUT(offsetof(S, g)); PUT(offsetof(S, m)); PUT(offsetof(S, rows));
       PUT(offsetof(S, cols)); PUT(offsetof(S, dtype)); PUT(offsetof(S, grad_dtype));
-      PUT(offsetof(S, rate)); PUT(offsetof(S, decay));
+      PUT(offsetof(S, rate)); PUT(offsetof(S, decay)); PUT(offsetof(S, precision));
       break;
     }
     case 12: {

@@ -1,12 +1,12 @@
 // Newton-Schulz orthogonalisation of matrix updates, and the step of the optimiser
 // that is built on it: argument checks, memory plans and the order of the launches.
-// The kernels are in ortho_norm.hpp and ortho_kernels.hpp.
+// The kernels are in ortho_kernels.hpp, ortho_norm.hpp and ortho_small.hpp.
 #include <algorithm>
 #include <cmath>
 #include <new>
 #include <vector>
 
-#include "ortho_norm.hpp"
+#include "ortho_small.hpp"
 
 using namespace scao;
 
@@ -25,6 +25,7 @@ struct Matrix {
   int64_t rows, cols, ld_src, ld_dst;
   int src_dtype, dst_dtype;
   float rate, decay;
+  int words;
   int64_t smaller() const { return std::min(rows, cols); }
   int64_t larger() const { return std::max(rows, cols); }
   // C's tiles of 256 x 256 in an update
@@ -113,10 +114,14 @@ struct Plan {
   OrthoPhase ph{};
 };
 
+bool same_group(const Matrix& a, const Matrix& b) {
+  return a.rows == b.rows && a.cols == b.cols && a.words == b.words;
+}
+
 struct Pass {
   const Matrix* m;
   const int* order;          // the pass's entries
-  int n, words;
+  int n;
   char* base;
   std::vector<OrthoGroup> groups;
   double* norms = nullptr;
@@ -130,21 +135,22 @@ struct Pass {
   }
   const Matrix& entry(int i) const { return m[order[i]]; }
 
-  Pass(const Matrix* matrices, const int* order_, int n_, int words_, char* base_, bool again)
-      : m(matrices), order(order_), n(n_), words(words_), base(base_) {
+  Pass(const Matrix* matrices, const int* order_, int n_, char* base_, bool again)
+      : m(matrices), order(order_), n(n_), base(base_) {
     norms = (double*)(base + take((int64_t)ORTHO_MATRICES * ORTHO_PARTS * 8));
     for (int i = 0; i < n;) {
       OrthoGroup g{};
       g.first = i;
       g.rows = (int)entry(i).rows;
       g.cols = (int)entry(i).cols;
-      while (i < n && entry(i).rows == g.rows && entry(i).cols == g.cols) ++i;
+      g.words = entry(i).words;
+      while (i < n && same_group(entry(i), entry(g.first))) ++i;
       g.count = i - g.first;
       const int64_t s = std::min(g.rows, g.cols);
       g.ldx = (int)round_up(g.cols, 8);
       g.lda = (int)round_up(s, 8);
-      g.x_step = round_up((int64_t)words * g.rows * g.ldx * 2, 256);
-      g.a_step = round_up(words * s * g.lda * 2, 256);
+      g.x_step = round_up((int64_t)g.words * g.rows * g.ldx * 2, 256);
+      g.a_step = round_up(g.words * s * g.lda * 2, 256);
       g.x = take(g.count * g.x_step);
       g.y = again ? take(g.count * g.x_step) : g.x;   // (one step writes the result alone)
       g.a = take(g.count * g.a_step);
@@ -153,14 +159,16 @@ struct Pass {
     }
   }
 
-  static int64_t sum_of(int phase, const OrthoGroup& g) {
-    return phase == ORTHO_GRAM ? std::max(g.rows, g.cols) : std::min(g.rows, g.cols);
+  // k steps of a tile
+  static int64_t steps_of(int phase, const OrthoGroup& g) {
+    const int k = phase == ORTHO_GRAM ? std::max(g.rows, g.cols) : std::min(g.rows, g.cols);
+    return (g.words == 2 ? 3 : 1) * ((k + FFN_BK - 1) / FFN_BK);
   }
   // The groups' tiles of `side`, the longest sums first.
   void lay(int phase, int side, OrthoPhase& ph) const {
     std::vector<OrthoGroup> g = groups;
     std::stable_sort(g.begin(), g.end(), [&](const OrthoGroup& a, const OrthoGroup& b) {
-      return sum_of(phase, a) > sum_of(phase, b);
+      return steps_of(phase, a) > steps_of(phase, b);
     });
     int64_t tiles = 0;
     for (size_t i = 0; i < g.size(); ++i) {
@@ -194,9 +202,6 @@ struct Pass {
     }
     return us;
   }
-  int64_t steps_of(int phase, const OrthoGroup& g) const {
-    return (words == 2 ? 3 : 1) * ((sum_of(phase, g) + FFN_BK - 1) / FFN_BK);
-  }
   // Which tile, how many of them run in one piece and in how many parts the others:
   // all of them, or those that do not fill a last round.  The join: a launch, and 8
   // bytes a part and element.
@@ -213,7 +218,7 @@ struct Pass {
           if (n == 1 ? whole != 0 : whole == ph.tiles) continue;
           const int rest = ph.tiles - whole;
           if (n > 1 && ((int64_t)rest * n > (big ? 1024 : 2048) ||
-                        2 * n > steps_of(phase, ph.g[ph.groups - 1])))
+                        2 * n > steps_of(phase, ph.g[0])))
             continue;
           double us = n == 1 ? rounds(phase, ph, c, 0, ph.tiles, 1)
                              : rounds(phase, ph, c, 0, whole, 1) +
@@ -247,6 +252,7 @@ struct Pass {
       s.cols = g.cols;
       s.ldx = g.ldx;
       s.first = g.first;
+      s.words = g.words;
       s.x = g.x;
       s.x_step = g.x_step;
       s.vecs = 1;
@@ -282,8 +288,7 @@ struct Pass {
     p.rest = (float)(1.0 - momentum);
     p.nesterov = nesterov;
     k_ortho_norm<<<blocks, 256, 0, st>>>(p);
-    if (words == 2) k_ortho_scale<2><<<blocks, 256, 0, st>>>(p);
-    else k_ortho_scale<1><<<blocks, 256, 0, st>>>(p);
+    k_ortho_scale<<<blocks, 256, 0, st>>>(p);
     SCAO_LAUNCH_CHECK(who);
     OrthoOut out{};
     for (int i = 0; i < n; ++i) {
@@ -293,7 +298,6 @@ struct Pass {
       out.rate[i] = entry(i).rate;
       out.decay[i] = entry(i).decay;
     }
-    const auto product = words == 2 ? ortho_product2 : ortho_product1;
     for (int k = 0; k < steps; ++k) {
       plans[ORTHO_GRAM].ph.by = sc.gram[k];
       plans[ORTHO_SQUARE].ph.by = sc.square[k];
@@ -301,9 +305,8 @@ struct Pass {
       plans[ORTHO_SQUARE].ph.diagonal = sc.diagonal[k];
       plans[ORTHO_UPDATE].ph.by = sc.update[k];
       for (int phase = 0; phase < 3; ++phase) {
-        product(plans[phase].big, phase,
-                phase == ORTHO_UPDATE && k + 1 == steps ? dest : ORTHO_NEXT, plans[phase].ph, out,
-                st);
+        const int to = phase == ORTHO_UPDATE && k + 1 == steps ? dest : ORTHO_NEXT;
+        (plans[phase].big ? ortho_tiles256 : ortho_tiles128)(phase, to, plans[phase].ph, out, st);
         SCAO_LAUNCH_CHECK(who);
       }
       for (Plan& q : plans)
@@ -324,7 +327,8 @@ int for_passes(const std::vector<Matrix>& m, F&& f) {
   std::stable_sort(order.begin(), order.end(), [&](int i, int j) {
     const Matrix &a = m[i], &b = m[j];
     if (a.smaller() != b.smaller()) return a.smaller() > b.smaller();
-    return a.rows != b.rows ? a.rows > b.rows : a.cols > b.cols;
+    if (a.rows != b.rows) return a.rows > b.rows;
+    return a.cols != b.cols ? a.cols > b.cols : a.words > b.words;
   });
   for (size_t i = 0; i < order.size();) {
     const size_t begin = i;
@@ -332,8 +336,7 @@ int for_passes(const std::vector<Matrix>& m, F&& f) {
     int groups = 0;
     while (i < order.size() && i - begin < ORTHO_MATRICES && tiles < PASS_TILES) {
       const Matrix& e = m[order[i]];
-      if (i == begin || e.rows != m[order[i - 1]].rows || e.cols != m[order[i - 1]].cols)
-        if (++groups > ORTHO_GROUPS) break;
+      if ((i == begin || !same_group(e, m[order[i - 1]])) && ++groups > ORTHO_GROUPS) break;
       tiles += e.tiles();
       ++i;
     }
@@ -342,10 +345,12 @@ int for_passes(const std::vector<Matrix>& m, F&& f) {
   return SCAO_OK;
 }
 
-int64_t workspace_of(const std::vector<Matrix>& m, int words, int steps) {
+bool all_small(const std::vector<Matrix>& m, int steps);
+int64_t workspace_of(const std::vector<Matrix>& m, int steps) {
   int64_t most = 0;
+  if (all_small(m, steps)) return 0;
   for_passes(m, [&](const int* order, int n) {
-    Pass p(m.data(), order, n, words, nullptr, steps > 1);
+    Pass p(m.data(), order, n, nullptr, steps > 1);
     for (int phase = 0; phase < 3; ++phase) p.plan(phase);
     most = std::max(most, p.peak);
     return SCAO_OK;
@@ -353,37 +358,93 @@ int64_t workspace_of(const std::vector<Matrix>& m, int words, int steps) {
   return most;
 }
 
+// Whether a workgroup holds every matrix whole: then the call is one launch for up to
+// 64 of them.  (Among larger ones small matrices share those's launches.)
+bool all_small(const std::vector<Matrix>& m, int steps) {
+  if (steps > SMALL_STEPS) return false;
+  for (const Matrix& e : m)
+    if (e.rows && e.cols &&
+        (e.smaller() > SMALL_SIDE || e.larger() > 4096 ||
+         small_lds((int)e.smaller(), (int)e.larger()) > SMALL_LDS))
+      return false;
+  return true;
+}
+int run_small(const char* who, const std::vector<Matrix>& m, const Scales& sc, int steps, double eps,
+              double momentum, bool nesterov, int dest, hipStream_t st) {
+  OrthoSmall p{};
+  for (int k = 0; k < steps; ++k) {
+    p.gram[k] = sc.gram[k];
+    p.square[k] = sc.square[k];
+    p.keep[k] = sc.square_keep[k];
+    p.diagonal[k] = sc.diagonal[k];
+    p.update[k] = sc.update[k];
+  }
+  p.steps = steps;
+  p.eps = eps;
+  p.scale = sc.first;
+  p.momentum = (float)momentum;
+  p.rest = (float)(1.0 - momentum);
+  p.nesterov = nesterov;
+  for (size_t i = 0; i < m.size();) {
+    int n = 0, lds = 0;
+    for (; i < m.size() && n < ORTHO_MATRICES; ++i) {
+      const Matrix& e = m[i];
+      if (!e.rows || !e.cols) continue;
+      p.src[n] = e.src;
+      p.buf[n] = e.buf;
+      p.dst[n] = e.dst;
+      p.rows[n] = (int)e.rows;
+      p.cols[n] = (int)e.cols;
+      p.ld_src[n] = (int)e.ld_src;
+      p.ld_dst[n] = (int)e.ld_dst;
+      p.rate[n] = e.rate;
+      p.decay[n] = e.decay;
+      p.src_dt[n] = (uint8_t)e.src_dtype;
+      p.dst_dt[n] = (uint8_t)e.dst_dtype;
+      lds = std::max(lds, small_lds((int)e.smaller(), (int)e.larger()));
+      ++n;
+    }
+    if (!n) break;
+    if (dest == ORTHO_RESULT) k_ortho_small<ORTHO_RESULT><<<n, SMALL_THREADS, lds, st>>>(p);
+    else k_ortho_small<ORTHO_PARAMETER><<<n, SMALL_THREADS, lds, st>>>(p);
+    SCAO_LAUNCH_CHECK(who);
+  }
+  return SCAO_OK;
+}
+
 int run_all(const char* who, const std::vector<Matrix>& m, const double* coefficients, int steps,
-            double eps, int words, double momentum, bool nesterov, int dest, void* workspace,
+            double eps, double momentum, bool nesterov, int dest, void* workspace,
             void* stream) {
   Scales sc;
   SCAO_CHECK_ARG(scales_of(coefficients, steps, sc),
                  "%s: with these coefficients singular values may grow beyond 1024", who);
+  if (all_small(m, steps))
+    return run_small(who, m, sc, steps, eps, momentum, nesterov, dest, (hipStream_t)stream);
   SCAO_CHECK_ARG((uintptr_t)workspace % 16 == 0, "%s: workspace is not aligned", who);
   return for_passes(m, [&](const int* order, int n) -> int {
     SCAO_CHECK_ARG(workspace, "%s: null workspace", who);
-    Pass p(m.data(), order, n, words, (char*)workspace, steps > 1);
+    Pass p(m.data(), order, n, (char*)workspace, steps > 1);
     return p.run(who, sc, steps, eps, momentum, nesterov, dest, (hipStream_t)stream);
   });
 }
 
 int check_scheme(const char* who, int n, const void* table, const double* coefficients, int steps,
-                 double eps, int precision) {
+                 double eps) {
   SCAO_CHECK_ARG(n >= 0 && (n == 0 || table), "%s: null table or negative count", who);
   SCAO_CHECK_ARG(steps >= 1 && steps <= MAX_STEPS, "%s: %d steps (1 to %d)", who, steps, MAX_STEPS);
   SCAO_CHECK_ARG(coefficients, "%s: null coefficients", who);
   for (int i = 0; i < 3 * steps; ++i)
     SCAO_CHECK_ARG(std::isfinite(coefficients[i]), "%s: coefficient %d is no finite number", who, i);
   SCAO_CHECK_ARG(eps > 0 && std::isfinite(eps), "%s: eps %g is not positive and finite", who, eps);
-  SCAO_CHECK_ARG(precision == SCAO_ORTHO_FAST || precision == SCAO_ORTHO_FP32, "%s: precision %d",
-                 who, precision);
   return SCAO_OK;
 }
-int check_sizes(const char* who, int i, int64_t rows, int64_t cols) {
+int check_sizes(const char* who, int i, int64_t rows, int64_t cols, int precision) {
   SCAO_CHECK_ARG(rows >= 0 && cols >= 0 && std::max(rows, cols) < MAX_SIDE &&
                      std::min(rows, cols) <= MAX_SMALLER,
                  "%s: matrix %d is %lld x %lld (sides below 2^20, the smaller one up to 2^15)", who,
                  i, (long long)rows, (long long)cols);
+  SCAO_CHECK_ARG(precision == SCAO_ORTHO_FAST || precision == SCAO_ORTHO_FP32,
+                 "%s: precision %d of matrix %d", who, precision, i);
   return SCAO_OK;
 }
 int check_matrix(const char* who, int i, const char* name, const void* p, int64_t rows, int64_t cols,
@@ -395,6 +456,13 @@ int check_matrix(const char* who, int i, const char* name, const void* p, int64_
                  "%s: row stride %lld of %s of matrix %d (%lld columns)", who, (long long)ld, name,
                  i, (long long)cols);
   return SCAO_OK;
+}
+
+// Words of an element.  Up to 128 rows or columns two in any case: a tile's beginning
+// and end are most of such a product, and one word's roundings spread over the fewer
+// singular values (results of 64 x 64 1.5e-3 off, of 1024 x 1024 1.2e-3).
+int words_of(int precision, int64_t rows, int64_t cols) {
+  return precision == SCAO_ORTHO_FP32 || std::min(rows, cols) <= 128 ? 2 : 1;
 }
 
 // what a call writes may not be what it writes or reads elsewhere
@@ -422,7 +490,7 @@ Range range_of(const void* p, int64_t rows, int64_t cols, int64_t ld, int dtype,
 int collect(const char* who, const scao_ortho_desc* t, int n, bool pointers, std::vector<Matrix>& m) {
   std::vector<Range> r;
   for (int i = 0; i < n; ++i) {
-    if (int rc = check_sizes(who, i, t[i].rows, t[i].cols)) return rc;
+    if (int rc = check_sizes(who, i, t[i].rows, t[i].cols, t[i].precision)) return rc;
     if (pointers && t[i].rows && t[i].cols) {
       if (int rc = check_matrix(who, i, "src", t[i].src, t[i].rows, t[i].cols, t[i].ld_src,
                                 t[i].src_dtype))
@@ -436,7 +504,8 @@ int collect(const char* who, const scao_ortho_desc* t, int n, bool pointers, std
     const int64_t one = t[i].cols;   // a single row's stride is never used
     m.push_back({t[i].src, nullptr, t[i].dst, t[i].rows, t[i].cols,
                  t[i].rows == 1 ? one : t[i].ld_src, t[i].rows == 1 ? one : t[i].ld_dst,
-                 t[i].src_dtype, t[i].dst_dtype, 0.f, 0.f});
+                 t[i].src_dtype, t[i].dst_dtype, 0.f, 0.f,
+                 words_of(t[i].precision, t[i].rows, t[i].cols)});
   }
   return check_apart(who, r);
 }
@@ -444,7 +513,7 @@ int collect(const char* who, const scao_muon_desc* t, int n, bool pointers, std:
   std::vector<Range> r;
   for (int i = 0; i < n; ++i) {
     const auto [rows, cols] = std::pair(t[i].rows, t[i].cols);
-    if (int rc = check_sizes(who, i, rows, cols)) return rc;
+    if (int rc = check_sizes(who, i, rows, cols, t[i].precision)) return rc;
     if (pointers && rows && cols) {
       if (int rc = check_matrix(who, i, "p", t[i].p, rows, cols, cols, t[i].dtype)) return rc;
       if (int rc = check_matrix(who, i, "g", t[i].g, rows, cols, cols, t[i].grad_dtype)) return rc;
@@ -456,12 +525,10 @@ int collect(const char* who, const scao_muon_desc* t, int n, bool pointers, std:
       r.push_back(range_of(t[i].m, rows, cols, cols, SCAO_F32, true));
     }
     m.push_back({t[i].g, t[i].m, t[i].p, rows, cols, cols, cols, t[i].grad_dtype, t[i].dtype,
-                 t[i].rate, t[i].decay});
+                 t[i].rate, t[i].decay, words_of(t[i].precision, rows, cols)});
   }
   return check_apart(who, r);
 }
-int words_of(int precision) { return precision == SCAO_ORTHO_FP32 ? 2 : 1; }
-
 }  // namespace
 
 namespace {
@@ -477,49 +544,47 @@ T guarded(const char* who, int n, T failed, F&& f) {
 }
 }  // namespace
 
-extern "C" int64_t scao_orthogonalize_workspace(const scao_ortho_desc* matrices, int n, int steps,
-                                                int precision) {
+extern "C" int64_t scao_orthogonalize_workspace(const scao_ortho_desc* matrices, int n, int steps) {
   const char* who = "scao_orthogonalize_workspace";
   return guarded<int64_t>(who, n, 0, [&]() -> int64_t {
     std::vector<Matrix> m;
     if (n <= 0 || !matrices || collect(who, matrices, n, false, m)) return 0;
-    return workspace_of(m, words_of(precision), steps);
+    return workspace_of(m, steps);
   });
 }
 
 extern "C" int scao_orthogonalize(const scao_ortho_desc* matrices, int n,
-                                  const double* coefficients, int steps, double eps, int precision,
+                                  const double* coefficients, int steps, double eps,
                                   void* workspace, void* stream) {
   const char* who = "scao_orthogonalize";
   return guarded<int>(who, n, SCAO_ERR_INVALID, [&]() -> int {
-    if (int rc = check_scheme(who, n, matrices, coefficients, steps, eps, precision)) return rc;
+    if (int rc = check_scheme(who, n, matrices, coefficients, steps, eps)) return rc;
     std::vector<Matrix> m;
     if (int rc = collect(who, matrices, n, true, m)) return rc;
-    return run_all(who, m, coefficients, steps, eps, words_of(precision), 0.0, false, ORTHO_RESULT,
+    return run_all(who, m, coefficients, steps, eps, 0.0, false, ORTHO_RESULT,
                    workspace, stream);
   });
 }
 
-extern "C" int64_t scao_muon_workspace(const scao_muon_desc* matrices, int n, int steps,
-                                       int precision) {
+extern "C" int64_t scao_muon_workspace(const scao_muon_desc* matrices, int n, int steps) {
   const char* who = "scao_muon_workspace";
   return guarded<int64_t>(who, n, 0, [&]() -> int64_t {
     std::vector<Matrix> m;
     if (n <= 0 || !matrices || collect(who, matrices, n, false, m)) return 0;
-    return workspace_of(m, words_of(precision), steps);
+    return workspace_of(m, steps);
   });
 }
 
 extern "C" int scao_muon_step(const scao_muon_desc* matrices, int n, double momentum, int nesterov,
-                              const double* coefficients, int steps, double eps, int precision,
+                              const double* coefficients, int steps, double eps,
                               void* workspace, void* stream) {
   const char* who = "scao_muon_step";
   return guarded<int>(who, n, SCAO_ERR_INVALID, [&]() -> int {
-    if (int rc = check_scheme(who, n, matrices, coefficients, steps, eps, precision)) return rc;
+    if (int rc = check_scheme(who, n, matrices, coefficients, steps, eps)) return rc;
     SCAO_CHECK_ARG(momentum >= 0 && momentum < 1, "%s: momentum %g is not in [0, 1)", who, momentum);
     std::vector<Matrix> m;
     if (int rc = collect(who, matrices, n, true, m)) return rc;
-    return run_all(who, m, coefficients, steps, eps, words_of(precision), momentum, nesterov != 0,
+    return run_all(who, m, coefficients, steps, eps, momentum, nesterov != 0,
                    ORTHO_PARAMETER, workspace, stream);
   });
 }

@@ -9,7 +9,7 @@
 // the diagonal are computed and the others stored as their mirror image.
 //
 // Words of the products.  X, A and B are fp16 (or, P = 2, a sum of two fp16 words,
-// 22 significant bits, multiplied as three products of words), scaled by powers of
+// 22 significant bits, multiplied as three products of words; a group's choice), scaled by powers of
 // two that the host chooses from what the polynomial can reach, so that neither end
 // of fp16's range matters: |X|, |A| and |B| are bounded by their largest singular
 // value.  fp16 has three bits more than bf16 at the same rate; each of the three is
@@ -38,6 +38,7 @@ struct OrthoGroup {
   int64_t x_step, a_step;    // bytes from a matrix's X to the next one's; of A and B
   int rows, cols, ldx, lda;
   int first, count;          // entries of the pass's tables
+  int words;                 // 1 or 2
   int per, tiles_m, tiles_n; // tiles of a matrix
   int tile0;                 // tiles of the groups before
 };
@@ -376,18 +377,12 @@ __device__ __forceinline__ void ortho_tile(char* smem, const OrthoPhase& ph, con
 }
 
 template <int P, int BM, int PHASE, int DEST>
-__global__ __launch_bounds__(BM * 2, 2) void k_ortho(const OrthoPhase ph, const OrthoOut out) {
+__device__ __forceinline__ void ortho_product(char* smem, const OrthoPhase& ph, const OrthoOut& out,
+                                              const OrthoGroup& g, int matrix, int tm, int tn,
+                                              int tile, int part) {
   using RR = OrthoGemm<BM, ROWS, ROWS>;
   using RC = OrthoGemm<BM, ROWS, COLS>;
   using CC = OrthoGemm<BM, COLS, COLS>;
-  static_assert(RR::THREADS == BM * 2, "a wave for every 32 rows");
-  __shared__ __attribute__((aligned(1024))) char smem[RR::LDS];
-  const int b = blockIdx.x, rest = ph.tiles - ph.whole;
-  const int part = b < ph.whole ? -1 : (b - ph.whole) / rest;
-  const int tile = part < 0 ? b : ph.whole + (b - ph.whole) % rest;
-  const OrthoGroup& g = ph.g[ortho_group_of(ph, tile)];
-  int matrix, tm, tn;
-  ortho_tile_of(g, PHASE != ORTHO_UPDATE, tile - g.tile0, matrix, tm, tn);
   const char* x = ph.base + matrix * g.x_step + g.x;
   const char* a = ph.base + matrix * g.a_step + (PHASE == ORTHO_SQUARE ? g.a : g.b);
   const bool wide = g.rows <= g.cols;
@@ -409,9 +404,27 @@ __global__ __launch_bounds__(BM * 2, 2) void k_ortho(const OrthoPhase ph, const 
     ortho_tile<RR, P, PHASE, DEST>(smem, ph, out, g, o, matrix, tm, tn, tile, part);
   }
 }
+template <int BM, int PHASE, int DEST>
+__global__ __launch_bounds__(BM * 2, 2) void k_ortho(const OrthoPhase ph, const OrthoOut out) {
+  using G = OrthoGemm<BM, ROWS, ROWS>;
+  static_assert(G::THREADS == BM * 2, "a wave for every 32 rows");
+  __shared__ __attribute__((aligned(1024))) char smem[G::LDS];
+  const int b = blockIdx.x, rest = ph.tiles - ph.whole;
+  const int part = b < ph.whole ? -1 : (b - ph.whole) / rest;
+  const int tile = part < 0 ? b : ph.whole + (b - ph.whole) % rest;
+  const OrthoGroup& g = ph.g[ortho_group_of(ph, tile)];
+  int matrix, tm, tn;
+  ortho_tile_of(g, PHASE != ORTHO_UPDATE, tile - g.tile0, matrix, tm, tn);
+  if (g.words == 2) ortho_product<2, BM, PHASE, DEST>(smem, ph, out, g, matrix, tm, tn, tile, part);
+  else ortho_product<1, BM, PHASE, DEST>(smem, ph, out, g, matrix, tm, tn, tile, part);
+}
 
 // The parts of split tiles, added in order: a wave takes two fragments.
-template <int P, int BM, int PHASE, int DEST>
+template <int P>
+struct OrthoWordCount {
+  static constexpr int value = P;
+};
+template <int BM, int PHASE, int DEST>
 __global__ __launch_bounds__(256) void k_ortho_join(const OrthoPhase ph, const OrthoOut out) {
   constexpr int F = BM / 16, PAIRS = F * F / 2;   // of a tile
   const int64_t at = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6);
@@ -422,13 +435,10 @@ __global__ __launch_bounds__(256) void k_ortho_join(const OrthoPhase ph, const O
   int matrix, tm, tn;
   ortho_tile_of(g, PHASE != ORTHO_UPDATE, tile - g.tile0, matrix, tm, tn);
   const OrthoTarget t = ortho_target<PHASE>(ph, g, matrix, tm > tn);
-  const OrthoPlace to = ortho_place<DEST>(out, g.first + matrix);
   const int fm = in / (F / 2), fn = in % (F / 2) * 2;
   const int m = tm * BM + fm * 16 + (lane & 15), n = tn * BM + fn * 16;
   // (whole fragments outside; the mirror image's padding columns are C's rows)
   if (tm * BM + fm * 16 >= ((t.M + 7) & ~7) || n >= t.cols) return;
-  OrthoPair<P, PHASE> add;
-  add.load(t, m, n, lane);
   const gv4f_a16* p = (const gv4f_a16*)ph.partial +
                       ((int64_t)(tile - ph.whole) * F * F + fm * F + fn) * 64 + lane;
   const int64_t all = (int64_t)rest * F * F * 64;
@@ -449,36 +459,36 @@ __global__ __launch_bounds__(256) void k_ortho_join(const OrthoPhase ph, const O
         d += pd[i];
       }
   }
-  ortho_finish<P, PHASE, DEST>(ph, to, t, add, m, n, lane, c, d);
+  const OrthoPlace to = ortho_place<DEST>(out, g.first + matrix);
+  auto finish = [&](auto words) {
+    constexpr int P = decltype(words)::value;
+    OrthoPair<P, PHASE> add;
+    add.load(t, m, n, lane);
+    ortho_finish<P, PHASE, DEST>(ph, to, t, add, m, n, lane, c, d);
+  };
+  if (g.words == 2) finish(OrthoWordCount<2>{});
+  else finish(OrthoWordCount<1>{});
 }
 
 // --------------------------------------------------------- launches --------
-template <int P, int BM, int PHASE, int DEST>
+template <int BM, int PHASE, int DEST>
 void ortho_launch(const OrthoPhase& ph, const OrthoOut& out, hipStream_t st) {
   const int rest = ph.tiles - ph.whole;
-  k_ortho<P, BM, PHASE, DEST><<<ph.whole + rest * ph.splits, BM * 2, 0, st>>>(ph, out);
+  k_ortho<BM, PHASE, DEST><<<ph.whole + rest * ph.splits, BM * 2, 0, st>>>(ph, out);
   if (rest)
-    k_ortho_join<P, BM, PHASE, DEST>
+    k_ortho_join<BM, PHASE, DEST>
         <<<(int)(((int64_t)rest * (BM / 16) * (BM / 16) / 2 + 3) / 4), 256, 0, st>>>(ph, out);
 }
-template <int P, int BM>
+template <int BM>
 void ortho_launch(int phase, int dest, const OrthoPhase& ph, const OrthoOut& out, hipStream_t st) {
-  if (phase == ORTHO_GRAM) ortho_launch<P, BM, ORTHO_GRAM, ORTHO_NEXT>(ph, out, st);
-  else if (phase == ORTHO_SQUARE) ortho_launch<P, BM, ORTHO_SQUARE, ORTHO_NEXT>(ph, out, st);
-  else if (dest == ORTHO_NEXT) ortho_launch<P, BM, ORTHO_UPDATE, ORTHO_NEXT>(ph, out, st);
-  else if (dest == ORTHO_RESULT) ortho_launch<P, BM, ORTHO_UPDATE, ORTHO_RESULT>(ph, out, st);
-  else ortho_launch<P, BM, ORTHO_UPDATE, ORTHO_PARAMETER>(ph, out, st);
+  if (phase == ORTHO_GRAM) ortho_launch<BM, ORTHO_GRAM, ORTHO_NEXT>(ph, out, st);
+  else if (phase == ORTHO_SQUARE) ortho_launch<BM, ORTHO_SQUARE, ORTHO_NEXT>(ph, out, st);
+  else if (dest == ORTHO_NEXT) ortho_launch<BM, ORTHO_UPDATE, ORTHO_NEXT>(ph, out, st);
+  else if (dest == ORTHO_RESULT) ortho_launch<BM, ORTHO_UPDATE, ORTHO_RESULT>(ph, out, st);
+  else ortho_launch<BM, ORTHO_UPDATE, ORTHO_PARAMETER>(ph, out, st);
 }
-template <int P>
-void ortho_product(int big, int phase, int dest, const OrthoPhase& ph, const OrthoOut& out,
-                   hipStream_t st) {
-  if (big) ortho_launch<P, 256>(phase, dest, ph, out, st);
-  else ortho_launch<P, 128>(phase, dest, ph, out, st);
-}
-// instantiated in ortho_words1.hip and ortho_words2.hip
-void ortho_product1(int big, int phase, int dest, const OrthoPhase& ph, const OrthoOut& out,
-                    hipStream_t st);
-void ortho_product2(int big, int phase, int dest, const OrthoPhase& ph, const OrthoOut& out,
-                    hipStream_t st);
+// instantiated in ortho_tiles128.hip and ortho_tiles256.hip
+void ortho_tiles128(int phase, int dest, const OrthoPhase& ph, const OrthoOut& out, hipStream_t st);
+void ortho_tiles256(int phase, int dest, const OrthoPhase& ph, const OrthoOut& out, hipStream_t st);
 
 }  // namespace scao

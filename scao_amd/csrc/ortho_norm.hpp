@@ -14,7 +14,7 @@ namespace scao {
 // row, or several short rows; a workgroup takes `per` units of one matrix.
 struct OrthoSource {
   int rows, cols, ldx;
-  int first;                 // entry of the tables
+  int first, words;          // entry of the tables; 1 or 2 words an element
   int vecs;                  // vectors of a row side by side in a unit (a power of two)
   int across, per, parts;    // units a row, units a workgroup, workgroups a matrix
   int block0;                // workgroups of the groups before
@@ -153,18 +153,8 @@ __global__ __launch_bounds__(256) void k_ortho_norm(const OrthoPrep p) {
 
 // X, with zeros up to its row stride's end; NaN throughout where the norm is none
 template <int P>
-__global__ __launch_bounds__(256) void k_ortho_scale(const OrthoPrep p) {
-  __shared__ double lds[4], total;
-  int matrix, part;
-  const OrthoSource& g = ortho_source(p, matrix, part);
-  double s[1] = {0.0};
-  for (int i = threadIdx.x; i < g.parts; i += 256)
-    s[0] += p.norms[(g.first + matrix) * ORTHO_PARTS + i];
-  block_sum(s, lds);
-  if (threadIdx.x == 0) total = s[0];
-  __syncthreads();
-  const double norm = sqrt(total);
-  const double scale = norm <= 1.7976931348623157e308 ? p.scale / (norm + p.eps) : norm - norm;
+__device__ __forceinline__ void ortho_scale(const OrthoPrep& p, const OrthoSource& g, int matrix,
+                                            int part, double scale) {
   uint16_t* x = (uint16_t*)(p.base + g.x + matrix * g.x_step);
   const int64_t plane = (int64_t)g.rows * g.ldx;
   ortho_walk<false>(p, g, matrix, part, g.ldx, [&](int r, int c, const OrthoVector& u) {
@@ -182,6 +172,21 @@ __global__ __launch_bounds__(256) void k_ortho_scale(const OrthoPrep p) {
       *(gv4u_a16*)(x + (int64_t)r * g.ldx + c + i * plane) =
           v4u_t{w[0][i][0], w[0][i][1], w[1][i][0], w[1][i][1]};
   });
+}
+__global__ __launch_bounds__(256) void k_ortho_scale(const OrthoPrep p) {
+  __shared__ double lds[4], total;
+  int matrix, part;
+  const OrthoSource& g = ortho_source(p, matrix, part);
+  double s[1] = {0.0};
+  for (int i = threadIdx.x; i < g.parts; i += 256)
+    s[0] += p.norms[(g.first + matrix) * ORTHO_PARTS + i];
+  block_sum(s, lds);
+  if (threadIdx.x == 0) total = s[0];
+  __syncthreads();
+  const double norm = sqrt(total);
+  const double scale = norm <= 1.7976931348623157e308 ? p.scale / (norm + p.eps) : norm - norm;
+  if (g.words == 2) ortho_scale<2>(p, g, matrix, part, scale);
+  else ortho_scale<1>(p, g, matrix, part, scale);
 }
 
 }  // namespace scao

@@ -29,6 +29,7 @@
 #include <torch/library.h>
 
 #include <algorithm>
+#include <cmath>
 #include <cstring>
 
 #include "../../include/scao_train.h"
@@ -576,20 +577,20 @@ PyObject* grad_clip(PyObject*, PyObject* const* args, Py_ssize_t n) {
 //   orthogonalize  fresh results of one type
 //   muon_step_     parameters and momenta written in place
 std::vector<Tensor> op_orthogonalize(at::TensorList updates, at::ArrayRef<double> coefficients,
-                                     double eps, at::ScalarType dtype, int64_t precision) {
+                                     double eps, std::optional<at::ScalarType> dtype) {
   static const auto op = c10::Dispatcher::singleton()
                              .findSchemaOrThrow("scao_amd::orthogonalize", "")
                              .typed<decltype(op_orthogonalize)>();
-  return op.call(updates, coefficients, eps, dtype, precision);
+  return op.call(updates, coefficients, eps, dtype);
 }
 void op_muon_step_(at::TensorList params, at::TensorList grads, at::TensorList momenta,
                    at::ArrayRef<double> rates, at::ArrayRef<double> decays, double momentum,
                    bool nesterov, at::ArrayRef<double> coefficients, double eps,
-                   int64_t precision) {
+                   at::IntArrayRef precisions) {
   static const auto op = c10::Dispatcher::singleton()
                              .findSchemaOrThrow("scao_amd::muon_step_", "")
                              .typed<decltype(op_muon_step_)>();
-  op.call(params, grads, momenta, rates, decays, momentum, nesterov, coefficients, eps, precision);
+  op.call(params, grads, momenta, rates, decays, momentum, nesterov, coefficients, eps, precisions);
 }
 
 void check_matrices(at::TensorList list, const char* name, c10::Device on) {
@@ -634,29 +635,32 @@ Tensor row_strided(const Tensor& t) {
 }
 
 std::vector<Tensor> orthogonalize_hip(at::TensorList updates, at::ArrayRef<double> coefficients,
-                                      double eps, at::ScalarType dtype, int64_t precision) {
+                                      double eps, std::optional<at::ScalarType> dtype) {
   check_scheme(coefficients);
   std::vector<Tensor> out;
   if (updates.empty()) return out;
   check_matrices(updates, "updates", updates[0].device());
-  TORCH_CHECK(code_of(dtype) >= 0, "orthogonalize: no result of type ", dtype);
+  TORCH_CHECK(!dtype || code_of(*dtype) >= 0, "orthogonalize: no result of type ", *dtype);
   const c10::DeviceGuard guard(updates[0].device());
   std::vector<Tensor> in;
   std::vector<scao_ortho_desc> table;
   for (const Tensor& t : updates) {
     in.push_back(row_strided(t.resolve_neg()));
-    out.push_back(at::empty(t.sizes(), t.options().dtype(dtype)));
+    const at::ScalarType type = dtype.value_or(t.scalar_type());
+    out.push_back(at::empty(t.sizes(), t.options().dtype(type)));
+    // one word an element where the result has fewer bits than it
+    const int precision = type == at::kBFloat16 ? SCAO_ORTHO_FAST : SCAO_ORTHO_FP32;
     char* to = (char*)out.back().data_ptr();
     for_matrices(in.back(), [&](char* p, int64_t rows, int64_t cols, int64_t ld) {
-      table.push_back({p, to, rows, cols, ld, cols, code_of(t.scalar_type()), code_of(dtype)});
+      table.push_back({p, to, rows, cols, ld, cols, code_of(t.scalar_type()), code_of(type),
+                       precision, 0});
       to += rows * cols * (int64_t)out.back().element_size();
     });
   }
   const int steps = (int)coefficients.size() / 3, n = (int)table.size();
-  const Tensor work =
-      bytes(lib.orthogonalize_workspace(table.data(), n, steps, (int)precision), updates[0]);
-  check(lib.orthogonalize(table.data(), n, coefficients.data(), steps, eps, (int)precision,
-                          work.data_ptr(), stream_of(updates[0])),
+  const Tensor work = bytes(lib.orthogonalize_workspace(table.data(), n, steps), updates[0]);
+  check(lib.orthogonalize(table.data(), n, coefficients.data(), steps, eps, work.data_ptr(),
+                          stream_of(updates[0])),
         "scao_orthogonalize");
   return out;
 }
@@ -664,10 +668,11 @@ std::vector<Tensor> orthogonalize_hip(at::TensorList updates, at::ArrayRef<doubl
 void muon_step_hip_(at::TensorList params, at::TensorList grads, at::TensorList momenta,
                     at::ArrayRef<double> rates, at::ArrayRef<double> decays, double momentum,
                     bool nesterov, at::ArrayRef<double> coefficients, double eps,
-                    int64_t precision) {
+                    at::IntArrayRef precisions) {
   check_scheme(coefficients);
   const size_t n = params.size();
-  TORCH_CHECK(grads.size() == n && momenta.size() == n && rates.size() == n && decays.size() == n,
+  TORCH_CHECK(grads.size() == n && momenta.size() == n && rates.size() == n && decays.size() == n &&
+                  precisions.size() == n,
               "muon_step_: lists of different lengths");
   if (!n) return;
   const c10::Device on = params[0].device();
@@ -688,26 +693,27 @@ void muon_step_hip_(at::TensorList params, at::TensorList grads, at::TensorList 
     const int64_t g_size = (int64_t)copies.back().element_size();
     for_matrices(p, [&](char* at, int64_t rows, int64_t cols, int64_t) {
       table.push_back({at, g, buf, rows, cols, code_of(p.scalar_type()),
-                       code_of(copies.back().scalar_type()), (float)rates[i], (float)decays[i]});
+                       code_of(copies.back().scalar_type()), (float)rates[i], (float)decays[i],
+                       (int32_t)precisions[i], 0});
       g += rows * cols * g_size;
       buf += rows * cols;
     });
   }
   const int steps = (int)coefficients.size() / 3, many = (int)table.size();
-  const Tensor work = bytes(lib.muon_workspace(table.data(), many, steps, (int)precision), params[0]);
+  const Tensor work = bytes(lib.muon_workspace(table.data(), many, steps), params[0]);
   check(lib.muon_step(table.data(), many, momentum, nesterov, coefficients.data(), steps, eps,
-                      (int)precision, work.data_ptr(), stream_of(params[0])),
+                      work.data_ptr(), stream_of(params[0])),
         "scao_muon_step");
 }
 // a graph that holds a parameter has to see that it changed
 void muon_step_version_(at::TensorList params, at::TensorList grads, at::TensorList momenta,
                         at::ArrayRef<double> rates, at::ArrayRef<double> decays, double momentum,
                         bool nesterov, at::ArrayRef<double> coefficients, double eps,
-                        int64_t precision) {
+                        at::IntArrayRef precisions) {
   {
     const at::AutoDispatchBelowADInplaceOrView below;
     op_muon_step_(params, grads, momenta, rates, decays, momentum, nesterov, coefficients, eps,
-                  precision);
+                  precisions);
   }
   for (const at::TensorList list : {params, momenta})
     for (const Tensor& t : list)
@@ -715,17 +721,17 @@ void muon_step_version_(at::TensorList params, at::TensorList grads, at::TensorL
 }
 
 std::vector<Tensor> orthogonalize_meta(at::TensorList updates, at::ArrayRef<double> coefficients,
-                                       double, at::ScalarType dtype, int64_t) {
+                                       double, std::optional<at::ScalarType> dtype) {
   check_scheme(coefficients);
   std::vector<Tensor> out;
   if (!updates.empty()) check_matrices(updates, "updates", updates[0].device());
   for (const Tensor& t : updates)
-    out.push_back(at::empty_symint(t.sym_sizes(), t.options().dtype(dtype)));
+    out.push_back(at::empty_symint(t.sym_sizes(), t.options().dtype(dtype.value_or(t.scalar_type()))));
   return out;
 }
 void muon_step_meta_(at::TensorList params, at::TensorList, at::TensorList, at::ArrayRef<double>,
                      at::ArrayRef<double>, double, bool, at::ArrayRef<double> coefficients, double,
-                     int64_t) {
+                     at::IntArrayRef) {
   check_scheme(coefficients);
   if (!params.empty()) check_matrices(params, "parameters", params[0].device());
 }
@@ -738,21 +744,21 @@ bool tangent(at::TensorList list) {
 }
 std::vector<Tensor> orthogonalize_autograd(at::TensorList updates,
                                            at::ArrayRef<double> coefficients, double eps,
-                                           at::ScalarType dtype, int64_t precision) {
+                                           std::optional<at::ScalarType> dtype) {
   bool wanted = tangent(updates);
   if (at::GradMode::is_enabled())
     for (const Tensor& t : updates) wanted = wanted || t.requires_grad();
   TORCH_CHECK_NOT_IMPLEMENTED(!wanted, "orthogonalize has no derivative: detach the updates");
   const at::AutoDispatchBelowADInplaceOrView below;
-  return op_orthogonalize(updates, coefficients, eps, dtype, precision);
+  return op_orthogonalize(updates, coefficients, eps, dtype);
 }
 
 TORCH_LIBRARY_FRAGMENT(scao_amd, m) {
-  m.def("orthogonalize(Tensor[] updates, float[] coefficients, float eps, ScalarType dtype, "
-        "int precision) -> Tensor[]");
+  m.def("orthogonalize(Tensor[] updates, float[] coefficients, float eps, ScalarType? dtype) "
+        "-> Tensor[]");
   m.def("muon_step_(Tensor(a!)[] params, Tensor[] grads, Tensor(b!)[] momenta, float[] rates, "
         "float[] decays, float momentum, bool nesterov, float[] coefficients, float eps, "
-        "int precision) -> ()");
+        "int[] precisions) -> ()");
 }
 TORCH_LIBRARY_IMPL(scao_amd, CUDA, m) {
   m.impl("orthogonalize", orthogonalize_hip);
@@ -791,7 +797,7 @@ std::vector<double> numbers(PyObject* list) {
   return out;
 }
 // muon_step(parameters, gradients, momenta, rates, decays, momentum, nesterov,
-// coefficients, eps, precision)
+// coefficients, eps, precisions)
 PyObject* muon_step(PyObject*, PyObject* const* args, Py_ssize_t n) {
   HANDLE_TH_ERRORS
   TORCH_CHECK_TYPE(n == 10, "muon_step() takes ten arguments");
@@ -801,11 +807,12 @@ PyObject* muon_step(PyObject*, PyObject* const* args, Py_ssize_t n) {
                             coefficients = numbers(args[7]);
   const double momentum = PyFloat_AsDouble(args[5]), eps = PyFloat_AsDouble(args[8]);
   const int nesterov = PyObject_IsTrue(args[6]);
-  const long precision = PyLong_AsLong(args[9]);
+  std::vector<int64_t> precisions;
+  for (const double p : numbers(args[9])) precisions.push_back((int64_t)p);
   if (PyErr_Occurred()) return nullptr;
   const at::AutoDispatchBelowAutograd below;
   op_muon_step_(params, grads, momenta, rates, decays, momentum, nesterov != 0, coefficients, eps,
-                precision);
+                precisions);
   Py_RETURN_NONE;
   END_HANDLE_TH_ERRORS
 }
@@ -851,6 +858,10 @@ void check_rope(ROPE_PARAMS) {
                   cos.sym_sizes() == sin.sym_sizes() && cos.sym_size(1) * 2 <= q.sym_size(3),
               "qk_norm_rope: cos and sin must be float32 tables of at most half a head's columns "
               "on q's device");
+  TORCH_CHECK(eps >= 0 && std::isfinite(eps), "qk_norm_rope: eps ", eps);
+  TORCH_CHECK(positions || cos.sym_size(1) == 0 || q.sym_size(1) <= cos.sym_size(0),
+              "qk_norm_rope: ", q.sym_size(1), " tokens and tables of ", cos.sym_size(0),
+              " positions");
   TORCH_CHECK(!positions || (on(*positions) && positions->dim() == 2 &&
                              (positions->scalar_type() == at::kLong ||
                               positions->scalar_type() == at::kInt) &&

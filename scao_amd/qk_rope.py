@@ -103,19 +103,23 @@ def qk_norm_rope(q: Tensor, k: Tensor, q_weight: Optional[Tensor], k_weight: Opt
     once in q, k and the weights, not in the tables, and not in forward mode.  A head
     with a NaN or an infinity gives NaN there (an infinity: zeros beside it), in its
     gradient and in the weight's, and in no other head."""
-    _check(q, k, q_weight, k_weight, cos, sin, positions, eps)
+    rest = q_weight, k_weight, cos, sin
+    if q.ndim == 4 and q.is_cuda:
+        # the operator checks for itself, in a sixth of the time; what it refuses is
+        # looked at again for the error's type and words
+        try:
+            return L.torch_host().qk_norm_rope(q, k, *rest, positions, eps, interleaved)
+        except (RuntimeError, TypeError):
+            _check(q, k, *rest, positions, eps)
+            raise
+    _check(q, k, *rest, positions, eps)
     lead = q.shape[:-2]
-    if len(lead) != 2:
-        tokens = lead[-1] if lead else 1
-        many = math.prod(lead[:-1])
-        q, k = (t.reshape(many, tokens, *t.shape[-2:]) for t in (q, k))
-        if positions is not None:
-            positions = positions.reshape(many, tokens)
-    yq, yk = L.torch_host().qk_norm_rope(q, k, q_weight, k_weight, cos, sin, positions, float(eps),
-                                         bool(interleaved))
-    if len(lead) != 2:
-        yq, yk = yq.reshape(*lead, *yq.shape[-2:]), yk.reshape(*lead, *yk.shape[-2:])
-    return yq, yk
+    tokens, many = lead[-1] if lead else 1, math.prod(lead[:-1])
+    q, k = (t.reshape(many, tokens, *t.shape[-2:]) for t in (q, k))
+    if positions is not None:
+        positions = positions.reshape(many, tokens)
+    yq, yk = L.torch_host().qk_norm_rope(q, k, *rest, positions, eps, interleaved)
+    return yq.reshape(*lead, *yq.shape[-2:]), yk.reshape(*lead, *yk.shape[-2:])
 
 
 class QKNormRope(nn.Module):

@@ -121,14 +121,14 @@ def _call(mats, dst, precision, coefficients, eps=1e-7):
     table = np.zeros(len(mats), dtype=L.ORTHO_DESC)
     for i, (s, d) in enumerate(zip(mats, dst)):
         table[i] = (s.data_ptr(), d.data_ptr(), *s.shape, s.stride(0), d.stride(0),
-                    L.DTYPE_CODE[s.dtype], L.DTYPE_CODE[d.dtype])
+                    L.DTYPE_CODE[s.dtype], L.DTYPE_CODE[d.dtype], precision, 0)
     co = np.array(coefficients, dtype=np.float64).reshape(-1)
     steps, at = len(coefficients), table.ctypes.data
-    ws = torch.empty(L.lib().scao_orthogonalize_workspace(at, len(mats), steps, precision),
+    ws = torch.empty(L.lib().scao_orthogonalize_workspace(at, len(mats), steps),
                      dtype=torch.uint8, device=mats[0].device)
     ws.fill_(0xff)   # NaN in any word
     L.call("scao_orthogonalize", at, len(mats), co.ctypes.data, steps, ctypes.c_double(eps),
-           precision, ws.data_ptr(), L.stream_ptr(mats[0].device))
+           ws.data_ptr(), L.stream_ptr(mats[0].device))
 
 
 @pytest.mark.parametrize("precision", ["fast", "fp32"])
