@@ -8,12 +8,21 @@
 // with its rows contiguous.  A and B are symmetric, so only the tiles on and below
 // the diagonal are computed and the others stored as their mirror image.
 //
-// Words of the products.  X, A and B are fp16 (or, P = 2, a sum of two fp16 words,
-// 22 significant bits, multiplied as three products of words; a group's choice), scaled by powers of
-// two that the host chooses from what the polynomial can reach, so that neither end
-// of fp16's range matters: |X|, |A| and |B| are bounded by their largest singular
-// value.  fp16 has three bits more than bf16 at the same rate; each of the three is
-// rounded once a step.  Sums, a X and b A are fp32.
+// Words of the products.  X, A and B are fp16 or, P = 2, a sum of two fp16 words (22
+// significant bits, multiplied as three products of words), a group's choice; scaled by
+// powers of two that the host chooses from what the polynomial can reach, so that
+// neither end of fp16's range matters: |X|, |A| and |B| are bounded by their largest
+// singular value.  fp16 has three bits more than bf16 at the same rate; each of the
+// three is rounded once a step, which leaves results of 512 x 512 1.2e-3 off (five
+// steps), a bf16 result's own rounding 1.7e-3.  Sums and b A are fp32.  a is part of B:
+// a X beside the product is no more exact (1.3e-3), and would read X once more at every
+// tile's end, when all of the chip does (3.6% of the time).
+//
+// What bounds it: the chip's power in long updates (14336 x 4096: matrix cores busy 66%
+// of the cycles at 1.85 GHz, 374 us an update, 1.29 PFLOP/s); the count of tiles in the
+// symmetric products (136 of 256 x 256 on 256 CUs: 98 us for 4096 x 4096, 230 in three
+// parts for the Gram matrix over 14336); launches for small matrices, about 5 us each
+// whatever they hold.
 //
 // All matrices of a call go through the same launches, whatever their shapes: a
 // launch's tiles are those of up to ORTHO_GROUPS groups of one shape each, the ones

@@ -1,8 +1,10 @@
 // From updates to the first X: the sums of squares of every matrix (of the
 // optimiser's update, with the momentum's own step), and X = G / (|G| + eps) in
-// fp16 words.  Two passes, as no element can be scaled before the last is summed;
-// both bound by HBM, and short beside the products (12 s multiplications an element
-// and step, s the smaller side).
+// fp16 words.  Two passes, as no element can be scaled before the last is summed; both
+// bound by HBM (134 M elements of eight 8192 x 2048 with bf16 gradients: 257 us with
+// the momentum's step, 5.2 TB/s, and 237, 4.5 TB/s; without four vectors under way and
+// with 256 workgroups a matrix instead of 1024, 58.7 M elements alone took 79 and 95 us
+// and now take 34 and 51), and short beside the products.
 #pragma once
 
 #include "ortho_kernels.hpp"
