@@ -998,7 +998,8 @@ struct QkNormRope : torch::autograd::Function<QkNormRope> {
     variable_list out(9);
     auto given = [](const Tensor& x) { return x.defined() ? std::optional<Tensor>(x) : std::nullopt; };
     int64_t wanted = 0;
-    for (int i = 0; i < 4; ++i) wanted |= (int64_t)(ctx->needs_input_grad(i) && t[i].defined()) << i;
+    for (int i = 0, edge = 0; i < 4; ++i)   // (a weight that is not given has no edge)
+      if (t[i].defined()) wanted |= (int64_t)ctx->needs_input_grad(edge++) << i;
     variable_list have;
     {
       const at::AutoDispatchBelowADInplaceOrView below;

@@ -181,6 +181,17 @@ def test_partial_gradients(hip_device):
         got = torch.autograd.grad([a for a, _ in outs], wanted, [b for _, b in outs])
         for g, want in zip(got, [g for i, g in enumerate(all_grads) if mask >> i & 1]):
             assert torch.equal(g, want)
+    # one of the weights alone
+    for i in range(2):
+        leaves = [t.clone().requires_grad_() for t in (q, k, w[i])]
+        pair = [None, None]
+        pair[i] = leaves[2]
+        y = scao_amd.qk_norm_rope(leaves[0], leaves[1], *pair, cos, sin)
+        got = torch.autograd.grad(y, leaves, d)
+        assert torch.equal(got[2], all_grads[2 + i]) and torch.equal(got[i], all_grads[i])
+        ones = [t.clone().requires_grad_() for t in (q, k)]
+        y = scao_amd.qk_norm_rope(*ones, None, None, cos, sin)
+        assert torch.equal(got[1 - i], torch.autograd.grad(y, ones, d)[1 - i])
     # one output alone
     leaves = [t.clone().requires_grad_() for t in (q, k, *w)]
     got = torch.autograd.grad(scao_amd.qk_norm_rope(*leaves, cos, sin)[0], leaves, d[0])
