@@ -101,6 +101,8 @@ int scao_ffn_backward(const scao_ffn_desc* desc, const void* dy, int64_t ld_dy, 
  * A matrix with a NaN or an infinity (or with a sum of squares beyond double's
  * range) gives NaN throughout, and no other matrix; one of zeros gives zeros.
  * Coefficients that may take a singular value of [0, 1] beyond 1024 are refused.
+ * eps, at least 1e-300, is meant to be small beside |G|: the first X is held to
+ * 2^-39 absolutely in either precision.
  * The norm is summed in double, no atomics: the same call gives the same bits.
  *
  * scao_muon_step: with the momentum m (fp32) and the gradient g
@@ -108,8 +110,8 @@ int scao_ffn_backward(const scao_ffn_desc* desc, const void* dy, int64_t ld_dy, 
  *   p <- decay p - rate orthogonalised(G)
  * p, g and m contiguous; p and g may have different types; p is rounded once.
  *
- * Written memory may not overlap with anything else of the table
- * (SCAO_ERR_INVALID).  workspace: the *_workspace() bytes for the same table and
+ * Written memory, from a matrix's first element to its last with the gaps between
+ * rows, may not overlap with anything else of the table (SCAO_ERR_INVALID).  workspace: the *_workspace() bytes for the same table and
  * steps, aligned to 16, contents of no meaning. */
 enum scao_ortho_precision { SCAO_ORTHO_FAST = 0, SCAO_ORTHO_FP32 = 1 };
 typedef struct scao_ortho_desc {   /* HOST */

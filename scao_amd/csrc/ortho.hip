@@ -435,7 +435,9 @@ int check_scheme(const char* who, int n, const void* table, const double* coeffi
   SCAO_CHECK_ARG(coefficients, "%s: null coefficients", who);
   for (int i = 0; i < 3 * steps; ++i)
     SCAO_CHECK_ARG(std::isfinite(coefficients[i]), "%s: coefficient %d is no finite number", who, i);
-  SCAO_CHECK_ARG(eps > 0 && std::isfinite(eps), "%s: eps %g is not positive and finite", who, eps);
+  // (1 / eps has to be a number: a matrix of zeros is one of zeros)
+  SCAO_CHECK_ARG(eps >= 1e-300 && std::isfinite(eps), "%s: eps %g (finite, at least 1e-300)", who,
+                 eps);
   return SCAO_OK;
 }
 int check_sizes(const char* who, int i, int64_t rows, int64_t cols, int precision) {

@@ -43,8 +43,8 @@ def _flat_coefficients(coefficients, steps: int) -> list:
 
 def _check_eps(eps: float) -> float:
     eps = float(eps)
-    if not 0.0 < eps < math.inf:
-        raise ValueError(f"eps must be positive and finite (got {eps})")
+    if not 1e-300 <= eps < math.inf:
+        raise ValueError(f"eps must be finite and at least 1e-300 (got {eps})")
     return eps
 
 
@@ -65,7 +65,9 @@ def orthogonalize(updates: Union[Tensor, Sequence[Tensor]], steps: int = 5,
     products of 22-bit words, at a third of the rate: pass ``dtype=torch.bfloat16``
     where that accuracy is not needed.  A matrix with a NaN or an infinity gives NaN
     throughout and no other matrix; one of zeros gives zeros.  Coefficients with
-    which a singular value may grow beyond 1024 are refused.  No derivative."""
+    which a singular value may grow beyond 1024 are refused.  eps is meant to be
+    small beside the norms: G / (|G| + eps) is held to 2^-39 absolutely, whatever the
+    precision.  No derivative."""
     flat, eps = _flat_coefficients(coefficients, steps), _check_eps(eps)
     single = isinstance(updates, Tensor)
     updates = [updates] if single else list(updates)

@@ -197,6 +197,22 @@ def test_nan_infinity_zeros_and_extremes(hip_device, dtype):
         assert rel <= 2 * ULP[dtype] if dtype != torch.float32 else rel <= 1e-5
 
 
+def test_the_smallest_and_a_large_eps(hip_device):
+    z = torch.zeros(300, 200, device=hip_device)
+    for dtype in (torch.bfloat16, torch.float32):
+        assert bool((scao_amd.orthogonalize(z, eps=1e-300, dtype=dtype) == 0).all())
+    assert bool((scao_amd.orthogonalize(z[:30, :40], eps=1e-300) == 0).all())
+    # a norm of 3 beside an eps of 200
+    g = _update(hip_device, 4, 300, 200, torch.float32)
+    g = g * (3.0 / g.norm())
+    co = triples(QUINTIC, 2)
+    want = orthogonalize(g, co, eps=200.0)
+    got = scao_amd.orthogonalize(g, steps=2, coefficients=QUINTIC, eps=200.0)
+    # X to 2^-39 an element, times 1.875 a step
+    room = bound(g, co, "fp32", eps=200.0) + 4 * 2.0 ** -39 * g.numel() ** 0.5
+    assert float((got.double() - want).norm()) <= room
+
+
 def test_low_rank_and_a_single_direction(hip_device):
     """A rank-one update: one singular value, the others zero throughout."""
     u = torch.randn(200, 1, device=hip_device)

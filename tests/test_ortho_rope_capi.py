@@ -47,6 +47,7 @@ def _call(t, coefficients=CO, steps=2, eps=1e-7, work=P, momentum=None, n=None):
 
 
 BAD_SCHEME = [dict(steps=0), dict(steps=65), dict(coefficients=None), dict(eps=0.0),
+              dict(eps=1e-310),
               dict(eps=float("nan")), dict(coefficients=np.array([np.inf] * 6)), dict(n=-1),
               dict(work=P + 8), dict(work=None),
               # 40^2 > 1024
@@ -190,6 +191,7 @@ def test_python_refuses_tensors_off_the_gpu():
 
 @pytest.mark.parametrize("kw", [dict(steps=0), dict(steps=2.5), dict(coefficients=(1.0, 2.0)),
                                 dict(coefficients=[(1.0, 2.0, 3.0)] * 4), dict(eps=-1.0),
+                                dict(eps=1e-310),
                                 dict(coefficients=(1.0, float("nan"), 0.0))])
 def test_python_refuses_schemes(kw):
     with pytest.raises(ValueError):
