@@ -98,8 +98,10 @@ __device__ __forceinline__ v4i buffer_of(const void* p, int64_t bytes) {
   return r;
 }
 
-// One operand's share of a step: R rows (of C's dimension) by 64 k, 16-bit.
-template <int L, int R, int NW>
+// One operand's share of a step: R rows (of C's dimension) by 64 k, 16-bit.  WORDS 2:
+// by 32 k of two words each, the lower ones behind the higher ones of all 32 k; in
+// memory they lie `low` elements behind them.
+template <int L, int R, int NW, int WORDS = 1>
 struct Tile {
   static constexpr int BYTES = R * FFN_BK * 2;
   static constexpr int LOADS = BYTES / 1024 / NW;   // per wave and step
@@ -108,20 +110,27 @@ struct Tile {
 
   // byte offset, relative to the step's origin, of what lane `lane` of load i
   // of wave w fetches
-  static __device__ __forceinline__ uint32_t offset(int i, int w, int lane, int64_t ld) {
+  static __device__ __forceinline__ uint32_t offset(int i, int w, int lane, int64_t ld,
+                                                    int low = 0) {
     const int at = (i * NW + w) * 1024 + lane * 16;
     if (L == ROWS) {
       const int r = at / 128, c = (at % 128) / 16 ^ (r & 7);
+      if (WORDS == 2) return (uint32_t)(r * ld * 2 + (c & 3) * 16 + (c >> 2) * low * 2);
       return (uint32_t)(r * ld * 2 + c * 16);
     }
     const int k = at / KROW, p = (at % KROW) / 16;
-    return (uint32_t)(k * ld * 2 + (((p >> 1) ^ fold(k)) * 2 + (p & 1)) * 16);
+    return (uint32_t)((WORDS == 2 ? k & 31 : k) * ld * 2 +
+                      (((p >> 1) ^ fold(k)) * 2 + (p & 1)) * 16);
+  }
+  // cols, WORDS 2: whether load i of wave w fetches lower words
+  static __device__ __forceinline__ bool lower(int i, int w) {
+    return WORDS == 2 && L == COLS && (i * NW + w) * 1024 >= 32 * KROW;
   }
   // its position in the dimension that has to be checked by hand: k for rows
   // (a row's tail is followed by the next row), r for cols
   static __device__ __forceinline__ int inner(int i, int w, int lane) {
     const int at = (i * NW + w) * 1024 + lane * 16;
-    if (L == ROWS) return ((at % 128) / 16 ^ ((at / 128) & 7)) * 8;
+    if (L == ROWS) return (((at % 128) / 16 ^ ((at / 128) & 7)) & (WORDS == 2 ? 3 : 7)) * 8;
     const int k = at / KROW, p = (at % KROW) / 16;
     return (((p >> 1) ^ fold(k)) * 2 + (p & 1)) * 8;
   }
@@ -174,15 +183,18 @@ __device__ __forceinline__ void tile_of(int b, int tm, int tn, int& m, int& n) {
 
 // GATED: B's tile rows 0 .. BN/2-1 are gate rows, the others the same columns'
 // up rows; each wave's fragments are half of either.  OPS: FfnOperands, or what
-// has its a[segment], b[segment], strides and sizes.
+// has its a[segment], b[segment], strides and sizes.  WORDS 2: every element of A and
+// B is a sum of two words; a step is 32 k and three products of words (the lower ones'
+// product is dropped), on four tiles where three products apart would fetch six.
 template <int BM, int BN, int WM, int WN, int LA, int LB, bool F16, bool GATED,
-          class OPS = FfnOperands>
+          class OPS = FfnOperands, int WORDS = 1>
 struct Gemm {
   static constexpr int NW = WM * WN, THREADS = NW * 64, BM_ = BM, BN_ = BN;
   static constexpr int FRAGS = BM / 16 * (BN / 16);   // of 16 x 16 sums
   static constexpr int MI = BM / WM / 16, NJ = BN / WN / 16;
-  using TA = Tile<LA, BM, NW>;
-  using TB = Tile<LB, BN, NW>;
+  static constexpr int BK = FFN_BK / WORDS;   // k of a step
+  using TA = Tile<LA, BM, NW, WORDS>;
+  using TB = Tile<LB, BN, NW, WORDS>;
   static constexpr int LDS = 3 * TA::BYTES + 2 * TB::BYTES;
   static constexpr int COLS_N = GATED ? BN / 2 : BN;   // of C
   static_assert(!GATED || LB == ROWS, "gated products have weights in rows");
@@ -202,17 +214,26 @@ struct Gemm {
     n0 = tn * COLS_N;
 #pragma unroll
     for (int i = 0; i < TA::LOADS; ++i) {
-      offa[i] = TA::offset(i, wave, lane, o.lda);
+      offa[i] = TA::offset(i, wave, lane, o.lda, low_a());
       ina[i] = TA::inner(i, wave, lane);
       if (LA == COLS && m0 + ina[i] >= o.M) offa[i] = OUT_OF_RANGE;
     }
 #pragma unroll
     for (int i = 0; i < TB::LOADS; ++i) {
-      offb[i] = TB::offset(i, wave, lane, o.ldb);
+      offb[i] = TB::offset(i, wave, lane, o.ldb, low_b());
       if (GATED && up_half(i)) offb[i] -= (uint32_t)(BN / 2 * o.ldb * 2);
       inb[i] = TB::inner(i, wave, lane);
       if (LB == COLS && n0 + inb[i] >= o.N) offb[i] = OUT_OF_RANGE;
     }
+  }
+  // where an element's lower word lies, in elements
+  __device__ __forceinline__ int low_a() const {
+    if constexpr (WORDS == 2) return o.low_a;
+    return 0;
+  }
+  __device__ __forceinline__ int low_b() const {
+    if constexpr (WORDS == 2) return o.low_b;
+    return 0;
   }
   __device__ __forceinline__ bool up_half(int i) const { return (i * NW + wave) * 8 >= BN / 2; }
 
@@ -243,7 +264,7 @@ struct Gemm {
   }
   template <int L>
   static __device__ __forceinline__ void advance(Cursor& c, int64_t ld) {
-    const int64_t step = L == ROWS ? FFN_BK * 2 : ld * FFN_BK * 2;
+    const int64_t step = L == ROWS ? BK * 2 : ld * BK * 2;
     c.at += step;
     c.left -= step;
   }
@@ -259,7 +280,7 @@ struct Gemm {
     if (GATED) w.u = cursor<LB>(o.b[w.seg + FFN_MAX_SEG / 2], o.ldb, n0, o.N, w.k0, o.K);
   }
   __device__ __forceinline__ void next(Walk& w) const {
-    w.k0 += FFN_BK;
+    w.k0 += BK;
     if (w.k0 < o.K) {
       advance<LA>(w.a, o.lda);
       advance<LB>(w.b, o.ldb);
@@ -278,20 +299,34 @@ struct Gemm {
     uint32_t lds;
     int k0;
   };
+  // the lower words': rows have them behind the higher ones, within one buffer; those
+  // of columns are a buffer of their own
+  template <int L>
+  static __device__ __forceinline__ v4i buffer(const Cursor& c, int low) {
+    if (WORDS == 2 && L == ROWS) return buffer_of(c.at, c.left > 0 ? c.left + low * 2 : 0);
+    return c.buffer();
+  }
+  template <int L>
+  static __device__ __forceinline__ v4i lower_buffer(const Cursor& c, int low, v4i same) {
+    if (WORDS == 2 && L == COLS) return buffer_of(c.at + low * 2, c.left);
+    return same;
+  }
   __device__ __forceinline__ Fetch fetch_a(const Walk& w, int at) const {
-    const v4i b = w.a.buffer();
-    return Fetch{b, b, (uint32_t)(uintptr_t)(lds + at) + wave * 1024, w.k0};
+    const v4i b = buffer<LA>(w.a, low_a());
+    return Fetch{b, lower_buffer<LA>(w.a, low_a(), b),
+                 (uint32_t)(uintptr_t)(lds + at) + wave * 1024, w.k0};
   }
   __device__ __forceinline__ Fetch fetch_b(const Walk& w, int at) const {
-    const v4i b = w.b.buffer();
-    return Fetch{b, GATED ? w.u.buffer() : b, (uint32_t)(uintptr_t)(lds + at) + wave * 1024, w.k0};
+    const v4i b = buffer<LB>(w.b, low_b());
+    return Fetch{b, GATED ? w.u.buffer() : lower_buffer<LB>(w.b, low_b(), b),
+                 (uint32_t)(uintptr_t)(lds + at) + wave * 1024, w.k0};
   }
   __device__ __forceinline__ void load_a(const Fetch& f, int i) const {
-    load_lds(f.buf, f.lds + i * NW * 1024,
+    load_lds(TA::lower(i, wave) ? f.up : f.buf, f.lds + i * NW * 1024,
              LA == ROWS && f.k0 + ina[i] >= o.K ? OUT_OF_RANGE : offa[i]);
   }
   __device__ __forceinline__ void load_b(const Fetch& f, int i) const {
-    load_lds(GATED && up_half(i) ? f.up : f.buf, f.lds + i * NW * 1024,
+    load_lds((GATED && up_half(i)) || TB::lower(i, wave) ? f.up : f.buf, f.lds + i * NW * 1024,
              LB == ROWS && f.k0 + inb[i] >= o.K ? OUT_OF_RANGE : offb[i]);
   }
 
@@ -321,6 +356,32 @@ struct Gemm {
     }
   }
 
+  // WORDS 2, behind half a step of the higher words' products: the products of A's
+  // lower and B's higher words, with one operand's loads dealt out between the rows;
+  // then those of A's higher and B's lower words, with the LDS reads of the next step's
+  // higher words, each into the registers of what is not needed any more.
+  __device__ __forceinline__ void lower_half(v8s (&a0)[MI], v8s (&b0)[NJ], const v8s (&a1)[MI],
+                                             const v8s (&b1)[NJ], v4f (&acc)[MI][NJ], int ta, int tb,
+                                             const Fetch& f) const {
+#pragma unroll
+    for (int i = 0; i < MI; ++i) {
+#pragma unroll
+      for (int j = 0; j < NJ; ++j) acc[i][j] = mma<F16>(b0[j], a1[i], acc[i][j]);
+#pragma unroll
+      for (int l = i * TB::LOADS / MI; l < (i + 1) * TB::LOADS / MI; ++l) load_b(f, l);
+      __builtin_amdgcn_sched_barrier(0);
+    }
+#pragma unroll
+    for (int i = 0; i < MI; ++i) {
+#pragma unroll
+      for (int j = i * NJ / MI; j < (i + 1) * NJ / MI; ++j) b0[j] = TB::frag(lds + tb, frag_n(j), 0, lane);
+#pragma unroll
+      for (int j = 0; j < NJ; ++j) acc[i][j] = mma<F16>(b1[j], a0[i], acc[i][j]);
+      a0[i] = TA::frag(lds + ta, frag_m(i), 0, lane);
+      __builtin_amdgcn_sched_barrier(0);
+    }
+  }
+
   // the k steps [begin, end) of all segments' steps in order
   __device__ __forceinline__ void run(int begin, int end, v4f (&acc)[MI][NJ]) const {
 #pragma unroll
@@ -328,10 +389,10 @@ struct Gemm {
 #pragma unroll
       for (int j = 0; j < NJ; ++j) acc[i][j] = v4f{0.f, 0.f, 0.f, 0.f};
     if (begin >= end) return;
-    const int steps = (o.K + FFN_BK - 1) / FFN_BK;
+    const int steps = (o.K + BK - 1) / BK;
     Walk w;
     w.seg = begin / steps;
-    w.k0 = (begin % steps) * FFN_BK;
+    w.k0 = (begin % steps) * BK;
     seek(w);
     // A's tiles of this step, the next and the one after, B's of this and the next
     int a0_ = 0, a1_ = TA::BYTES, a2_ = 2 * TA::BYTES;
@@ -363,7 +424,8 @@ struct Gemm {
       wait_loads<TA::LOADS>();
       __builtin_amdgcn_sched_barrier(0);
       // (after the last step the reads are of no use, within LDS)
-      half<false>(fa1, fb1, acc, a1_, b1_, 0, fa0, fb0, fb);
+      if constexpr (WORDS == 2) lower_half(fa0, fb0, fa1, fb1, acc, a1_, b1_, fb);
+      else half<false>(fa1, fb1, acc, a1_, b1_, 0, fa0, fb0, fb);
       next(w);
       const int a = a0_, b = b0_;
       a0_ = a1_;

@@ -162,7 +162,8 @@ struct Pass {
   // k steps of a tile
   static int64_t steps_of(int phase, const OrthoGroup& g) {
     const int k = phase == ORTHO_GRAM ? std::max(g.rows, g.cols) : std::min(g.rows, g.cols);
-    return (g.words == 2 ? 3 : 1) * ((k + FFN_BK - 1) / FFN_BK);
+    const int bk = FFN_BK / g.words;
+    return (k + bk - 1) / bk;
   }
   // The groups' tiles of `side`, the longest sums first.
   void lay(int phase, int side, OrthoPhase& ph) const {
@@ -198,7 +199,9 @@ struct Pass {
       const int tile = begin + (int)(at / n);
       while (k + 1 < ph.groups && ph.g[k + 1].tile0 <= tile) ++k;
       const int64_t steps = steps_of(phase, ph.g[k]);
-      us += (steps + n - 1) / n * c.step(std::min<int64_t>(c.slots, all - at)) + c.ends;
+      // (a step of two words has half as many products again)
+      us += (steps + n - 1) / n * c.step(std::min<int64_t>(c.slots, all - at)) *
+                (ph.g[k].words == 2 ? 1.3 : 1.0) + c.ends;
     }
     return us;
   }

@@ -70,28 +70,23 @@ struct OrthoOut {
   uint8_t dt[ORTHO_MATRICES];
 };
 
-// a matrix's words: segment `low` takes the lower ones
+// What the tiled product needs of one of this group's products: one segment, and where
+// an element's lower word lies.
 struct OrthoWords {
-  const uint16_t* p;
-  int64_t plane;
-  int low;
-  __device__ __forceinline__ const void* operator[](int seg) const {
-    return p + (seg == low ? plane : 0);
-  }
+  const char* p;
+  __device__ __forceinline__ const void* operator[](int) const { return p; }
 };
 struct OrthoOperands {
   OrthoWords a, b;
   int64_t lda, ldb;
+  int low_a, low_b;
   int M, N, K, nseg, row0;
 };
-// P = 2: low x high, high x low, high x high
+// ld: elements of a row of one word; the rows of both words take turns
 template <int P>
-__device__ __forceinline__ OrthoOperands ortho_operands(const char* a, int64_t plane_a, int lda,
-                                                        const char* b, int64_t plane_b, int ldb,
-                                                        int M, int N, int K) {
-  return OrthoOperands{{(const uint16_t*)a, plane_a, P == 2 ? 0 : -1},
-                       {(const uint16_t*)b, plane_b, P == 2 ? 1 : -1},
-                       lda, ldb, M, N, K, P == 2 ? 3 : 1, 0};
+__device__ __forceinline__ OrthoOperands ortho_operands(const char* a, int lda, const char* b,
+                                                        int ldb, int M, int N, int K) {
+  return OrthoOperands{{a}, {b}, (int64_t)P * lda, (int64_t)P * ldb, lda, ldb, M, N, K, 1, 0};
 }
 
 // four values as fp16 words: rounded, or with the rest in a second word
@@ -133,8 +128,8 @@ __device__ __forceinline__ int ortho_group_of(const OrthoPhase& ph, int tile) {
 struct OrthoTarget {
   uint16_t* to;
   const uint16_t* add;
-  int64_t plane;
-  int ld, M, N, cols;      // cols: with the padding, N rounded up to 8
+  int plane, M, N, cols;   // from one word's row to the next's; cols: N rounded up to 8
+  int64_t ld;
   bool mirror;             // a tile below the diagonal
 };
 template <int PHASE>
@@ -147,17 +142,16 @@ __device__ __forceinline__ OrthoTarget ortho_target(const OrthoPhase& ph, const 
   if (PHASE == ORTHO_UPDATE) {
     t.to = (uint16_t*)(x + g.y);
     t.add = nullptr;
-    t.plane = (int64_t)g.rows * g.ldx;
-    t.ld = g.ldx;
+    t.plane = g.ldx;
     t.M = g.rows;
     t.N = g.cols;
   } else {
     t.to = (uint16_t*)(a + (PHASE == ORTHO_GRAM ? g.a : g.b));
     t.add = (const uint16_t*)(a + g.a);
     t.M = t.N = min(g.rows, g.cols);
-    t.plane = (int64_t)t.M * g.lda;
-    t.ld = g.lda;
+    t.plane = g.lda;
   }
+  t.ld = (int64_t)g.words * t.plane;
   t.cols = (t.N + 7) & ~7;
   return t;
 }
@@ -193,7 +187,7 @@ struct OrthoPair {
     const bool in = m < t.M && n < t.cols;
 #pragma unroll
     for (int i = 0; i < P; ++i)
-      w[i] = in ? (v4u_t) * (const gv4u_a16*)(t.add + (int64_t)m * t.ld + n + i * t.plane)
+      w[i] = in ? (v4u_t) * (const gv4u_a16*)(t.add + m * t.ld + n + i * t.plane)
                 : v4u_t{0, 0, 0, 0};
   }
   // by c, of a square by c + keep A + diagonal, likewise d
@@ -233,7 +227,7 @@ __device__ __forceinline__ void ortho_store(const OrthoTarget& t, int m, int n, 
 #pragma unroll
   for (int i = 0; i < P; ++i) {
     const v4u_t w = join_pair(p[i], q[i]);
-    if (in) *(gv4u_a16*)(t.to + (int64_t)m * t.ld + at + i * t.plane) = w;
+    if (in) *(gv4u_a16*)(t.to + m * t.ld + at + i * t.plane) = w;
   }
   if (!t.mirror) return;
   // (a row of C is a column of the image, so C's padding rows are stored as the
@@ -243,10 +237,10 @@ __device__ __forceinline__ void ortho_store(const OrthoTarget& t, int m, int n, 
   for (int i = 0; i < P; ++i) {
     const v2u a = turn4(p[i], lane), b = turn4(q[i], lane);
     if (col < t.cols) {
-      uint16_t* to = t.to + (int64_t)row * t.ld + col + i * t.plane;
+      uint16_t* to = t.to + row * t.ld + col + i * t.plane;
       typedef __attribute__((address_space(1))) v2u gv2u_a8;
       *(gv2u_a8*)to = a;
-      *(gv2u_a8*)(to + (int64_t)16 * t.ld) = b;
+      *(gv2u_a8*)(to + 16 * t.ld) = b;
     }
   }
 }
@@ -334,15 +328,15 @@ __device__ __forceinline__ OrthoPlace ortho_place(const OrthoOut& o, int e) {
   return OrthoPlace{o.p[e], o.ld[e], o.dt[e], o.rate[e], o.decay[e]};
 }
 
-template <int BM, int LA, int LB>
-using OrthoGemm = Gemm<BM, BM, 2, BM == 256 ? 4 : 2, LA, LB, true, false, OrthoOperands>;
+template <int P, int BM, int LA, int LB>
+using OrthoGemm = Gemm<BM, BM, 2, BM == 256 ? 4 : 2, LA, LB, true, false, OrthoOperands, P>;
 
 template <class G, int P, int PHASE, int DEST>
 __device__ __forceinline__ void ortho_tile(char* smem, const OrthoPhase& ph, const OrthoOut& out,
                                            const OrthoGroup& g, const OrthoOperands& o, int matrix,
                                            int tm, int tn, int tile, int part) {
   G gm(o, (lchar*)smem, tm, tn);
-  const int steps = o.nseg * ((o.K + FFN_BK - 1) / FFN_BK);
+  const int steps = (o.K + G::BK - 1) / G::BK;
   const bool split = part >= 0;
   const int per = split ? (steps + ph.splits - 1) / ph.splits : steps;
   const int begin = split ? part * per : 0;
@@ -389,33 +383,32 @@ template <int P, int BM, int PHASE, int DEST>
 __device__ __forceinline__ void ortho_product(char* smem, const OrthoPhase& ph, const OrthoOut& out,
                                               const OrthoGroup& g, int matrix, int tm, int tn,
                                               int tile, int part) {
-  using RR = OrthoGemm<BM, ROWS, ROWS>;
-  using RC = OrthoGemm<BM, ROWS, COLS>;
-  using CC = OrthoGemm<BM, COLS, COLS>;
+  using RR = OrthoGemm<P, BM, ROWS, ROWS>;
+  using RC = OrthoGemm<P, BM, ROWS, COLS>;
+  using CC = OrthoGemm<P, BM, COLS, COLS>;
   const char* x = ph.base + matrix * g.x_step + g.x;
   const char* a = ph.base + matrix * g.a_step + (PHASE == ORTHO_SQUARE ? g.a : g.b);
   const bool wide = g.rows <= g.cols;
   const int s = wide ? g.rows : g.cols;
-  const int64_t px = (int64_t)g.rows * g.ldx, pa = (int64_t)s * g.lda;
   if constexpr (PHASE == ORTHO_SQUARE) {
-    const OrthoOperands o = ortho_operands<P>(a, pa, g.lda, a, pa, g.lda, s, s, s);
+    const OrthoOperands o = ortho_operands<P>(a, g.lda, a, g.lda, s, s, s);
     ortho_tile<RR, P, PHASE, DEST>(smem, ph, out, g, o, matrix, tm, tn, tile, part);
   } else if constexpr (PHASE == ORTHO_GRAM) {
     const OrthoOperands o =
-        ortho_operands<P>(x, px, g.ldx, x, px, g.ldx, s, s, wide ? g.cols : g.rows);
+        ortho_operands<P>(x, g.ldx, x, g.ldx, s, s, wide ? g.cols : g.rows);
     if (wide) ortho_tile<RR, P, PHASE, DEST>(smem, ph, out, g, o, matrix, tm, tn, tile, part);
     else ortho_tile<CC, P, PHASE, DEST>(smem, ph, out, g, o, matrix, tm, tn, tile, part);
   } else if (wide) {
-    const OrthoOperands o = ortho_operands<P>(a, pa, g.lda, x, px, g.ldx, g.rows, g.cols, s);
+    const OrthoOperands o = ortho_operands<P>(a, g.lda, x, g.ldx, g.rows, g.cols, s);
     ortho_tile<RC, P, PHASE, DEST>(smem, ph, out, g, o, matrix, tm, tn, tile, part);
   } else {
-    const OrthoOperands o = ortho_operands<P>(x, px, g.ldx, a, pa, g.lda, g.rows, g.cols, s);
+    const OrthoOperands o = ortho_operands<P>(x, g.ldx, a, g.lda, g.rows, g.cols, s);
     ortho_tile<RR, P, PHASE, DEST>(smem, ph, out, g, o, matrix, tm, tn, tile, part);
   }
 }
 template <int BM, int PHASE, int DEST>
 __global__ __launch_bounds__(BM * 2, 2) void k_ortho(const OrthoPhase ph, const OrthoOut out) {
-  using G = OrthoGemm<BM, ROWS, ROWS>;
+  using G = OrthoGemm<1, BM, ROWS, ROWS>;
   static_assert(G::THREADS == BM * 2, "a wave for every 32 rows");
   __shared__ __attribute__((aligned(1024))) char smem[G::LDS];
   const int b = blockIdx.x, rest = ph.tiles - ph.whole;

@@ -158,7 +158,6 @@ template <int P>
 __device__ __forceinline__ void ortho_scale(const OrthoPrep& p, const OrthoSource& g, int matrix,
                                             int part, double scale) {
   uint16_t* x = (uint16_t*)(p.base + g.x + matrix * g.x_step);
-  const int64_t plane = (int64_t)g.rows * g.ldx;
   ortho_walk<false>(p, g, matrix, part, g.ldx, [&](int r, int c, const OrthoVector& u) {
     v2u w[2][P];
 #pragma unroll
@@ -171,7 +170,7 @@ __device__ __forceinline__ void ortho_scale(const OrthoPrep& p, const OrthoSourc
     }
 #pragma unroll
     for (int i = 0; i < P; ++i)
-      *(gv4u_a16*)(x + (int64_t)r * g.ldx + c + i * plane) =
+      *(gv4u_a16*)(x + ((int64_t)r * P + i) * g.ldx + c) =
           v4u_t{w[0][i][0], w[0][i][1], w[1][i][0], w[1][i][1]};
   });
 }
