@@ -216,9 +216,38 @@ struct OrthoPair {
   }
 };
 
+// A tile's mirror image goes through LDS, which the products need no more: rows of
+// 16-byte stores.  (Stored from the registers, 32 bytes of a row at a time, it took 8 us
+// of a 256 x 256 tile's 16 beside its k steps, 16 of 26 with two words.)  Rows of BM
+// elements and 32 bytes, so that the 16 lanes that write four rows each meet all banks.
+template <int BM>
+struct OrthoImage {
+  static constexpr int ROW = BM * 2 + 32;
+  static constexpr int BYTES = BM * ROW;
+  typedef __attribute__((address_space(3))) v2u lv2u;
+  typedef __attribute__((address_space(3))) v4u_t lv4u;
+  // a fragment's words, from row m and column n of the tile
+  static __device__ __forceinline__ void put(lchar* lds, int m, int n, int lane, v2u w) {
+    const int q = lane & 3;
+    *(lv2u*)(lds + (n + 4 * (lane >> 4) + q) * ROW + (m + (lane & 15) - q) * 2) = turn4(w, lane);
+  }
+  // plane `to` of the matrix; row0, col0: the image's place
+  static __device__ __forceinline__ void store(const lchar* lds, const OrthoTarget& t, uint16_t* to,
+                                               int row0, int col0) {
+    constexpr int PIECES = BM / 8, THREADS = BM * 2;
+#pragma unroll 4
+    for (int i = 0; i < BM * PIECES / THREADS; ++i) {
+      const int at = i * THREADS + threadIdx.x, r = at / PIECES, c = at % PIECES * 8;
+      if (col0 + c < t.cols)
+        *(gv4u_a16*)(to + (row0 + r) * t.ld + col0 + c) = *(const lv4u*)(lds + r * ROW + c * 2);
+    }
+  }
+};
+
+// mirror: the image too, 32 bytes of a row at a time
 template <int P>
-__device__ __forceinline__ void ortho_store(const OrthoTarget& t, int m, int n, int lane, v4f c,
-                                            v4f d) {
+__device__ __forceinline__ void ortho_store(const OrthoTarget& t, bool mirror, int m, int n, int lane,
+                                            v4f c, v4f d) {
   v2u p[P], q[P];
   ortho_words<P>(c, p);
   ortho_words<P>(d, q);
@@ -229,7 +258,7 @@ __device__ __forceinline__ void ortho_store(const OrthoTarget& t, int m, int n, 
     const v4u_t w = join_pair(p[i], q[i]);
     if (in) *(gv4u_a16*)(t.to + m * t.ld + at + i * t.plane) = w;
   }
-  if (!t.mirror) return;
+  if (!mirror) return;
   // (a row of C is a column of the image, so C's padding rows are stored as the
   // image's padding columns; a tile below the diagonal has no padding columns)
   const int dm = lane & 15, row = n + 4 * (lane >> 4) + (dm & 3), col = m - (dm & 3);
@@ -317,9 +346,9 @@ __device__ __forceinline__ void ortho_put(const OrthoPlace& o, const OrthoTarget
 template <int P, int PHASE, int DEST>
 __device__ __forceinline__ void ortho_finish(const OrthoPhase& ph, const OrthoPlace& o,
                                              const OrthoTarget& t, const OrthoPair<P, PHASE>& add,
-                                             int m, int n, int lane, v4f c, v4f d) {
+                                             bool mirror, int m, int n, int lane, v4f& c, v4f& d) {
   add.sum(ph, m, n, lane, c, d);
-  if constexpr (DEST == ORTHO_NEXT) ortho_store<P>(t, m, n, lane, c, d);
+  if constexpr (DEST == ORTHO_NEXT) ortho_store<P>(t, mirror, m, n, lane, c, d);
   else ortho_put<DEST>(o, t, m, n, lane, c, d);
 }
 template <int DEST>
@@ -372,10 +401,35 @@ __device__ __forceinline__ void ortho_tile(char* smem, const OrthoPhase& ph, con
     for (int i = 0; i < BATCH; ++i)
 #pragma unroll
       for (int j = 0; j < G::NJ; j += 2)
-        ortho_finish<P, PHASE, DEST>(ph, to, t, add[i][j / 2],
+        ortho_finish<P, PHASE, DEST>(ph, to, t, add[i][j / 2], false,
                                      gm.m0 + gm.frag_m(i0 + i) + (lane & 15), gm.n0 + gm.frag_n(j),
                                      lane, acc[i0 + i][j], acc[i0 + i][j + 1]);
     __builtin_amdgcn_sched_barrier(0);
+  }
+  if constexpr (PHASE != ORTHO_UPDATE) {
+    if (!t.mirror) return;
+    using Image = OrthoImage<G::BM_>;
+    static_assert(Image::BYTES <= G::LDS, "the image fits");
+    // (the last of run() was a barrier: nobody reads the products' tiles any more.  The
+    // lane is hidden from the compiler, which would keep the addresses that follow from
+    // it in registers from before the products on: there are none to spare.)
+    int at = lane;
+    asm volatile("" : "+v"(at));
+#pragma unroll
+    for (int p = 0; p < P; ++p) {
+      if (p) __syncthreads();
+#pragma unroll
+      for (int i = 0; i < G::MI; ++i)
+#pragma unroll
+        for (int j = 0; j < G::NJ; ++j) {
+          v2u w[P];
+          ortho_words<P>(acc[i][j], w);
+          Image::put((lchar*)smem, gm.frag_m(i), gm.frag_n(j), at, w[p]);
+          __builtin_amdgcn_sched_barrier(0);
+        }
+      __syncthreads();
+      Image::store((const lchar*)smem, t, t.to + p * t.plane, gm.n0, gm.m0);
+    }
   }
 }
 
@@ -466,7 +520,7 @@ __global__ __launch_bounds__(256) void k_ortho_join(const OrthoPhase ph, const O
     constexpr int P = decltype(words)::value;
     OrthoPair<P, PHASE> add;
     add.load(t, m, n, lane);
-    ortho_finish<P, PHASE, DEST>(ph, to, t, add, m, n, lane, c, d);
+    ortho_finish<P, PHASE, DEST>(ph, to, t, add, t.mirror, m, n, lane, c, d);
   };
   if (g.words == 2) finish(OrthoWordCount<2>{});
   else finish(OrthoWordCount<1>{});
