@@ -94,20 +94,22 @@ bool scales_of(const double* co, int steps, Scales& s) {
 }
 
 // -------------------------------------------------------------- one pass ---
-// us of a k step with one workgroup a CU and with all a CU holds, and of a tile's
-// beginning and end: those of the feed-forward block's products on the same tiles
+// Estimated us of the products' tiles, by words and tile: of a k step (64 k, or 32 of
+// two words) with a CU's LDS to one tile and with all it holds, and of a tile's beginning
+// and end (sums alone, an update's, a symmetric product's with its image); of a join, a
+// part and element.  Fitted to 132 launches of 10 to 1296 tiles and 6 to 72 steps.
 struct Cost {
   int side, slots;
-  double lone, full, ends;
+  double lone, full, parts, update, symmetric;
+  // 128 x 128 tiles: two on a CU as soon as there are more than CUs
   double step(int64_t groups) const {
-    const double crowd = groups >= slots  ? 1.0
-                         : slots == 256   ? groups / 256.0
-                         : groups <= 256  ? 0.0
-                                          : (groups - 256.0) / (slots - 256.0);
-    return lone + (full - lone) * crowd;
+    if (slots > 256) return groups > 256 ? full : lone;
+    return lone + (full - lone) * std::min(1.0, groups / 256.0);
   }
 };
-const Cost COSTS[2] = {{128, 512, 0.62, 1.14, 5.2}, {256, 256, 1.15, 1.50, 4.9}};
+const Cost COSTS[2][2] = {{{128, 512, 0.50, 0.94, 6.5, 6.5, 7.5}, {256, 256, 1.00, 1.40, 13, 13, 16}},
+                          {{128, 512, 0.67, 1.28, 6.5, 8.0, 9.0}, {256, 256, 1.60, 2.18, 13, 16, 24}}};
+const double JOIN[2] = {0.87e-6, 1.6e-6};
 
 struct Plan {
   int big = 0;
@@ -190,32 +192,39 @@ struct Pass {
     ph.tiles = (int)tiles;
   }
   // Estimated us of the tiles from `begin` on, each in n parts: rounds of as many
-  // workgroups as the chip holds, as long as their first.
-  double rounds(int phase, const OrthoPhase& ph, const Cost& c, int begin, int end, int n) const {
+  // workgroups as the chip holds, as long as their first, with the CUs shared by as many
+  // as would do the round's steps at that length (a few long tiles among short ones have
+  // their CUs alone: 4 Gram matrices of 384 over 6246 rows and 16 of 256 over 599).
+  static double rounds(int phase, const OrthoPhase& ph, int big, int begin, int end, int n) {
     double us = 0;
     int k = 0;
-    const int64_t all = (int64_t)(end - begin) * n;
-    for (int64_t at = 0; at < all; at += c.slots) {
-      const int tile = begin + (int)(at / n);
-      while (k + 1 < ph.groups && ph.g[k + 1].tile0 <= tile) ++k;
-      const int64_t steps = steps_of(phase, ph.g[k]);
-      // (a step of two words has half as many products again)
-      us += (steps + n - 1) / n * c.step(std::min<int64_t>(c.slots, all - at)) *
-                (ph.g[k].words == 2 ? 1.3 : 1.0) + c.ends;
+    const int64_t slots = COSTS[0][big].slots, stop = (int64_t)end * n;
+    for (int64_t at = (int64_t)begin * n; at < stop; at += slots) {
+      while (k + 1 < ph.groups && (int64_t)ph.g[k + 1].tile0 * n <= at) ++k;
+      const int64_t last = std::min(stop, at + slots);
+      const Cost& c = COSTS[ph.g[k].words - 1][big];
+      const int first = (steps_of(phase, ph.g[k]) + n - 1) / n;
+      int64_t steps = 0;
+      for (int i = k; i < ph.groups && (int64_t)ph.g[i].tile0 * n < last; ++i) {
+        const int64_t from = std::max(at, (int64_t)ph.g[i].tile0 * n);
+        const int64_t to = i + 1 < ph.groups ? std::min(last, (int64_t)ph.g[i + 1].tile0 * n) : last;
+        steps += (to - from) * ((steps_of(phase, ph.g[i]) + n - 1) / n);
+      }
+      us += first * c.step(steps / first) +
+            (n > 1 ? c.parts : phase == ORTHO_UPDATE ? c.update : c.symmetric);
     }
     return us;
   }
   // Which tile, how many of them run in one piece and in how many parts the others:
-  // all of them, or those that do not fill a last round.  The join: a launch, and 8
-  // bytes a part and element.
+  // all of them, or those that do not fill a last round.
   Plan plan(int phase) {
     Plan best;
     double least = 1e30;
     for (int big = 0; big < 2; ++big) {
-      const Cost& c = COSTS[big];
+      const int side = COSTS[0][big].side, slots = COSTS[0][big].slots;
       OrthoPhase ph{};
-      lay(phase, c.side, ph);
-      const int whole_rounds = ph.tiles / c.slots * c.slots;
+      lay(phase, side, ph);
+      const int whole_rounds = ph.tiles / slots * slots;
       for (int n : {1, 2, 3, 4, 6, 8, 12, 16})
         for (int whole : {0, whole_rounds}) {
           if (n == 1 ? whole != 0 : whole == ph.tiles) continue;
@@ -223,10 +232,10 @@ struct Pass {
           if (n > 1 && ((int64_t)rest * n > (big ? 1024 : 2048) ||
                         2 * n > steps_of(phase, ph.g[0])))
             continue;
-          double us = n == 1 ? rounds(phase, ph, c, 0, ph.tiles, 1)
-                             : rounds(phase, ph, c, 0, whole, 1) +
-                                   rounds(phase, ph, c, whole, ph.tiles, n) + 3 +
-                                   (8 / 7.4e6 * n + 4 / 5e6) * rest * c.side * c.side;
+          double us = n == 1 ? rounds(phase, ph, big, 0, ph.tiles, 1)
+                             : rounds(phase, ph, big, 0, whole, 1) +
+                                   rounds(phase, ph, big, whole, ph.tiles, n) + 4 +
+                                   JOIN[ph.g[0].words - 1] * n * rest * side * side;
           if (us < least) {
             least = us;
             best.big = big;
@@ -239,7 +248,7 @@ struct Pass {
     const int64_t rest = best.ph.tiles - best.ph.whole;
     best.ph.base = base;
     if (rest) {   // the parts' room is given back
-      const int64_t at = used, side = COSTS[best.big].side;
+      const int64_t at = used, side = COSTS[0][best.big].side;
       best.ph.partial = (float*)(base + take(rest * best.ph.splits * side * side * 4));
       used = at;
     }
