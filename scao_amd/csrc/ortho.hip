@@ -1,12 +1,13 @@
 // Newton-Schulz orthogonalisation of matrix updates, and the step of the optimiser
 // that is built on it: argument checks, memory plans and the order of the launches.
-// The kernels are in ortho_kernels.hpp, ortho_norm.hpp and ortho_small.hpp.
+// The kernels are in ortho_kernels.hpp, ortho_norm.hpp, ortho_small.hpp and
+// ortho_panels.hpp.
 #include <algorithm>
 #include <cmath>
 #include <new>
 #include <vector>
 
-#include "ortho_small.hpp"
+#include "ortho_panels.hpp"
 
 using namespace scao;
 
@@ -71,6 +72,8 @@ struct Scales {
   double first;                       // of the first X
   float gram[MAX_STEPS], square[MAX_STEPS], square_keep[MAX_STEPS];
   float diagonal[MAX_STEPS], update[MAX_STEPS];
+  // by panels: of A X and (A X) X^T as words; of X, A X and A A X in the next X
+  float second[MAX_STEPS], third[MAX_STEPS], a[MAX_STEPS], b[MAX_STEPS], c[MAX_STEPS];
 };
 // false: some singular value may grow past what the words hold
 bool scales_of(const double* co, int steps, Scales& s) {
@@ -87,6 +90,12 @@ bool scales_of(const double* co, int steps, Scales& s) {
     s.square_keep[k] = (float)(b * sb / sa);
     s.diagonal[k] = (float)(a * sb);
     s.update[k] = (float)(to / (sb * sx));
+    const double sy = power_for(u * u * u, 28), sz = power_for(u * u * u * u, 28);
+    s.second[k] = (float)(sy / (sa * sx));
+    s.third[k] = (float)(sz / (sy * sx));
+    s.a[k] = (float)(a * to / sx);
+    s.b[k] = (float)(b * to / (sa * sx));
+    s.c[k] = (float)(c * to / (sz * sx));
     u = next;
     sx = to;
   }
@@ -113,6 +122,7 @@ const double JOIN[2] = {0.87e-6, 1.6e-6};
 
 struct Plan {
   int big = 0;
+  double us = 0;
   OrthoPhase ph{};
 };
 
@@ -242,6 +252,7 @@ struct Pass {
             best.ph = ph;
             best.ph.splits = n;
             best.ph.whole = n == 1 ? ph.tiles : whole;
+            best.us = us;
           }
         }
     }
@@ -253,6 +264,107 @@ struct Pass {
       used = at;
     }
     return best;
+  }
+
+  // The groups' places if a step is shorter by panels than in these launches, or none.
+  // (What the plans have taken is taken again: one or the other runs.)
+  std::vector<PanelGroup> panels_of(const Plan (&plans)[3]) {
+    std::vector<PanelGroup> to;
+    double us = 4;
+    int blocks = 0;
+    used = round_up((int64_t)ORTHO_MATRICES * ORTHO_PARTS * 8, 256);
+    for (const OrthoGroup& g : groups) {
+      PanelGroup q{};
+      q.wide = g.rows <= g.cols;
+      q.source_s = std::min(g.rows, g.cols);
+      q.source_l = std::max(g.rows, g.cols);
+      q.s = (int)round_up(q.source_s, 32);
+      q.l = (int)round_up(q.source_l, 32);
+      q.first = g.first;
+      q.count = g.count;
+      q.words = g.words;
+      if (q.s > PANEL_SIDE || q.l > PANEL_LENGTH || panel_lds(q) > PANEL_LDS) return {};
+      q.per = q.s / PANEL;
+      q.block0 = blocks;
+      blocks += q.per * q.count;
+      to.push_back(q);
+    }
+    // Rounds of a panel a CU, by the longest of each: 0.8 us a product, and 7.5 a MB of X
+    // with a CU alone, 15 where all read (20 with nothing else to wait for).  Fitted to
+    // 52 calls of 160 x 160 to 512 x 1024; small launches of tiles take 15% less than
+    // their estimate.
+    for (int64_t at = 0; at < blocks; at += 256) {
+      double most = 0;
+      const double fill = std::min<int64_t>(256, blocks - at) / 256.0;
+      for (const PanelGroup& q : to)
+        if (q.block0 < at + 256 && q.block0 + (int64_t)q.per * q.count > at) {
+          const bool held = panel_held(q);
+          const int products = 2 * ((q.s + 255) / 256 + (q.l + 255) / 256);
+          most = std::max(most, 0.8 * products + 1e-6 * panel_bytes(q) * (held ? 2 : 4) *
+                                                     (7.5 + (held ? 12.5 : 7.5) * fill));
+        }
+      us += most;
+    }
+    if (1.15 * us > plans[0].us + plans[1].us + plans[2].us) return {};
+    for (PanelGroup& q : to)
+      for (int64_t PanelGroup::*at : {&PanelGroup::rows, &PanelGroup::columns,
+                                      &PanelGroup::next_rows, &PanelGroup::next_columns})
+        q.*at = take((int64_t)q.count * panel_bytes(q));
+    return to;
+  }
+  int run_panels(const char* who, const Scales& sc, int steps, int dest, const OrthoPrep& prep,
+                 const std::vector<PanelGroup>& panels, const OrthoOut& out, hipStream_t st) {
+    OrthoPanels p{};
+    PanelSources first{};
+    int blocks = 0, lds = 0;
+    bool all = true;
+    for (const PanelGroup& q : panels) {
+      all = all && panel_held(q);
+      p.g[p.groups] = first.g[p.groups] = q;
+      first.g[p.groups].parts = prep.g[p.groups].parts;
+      ++p.groups;
+      blocks += q.per * q.count;
+      lds = std::max(lds, panel_lds(q));
+    }
+    for (int i = 0; i < n; ++i) {
+      first.src[i] = prep.src[i];
+      first.buf[i] = prep.buf[i];
+      first.ld[i] = prep.ld[i];
+      first.dt[i] = prep.dt[i];
+    }
+    first.base = base;
+    first.norms = norms;
+    first.eps = prep.eps;
+    first.scale = prep.scale;
+    first.momentum = prep.momentum;
+    first.rest = prep.rest;
+    first.groups = p.groups;
+    first.nesterov = prep.nesterov;
+    k_panel_first<<<blocks, PANEL_THREADS, 0, st>>>(first);
+    SCAO_LAUNCH_CHECK(who);
+    p.base = base;
+    for (int k = 0; k < steps; ++k) {
+      p.gram = sc.gram[k];
+      p.second = sc.second[k];
+      p.third = sc.third[k];
+      p.a = sc.a[k];
+      p.b = sc.b[k];
+      p.c = sc.c[k];
+      const int to = k + 1 < steps ? ORTHO_NEXT : dest;
+      auto* kernel = all ? (to == ORTHO_NEXT     ? k_ortho_panels<true, ORTHO_NEXT>
+                            : to == ORTHO_RESULT ? k_ortho_panels<true, ORTHO_RESULT>
+                                                 : k_ortho_panels<true, ORTHO_PARAMETER>)
+                         : (to == ORTHO_NEXT     ? k_ortho_panels<false, ORTHO_NEXT>
+                            : to == ORTHO_RESULT ? k_ortho_panels<false, ORTHO_RESULT>
+                                                 : k_ortho_panels<false, ORTHO_PARAMETER>);
+      kernel<<<blocks, PANEL_THREADS, lds, st>>>(p, out);
+      SCAO_LAUNCH_CHECK(who);
+      for (int i = 0; i < p.groups; ++i) {
+        std::swap(p.g[i].rows, p.g[i].next_rows);
+        std::swap(p.g[i].columns, p.g[i].next_columns);
+      }
+    }
+    return SCAO_OK;
   }
 
   void prep(OrthoPrep& p, int& blocks) const {
@@ -291,6 +403,7 @@ struct Pass {
   int run(const char* who, const Scales& sc, int steps, double eps, double momentum, bool nesterov,
           int dest, hipStream_t st) {
     Plan plans[3] = {plan(ORTHO_GRAM), plan(ORTHO_SQUARE), plan(ORTHO_UPDATE)};
+    const std::vector<PanelGroup> panels = panels_of(plans);
     OrthoPrep p{};
     int blocks;
     prep(p, blocks);
@@ -300,7 +413,7 @@ struct Pass {
     p.rest = (float)(1.0 - momentum);
     p.nesterov = nesterov;
     k_ortho_norm<<<blocks, 256, 0, st>>>(p);
-    k_ortho_scale<<<blocks, 256, 0, st>>>(p);
+    if (panels.empty()) k_ortho_scale<<<blocks, 256, 0, st>>>(p);
     SCAO_LAUNCH_CHECK(who);
     OrthoOut out{};
     for (int i = 0; i < n; ++i) {
@@ -310,6 +423,7 @@ struct Pass {
       out.rate[i] = entry(i).rate;
       out.decay[i] = entry(i).decay;
     }
+    if (!panels.empty()) return run_panels(who, sc, steps, dest, p, panels, out, st);
     for (int k = 0; k < steps; ++k) {
       plans[ORTHO_GRAM].ph.by = sc.gram[k];
       plans[ORTHO_SQUARE].ph.by = sc.square[k];
@@ -363,7 +477,8 @@ int64_t workspace_of(const std::vector<Matrix>& m, int steps) {
   if (all_small(m, steps)) return 0;
   for_passes(m, [&](const int* order, int n) {
     Pass p(m.data(), order, n, nullptr, steps > 1);
-    for (int phase = 0; phase < 3; ++phase) p.plan(phase);
+    const Plan plans[3] = {p.plan(ORTHO_GRAM), p.plan(ORTHO_SQUARE), p.plan(ORTHO_UPDATE)};
+    p.panels_of(plans);
     most = std::max(most, p.peak);
     return SCAO_OK;
   });

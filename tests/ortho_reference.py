@@ -14,7 +14,13 @@ function on [-u, u] are values of its derivative).  Its own errors:
     and four times that for what a partial sum may exceed its end.
 
 Errors of A reach B as |b| + 2 |c| |A|, errors of B reach X times |X|, both in the
-spectral norm."""
+spectral norm.
+
+Matrices of up to 512 x 1024 may take their steps by panels: Y = A X, A'' = Y X^T and
+Z = A'' X instead of A A and B X, a X + b Y + c Z in fp32.  An error of A reaches Y times
+|X|, one of Y reaches A'' times |X|, one of A'' reaches Z times |X|; Y and A'' are
+rounded to words where they are a product's factor (b Y is not), and every product has
+the sums' and the dropped words' errors.  The larger of the two ways' errors counts."""
 
 from __future__ import annotations
 
@@ -63,8 +69,17 @@ def bound(g, coefficients, precision, eps=1e-7):
         ea = w * na + _sums(l) * nx * nx + 2 * w * math.sqrt(top) * nx
         eb = (abs(b) + 2 * abs(c) * top) * ea + w * float(factor.norm()) + (
             _sums(s) + 2 * w) * abs(c) * na * na
-        x, ex = a * x + factor @ x, math.sqrt(top) * eb + (_sums(s) + 2 * w) * float(
+        ex = math.sqrt(top) * eb + (_sums(s) + 2 * w) * float(
             factor.norm()) * nx + 2.0 ** -23 * abs(a) * nx
+        if s <= 512 and l <= 1024:
+            y, z = gram @ x, square @ x
+            ny, nz, root = float(y.norm()), float(z.norm()), math.sqrt(top)
+            ey = root * ea + (_sums(s) + 2 * w) * na * nx
+            e2 = root * (ey + w * ny) + (_sums(l) + 2 * w) * ny * nx + w * float(square.norm())
+            ez = root * e2 + (_sums(s) + 2 * w) * float(square.norm()) * nx
+            ex = max(ex, abs(b) * ey + abs(c) * ez
+                     + 2.0 ** -22 * (abs(a) * nx + abs(b) * ny + abs(c) * nz))
+        x = a * x + factor @ x
         err = slope * err + ex + w * float(x.norm())
         u = float((a * grid + b * grid ** 3 + c * grid ** 5).abs().max())
     return err

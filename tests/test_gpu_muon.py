@@ -72,6 +72,31 @@ def test_steps(hip_device, dtype, nesterov, adjust):
                 m[at] = mom
 
 
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("nesterov", [True, False])
+def test_steps_of_a_few_hundred_rows(hip_device, dtype, nesterov):
+    lr, wd, mu, co = 0.03, 0.2, 0.9, triples(QUINTIC, 2)
+    params = [torch.nn.Parameter((torch.randn(shape, device=hip_device) * 0.05).to(dtype))
+              for shape in ((256, 256), (300, 160), (2, 140, 333))]
+    opt = scao_amd.Muon(params, lr=lr, weight_decay=wd, momentum=mu, nesterov=nesterov,
+                        ns_coefficients=QUINTIC, ns_steps=2)
+    momenta = [torch.zeros(p.shape, dtype=torch.float64, device=hip_device) for p in params]
+    precision = "fp32" if dtype == torch.float32 else "fast"
+    for step in range(2):
+        before = [p.detach().clone() for p in params]
+        for p in params:
+            p.grad = torch.randn(p.shape, device=hip_device).mul_(1e-2).to(dtype)
+        opt.step()
+        for p, old, m in zip(params, before, momenta):
+            for k in range(p.shape[0] if p.ndim == 3 else 1):
+                at = (k,) if p.ndim == 3 else ()
+                want, mom, room = _reference(old[at], p.grad[at], m[at], lr, wd, mu, nesterov, co,
+                                             None, precision)
+                err = float((p.detach()[at].double() - want).norm())
+                assert err <= room, (step, p.shape, err, room)
+                m[at] = mom
+
+
 @pytest.mark.parametrize("ns_dtype,precision", [(torch.bfloat16, "fast"), (torch.float32, "fp32")])
 def test_precision_by_choice(hip_device, ns_dtype, precision):
     for dtype in (torch.float32, torch.bfloat16):

@@ -155,6 +155,47 @@ def test_many_shapes_types_and_strides_in_one_call(hip_device, precision):
     assert float((single - dst[0]).norm()) <= 2 * bound(mats[0], co, precision)
 
 
+# Sizes whose steps go by panels: sides just behind a multiple of 16 and 32, one to
+# four blocks of columns a wave, all pieces kept or not, and several shapes at once.
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("shapes", [
+    [(129, 129)], [(256, 256)], [(241, 255)], [(257, 225)], [(160, 900)], [(1000, 145)],
+    [(384, 384)], [(256, 512)], [(513, 256)], [(512, 512)], [(300, 449)] * 3,
+    [(200, 256)] * 17, [(384, 300), (150, 150), (150, 150), (100, 400), (401, 140)]])
+def test_panels(hip_device, shapes, dtype):
+    mats = [_update(hip_device, i, m, n, dtype, i % 3, i % 2) for i, (m, n) in enumerate(shapes)]
+    precision = "fast" if dtype == torch.bfloat16 else "fp32"
+    for co in (triples(QUINTIC, 3), triples((3.4445, -4.7750, 2.0315), 2), triples(CUBIC, 1)):
+        dst = [torch.full((m, n + 3), 7.0, device=hip_device)[:, :n] for m, n in shapes]
+        _call(mats, dst, L.ORTHO_FAST if precision == "fast" else L.ORTHO_FP32, co)
+        for i in {0, len(mats) // 2, len(mats) - 1}:
+            _check(dst[i], mats[i], co, precision, f"matrix {i}")
+        assert all(bool((d.as_strided((d.shape[0], 3), (d.stride(0), 1), d.shape[1]) == 7.0).all())
+                   for d in dst)
+
+
+def test_panels_of_nan_and_zeros(hip_device):
+    for dtype in TYPES:
+        mats = [_update(hip_device, i, 300, 200, dtype) for i in range(4)]
+        alone = scao_amd.orthogonalize(mats)
+        bad = [t.clone() for t in mats]
+        bad[1][299, 199] = float("nan")
+        bad[2].zero_()
+        got = scao_amd.orthogonalize(bad)
+        assert torch.equal(got[0], alone[0]) and torch.equal(got[3], alone[3])
+        assert bool(got[1].isnan().all()) and bool((got[2] == 0).all())
+
+
+@pytest.mark.parametrize("m,n", [(256, 256), (300, 160)])
+def test_panels_with_strong_growth(hip_device, m, n):
+    """Singular values that the first step takes far up and the second far down."""
+    g = _update(hip_device, 9, m, n, torch.float32)
+    co = [(30.0, 0.0, 0.0), (1.0 / 16, 2.0 ** -14, 2.0 ** -24), (0.5, 0.125, 0.0)]
+    for dtype, precision in ((torch.float32, "fp32"), (torch.bfloat16, "fast")):
+        got = scao_amd.orthogonalize(g, steps=3, coefficients=co, dtype=dtype)
+        _check(got, g, co, precision, "growth")
+
+
 # sizes whose products take 256 x 256 tiles, tiles in parts, and both
 @pytest.mark.parametrize("m,n,many", [(2048, 2048, 1), (2048, 2048, 3), (4096, 512, 2),
                                       (1030, 4100, 2), (4100, 1030, 2), (640, 640, 30)])
