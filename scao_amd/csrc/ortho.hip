@@ -486,15 +486,22 @@ int64_t workspace_of(const std::vector<Matrix>& m, int steps) {
 }
 
 // Whether a workgroup holds every matrix whole: then the call is one launch for up to
-// 64 of them.  (Among larger ones small matrices share those's launches.)
+// 64 of them.  (Among larger ones small matrices share those's launches.)  A few of
+// more than 96 rows are shorter by panels, which share a matrix among workgroups: one of
+// 112 x 112 62 us and 48, of 128 x 128 65 and 49, eight 67 and 55, but 32 68 and 75.
 bool all_small(const std::vector<Matrix>& m, int steps) {
   if (steps > SMALL_STEPS) return false;
-  for (const Matrix& e : m)
-    if (e.rows && e.cols &&
-        (e.smaller() > SMALL_SIDE || e.larger() > 4096 ||
-         small_lds((int)e.smaller(), (int)e.larger()) > SMALL_LDS))
+  int n = 0;
+  int64_t most = 0;
+  for (const Matrix& e : m) {
+    if (!e.rows || !e.cols) continue;
+    if (e.smaller() > SMALL_SIDE || e.larger() > 4096 ||
+        small_lds((int)e.smaller(), (int)e.larger()) > SMALL_LDS)
       return false;
-  return true;
+    ++n;
+    most = std::max(most, e.smaller());
+  }
+  return most <= 96 || n > 16;
 }
 int run_small(const char* who, const std::vector<Matrix>& m, const Scales& sc, int steps, double eps,
               double momentum, bool nesterov, int dest, hipStream_t st) {

@@ -16,6 +16,15 @@
 // a load, a step of 256 x 256 took 22 us).  Zeros up to 32 rows and columns.
 //
 // Sums, b Y and a X' are fp32; A', Y and A'' are rounded to the words of the group.
+//
+// What bounds it: reads of X from L2, 13 to 20 us a MB and panel, and about 0.8 us a
+// product until its first sums.  Five steps of 256 x 256 in one word: 59 us, of which
+// the launches alone are 25 (tiles 125; 16 matrices 85 and 129, 64 240 and 151); of two
+// words 89 (162); 384 x 384 105 (145), 512 x 512 155 (161), 256 x 1024 177 (138).  The
+// host takes whichever its estimates say.  With one word and up to 256 columns a wave's
+// pieces of X, in either order, stay in its registers for the step: 70 to 63 us of 256 x
+// 256.  The first pieces of a product fetched before the barrier ahead of it spill:
+// slower in every other case (512 x 512: 156 to 184).
 #pragma once
 
 #include "ortho_small.hpp"

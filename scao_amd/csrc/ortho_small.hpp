@@ -3,8 +3,9 @@
 //
 // A tile's beginning and end and a launch's own time are nearly all of a small
 // product: a call of 2 + 3 launches a step takes 8 us a launch whatever it multiplies.
-// Here a step is three passes over LDS.  Five steps of 32 x 32 take 15 us, of 64 x 64
-// 21, 96 x 160 47, 128 x 128 66 (by tiles 135 and more); 64 matrices as long as one.
+// Here a step is three passes over LDS.  Five steps of 32 x 32 take 16 us, of 64 x 64
+// 21, 96 x 96 37, 128 x 128 65 (by tiles 135 and more, by panels 34, 37, 43 and 49);
+// 32 matrices as long as one.
 // Bound by LDS reads (a fragment of either operand, 4 KB, for three 16 x 16 x 32
 // products) and their latency: eight waves instead of sixteen take half as long again.
 //

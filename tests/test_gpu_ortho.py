@@ -174,6 +174,17 @@ def test_panels(hip_device, shapes, dtype):
                    for d in dst)
 
 
+def test_many_of_128_rows(hip_device):
+    """17 of them are a workgroup's each, 16 go by panels."""
+    for dtype, precision in ((torch.float32, "fp32"), (torch.bfloat16, "fast")):
+        mats = [_update(hip_device, i, *((128, 128), (100, 120), (121, 97))[i % 3], dtype)
+                for i in range(17)]
+        for n in (17, 16):
+            got = scao_amd.orthogonalize(mats[:n], steps=3, coefficients=QUINTIC)
+            for i in range(5):
+                _check(got[i], mats[i], triples(QUINTIC, 3), precision, f"{n} of")
+
+
 def test_panels_of_nan_and_zeros(hip_device):
     for dtype in TYPES:
         mats = [_update(hip_device, i, 300, 200, dtype) for i in range(4)]
