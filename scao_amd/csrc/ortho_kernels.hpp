@@ -19,10 +19,10 @@
 // tile's end, when all of the chip does (3.6% of the time).
 //
 // What bounds it: the chip's power in long updates (14336 x 4096: matrix cores busy 66%
-// of the cycles at 1.85 GHz, 374 us an update, 1.29 PFLOP/s); the count of tiles in the
-// symmetric products (136 of 256 x 256 on 256 CUs: 98 us for 4096 x 4096, 230 in three
-// parts for the Gram matrix over 14336); launches for small matrices, about 5 us each
-// whatever they hold.
+// of the cycles at 1.85 GHz, 378 us an update, 1.27 PFLOP/s); the count of tiles in the
+// symmetric products (136 of 256 x 256 on 256 CUs; 528 of 128 x 128, the 16 behind the
+// last round in 16 parts: 86 us for 4096 x 4096 with their join, 271 for the Gram matrix
+// over 14336); launches for small matrices, about 5 us each whatever they hold.
 //
 // All matrices of a call go through the same launches, whatever their shapes: a
 // launch's tiles are those of up to ORTHO_GROUPS groups of one shape each, the ones
