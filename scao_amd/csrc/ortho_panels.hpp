@@ -17,7 +17,7 @@
 //
 // Sums, b Y and a X' are fp32; A', Y and A'' are rounded to the words of the group.
 //
-// What bounds it: reads of X from L2, 13 to 20 us a MB and panel, and about 0.8 us a
+// What bounds it: reads of X from L2, 7.5 to 15 us a MB and panel, and about 0.8 us a
 // product until its first sums.  Five steps of 256 x 256 in one word: 59 us, of which
 // the launches alone are 25 (tiles 125; 16 matrices 85 and 129, 64 240 and 151); of two
 // words 89 (162); 384 x 384 105 (145), 512 x 512 155 (161), 256 x 1024 177 (138).  The
