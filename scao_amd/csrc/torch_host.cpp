@@ -873,6 +873,15 @@ void check_rope(ROPE_PARAMS) {
 Tensor unit_columns(const Tensor& t) {
   return t.stride(-1) == 1 || t.size(-1) <= 1 ? t : t.contiguous();
 }
+// Fresh memory for what the kernels write of t's shape: in t's order where the columns
+// come out with unit stride, which is how they are written.  (Of a view whose tokens or
+// sequences overlap, empty_like may put the columns outside of them.)
+Tensor empty_columns(const Tensor& t) {
+  const Tensor out = at::empty_like(t);
+  return out.stride(-1) == 1 || out.size(-1) <= 1
+             ? out
+             : at::empty_like(t, t.options(), at::MemoryFormat::Contiguous);
+}
 scao_rope_tensor rope_tensor(const Tensor& t) {
   return {t.data_ptr(), t.stride(0), t.stride(1), t.stride(2)};
 }
@@ -927,7 +936,7 @@ std::tuple<Tensor, Tensor> qk_norm_rope_hip(ROPE_PARAMS) {
   check_rope(ROPE_ARGS);
   const c10::DeviceGuard guard(q.device());
   const Rope r(ROPE_ARGS);
-  const Tensor yq = at::empty_like(r.q), yk = at::empty_like(r.k);
+  const Tensor yq = empty_columns(r.q), yk = empty_columns(r.k);
   const scao_rope_tensor y[2] = {rope_tensor(yq), rope_tensor(yk)};
   check(lib.rope_forward(&r.d, y, stream_of(q)), "scao_qk_rope_forward");
   return {yq, yk};
@@ -950,7 +959,7 @@ std::vector<Tensor> qk_norm_rope_backward_hip(const Tensor& dq_, const Tensor& d
   void* dw[2] = {};
   for (int i = 0; i < 2; ++i)
     if (wanted >> i & 1) {
-      out.push_back(at::empty_like(i ? r.k : r.q));
+      out.push_back(empty_columns(i ? r.k : r.q));
       dx[i] = rope_tensor(out.back());
     }
   for (int i = 0; i < 2; ++i)
@@ -967,13 +976,13 @@ std::vector<Tensor> qk_norm_rope_backward_hip(const Tensor& dq_, const Tensor& d
 
 std::tuple<Tensor, Tensor> qk_norm_rope_meta(ROPE_PARAMS) {
   check_rope(ROPE_ARGS);
-  return {at::empty_like(q), at::empty_like(k)};
+  return {empty_columns(q), empty_columns(k)};
 }
 std::vector<Tensor> qk_norm_rope_backward_meta(const Tensor&, const Tensor&, ROPE_PARAMS,
                                                int64_t wanted) {
   std::vector<Tensor> out;
-  if (wanted & 1) out.push_back(at::empty_like(q));
-  if (wanted & 2) out.push_back(at::empty_like(k));
+  if (wanted & 1) out.push_back(empty_columns(q));
+  if (wanted & 2) out.push_back(empty_columns(k));
   if (wanted & 4) out.push_back(at::empty_like(*wq));
   if (wanted & 8) out.push_back(at::empty_like(*wk));
   return out;

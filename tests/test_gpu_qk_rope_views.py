@@ -1,0 +1,41 @@
+"""Queries and keys in views of any strides, overlapping ones among them: the same bits
+as of contiguous copies, forward and backward."""
+
+from __future__ import annotations
+
+import pytest
+import torch
+
+import scao_amd
+from tests.test_qk_rope_layouts import VIEWS, view
+
+pytestmark = pytest.mark.gpu
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("which", VIEWS)
+def test_views(hip_device, which, dtype):
+    g = torch.Generator(device=hip_device).manual_seed(3)
+
+    def normal(*shape):
+        return torch.randn(*shape, generator=g, device=hip_device).to(dtype)
+
+    def pair():
+        return view(normal(4, 1000), which), view(normal(4, 1000), which)[:, :, :1]
+
+    inputs, gradients = pair(), pair()
+    dim = inputs[0].shape[-1]
+    weights = normal(dim), normal(dim)
+    cos, sin = scao_amd.rotary_table(64, dim // 2 * 2, device=hip_device)
+
+    def run(form):
+        # (the leaves keep their strides: nothing copies them ahead of the operator)
+        leaves = [form(t).detach().requires_grad_() for t in inputs]
+        leaves += [w.clone().requires_grad_() for w in weights]
+        alone = scao_amd.qk_norm_rope(*(t.detach() for t in leaves), cos, sin)
+        y = scao_amd.qk_norm_rope(*leaves, cos, sin)
+        return *alone, *y, *torch.autograd.grad(y, leaves, [form(t) for t in gradients])
+
+    for a, b in zip(run(lambda t: t), run(lambda t: t.contiguous())):
+        assert a.shape == b.shape and torch.equal(a, b)
+        assert not bool(a.isnan().any())
