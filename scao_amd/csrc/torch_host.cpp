@@ -976,13 +976,13 @@ std::vector<Tensor> qk_norm_rope_backward_hip(const Tensor& dq_, const Tensor& d
 
 std::tuple<Tensor, Tensor> qk_norm_rope_meta(ROPE_PARAMS) {
   check_rope(ROPE_ARGS);
-  return {empty_columns(q), empty_columns(k)};
+  return {empty_columns(unit_columns(q)), empty_columns(unit_columns(k))};
 }
 std::vector<Tensor> qk_norm_rope_backward_meta(const Tensor&, const Tensor&, ROPE_PARAMS,
                                                int64_t wanted) {
   std::vector<Tensor> out;
-  if (wanted & 1) out.push_back(empty_columns(q));
-  if (wanted & 2) out.push_back(empty_columns(k));
+  if (wanted & 1) out.push_back(empty_columns(unit_columns(q)));
+  if (wanted & 2) out.push_back(empty_columns(unit_columns(k)));
   if (wanted & 4) out.push_back(at::empty_like(*wq));
   if (wanted & 8) out.push_back(at::empty_like(*wk));
   return out;

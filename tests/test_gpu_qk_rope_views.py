@@ -39,3 +39,18 @@ def test_views(hip_device, which, dtype):
     for a, b in zip(run(lambda t: t), run(lambda t: t.contiguous())):
         assert a.shape == b.shape and torch.equal(a, b)
         assert not bool(a.isnan().any())
+
+
+@pytest.mark.parametrize("which", VIEWS)
+def test_a_trace_says_how_outputs_lie(hip_device, which):
+    scao_amd._lib.torch_host()
+    x = torch.randn(4, 1000, device=hip_device)
+    strides = []
+    for t in (x, x.to("meta")):
+        q = view(t, which)
+        table = torch.ones(64, q.shape[-1] // 2, device=t.device)
+        rest = q, q, None, None, table, table, None, 1e-6, False
+        y = torch.ops.scao_amd.qk_norm_rope(*rest)
+        dx = torch.ops.scao_amd.qk_norm_rope_backward(q, q, *rest, 3)
+        strides.append([o.stride() for o in (*y, *dx)])
+    assert strides[0] == strides[1]

@@ -44,3 +44,17 @@ def test_outputs_have_unit_columns(which):
         assert t.stride(-1) == 1 or t.shape[-1] == 1
         # no two elements of one place
         assert torch._prims_common.is_non_overlapping_and_dense(t)
+
+
+def test_copied_inputs_have_contiguous_outputs():
+    """Columns of another stride are copied ahead of the kernels, which is what a trace has
+    to say of their outputs."""
+    scao_amd._lib.torch_host()
+    q = view(torch.empty(4, 1000, device="meta"), "columns before heads")
+    assert q.stride() == (1000, 320, 1, 5)
+    table = torch.empty(8, 32, device="meta")
+    y = torch.ops.scao_amd.qk_norm_rope(q, q, None, None, table, table, None, 1e-6, False)
+    dx = torch.ops.scao_amd.qk_norm_rope_backward(*y, q, q, None, None, table, table, None, 1e-6,
+                                                  False, 3)
+    for t in (*y, *dx):
+        assert t.shape == q.shape and t.is_contiguous()
