@@ -858,6 +858,10 @@ void check_rope(ROPE_PARAMS) {
                   cos.sym_sizes() == sin.sym_sizes() && cos.sym_size(1) * 2 <= q.sym_size(3),
               "qk_norm_rope: cos and sin must be float32 tables of at most half a head's columns "
               "on q's device");
+  TORCH_CHECK(q.sym_size(3) >= 1 && q.sym_size(3) <= 512 && q.sym_size(2) >= 1 &&
+                  k.sym_size(2) >= 1,
+              "qk_norm_rope takes heads of 1 to 512 columns, one at least: q ", q.sym_sizes(),
+              ", k ", k.sym_sizes());
   TORCH_CHECK(eps >= 0 && std::isfinite(eps), "qk_norm_rope: eps ", eps);
   TORCH_CHECK(positions || cos.sym_size(1) == 0 || q.sym_size(1) <= cos.sym_size(0),
               "qk_norm_rope: ", q.sym_size(1), " tokens and tables of ", cos.sym_size(0),
@@ -868,6 +872,17 @@ void check_rope(ROPE_PARAMS) {
                              positions->sym_size(0) == q.sym_size(0) &&
                              positions->sym_size(1) == q.sym_size(1)),
               "qk_norm_rope: positions must be int64 or int32, one a token, on q's device");
+}
+
+void check_rope_gradients(const Tensor& dq, const Tensor& dk, const Tensor& q, const Tensor& k,
+                          const std::optional<Tensor>& wq, const std::optional<Tensor>& wk,
+                          int64_t wanted) {
+  TORCH_CHECK(dq.sym_sizes() == q.sym_sizes() && dk.sym_sizes() == k.sym_sizes() &&
+                  dq.scalar_type() == q.scalar_type() && dk.scalar_type() == k.scalar_type() &&
+                  dq.device() == q.device() && dk.device() == q.device(),
+              "qk_norm_rope_backward: the gradients are not like q and k");
+  TORCH_CHECK((wq || !(wanted & 4)) && (wk || !(wanted & 8)),
+              "qk_norm_rope_backward: no weight, no gradient");
 }
 
 Tensor unit_columns(const Tensor& t) {
@@ -945,12 +960,7 @@ std::tuple<Tensor, Tensor> qk_norm_rope_hip(ROPE_PARAMS) {
 std::vector<Tensor> qk_norm_rope_backward_hip(const Tensor& dq_, const Tensor& dk_, ROPE_PARAMS,
                                               int64_t wanted) {
   check_rope(ROPE_ARGS);
-  TORCH_CHECK(dq_.sizes() == q.sizes() && dk_.sizes() == k.sizes() &&
-                  dq_.scalar_type() == q.scalar_type() && dk_.scalar_type() == k.scalar_type() &&
-                  dq_.device() == q.device() && dk_.device() == q.device(),
-              "qk_norm_rope_backward: the gradients are not like q and k");
-  TORCH_CHECK((wq || !(wanted & 4)) && (wk || !(wanted & 8)),
-              "qk_norm_rope_backward: no weight, no gradient");
+  check_rope_gradients(dq_, dk_, q, k, wq, wk, wanted);
   const c10::DeviceGuard guard(q.device());
   const Rope r(ROPE_ARGS);
   const Tensor dq = unit_columns(dq_), dk = unit_columns(dk_);
@@ -978,8 +988,10 @@ std::tuple<Tensor, Tensor> qk_norm_rope_meta(ROPE_PARAMS) {
   check_rope(ROPE_ARGS);
   return {empty_columns(unit_columns(q)), empty_columns(unit_columns(k))};
 }
-std::vector<Tensor> qk_norm_rope_backward_meta(const Tensor&, const Tensor&, ROPE_PARAMS,
+std::vector<Tensor> qk_norm_rope_backward_meta(const Tensor& dq, const Tensor& dk, ROPE_PARAMS,
                                                int64_t wanted) {
+  check_rope(ROPE_ARGS);
+  check_rope_gradients(dq, dk, q, k, wq, wk, wanted);
   std::vector<Tensor> out;
   if (wanted & 1) out.push_back(empty_columns(unit_columns(q)));
   if (wanted & 2) out.push_back(empty_columns(unit_columns(k)));
