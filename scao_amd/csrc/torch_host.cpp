@@ -600,12 +600,21 @@ void check_matrices(at::TensorList list, const char* name, c10::Device on) {
                 t.scalar_type(), ", ", t.layout(), ", ", t.device(), ")");
     TORCH_CHECK(t.dim() >= 2, name, " must be matrices or stacks of matrices (got ",
                 t.sym_sizes(), ")");
+    const auto rows = t.sym_size(-2), cols = t.sym_size(-1);
+    constexpr int64_t SIDE = (int64_t)1 << 20, SMALLER = (int64_t)1 << 15;   // scao_train.h's
+    TORCH_CHECK(t.sym_numel() == 0 ||
+                    (rows < SIDE && cols < SIDE && (rows <= SMALLER || cols <= SMALLER)), name,
+                " must have sides below 2^20, the smaller one up to 2^15 (got ", t.sym_sizes(), ")");
   }
+}
+void check_result(std::optional<at::ScalarType> dtype) {
+  TORCH_CHECK(!dtype || code_of(*dtype) >= 0, "orthogonalize: no result of type ", *dtype);
 }
 void check_scheme(at::ArrayRef<double> coefficients) {
   TORCH_CHECK(lib.orthogonalize, "orthogonalize: scao_amd has not loaded its library");
-  TORCH_CHECK(!coefficients.empty() && coefficients.size() % 3 == 0,
-              "orthogonalize: three coefficients a step");
+  TORCH_CHECK(!coefficients.empty() && coefficients.size() % 3 == 0 &&
+                  coefficients.size() <= 3 * 64,
+              "orthogonalize: three coefficients a step, up to 64 steps");
 }
 
 // the matrices of a stack, whose rows are unit-strided and apart
@@ -640,7 +649,7 @@ std::vector<Tensor> orthogonalize_hip(at::TensorList updates, at::ArrayRef<doubl
   std::vector<Tensor> out;
   if (updates.empty()) return out;
   check_matrices(updates, "updates", updates[0].device());
-  TORCH_CHECK(!dtype || code_of(*dtype) >= 0, "orthogonalize: no result of type ", *dtype);
+  check_result(dtype);
   const c10::DeviceGuard guard(updates[0].device());
   std::vector<Tensor> in;
   std::vector<scao_ortho_desc> table;
@@ -665,11 +674,9 @@ std::vector<Tensor> orthogonalize_hip(at::TensorList updates, at::ArrayRef<doubl
   return out;
 }
 
-void muon_step_hip_(at::TensorList params, at::TensorList grads, at::TensorList momenta,
-                    at::ArrayRef<double> rates, at::ArrayRef<double> decays, double momentum,
-                    bool nesterov, at::ArrayRef<double> coefficients, double eps,
-                    at::IntArrayRef precisions) {
-  check_scheme(coefficients);
+void check_step(at::TensorList params, at::TensorList grads, at::TensorList momenta,
+                at::ArrayRef<double> rates, at::ArrayRef<double> decays,
+                at::IntArrayRef precisions) {
   const size_t n = params.size();
   TORCH_CHECK(grads.size() == n && momenta.size() == n && rates.size() == n && decays.size() == n &&
                   precisions.size() == n,
@@ -678,15 +685,29 @@ void muon_step_hip_(at::TensorList params, at::TensorList grads, at::TensorList 
   const c10::Device on = params[0].device();
   check_matrices(params, "parameters", on);
   check_matrices(grads, "gradients", on);
+  for (size_t i = 0; i < n; ++i) {
+    const Tensor &p = params[i], &m = momenta[i];
+    TORCH_CHECK(p.is_contiguous() && !p.is_neg() && m.is_contiguous() && !m.is_neg() &&
+                    m.scalar_type() == at::kFloat && m.device() == on &&
+                    m.sym_sizes() == p.sym_sizes() && grads[i].sym_sizes() == p.sym_sizes(),
+                "muon_step_: a parameter and its momentum must be contiguous, the momentum "
+                "float32, and both and the gradient of one shape");
+  }
+}
+void muon_step_hip_(at::TensorList params, at::TensorList grads, at::TensorList momenta,
+                    at::ArrayRef<double> rates, at::ArrayRef<double> decays, double momentum,
+                    bool nesterov, at::ArrayRef<double> coefficients, double eps,
+                    at::IntArrayRef precisions) {
+  check_scheme(coefficients);
+  check_step(params, grads, momenta, rates, decays, precisions);
+  const size_t n = params.size();
+  if (!n) return;
+  const c10::Device on = params[0].device();
   const c10::DeviceGuard guard(on);
   std::vector<Tensor> copies;
   std::vector<scao_muon_desc> table;
   for (size_t i = 0; i < n; ++i) {
     const Tensor &p = params[i], &m = momenta[i];
-    TORCH_CHECK(p.is_contiguous() && !p.is_neg() && m.is_contiguous() && !m.is_neg() && m.scalar_type() == at::kFloat &&
-                    m.device() == on && m.sizes() == p.sizes() && grads[i].sizes() == p.sizes(),
-                "muon_step_: a parameter and its momentum must be contiguous, the momentum "
-                "float32, and both and the gradient of one shape");
     copies.push_back(grads[i].resolve_neg().contiguous());
     const char* g = (const char*)copies.back().data_ptr();
     float* buf = (float*)m.data_ptr();
@@ -725,15 +746,16 @@ std::vector<Tensor> orthogonalize_meta(at::TensorList updates, at::ArrayRef<doub
   check_scheme(coefficients);
   std::vector<Tensor> out;
   if (!updates.empty()) check_matrices(updates, "updates", updates[0].device());
+  check_result(dtype);
   for (const Tensor& t : updates)
     out.push_back(at::empty_symint(t.sym_sizes(), t.options().dtype(dtype.value_or(t.scalar_type()))));
   return out;
 }
-void muon_step_meta_(at::TensorList params, at::TensorList, at::TensorList, at::ArrayRef<double>,
-                     at::ArrayRef<double>, double, bool, at::ArrayRef<double> coefficients, double,
-                     at::IntArrayRef) {
+void muon_step_meta_(at::TensorList params, at::TensorList grads, at::TensorList momenta,
+                     at::ArrayRef<double> rates, at::ArrayRef<double> decays, double, bool,
+                     at::ArrayRef<double> coefficients, double, at::IntArrayRef precisions) {
   check_scheme(coefficients);
-  if (!params.empty()) check_matrices(params, "parameters", params[0].device());
+  check_step(params, grads, momenta, rates, decays, precisions);
 }
 
 bool tangent(at::TensorList list) {

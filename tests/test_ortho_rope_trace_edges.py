@@ -36,3 +36,36 @@ def test_a_trace_refuses_the_heads_that_the_kernels_refuse():
             back(*gradients, *_heads(), 3)
     with pytest.raises(RuntimeError, match="no weight"):
         back(*y, *_heads(), 4)
+
+
+def test_a_trace_refuses_the_updates_that_the_kernels_refuse():
+    scao_amd._lib.torch_host()
+    op, co = torch.ops.scao_amd.orthogonalize, [1.5, -0.5, 0.0]
+    m = torch.empty(8, 16, device="meta")
+    assert op([m], co, 1e-7, torch.bfloat16)[0].dtype == torch.bfloat16
+    assert op([torch.empty(0, 1 << 21, device="meta")], co, 1e-7, None)[0].shape == (0, 1 << 21)
+    for args in (([m], co, 1e-7, torch.float64), ([m.double()], co, 1e-7, None),
+                 ([m[0]], co, 1e-7, None), ([m], co[:2], 1e-7, None), ([m], co * 65, 1e-7, None),
+                 ([m], [], 1e-7, None), ([torch.empty(1 << 20, 4, device="meta")], co, 1e-7, None),
+                 ([torch.empty(40000, 40000, device="meta")], co, 1e-7, None)):
+        with pytest.raises(RuntimeError):
+            op(*args)
+
+
+def test_a_trace_refuses_the_steps_that_the_kernels_refuse():
+    scao_amd._lib.torch_host()
+    op = torch.ops.scao_amd.muon_step_
+    p, m = torch.empty(8, 16, device="meta"), torch.empty(8, 16, device="meta")
+
+    def step(params=(p,), grads=(p,), momenta=(m,), rates=(0.1,), decays=(1.0,), precisions=(0,)):
+        op(list(params), list(grads), list(momenta), list(rates), list(decays), 0.9, True,
+           [1.5, -0.5, 0.0], 1e-7, list(precisions))
+
+    step()
+    for bad in (dict(grads=()), dict(momenta=(m, m)), dict(rates=()), dict(decays=(1.0, 1.0)),
+                dict(precisions=()), dict(momenta=(m.bfloat16(),)), dict(momenta=(m[:, :8],)),
+                dict(grads=(p.t(),)), dict(grads=(p.double(),)),
+                dict(params=(p.t(),), grads=(p.t(),), momenta=(m.t(),)),
+                dict(params=(p[0],), grads=(p[0],), momenta=(m[0],))):
+        with pytest.raises(RuntimeError):
+            step(**bad)
