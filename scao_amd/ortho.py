@@ -161,6 +161,12 @@ class Muon(torch.optim.Optimizer):
             buf = state["momentum_buffer"] = buf.to(torch.float32).contiguous()
         return buf
 
+    def __setstate__(self, state: dict) -> None:
+        """(the groups of torch.optim.Muon know no ns_dtype)"""
+        super().__setstate__(state)
+        for group in self.param_groups:
+            group.setdefault("ns_dtype", self.defaults["ns_dtype"])
+
     def load_state_dict(self, state_dict: dict) -> None:
         """(torch's own would round the momentum to the parameter's type.)"""
         super().load_state_dict(state_dict)

@@ -1,0 +1,36 @@
+"""What Muon does on the host, over tensors without memory: no GPU needed."""
+
+from __future__ import annotations
+
+import copy
+import pickle
+
+import pytest
+import torch
+from torch._subclasses.fake_tensor import FakeTensorMode
+
+import scao_amd
+
+
+def _params(n=2):
+    return [torch.nn.Parameter(torch.randn(3, 5)) for _ in range(n)]
+
+
+@pytest.mark.parametrize("ns_dtype", [None, torch.bfloat16])
+def test_a_state_of_the_optimizer_whose_arguments_these_are(ns_dtype):
+    """torch.optim.Muon's groups know no ns_dtype: it stays as it was given here."""
+    if not hasattr(torch.optim, "Muon"):
+        pytest.skip("a torch without Muon")
+    theirs = torch.optim.Muon(_params(), lr=0.3, weight_decay=0.2)
+    for p in theirs.param_groups[0]["params"]:
+        theirs.state[p]["momentum_buffer"] = torch.randn(3, 5)
+    ours = scao_amd.Muon(_params(), ns_dtype=ns_dtype)
+    ours.load_state_dict(theirs.state_dict())
+    group = ours.param_groups[0]
+    assert (group["lr"], group["weight_decay"], group["ns_dtype"]) == (0.3, 0.2, ns_dtype)
+    assert len(ours._check(group)) == 3 * 5
+    for p, q in zip(group["params"], theirs.param_groups[0]["params"]):
+        assert torch.equal(ours.state[p]["momentum_buffer"], theirs.state[q]["momentum_buffer"])
+    # and what is copied or pickled has it too
+    for twin in (copy.deepcopy(ours), pickle.loads(pickle.dumps(ours))):
+        assert twin.param_groups[0]["ns_dtype"] is ns_dtype
