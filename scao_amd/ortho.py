@@ -103,7 +103,8 @@ class Muon(torch.optim.Optimizer):
     ``momentum_buffer`` are those of ``torch.optim.Muon``; the buffer is float32
     whatever the parameter's type is.  Parameters are contiguous matrices, or
     stacks of them with the matrices last; vectors and embeddings belong to
-    another optimizer, such as ``SCAO``.  One call steps all parameters.
+    another optimizer, such as ``SCAO``.  One call steps all parameters.  A step can be
+    captured into a graph once a step before it has made the momentum.
 
     ns_dtype: how exact the orthogonalised update is (``orthogonalize``):
     torch.float32, torch.bfloat16, or None: float32 for float32 parameters."""
@@ -154,10 +155,15 @@ class Muon(torch.optim.Optimizer):
     def _momentum(self, p: Tensor) -> Tensor:
         state = self.state[p]
         buf = state.get("momentum_buffer")
+        ready = buf is not None and buf.dtype == torch.float32 and buf.is_contiguous()
+        if not ready and torch.cuda.is_initialized() and torch.cuda.is_current_stream_capturing():
+            # every replay would start again from the momentum as it is made here
+            raise RuntimeError("Muon's first step, which makes the momentum, cannot be captured: "
+                               "take one before the capture")
         if buf is None:
             buf = state["momentum_buffer"] = torch.zeros(p.shape, dtype=torch.float32,
                                                          device=p.device)
-        elif buf.dtype != torch.float32 or not buf.is_contiguous():   # another optimizer's state
+        elif not ready:   # another optimizer's state
             buf = state["momentum_buffer"] = buf.to(torch.float32).contiguous()
         return buf
 

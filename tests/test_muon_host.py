@@ -34,3 +34,23 @@ def test_a_state_of_the_optimizer_whose_arguments_these_are(ns_dtype):
     # and what is copied or pickled has it too
     for twin in (copy.deepcopy(ours), pickle.loads(pickle.dumps(ours))):
         assert twin.param_groups[0]["ns_dtype"] is ns_dtype
+
+
+def test_a_first_step_is_not_captured(monkeypatch):
+    """Replays of a graph that holds the momentum's zeroing would all start from zero."""
+    with FakeTensorMode():
+        p = torch.nn.Parameter(torch.empty(8, 16, device="cuda"))
+        p.grad = torch.empty(8, 16, device="cuda")
+        opt = scao_amd.Muon([p])
+        monkeypatch.setattr(torch.cuda, "is_initialized", lambda: True)
+        monkeypatch.setattr(torch.cuda, "current_device", lambda: 0)
+        monkeypatch.setattr(torch.cuda, "is_current_stream_capturing", lambda: True)
+        with pytest.raises(RuntimeError, match="captured"):
+            opt.step()
+        assert "momentum_buffer" not in opt.state[p]
+        # one of another type would be converted at every replay, from where it was
+        opt.state[p]["momentum_buffer"] = torch.empty(8, 16, device="cuda", dtype=torch.bfloat16)
+        with pytest.raises(RuntimeError, match="captured"):
+            opt.step()
+        opt.state[p]["momentum_buffer"] = torch.empty(8, 16, device="cuda")
+        opt.step()
