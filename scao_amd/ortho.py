@@ -191,6 +191,7 @@ class Muon(torch.optim.Optimizer):
             with torch.enable_grad():
                 loss = closure()
         host = L.torch_host()
+        queue = []   # what is refused here is refused before any group's step
         for group in self.param_groups:
             flat = self._check(group)
             lr, wd = float(group["lr"]), float(group["weight_decay"])
@@ -218,7 +219,8 @@ class Muon(torch.optim.Optimizer):
                 for to, x in zip(lists, (p, g, self._momentum(p), lr * ratio, 1.0 - lr * wd,
                                          L.ORTHO_FP32 if precise else L.ORTHO_FAST)):
                     to.append(x)
-            for *lists, precisions in calls.values():
-                host.muon_step(*lists, float(group["momentum"]), bool(group["nesterov"]), flat,
-                               float(group["eps"]), precisions)
+            queue += [(*lists, float(group["momentum"]), bool(group["nesterov"]), flat,
+                       float(group["eps"]), precisions) for *lists, precisions in calls.values()]
+        for call in queue:
+            host.muon_step(*call)
         return loss

@@ -54,3 +54,24 @@ def test_a_first_step_is_not_captured(monkeypatch):
             opt.step()
         opt.state[p]["momentum_buffer"] = torch.empty(8, 16, device="cuda")
         opt.step()
+
+
+def test_a_refused_step_steps_no_group(monkeypatch):
+    steps = []
+    monkeypatch.setattr(scao_amd._lib.torch_host(), "muon_step", lambda *a: steps.append(a))
+    with FakeTensorMode():
+        good, bad = (torch.nn.Parameter(torch.empty(s, device="cuda")) for s in ((8, 16), (4, 4)))
+        good.grad, bad.grad = torch.empty(8, 16, device="cuda"), torch.empty(4, 4, device="cuda")
+        opt = scao_amd.Muon([dict(params=[good]), dict(params=[bad])])
+        opt.step()
+        assert len(steps) == 2
+        turned = torch.nn.Parameter(torch.empty(4, 6, device="cuda").t())
+        turned.grad = torch.empty(6, 4, device="cuda")
+        opt.add_param_group(dict(params=[turned]))
+        with pytest.raises(ValueError, match="contiguous"):
+            opt.step()
+        turned.grad = None
+        opt.param_groups[1]["lr"] = float("nan")
+        with pytest.raises(ValueError, match="lr"):
+            opt.step()
+        assert len(steps) == 2
