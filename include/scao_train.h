@@ -149,6 +149,7 @@ int scao_muon_step(const scao_muon_desc* matrices, int n, double momentum, int n
  * columns.  w null: ones.  backward: dx (p null: not wanted) and dw (null: not
  * wanted), summed in a fixed order without atomics; the angles have no gradient.
  * Batch, token and head strides of any tensor are free; outputs may not overlap.
+ * A call takes fewer than 2^32 lanes: up to 64 for four heads of q or k of a token.
  * workspace: scao_qk_rope_backward_workspace() bytes, aligned to 16; needed for
  * the weights' gradients. */
 typedef struct scao_rope_tensor {  /* HOST; strides in elements                  */

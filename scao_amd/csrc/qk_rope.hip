@@ -59,7 +59,7 @@ struct Args {
   int64_t table;             // rows of the tables
   int dim, half;             // columns; half the rotated ones
   int wide_positions;
-  int lanes, pairs;          // a head's lanes and pairs of pieces
+  int lanes;                 // of a head
   float eps;
 };
 
@@ -524,9 +524,9 @@ Args args_of(const scao_rope_desc& d, int run, int v) {
   a.half = d.rotary / 2;
   a.wide_positions = d.wide_positions != 0;
   a.eps = d.eps;
-  a.pairs = (d.dim + 2 * v - 1) / (2 * v);
+  const int pairs = (d.dim + 2 * v - 1) / (2 * v);   // of pieces
   a.lanes = 1;
-  while (a.lanes < a.pairs && a.lanes < 64) a.lanes *= 2;
+  while (a.lanes < pairs && a.lanes < 64) a.lanes *= 2;
   for (int i = 0; i < 2; ++i) {
     Side& s = a.s[i];
     const scao_rope_tensor& x = d.x[i];
@@ -601,6 +601,9 @@ extern "C" int scao_qk_rope_forward(const scao_rope_desc* d, const scao_rope_ten
   for (int i = 0; i < 2; ++i) to_out(a.s[i], y[i]);
   const int64_t threads = (int64_t)a.tokens * (a.s[0].runs + a.s[1].runs) * a.lanes;
   const int64_t blocks = (threads + THREADS - 1) / THREADS;
+  SCAO_CHECK_ARG(blocks * THREADS < (int64_t)1 << 32,
+                 "%s: %lld tokens' heads take %lld lanes (below 2^32)", who, (long long)a.tokens,
+                 (long long)threads);
   for_variant(d->dtype, v, d->interleaved != 0, [&](auto type, auto piece, auto beside) {
     k_rope_forward<decltype(type)::value, decltype(piece)::value, decltype(beside)::value != 0>
         <<<(uint32_t)blocks, THREADS, 0, (hipStream_t)stream>>>(a);
