@@ -93,10 +93,11 @@ int scao_ffn_backward(const scao_ffn_desc* desc, const void* dy, int64_t ld_dy, 
  * polynomials a s + b s^3 + c s^5.  The matrices of a HOST table may differ in
  * shape, type and precision; all of them share the launches.  Rows have unit column
  * stride and a row stride of at least a row; src and dst may differ in type.
- *   SCAO_ORTHO_FAST  products of fp16 words with fp32 sums, X, A and B rounded to
- *                    11 significant bits once a step (the published five steps:
- *                    results about 1.2e-3 off, a bf16's own rounding 1.7e-3;
- *                    with up to 128 rows or columns as SCAO_ORTHO_FP32);
+ *   SCAO_ORTHO_FAST  products of fp16 words with fp32 sums, X, A and B (of some
+ *                    matrices of up to 512 x 1024: X and A X) rounded to 11
+ *                    significant bits once a step.  The published five steps:
+ *                    results 0.6e-3 to 1.4e-3 off, a bf16's own rounding 1.7e-3.
+ *                    With up to 128 rows or columns as SCAO_ORTHO_FP32;
  *   SCAO_ORTHO_FP32  words of 22 bits, three products each: fp32's accuracy.
  * A matrix with a NaN or an infinity (or with a sum of squares beyond double's
  * range) gives NaN throughout, and no other matrix; one of zeros gives zeros.

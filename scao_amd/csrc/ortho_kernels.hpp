@@ -13,8 +13,8 @@
 // powers of two that the host chooses from what the polynomial can reach, so that
 // neither end of fp16's range matters: |X|, |A| and |B| are bounded by their largest
 // singular value.  fp16 has three bits more than bf16 at the same rate; each of the
-// three is rounded once a step, which leaves results of 512 x 512 1.2e-3 off (five
-// steps), a bf16 result's own rounding 1.7e-3.  Sums and b A are fp32.  a is part of B:
+// three is rounded once a step, which leaves results of 640 x 640 1.2e-3 off (five
+// steps; 4096 x 1024 0.8e-3, 2048 x 512 1.4e-3), a bf16 result's own rounding 1.7e-3.  Sums and b A are fp32.  a is part of B:
 // a X beside the product is no more exact (1.3e-3), and would read X once more at every
 // tile's end, when all of the chip does (3.6% of the time).
 //

@@ -15,12 +15,17 @@
 // such piece, and none of X is read twice in a product (as rows, 16 pieces of 64 bytes
 // a load, a step of 256 x 256 took 22 us).  Zeros up to 32 rows and columns.
 //
-// Sums, b Y and a X' are fp32; A', Y and A'' are rounded to the words of the group.
+// Sums, b Y and a X' are fp32.  A' and A'' are rounded to two words whatever the group's
+// are, as an error of theirs reaches all that follows from them: with one word each,
+// results of 256 x 256 were 1.5e-3 off after the published five steps and those of 256 x
+// 1024 1.9e-3, where tiles leave 1.3e-3 and 1.1e-3; with two they are 1.0e-3 and 0.7e-3
+// off, in the time of one (256 x 256 59 us, 384 x 384 106 for 101).  X, and Y beside A' X,
+// have the group's words.
 //
 // What bounds it: reads of X from L2, 7.5 to 15 us a MB and panel, and about 0.8 us a
 // product until its first sums.  Five steps of 256 x 256 in one word: 59 us, of which
-// the launches alone are 25 (tiles 125; 16 matrices 85 and 129, 64 240 and 151); of two
-// words 89 (162); 384 x 384 105 (145), 512 x 512 155 (161), 256 x 1024 177 (138).  The
+// the launches alone are 25 (tiles 125; 16 matrices 82 and 129, 64 240 and 151); of two
+// words 86 (162); 384 x 384 106 (145), 512 x 512 152 (161), 256 x 1024 177 (138).  The
 // host takes whichever its estimates say.  With one word and up to 256 columns a wave's
 // pieces of X, in either order, stay in its registers for the step: 70 to 63 us of 256 x
 // 256.  The first pieces of a product fetched before the barrier ahead of it spill:
@@ -51,13 +56,14 @@ struct OrthoPanels {
   PanelGroup g[ORTHO_GROUPS];
   char* base;
   int groups;
-  float gram, second, third;        // of A', Y and A'' when they become words
+  float gram, second, third;        // of A', Y and A'' when they become words (A's two)
   float a, b, c;                    // of X's words, of Y's and of Z's sums
 };
 static_assert(sizeof(OrthoPanels) + sizeof(OrthoOut) <= 4096, "kernel arguments are limited to 4 KiB");
 
+// (panels of A and A A have two words whatever X has)
 __host__ __device__ inline int panel_lds(const PanelGroup& g) {
-  return g.words * PANEL * 2 * (2 * g.l + g.s);
+  return PANEL * 2 * (g.words * 2 * g.l + 2 * g.s);
 }
 // whether a wave's 128 registers hold its pieces of X in either order
 __host__ __device__ inline bool panel_held(const PanelGroup& g) { return g.words == 1 && g.l <= 256; }
@@ -74,8 +80,8 @@ __device__ __forceinline__ const PanelGroup& panel_group(const PanelGroup* g, in
 
 // Rows j .. j + 15 of a matrix in memory times the panel's, over k: what this lane holds
 // is of panel row lane % 16 and of rows j + 4 (lane / 16) .. + 3.  The next pieces are
-// under way during the products of some.
-template <int P>
+// under way during the products of some.  The panel has W words an element, the matrix P.
+template <int P, int W>
 struct PanelRows {
   static constexpr int STEPS = P == 1 ? 8 : 4;
   typedef v8s Pieces[STEPS][P];
@@ -100,15 +106,15 @@ struct PanelRows {
 #pragma unroll
     for (int h = 0; h < STEPS; ++h)
       if (k0 + h < pieces) {
-        const lchar* t = panel + (k0 + h) * P * 1024 + lane * 16;
+        const lchar* t = panel + (k0 + h) * W * 1024 + lane * 16;
         const v8s hi = *(const lv8s*)t;
-        if constexpr (P == 1) {
+        if constexpr (W == 1) {
           c[h & 1] = mma<true>(w[h][0], hi, c[h & 1]);
         } else {
           const v8s lo = *(const lv8s*)(t + 1024);
-          c[0] = mma<true>(w[h][1], hi, c[0]);
-          c[1] = mma<true>(w[h][0], lo, c[1]);
-          c[2] = mma<true>(w[h][0], hi, c[2]);
+          if constexpr (P == 2) c[2] = mma<true>(w[h][1], hi, c[2]);
+          c[0] = mma<true>(w[h][0], lo, c[0]);
+          c[1] = mma<true>(w[h][0], hi, c[1]);
         }
       }
   }
@@ -119,14 +125,14 @@ struct PanelRows {
     return sum(c);
   }
   static __device__ __forceinline__ v4f sum(const v4f (&c)[3]) {
-    return P == 1 ? c[0] + c[1] : (c[0] + c[1]) + c[2];
+    return P == 1 ? c[0] + c[1] : (c[2] + c[0]) + c[1];
   }
 };
-template <int P>
+template <int P, int W>
 __device__ __forceinline__ v4f panel_product(const char* x, int j, int k_end, const lchar* panel,
                                              int lane) {
-  PanelRows<P> r;
-  typename PanelRows<P>::Pieces next;
+  PanelRows<P, W> r;
+  typename PanelRows<P, W>::Pieces next;
   r.begin(x, j, k_end, lane);
   v4f c[3] = {};
   for (int k = 0; k < r.pieces; k += 2 * r.STEPS) {
@@ -167,7 +173,8 @@ __device__ __forceinline__ void ortho_panel(const OrthoPanels& p, const OrthoOut
   const int dm = lane & 15, dn = 4 * (lane >> 4);
 
   const int j0 = wave * 16;
-  PanelRows<P> r, c;
+  PanelRows<P, P> r;
+  PanelRows<P, 2> c;
   if (ALL && j0 < s) r.begin(rows, j0, l, lane);
   if (ALL && j0 < l) c.begin(columns, j0, s, lane);
   const char* mine = rows + (int64_t)panel * P * PANEL * l * 2;
@@ -178,14 +185,14 @@ __device__ __forceinline__ void ortho_panel(const OrthoPanels& p, const OrthoOut
     for (int j = j0; j < s; j += PANEL_WAVES * 16) {
       v4f u;
       if constexpr (ALL) u = r.product(t, lane);
-      else u = panel_product<P>(rows, j, l, t, lane);
-      panel_put<P>(a, dm, j + dn, u * scale);
+      else u = panel_product<P, P>(rows, j, l, t, lane);
+      panel_put<2>(a, dm, j + dn, u * scale);
     }
   };
   // the panel a times X
   auto by_columns = [&](int j) {
     if constexpr (ALL) return c.product(a, lane);
-    else return panel_product<P>(columns, j, s, a, lane);
+    else return panel_product<P, 2>(columns, j, s, a, lane);
   };
   __syncthreads();
   by_rows(x, p.gram);

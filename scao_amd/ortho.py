@@ -60,7 +60,8 @@ def orthogonalize(updates: Union[Tensor, Sequence[Tensor]], steps: int = 5,
     results' type, that of each update by default.
 
     bfloat16 results go through products of fp16 words (three bits more than
-    bfloat16's own, sums in float32; about 1.2e-3 off, their last rounding 1.7e-3);
+    bfloat16's own, sums in float32; 0.6e-3 to 1.4e-3 off with the defaults, their last
+    rounding 1.7e-3);
     float32 and float16 ones, and matrices of up to 128 rows or columns, through
     products of 22-bit words, at a third of the rate: pass ``dtype=torch.bfloat16``
     where that accuracy is not needed.  A matrix with a NaN or an infinity gives NaN
