@@ -119,6 +119,16 @@ struct Cost {
 const Cost COSTS[2][2] = {{{128, 512, 0.50, 0.94, 6.5, 6.5, 7.5}, {256, 256, 1.00, 1.40, 13, 13, 16}},
                           {{128, 512, 0.67, 1.28, 6.5, 8.0, 9.0}, {256, 256, 1.60, 2.18, 13, 16, 24}}};
 const double JOIN[2] = {0.87e-6, 1.6e-6};
+// k steps of two words that a 256 x 256 tile adds up in the matrix cores, whose errors
+// grow with the root of a sum's length: such a tile has no registers to put sums aside
+// (128 x 128 tiles do, every eight steps).  The published
+// five steps in fp32: with Gram matrices on 256 x 256 tiles results of 512 x 2048 (64
+// steps) are 2.2e-6 off where 128 x 128 tiles leave 1.7e-6, of 512 x 14336 (448) 5.7e-6
+// and 1.7e-6, of 512 x 65536 1.1e-5 and 2.1e-6; all phases on 256 x 256 tiles, 2048 x 2048
+// (64) 2.4e-6 and 0.9e-6, 4096 x 4096 (128) 3.3e-6 and 1.0e-6 (in a library's products
+// 3.6e-6 and 4.8e-6).  Longer sums take smaller tiles, or parts, which are joined with
+// rounding; their updates take a sixth longer.
+constexpr int64_t LONG_SUM = 64;
 
 struct Plan {
   int big = 0;
@@ -234,10 +244,14 @@ struct Pass {
       const int side = COSTS[0][big].side, slots = COSTS[0][big].slots;
       OrthoPhase ph{};
       lay(phase, side, ph);
+      int64_t sum = 0;   // the longest of two words
+      for (const OrthoGroup& g : groups)
+        if (g.words == 2) sum = std::max(sum, steps_of(phase, g));
       const int whole_rounds = ph.tiles / slots * slots;
       for (int n : {1, 2, 3, 4, 6, 8, 12, 16})
         for (int whole : {0, whole_rounds}) {
           if (n == 1 ? whole != 0 : whole == ph.tiles) continue;
+          if (big && (whole || n == 1 ? sum : (sum + n - 1) / n) > LONG_SUM) continue;
           const int rest = ph.tiles - whole;
           if (n > 1 && ((int64_t)rest * n > (big ? 1024 : 2048) ||
                         2 * n > steps_of(phase, ph.g[0])))

@@ -1,0 +1,89 @@
+"""How the orthogonalisation of updates cuts its products, planned without a GPU."""
+
+from __future__ import annotations
+
+import ctypes
+import math
+import os
+import random
+import shutil
+import subprocess
+
+import numpy as np
+import pytest
+
+from scao_amd import _lib as L
+from scao_amd.build import FLAGS, HIPCC, ROOT
+
+GRAM, SQUARE, UPDATE = range(3)
+
+
+@pytest.fixture(scope="module")
+def plan(tmp_path_factory):
+    """plan([(rows, cols, precision)]): a dict for every phase of every pass"""
+    if shutil.which(HIPCC) is None:
+        pytest.skip("no hipcc")
+    so = str(tmp_path_factory.mktemp("plan") / "ortho_plan.so")
+    subprocess.run([HIPCC, *FLAGS, "-O1", "-shared", "-o", so,
+                    os.path.join(ROOT, "tests", "ortho_plan.hip")], check=True)
+    lib = ctypes.CDLL(so)
+    lib.ortho_plan.argtypes = [ctypes.c_void_p, ctypes.c_int, ctypes.c_int, ctypes.c_void_p,
+                               ctypes.c_void_p, ctypes.c_int]
+    out, us = np.zeros((256, 8), dtype=np.int32), np.zeros(256)
+
+    def call(matrices, steps=5):
+        t = np.zeros(len(matrices), dtype=L.ORTHO_DESC)
+        for i, (rows, cols, precision) in enumerate(matrices):
+            t[i]["rows"], t[i]["cols"], t[i]["precision"] = rows, cols, precision
+        n = lib.ortho_plan(t.ctypes.data, len(t), steps, out.ctypes.data, us.ctypes.data, len(out))
+        assert 0 <= n <= len(out)
+        names = ("run", "phase", "side", "tiles", "whole", "parts", "matrices", "panels")
+        return [dict(zip(names, row.tolist()), us=float(t)) for row, t in zip(out[:n], us)]
+
+    return call
+
+
+def _sum(phase, rows, cols, words):
+    """k steps of a tile: 64 k, or 32 of two words"""
+    k = max(rows, cols) if phase == GRAM else min(rows, cols)
+    return -(-k * words // 64)
+
+
+def _words(rows, cols, precision):
+    return 2 if precision == L.ORTHO_FP32 or min(rows, cols) <= 128 else 1
+
+
+def _lists(seed, many):
+    """lists of up to three shapes, one to 24 matrices of each, in one pass"""
+    rng = random.Random(seed)
+    for _ in range(many):
+        matrices = []
+        for _ in range(rng.randint(1, 3)):
+            m, n = (max(1, int(math.exp(rng.uniform(math.log(16), math.log(16384)))))
+                    for _ in range(2))
+            m, n = (v // 64 * 64 if rng.random() < 0.5 and v >= 64 else v for v in (m, n))
+            matrices += [(m, n, rng.randint(0, 1))] * rng.choice([1, 1, 2, 4, 8, 24])
+        yield matrices
+
+
+def test_long_sums_of_two_words_are_not_left_to_the_matrix_cores(plan):
+    """Tiles of 256 x 256 add up to 64 steps of two words each."""
+    fixed = [[(4096, 14336, 1)] * 2, [(2048, 8192, 1)] * 8, [(4096, 4096, 1)] * 4,
+             [(512, 65536, 1)] * 64, [(4096, 14336, 1), (4096, 14336, 0)], [(120, 1 << 19, 0)] * 9,
+             [(32768, 32768, 1)]]
+    large = 0
+    for matrices in fixed + list(_lists(5, 400)):
+        left = sorted(matrices, key=lambda s: (-min(s[:2]), -s[0], -s[1], -_words(*s)))
+        for row in plan(matrices):
+            if row["phase"] == GRAM:
+                mine, left = left[:row["matrices"]], left[row["matrices"]:]
+            if row["side"] == 128:
+                continue
+            sums = [_sum(row["phase"], m, n, 2) for m, n, p in mine if _words(m, n, p) == 2]
+            if not sums:
+                continue
+            large += 1
+            parts = 1 if row["whole"] else row["parts"]
+            assert -(-max(sums) // parts) <= 64, (matrices, row)
+        assert not left or not plan(matrices)
+    assert large > 20
