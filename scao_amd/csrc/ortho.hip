@@ -127,7 +127,7 @@ const double JOIN[2] = {0.87e-6, 1.6e-6};
 // and 1.7e-6, of 512 x 65536 1.1e-5 and 2.1e-6; all phases on 256 x 256 tiles, 2048 x 2048
 // (64) 2.4e-6 and 0.9e-6, 4096 x 4096 (128) 3.3e-6 and 1.0e-6 (in a library's products
 // 3.6e-6 and 4.8e-6).  Longer sums take smaller tiles, or parts, which are joined with
-// rounding; their updates take a sixth longer.
+// rounding: two of 4096 x 4096 take a sixth longer so, two of 4096 x 14336 a quarter.
 constexpr int64_t LONG_SUM = 64;
 
 struct Plan {

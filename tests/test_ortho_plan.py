@@ -14,8 +14,9 @@ import pytest
 
 from scao_amd import _lib as L
 from scao_amd.build import FLAGS, HIPCC, ROOT
+from tests.ortho_paths import LISTS, matrices
 
-GRAM, SQUARE, UPDATE = range(3)
+GRAM = 0   # the first phase of a pass's rows
 
 
 @pytest.fixture(scope="module")
@@ -31,9 +32,9 @@ def plan(tmp_path_factory):
                                ctypes.c_void_p, ctypes.c_int]
     out, us = np.zeros((256, 8), dtype=np.int32), np.zeros(256)
 
-    def call(matrices, steps=5):
-        t = np.zeros(len(matrices), dtype=L.ORTHO_DESC)
-        for i, (rows, cols, precision) in enumerate(matrices):
+    def call(shapes, steps=5):
+        t = np.zeros(len(shapes), dtype=L.ORTHO_DESC)
+        for i, (rows, cols, precision) in enumerate(shapes):
             t[i]["rows"], t[i]["cols"], t[i]["precision"] = rows, cols, precision
         n = lib.ortho_plan(t.ctypes.data, len(t), steps, out.ctypes.data, us.ctypes.data, len(out))
         assert 0 <= n <= len(out)
@@ -57,13 +58,13 @@ def _lists(seed, many):
     """lists of up to three shapes, one to 24 matrices of each, in one pass"""
     rng = random.Random(seed)
     for _ in range(many):
-        matrices = []
+        shapes = []
         for _ in range(rng.randint(1, 3)):
             m, n = (max(1, int(math.exp(rng.uniform(math.log(16), math.log(16384)))))
                     for _ in range(2))
             m, n = (v // 64 * 64 if rng.random() < 0.5 and v >= 64 else v for v in (m, n))
-            matrices += [(m, n, rng.randint(0, 1))] * rng.choice([1, 1, 2, 4, 8, 24])
-        yield matrices
+            shapes += [(m, n, rng.randint(0, 1))] * rng.choice([1, 1, 2, 4, 8, 24])
+        yield shapes
 
 
 def test_long_sums_of_two_words_are_not_left_to_the_matrix_cores(plan):
@@ -72,9 +73,9 @@ def test_long_sums_of_two_words_are_not_left_to_the_matrix_cores(plan):
              [(512, 65536, 1)] * 64, [(4096, 14336, 1), (4096, 14336, 0)], [(120, 1 << 19, 0)] * 9,
              [(32768, 32768, 1)]]
     large = 0
-    for matrices in fixed + list(_lists(5, 400)):
-        left = sorted(matrices, key=lambda s: (-min(s[:2]), -s[0], -s[1], -_words(*s)))
-        for row in plan(matrices):
+    for shapes in fixed + list(_lists(5, 400)):
+        left = sorted(shapes, key=lambda s: (-min(s[:2]), -s[0], -s[1], -_words(*s)))
+        for row in plan(shapes):
             if row["phase"] == GRAM:
                 mine, left = left[:row["matrices"]], left[row["matrices"]:]
             if row["side"] == 128:
@@ -84,6 +85,43 @@ def test_long_sums_of_two_words_are_not_left_to_the_matrix_cores(plan):
                 continue
             large += 1
             parts = 1 if row["whole"] else row["parts"]
-            assert -(-max(sums) // parts) <= 64, (matrices, row)
-        assert not left or not plan(matrices)
+            assert -(-max(sums) // parts) <= 64, (shapes, row)
+        assert not left or not plan(shapes)
     assert large > 20
+
+
+def _paths(plan, shapes):
+    """of a list: panels, or what each phase does with every kind of matrix"""
+    paths = set()
+    left = sorted(shapes, key=lambda s: (-min(s[:2]), -s[0], -s[1], -_words(*s)))
+    for row in plan(shapes):
+        if row["phase"] == GRAM:
+            mine, left = left[:row["matrices"]], left[row["matrices"]:]
+        if row["panels"]:
+            paths.add("panels")
+            continue
+        assert 0 <= row["whole"] <= row["tiles"]
+        assert (row["parts"] > 1) == (row["whole"] < row["tiles"])
+        mode = ("whole" if row["whole"] == row["tiles"] else
+                "split" if row["whole"] == 0 else "last round split")
+        for m, n, p in mine:
+            paths.add((row["phase"], row["side"], mode, _words(m, n, p), m <= n))
+    return paths
+
+
+def test_the_tests_take_every_path(plan):
+    tested = set()
+    for precision, shapes in LISTS:
+        p = L.ORTHO_FP32 if precision == "fp32" else L.ORTHO_FAST
+        tested |= _paths(plan, [(*s, p) for s in matrices(shapes)])
+    assert len(tested) > 60
+    rng = random.Random(3)
+    for _ in range(8000):
+        shapes, p = [], rng.randint(0, 1)
+        for _ in range(rng.randint(1, 3)):
+            m, n = (max(1, int(math.exp(rng.uniform(math.log(16), math.log(6000)))))
+                    for _ in range(2))
+            m, n = (v // 64 * 64 if rng.random() < 0.4 and v >= 64 else v for v in (m, n))
+            shapes += [(m, n, p)] * rng.choice([1, 1, 2, 4, 8, 24])
+        left = _paths(plan, shapes) - tested
+        assert not left, (shapes, left)
