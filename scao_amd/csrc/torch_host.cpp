@@ -577,11 +577,12 @@ PyObject* grad_clip(PyObject*, PyObject* const* args, Py_ssize_t n) {
 //   orthogonalize  fresh results of one type
 //   muon_step_     parameters and momenta written in place
 std::vector<Tensor> op_orthogonalize(at::TensorList updates, at::ArrayRef<double> coefficients,
-                                     double eps, std::optional<at::ScalarType> dtype) {
+                                     double eps, std::optional<at::ScalarType> dtype,
+                                     std::optional<at::ScalarType> ns_dtype) {
   static const auto op = c10::Dispatcher::singleton()
                              .findSchemaOrThrow("scao_amd::orthogonalize", "")
                              .typed<decltype(op_orthogonalize)>();
-  return op.call(updates, coefficients, eps, dtype);
+  return op.call(updates, coefficients, eps, dtype, ns_dtype);
 }
 void op_muon_step_(at::TensorList params, at::TensorList grads, at::TensorList momenta,
                    at::ArrayRef<double> rates, at::ArrayRef<double> decays, double momentum,
@@ -607,8 +608,10 @@ void check_matrices(at::TensorList list, const char* name, c10::Device on) {
                 " must have sides below 2^20, the smaller one up to 2^15 (got ", t.sym_sizes(), ")");
   }
 }
-void check_result(std::optional<at::ScalarType> dtype) {
+void check_result(std::optional<at::ScalarType> dtype, std::optional<at::ScalarType> ns_dtype) {
   TORCH_CHECK(!dtype || code_of(*dtype) >= 0, "orthogonalize: no result of type ", *dtype);
+  TORCH_CHECK(!ns_dtype || *ns_dtype == at::kFloat || *ns_dtype == at::kBFloat16,
+              "orthogonalize: no products of type ", *ns_dtype);
 }
 void check_scheme(at::ArrayRef<double> coefficients) {
   TORCH_CHECK(lib.orthogonalize, "orthogonalize: scao_amd has not loaded its library");
@@ -644,12 +647,13 @@ Tensor row_strided(const Tensor& t) {
 }
 
 std::vector<Tensor> orthogonalize_hip(at::TensorList updates, at::ArrayRef<double> coefficients,
-                                      double eps, std::optional<at::ScalarType> dtype) {
+                                      double eps, std::optional<at::ScalarType> dtype,
+                                      std::optional<at::ScalarType> ns_dtype) {
   check_scheme(coefficients);
   std::vector<Tensor> out;
   if (updates.empty()) return out;
   check_matrices(updates, "updates", updates[0].device());
-  check_result(dtype);
+  check_result(dtype, ns_dtype);
   const c10::DeviceGuard guard(updates[0].device());
   std::vector<Tensor> in;
   std::vector<scao_ortho_desc> table;
@@ -657,8 +661,9 @@ std::vector<Tensor> orthogonalize_hip(at::TensorList updates, at::ArrayRef<doubl
     in.push_back(row_strided(t.resolve_neg()));
     const at::ScalarType type = dtype.value_or(t.scalar_type());
     out.push_back(at::empty(t.sizes(), t.options().dtype(type)));
-    // one word an element where the result has fewer bits than it
-    const int precision = type == at::kBFloat16 ? SCAO_ORTHO_FAST : SCAO_ORTHO_FP32;
+    // by default one word an element where the result has fewer bits than it
+    const int precision =
+        ns_dtype.value_or(type) == at::kBFloat16 ? SCAO_ORTHO_FAST : SCAO_ORTHO_FP32;
     char* to = (char*)out.back().data_ptr();
     for_matrices(in.back(), [&](char* p, int64_t rows, int64_t cols, int64_t ld) {
       table.push_back({p, to, rows, cols, ld, cols, code_of(t.scalar_type()), code_of(type),
@@ -742,11 +747,12 @@ void muon_step_version_(at::TensorList params, at::TensorList grads, at::TensorL
 }
 
 std::vector<Tensor> orthogonalize_meta(at::TensorList updates, at::ArrayRef<double> coefficients,
-                                       double, std::optional<at::ScalarType> dtype) {
+                                       double, std::optional<at::ScalarType> dtype,
+                                       std::optional<at::ScalarType> ns_dtype) {
   check_scheme(coefficients);
   std::vector<Tensor> out;
   if (!updates.empty()) check_matrices(updates, "updates", updates[0].device());
-  check_result(dtype);
+  check_result(dtype, ns_dtype);
   for (const Tensor& t : updates)
     out.push_back(at::empty_symint(t.sym_sizes(), t.options().dtype(dtype.value_or(t.scalar_type()))));
   return out;
@@ -766,18 +772,19 @@ bool tangent(at::TensorList list) {
 }
 std::vector<Tensor> orthogonalize_autograd(at::TensorList updates,
                                            at::ArrayRef<double> coefficients, double eps,
-                                           std::optional<at::ScalarType> dtype) {
+                                           std::optional<at::ScalarType> dtype,
+                                           std::optional<at::ScalarType> ns_dtype) {
   bool wanted = tangent(updates);
   if (at::GradMode::is_enabled())
     for (const Tensor& t : updates) wanted = wanted || t.requires_grad();
   TORCH_CHECK_NOT_IMPLEMENTED(!wanted, "orthogonalize has no derivative: detach the updates");
   const at::AutoDispatchBelowADInplaceOrView below;
-  return op_orthogonalize(updates, coefficients, eps, dtype);
+  return op_orthogonalize(updates, coefficients, eps, dtype, ns_dtype);
 }
 
 TORCH_LIBRARY_FRAGMENT(scao_amd, m) {
-  m.def("orthogonalize(Tensor[] updates, float[] coefficients, float eps, ScalarType? dtype) "
-        "-> Tensor[]");
+  m.def("orthogonalize(Tensor[] updates, float[] coefficients, float eps, ScalarType? dtype, "
+        "ScalarType? ns_dtype=None) -> Tensor[]");
   m.def("muon_step_(Tensor(a!)[] params, Tensor[] grads, Tensor(b!)[] momenta, float[] rates, "
         "float[] decays, float momentum, bool nesterov, float[] coefficients, float eps, "
         "int[] precisions) -> ()");

@@ -48,9 +48,15 @@ def _check_eps(eps: float) -> float:
     return eps
 
 
+def _check_ns_dtype(ns_dtype) -> None:
+    if ns_dtype not in (None, torch.float32, torch.bfloat16):
+        raise ValueError(f"ns_dtype must be None, torch.float32 or torch.bfloat16 (got {ns_dtype})")
+
+
 def orthogonalize(updates: Union[Tensor, Sequence[Tensor]], steps: int = 5,
                   coefficients=NS_COEFFICIENTS, eps: float = 1e-7,
-                  dtype: Optional[torch.dtype] = None) -> Union[Tensor, list]:
+                  dtype: Optional[torch.dtype] = None, ns_dtype: Optional[torch.dtype] = None
+                  ) -> Union[Tensor, list]:
     """The matrices of ``updates`` with their singular values taken through
     ``steps`` Newton-Schulz steps, as fresh contiguous tensors.
 
@@ -59,16 +65,16 @@ def orthogonalize(updates: Union[Tensor, Sequence[Tensor]], steps: int = 5,
     stride.  coefficients: (a, b, c), or one such triple a step.  dtype: the
     results' type, that of each update by default.
 
-    bfloat16 results go through products of fp16 words (three bits more than
-    bfloat16's own, sums in float32; 0.6e-3 to 1.4e-3 off with the defaults, their last
-    rounding 1.7e-3);
-    float32 and float16 ones, and matrices of up to 128 rows or columns, through
-    products of 22-bit words, at a third of the rate: pass ``dtype=torch.bfloat16``
-    where that accuracy is not needed.  A matrix with a NaN or an infinity gives NaN
-    throughout and no other matrix; one of zeros gives zeros.  Coefficients with
-    which a singular value may grow beyond 1024 are refused.  eps is meant to be
-    small beside the norms: G / (|G| + eps) is held to 2^-39 absolutely, whatever the
-    precision.  No derivative."""
+    ns_dtype: how exact the products are.  torch.bfloat16: of fp16 words (three bits
+    more than bfloat16's own), sums in float32; with the defaults 0.6e-3 to 1.4e-3 off,
+    where a bfloat16's last rounding is 1.7e-3.  torch.float32: of 22-bit words, at a
+    third of the rate (1e-6 to 2e-6 off); matrices of up to 128 rows or columns have
+    them in any case.  None: bfloat16 for results of that type, else float32.
+
+    A matrix with a NaN or an infinity gives NaN throughout and no other matrix; one of
+    zeros gives zeros.  Coefficients with which a singular value may grow beyond 1024 are
+    refused.  eps is meant to be small beside the norms: G / (|G| + eps) is held to 2^-39
+    absolutely, whatever the precision.  No derivative."""
     flat, eps = _flat_coefficients(coefficients, steps), _check_eps(eps)
     single = isinstance(updates, Tensor)
     updates = [updates] if single else list(updates)
@@ -86,10 +92,11 @@ def orthogonalize(updates: Union[Tensor, Sequence[Tensor]], steps: int = 5,
             raise RuntimeError(f"updates on {updates[0].device} and {t.device}")
     if dtype is not None and dtype not in L.DTYPE_CODE:
         raise TypeError(f"dtype must be float32, bfloat16 or float16 (got {dtype})")
+    _check_ns_dtype(ns_dtype)
     if not updates:
         return []
     L.torch_host()
-    out = torch.ops.scao_amd.orthogonalize(updates, flat, eps, dtype)
+    out = torch.ops.scao_amd.orthogonalize(updates, flat, eps, dtype, ns_dtype)
     return out[0] if single else out
 
 
@@ -140,9 +147,7 @@ class Muon(torch.optim.Optimizer):
         if group["adjust_lr_fn"] not in (None, "original", "match_rms_adamw"):
             raise ValueError('adjust_lr_fn must be None, "original" or "match_rms_adamw" '
                              f"(got {group['adjust_lr_fn']!r})")
-        if group["ns_dtype"] not in (None, torch.float32, torch.bfloat16):
-            raise ValueError("ns_dtype must be None, torch.float32 or torch.bfloat16 "
-                             f"(got {group['ns_dtype']})")
+        _check_ns_dtype(group["ns_dtype"])
         _check_eps(group["eps"])
         for p in group["params"]:
             if p.ndim < 2:

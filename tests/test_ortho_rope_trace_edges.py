@@ -44,7 +44,9 @@ def test_a_trace_refuses_the_updates_that_the_kernels_refuse():
     m = torch.empty(8, 16, device="meta")
     assert op([m], co, 1e-7, torch.bfloat16)[0].dtype == torch.bfloat16
     assert op([torch.empty(0, 1 << 21, device="meta")], co, 1e-7, None)[0].shape == (0, 1 << 21)
-    for args in (([m], co, 1e-7, torch.float64), ([m.double()], co, 1e-7, None),
+    assert op([m], co, 1e-7, torch.float16, torch.float32)[0].dtype == torch.float16
+    for args in (([m], co, 1e-7, None, torch.float16), ([m], co, 1e-7, torch.float64),
+                 ([m.double()], co, 1e-7, None),
                  ([m[0]], co, 1e-7, None), ([m], co[:2], 1e-7, None), ([m], co * 65, 1e-7, None),
                  ([m], [], 1e-7, None), ([torch.empty(1 << 20, 4, device="meta")], co, 1e-7, None),
                  ([torch.empty(40000, 40000, device="meta")], co, 1e-7, None)):
