@@ -2,6 +2,7 @@
 
 from __future__ import annotations
 
+import csv
 import ctypes
 import math
 import os
@@ -125,3 +126,44 @@ def test_the_tests_take_every_path(plan):
             shapes += [(m, n, p)] * rng.choice([1, 1, 2, 4, 8, 24])
         left = _paths(plan, shapes) - tested
         assert not left, (shapes, left)
+
+
+def _matrices(text, words):
+    return [(*map(int, shape.split("x")), words - 1) for shape, many in
+            (part.split("*") for part in text.split(",")) for _ in range(int(many))]
+
+
+def test_choice_against_measured_products(plan):
+    """Tiles, parts and panels as they are chosen, against the best of what
+    perf/ortho_tiles.hip measured."""
+    tiles, panels = {}, {}
+    with open(os.path.join(ROOT, "profiles", "ortho_tiles.csv")) as fh:
+        for r in csv.DictReader(fh):
+            key = r["list"], int(r["words"])
+            if r["phase"] == "panels":
+                panels[key] = float(r["us"])
+            else:
+                forms = tiles.setdefault(key, {}).setdefault(int(r["phase"]), {})
+                forms[int(r["side"]), int(r["parts"]), int(r["whole"])] = float(r["us"])
+    behind, steps = [], []
+    for (text, words), phases in tiles.items():
+        shapes = _matrices(text, words)
+        rows = plan(shapes)
+        assert len(rows) == 3
+        took = 0.0
+        for row in rows:
+            forms = phases[row["phase"]]
+            chosen = forms[row["side"], row["parts"], row["whole"]]
+            long = max((_sum(row["phase"], m, n, 2) for m, n, p in shapes
+                        if _words(m, n, p) == 2), default=0)
+            allowed = [us for (side, parts, whole), us in forms.items()
+                       if side == 128 or (long if whole else -(-long // parts)) <= 64]
+            behind.append(chosen / min(allowed))
+            took += chosen
+        if (text, words) in panels:
+            by = panels[text, words]
+            steps.append((by if rows[0]["panels"] else took) / min(by, took))
+    print(f"{len(behind)} launches: {np.exp(np.log(behind).mean()):.4f}, {max(behind):.3f}; "
+          f"{len(steps)} steps: {np.exp(np.log(steps).mean()):.4f}, {max(steps):.3f}")
+    assert len(behind) == 222 and np.exp(np.log(behind).mean()) < 1.03 and max(behind) < 1.4
+    assert len(steps) == 33 and np.exp(np.log(steps).mean()) < 1.05 and max(steps) < 1.3
