@@ -110,7 +110,8 @@ class Muon(torch.optim.Optimizer):
     0.2 sqrt(max(rows, cols)) ("match_rms_adamw").  The arguments and the state's
     ``momentum_buffer`` are those of ``torch.optim.Muon``; the buffer is float32
     whatever the parameter's type is.  Parameters are contiguous matrices, or
-    stacks of them with the matrices last; vectors and embeddings belong to
+    stacks of them with the matrices last (a convolution's weight would be a stack of its
+    kernels: flatten it to a matrix before); vectors and embeddings belong to
     another optimizer, such as ``SCAO``.  One call steps all parameters.  A step can be
     captured into a graph once a step before it has made the momentum.
 

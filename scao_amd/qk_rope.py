@@ -102,7 +102,8 @@ def qk_norm_rope(q: Tensor, k: Tensor, q_weight: Optional[Tensor], k_weight: Opt
     Sums and products are float32, every output is rounded once.  Differentiable
     once in q, k and the weights, not in the tables, and not in forward mode.  A head
     with a NaN or an infinity gives NaN there (an infinity: zeros beside it), in its
-    gradient and in the weight's, and in no other head."""
+    gradient and in the weight's, and in no other head; one whose sum of squares is past
+    float32's range (values of 1e19) is all zeros, as beside an infinity."""
     rest = q_weight, k_weight, cos, sin
     if q.ndim == 4 and q.is_cuda:
         # the operator checks for itself, in a sixth of the time; what it refuses is

@@ -55,3 +55,16 @@ def test_up_to_128_rows_have_two_words(hip_device, m, n):
     g = _update(hip_device, m + n, m, n, torch.bfloat16)
     want = orthogonalize(g, PUBLISHED)
     assert relative(scao_amd.orthogonalize(g), want) <= 1.01 * relative(want.bfloat16(), want)
+
+
+@pytest.mark.parametrize("m,n", [(256, 256), (300, 160), (640, 700)])
+def test_one_word_with_strong_growth(hip_device, m, n):
+    """Singular values that the first step takes far up and the second far down."""
+    g = _update(hip_device, 9, m, n, torch.float32)
+    co = [(30.0, 0.0, 0.0), (1.0 / 16, 2.0 ** -14, 2.0 ** -24), (0.5, 0.125, 0.0)]
+    full = torch.empty(m, n, device=hip_device)
+    _call([g], [full], L.ORTHO_FAST, co)
+    want, room = allowed(g, co, torch.float32)
+    err = relative(full, want)
+    print(f"{m}x{n}: {err:.2e} of {room:.2e}", flush=True)
+    assert err <= room <= 2e-3

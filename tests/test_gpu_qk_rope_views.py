@@ -54,3 +54,19 @@ def test_a_trace_says_how_outputs_lie(hip_device, which):
         dx = torch.ops.scao_amd.qk_norm_rope_backward(q, q, *rest, 3)
         strides.append([o.stride() for o in (*y, *dx)])
     assert strides[0] == strides[1]
+
+
+def test_vmapped(hip_device):
+    """torch maps the operator over a dimension by calling it for every entry."""
+    q = torch.randn(3, 2, 5, 4, 32, device=hip_device)
+    w = torch.randn(3, 32, device=hip_device)
+    cos, sin = scao_amd.rotary_table(5, 32, device=hip_device)
+    got = torch.func.vmap(lambda a, b: scao_amd.qk_norm_rope(a, a[:, :, :1], b, b, cos, sin))(q, w)
+    for i in range(3):
+        one = scao_amd.qk_norm_rope(q[i], q[i, :, :, :1], w[i], w[i], cos, sin)
+        assert all(torch.equal(a[i], b) for a, b in zip(got, one))
+    # what torch cannot map is refused
+    with pytest.raises(RuntimeError):
+        torch.func.vmap(lambda a: scao_amd.orthogonalize(a))(q[:, 0, 0])
+    with pytest.raises(RuntimeError):
+        torch.func.grad(lambda a: scao_amd.qk_norm_rope(a, a, None, None, cos, sin)[0].sum())(q[0])
