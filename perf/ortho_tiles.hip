@@ -32,7 +32,7 @@ const char* LISTS[] = {
     "1024x1024*8", "1024x1024*16", "1024x1024*20", "512x2048*8", "2048x2048*1", "2048x2048*2",
     "2048x2048*4", "2048x2048*8", "336x1000*12", "1001x333*12,333x1001*5,77x2049*7",
     "768x2304*12,768x768*12", "6246x384*4,599x256*16", "384x1536*4,448x1024*4,1593x2112*1",
-    "63x1599*16,320x46*3", "1024x4096*4", "2048x8192*3", "14336x4096*1"};
+    "63x1599*16,320x46*3", "1024x4096*4", "2048x8192*4", "14336x4096*1"};
 
 constexpr int64_t ROOM = (int64_t)4 << 30, PARTS = (int64_t)512 << 20;
 char *buffer, *parts_buffer;

@@ -108,7 +108,7 @@ bool scales_of(const double* co, int steps, Scales& s) {
 // and end (sums alone, an update's, a symmetric product's with its image); of a join, a
 // part and element.  Fitted to launches of 10 to 1296 tiles and 6 to 72 steps; of the 222
 // launches of profiles/ortho_tiles.csv (perf/ortho_tiles.hip measured them) the chosen
-// form is 0.9% behind the best one on the geometric average, 31% at most.
+// form is 0.8% behind the best one on the geometric average, 18% at most.
 struct Cost {
   int side, slots;
   double lone, full, parts, update, symmetric;
@@ -309,7 +309,7 @@ struct Pass {
     // with a CU alone, 15 where all read (20 with nothing else to wait for).  Fitted to
     // calls of 160 x 160 to 512 x 1024; small launches of tiles take 15% less than their
     // estimate.  Of the 33 steps of profiles/ortho_tiles.csv that either could take, the
-    // chosen one is 2.3% behind on the geometric average, 19% at most.
+    // chosen one is 2.2% behind on the geometric average, 19% at most.
     for (int64_t at = 0; at < blocks; at += 256) {
       double most = 0;
       const double fill = std::min<int64_t>(256, blocks - at) / 256.0;
